@@ -282,6 +282,82 @@ int slotscan_read_bwd(const slotscan_read_params* p, const void* qr, const float
                       const void* vbuf, const float* kinv, const uint8_t* valid, const void* drd, void* dqr,
                       float* dsharp, void* dkbuf, void* dvbuf, float* dkinv, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * The token half of a mixer layer: what stands beside the slot memory.  [The reference leaves it to library calls: the
+ * 16-token window of memlm_sh.py:349-359, rotated queries and keys.]
+ * Strides are in elements, of a sequence, a token and a head; the channels of a head are adjacent.  Strides and base
+ * addresses are multiples of 16 bytes, so that slices of a fused projection are read where they lie.
+ *
+ * Norms of queries and keys per head with the position rotation.  Per row x of D channels
+ *     r = (mean x^2 + eps)^(-1/2),   y = x r w,   then the channel pairs (i, i + R/2), i < R/2, turn by the angle of the
+ * token's position:  y_i' = y_i cos - y_j sin,  y_j' = y_j cos + y_i sin.
+ *   q (B,T,H,D), k (B,T,KV,D) of `dtype`, strided;  table (table_len, R/2, 2) fp32: cosine and sine of every position
+ *   pos   (B,T) int32, or NULL: token t of a sequence stands at position t.  A position outside the table gives NaN.
+ *   qw, kw (D) fp32, or NULL for ones
+ *   qo (B,T,H,D), ko (B,T,KV,D) contiguous
+ * D a multiple of 8 up to 256, R a multiple of 16 up to D (0: no rotation, table NULL).
+ * slotscan_norm_rope_bwd: gradients dqo, dko (contiguous) to dq, dk (contiguous) and dqw, dkw (D) fp32 (both or neither; scratch
+ * of slotscan_norm_rope_bwd_scratch_bytes, only with them); sums in a fixed order, equal from run to run. */
+typedef struct {
+    int32_t B, T, H, KV, D, R, table_len, dtype;
+    float eps;
+    int64_t q_stride[3], k_stride[3];
+} slotscan_norm_params;
+int slotscan_norm_rope_check(const slotscan_norm_params* p);
+int slotscan_norm_rope_fwd(const slotscan_norm_params* p, const void* q, const void* k, const float* table, const int32_t* pos,
+                           const float* qw, const float* kw, void* qo, void* ko, void* stream);
+size_t slotscan_norm_rope_bwd_scratch_bytes(const slotscan_norm_params* p);
+int slotscan_norm_rope_bwd(const slotscan_norm_params* p, const void* q, const void* k, const float* table, const int32_t* pos,
+                           const float* qw, const float* kw, const void* dqo, const void* dko, void* dq, void* dk, float* dqw,
+                           float* dkw, void* scratch, size_t scratch_bytes, void* stream);
+/* The same for the next T tokens of running sequences: token t of sequence b stands at position pos[b] + t, and its rotated key
+ * and its value v (B,T,KV,D) go to row (pos[b] + t) mod L of the caches (B,L,KV,D), whose strides are of a sequence, a row and a
+ * head.  T <= L.  Negative positions store nothing. */
+typedef struct {
+    slotscan_norm_params base;
+    int32_t L;
+    int64_t v_stride[3], kc_stride[3], vc_stride[3];
+} slotscan_append_params;
+int slotscan_norm_rope_append(const slotscan_append_params* p, const void* q, const void* k, const void* v, const float* table,
+                              const int32_t* pos, const float* qw, const float* kw, void* qo, void* kc, void* vc, void* stream);
+
+/* Attention over tokens.  Query i of Tq stands at position i + Tk - Tq, key j of Tk at j; query head h reads key head
+ * h / (H / KV).   s = scale <q_i, k_j>;  s <- cap tanh(s / cap) if cap > 0;  s <- s - slopes[h] |i - j|;  softmax over the
+ * visible keys;  o_i = sum p v_j.  Visible, with positions i and j:
+ *     docs[i].begin <= j < docs[i].end   and   |i - j| < window (if window > 0)   and   (j <= i  or  j < prefix[b])
+ * A row without a visible key gives zeros and takes no part in the gradients; values that are hidden from a query, NaN and
+ * infinities among them, do not reach it.
+ *   slopes (H) fp32 or NULL;  docs (B,Tk,2) int32 or NULL: where the document of each position begins and ends; documents are
+ *   intervals, and padding stands in one of no length at its own place;  prefix (B) int32 or NULL
+ *   o (B,Tq,H,D) contiguous;  lse (B,H,Tq) fp32 or NULL: what the backward needs of the softmax (base-2 logarithm of its sum;
+ *   minus infinity for an empty row, plus infinity for a row of a single key, whose weight is 1 and whose scores have no gradient)
+ * D a multiple of 8 up to 128.
+ * slotscan_attn_bwd: gradient dout (contiguous like o) to dq, dk, dv, contiguous.  delta: (B,H,Tq) fp32 scratch.  No atomics: the
+ * results are equal from run to run. */
+typedef struct {
+    int32_t B, Tq, Tk, H, KV, D, window, dtype;
+    float scale, cap;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+} slotscan_attn_params;
+int slotscan_attn_check(const slotscan_attn_params* p);
+int slotscan_attn_fwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
+                      const int32_t* docs, const int32_t* prefix, void* o, float* lse, void* stream);
+int slotscan_attn_bwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
+                      const int32_t* docs, const int32_t* prefix, const void* o, const float* lse, const void* dout, float* delta,
+                      void* dq, void* dk, void* dv, void* stream);
+/* One query for each sequence over ring caches (B,L,KV,D) whose row j mod L holds position j: the query stands at pos[b] and sees
+ * the positions from max(start[b], pos[b] - min(window, L) + 1, 0) to pos[b] (start NULL: 0).  q strides: of a sequence and a
+ * head.  o (B,H,D) contiguous.  scratch: slotscan_attn_step_scratch_bytes, which depends on p alone. */
+typedef struct {
+    int32_t B, H, KV, D, L, window, dtype;
+    float scale, cap;
+    int64_t q_stride[2], k_stride[3], v_stride[3];
+} slotscan_attn_step_params;
+int slotscan_attn_step_check(const slotscan_attn_step_params* p);
+size_t slotscan_attn_step_scratch_bytes(const slotscan_attn_step_params* p);
+int slotscan_attn_step(const slotscan_attn_step_params* p, const void* q, const void* k, const void* v, const int32_t* pos,
+                       const int32_t* start, const float* slopes, void* o, void* scratch, size_t scratch_bytes, void* stream);
+
 /* Registers / spilled bytes / static shared memory / max threads of each kernel, the analogue of kernel_attrs
  * (gqa25/slotkern_cuda.py:467-479).  Fills up to `cap` entries (HOST memory), returns how many kernels exist. */
 typedef struct {

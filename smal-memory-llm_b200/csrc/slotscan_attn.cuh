@@ -1,0 +1,66 @@
+// Attention over tokens: what its kernels share.
+//
+// A query at position i sees, of the keys, one interval [lo, hi): its document's bounds, the window and the causal rule (or the prefix)
+// are intervals each.  Read from a key's side, the queries that see it are one interval too.  So a tile of rows visits the tiles of
+// the other side between the least lo and the greatest hi of its rows, and masks the ones that some row does not see whole.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "slotscan.h"
+#include "slotscan_common.cuh"
+
+namespace slotscan {
+
+typedef __nv_bfloat16 bf16;
+constexpr float LOG2E = 1.44269504088896f;
+
+struct AttnArgs {
+    int B, Tq, Tk, H, KV, D;
+    int window;                                          // 1 .. Tk: |i - j| < window
+    float scale, cap;                                    // cap 0: none
+    long long qs[3], ks[3], vs[3];                       // elements from sequence to sequence, token to token, head to head
+    const float* slopes;                                 // per query head, or NULL
+    const int2* docs;                                    // (B, Tk) bounds, or NULL
+    const int32_t* prefix;                               // (B), or NULL
+};
+
+struct Span { int lo, hi; };                             // empty where hi <= lo
+
+// keys that query row i (of Tq) sees
+__device__ __forceinline__ Span keys_of(const AttnArgs& a, int b, int i) {
+    const int at = i + a.Tk - a.Tq;
+    const int2 d = a.docs != nullptr ? a.docs[(size_t)b * a.Tk + at] : make_int2(0, a.Tk);
+    const int reach = a.prefix != nullptr ? max(at + 1, a.prefix[b]) : at + 1;
+    return {max(max(d.x, 0), at - a.window + 1), min(min(d.y, a.Tk), min(reach, at + a.window))};
+}
+// query rows that see key j
+__device__ __forceinline__ Span queries_of(const AttnArgs& a, int b, int j) {
+    const int off = a.Tk - a.Tq;
+    const int2 d = a.docs != nullptr ? a.docs[(size_t)b * a.Tk + j] : make_int2(0, a.Tk);
+    const int from = a.prefix != nullptr && j < a.prefix[b] ? 0 : j;
+    return {max(max(max(d.x, from), j - a.window + 1) - off, 0), min(min(d.y, a.Tk), j + a.window) - off};
+}
+
+// a score as the base-2 exponent of its weight, before the softmax's shift.  Of the cap, t = tanh(scale <q, k> / cap), whose
+// derivative is 1 - t^2.
+struct Score {
+    float lin, cap_in, cap_out, slope;                   // slope in base 2
+    __device__ __forceinline__ Score(const AttnArgs& a, int h) {
+        lin = a.scale * LOG2E;
+        cap_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
+        cap_out = a.cap * LOG2E;
+        slope = a.slopes != nullptr ? a.slopes[h] * LOG2E : 0.f;
+    }
+};
+
+// the launches of the two families, float32 and bf16
+cudaError_t run_attn_fwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st);
+cudaError_t run_attn_bwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                             float* delta, void* dq, void* dk, void* dv, cudaStream_t st);
+cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st);
+cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                              float* delta, void* dq, void* dk, void* dv, cudaStream_t st);
+
+}  // namespace slotscan

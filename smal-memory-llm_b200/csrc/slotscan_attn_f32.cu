@@ -1,0 +1,333 @@
+// Attention over tokens on the CUDA cores: float32, whose products the tensor cores would round to 11 bits or fewer.
+//
+// Forward: a CTA holds 64 queries of a head and passes over their keys 64 at a time, with the running maximum and sum of each
+// row's softmax.  Backward: the same walk twice, once with rows of queries (dq, and delta = <do, o> for the other), once with
+// rows of keys over the queries of all heads that share the key head (dk, dv): one more pair of products than a single walk with
+// atomic sums would take, and the same bits from run to run.
+//   rows X0, X1 / stream Y0, Y1:   queries: q, do / k, v      keys: k, v / q, do
+//   s = X0 Y0^T, dp = X1 Y1^T, p = exp(s - lse), ds = p (dp - delta) (1 - tanh^2),  out1 += ds Y0,  keys also out0 += p Y1
+// Bound by shared memory: two 16-byte reads for 8 multiply-adds of a thread's 4 x 4 block.
+#include "slotscan_attn.cuh"
+#include "slotscan_launch.h"
+
+namespace slotscan {
+
+constexpr int SA_THREADS = 256, SA_M = 64, SA_N = 64, SA_LDP = SA_N + 4;
+
+template <typename T>
+__device__ __forceinline__ float4 ld4or0(const T* p, bool ok) { return ok ? ld4(p) : make_float4(0.f, 0.f, 0.f, 0.f); }
+
+// rows [r0, r0 + 64) of a strided matrix into shared memory, zeros beyond `rows` and beyond D channels
+template <int DP, typename T>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, int r0, int rows, int D) {
+    for (int i = threadIdx.x; i < SA_M * (DP / 4); i += SA_THREADS) {
+        const int r = i / (DP / 4), c = i % (DP / 4) * 4;
+        st4(dst + r * (DP + 4) + c, ld4or0(src + (long long)(r0 + r) * stride + c, r0 + r < rows && c < D));
+    }
+}
+// C[r][c] = <A row 4 ty + r, B row tx + 16 c>
+template <int DP>
+__device__ __forceinline__ void dot_block(float (&C)[4][4], const float* A, const float* Bm, int ty, int tx) {
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) C[r][c] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = ld4(A + (4 * ty + r) * (DP + 4) + d);
+#pragma unroll
+        for (int c = 0; c < 4; c++) y[c] = ld4(Bm + (tx + 16 * c) * (DP + 4) + d);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                C[r][c] = fmaf(x[r].x, y[c].x, fmaf(x[r].y, y[c].y, fmaf(x[r].z, y[c].z, fmaf(x[r].w, y[c].w, C[r][c]))));
+    }
+}
+// acc[r][8 channels of tx] += sum_j P[4 ty + r][j] Y[j]
+template <int DP>
+__device__ __forceinline__ void product_block(float (&acc)[4][DP / 16], const float* P, const float* Y, int ty, int tx) {
+    for (int j = 0; j < SA_N; j += 4) {
+        float4 p[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) p[r] = ld4(P + (4 * ty + r) * SA_LDP + j);
+#pragma unroll
+        for (int jj = 0; jj < 4; jj++) {
+#pragma unroll
+            for (int c = 0; c < DP / 64; c++) {
+                const float4 y = ld4(Y + (j + jj) * (DP + 4) + tx * 4 + 64 * c);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float w = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+                    acc[r][4 * c] = fmaf(w, y.x, acc[r][4 * c]);
+                    acc[r][4 * c + 1] = fmaf(w, y.y, acc[r][4 * c + 1]);
+                    acc[r][4 * c + 2] = fmaf(w, y.z, acc[r][4 * c + 2]);
+                    acc[r][4 * c + 3] = fmaf(w, y.w, acc[r][4 * c + 3]);
+                }
+            }
+        }
+    }
+}
+__device__ __forceinline__ float max16(float v) {        // over the 16 lanes of a row block
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, off));
+    return v;
+}
+// base-2 exponent of a score and the factor of its derivative (1 - tanh^2)
+__device__ __forceinline__ float score2(const Score& sc, float s, int dist, float& slope_of_cap) {
+    if (sc.cap_in != 0.f) {
+        const float t = tanhf(s * sc.cap_in);
+        slope_of_cap = 1.f - t * t;
+        return fmaf(-sc.slope, (float)dist, sc.cap_out * t);
+    }
+    slope_of_cap = 1.f;
+    return fmaf(-sc.slope, (float)dist, s * sc.lin);
+}
+// least lo and greatest hi of the CTA's 64 rows (the rows that do not exist have an empty span)
+__device__ __forceinline__ Span cta_span(Span mine, bool counts, int* s_red) {
+    if (threadIdx.x == 0) { s_red[0] = BIGI; s_red[1] = 0; }
+    __syncthreads();
+    if (counts && mine.hi > mine.lo) { atomicMin(&s_red[0], mine.lo); atomicMax(&s_red[1], mine.hi); }
+    __syncthreads();
+    return {s_red[0], s_red[1]};
+}
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(SA_THREADS) attn_fwd_cores_kernel(AttnArgs a, const T* q, const T* k, const T* v, T* o, float* lse) {
+    extern __shared__ float4 smem4[];
+    float* Qs = reinterpret_cast<float*>(smem4);
+    float* Ys = Qs + SA_M * (DP + 4);                    // keys, then values
+    float* Ps = Ys + SA_N * (DP + 4);
+    __shared__ int s_red[2];
+    const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.KV);
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * SA_M;                            // the long rows first
+    const T* kb = k + b * a.ks[0] + hk * a.ks[2];
+    const T* vb = v + b * a.vs[0] + hk * a.vs[2];
+    load_tile<DP>(Qs, q + b * a.qs[0] + h * a.qs[2], a.qs[1], i0, a.Tq, a.D);
+    Span sp[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) sp[r] = i0 + 4 * ty + r < a.Tq ? keys_of(a, b, i0 + 4 * ty + r) : Span{0, 0};
+    const Span all = cta_span(i0 + tid < a.Tq && tid < SA_M ? keys_of(a, b, i0 + tid) : Span{0, 0}, tid < SA_M, s_red);
+    const Score sc(a, h);
+    float m[4], l[4], acc[4][DP / 16];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        m[r] = -INFINITY; l[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) acc[r][c] = 0.f;
+    }
+    for (int j0 = all.lo; j0 < all.hi; j0 += SA_N) {
+        __syncthreads();
+        load_tile<DP>(Ys, kb, a.ks[1], j0, a.Tk, a.D);
+        __syncthreads();
+        float s[4][4];
+        dot_block<DP>(s, Qs, Ys, ty, tx);
+        float shrink[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int at = i0 + 4 * ty + r + a.Tk - a.Tq;
+            float top = -INFINITY, unused;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int j = j0 + tx + 16 * c;
+                s[r][c] = j >= sp[r].lo && j < sp[r].hi ? score2(sc, s[r][c], abs(at - j), unused) : -INFINITY;
+                top = fmaxf(top, s[r][c]);
+            }
+            top = fmaxf(m[r], max16(top));
+            const float base = top == -INFINITY ? 0.f : top;
+            shrink[r] = exp2f(m[r] - base);
+            m[r] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float p = exp2f(s[r][c] - base);
+                sum += p;
+                Ps[(4 * ty + r) * SA_LDP + tx + 16 * c] = p;
+            }
+            l[r] = fmaf(l[r], shrink[r], group_sum<16>(sum));
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) acc[r][c] *= shrink[r];
+        }
+        __syncthreads();
+        load_tile<DP>(Ys, vb, a.vs[1], j0, a.Tk, a.D);
+        __syncthreads();
+        product_block<DP>(acc, Ps, Ys, ty, tx);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int i = i0 + 4 * ty + r;
+        if (i >= a.Tq) continue;
+        const bool empty = sp[r].hi <= sp[r].lo;
+        const float inv = empty ? 0.f : 1.f / l[r];
+#pragma unroll
+        for (int c = 0; c < DP / 64; c++) {
+            const int d = tx * 4 + 64 * c;
+            if (d < a.D)
+                st4(o + (((size_t)b * a.Tq + i) * a.H + h) * a.D + d,
+                    make_float4(acc[r][4 * c] * inv, acc[r][4 * c + 1] * inv, acc[r][4 * c + 2] * inv, acc[r][4 * c + 3] * inv));
+        }
+        if (lse != nullptr && tx == 0)
+            lse[((size_t)b * a.H + h) * a.Tq + i] = empty ? -INFINITY : sp[r].hi - sp[r].lo == 1 ? INFINITY : m[r] + log2f(l[r]);
+    }
+}
+
+// KEYS: rows of keys (dk, dv); else rows of queries (dq, and delta)
+template <int DP, bool KEYS, typename T>
+__global__ void __launch_bounds__(SA_THREADS) attn_bwd_cores_kernel(AttnArgs a, const T* q, const T* k, const T* v, const T* o, const float* lse,
+                                                                    const T* dout, float* delta, T* d0, T* d1) {
+    extern __shared__ float4 smem4[];
+    float* X0 = reinterpret_cast<float*>(smem4);
+    float* X1 = X0 + SA_M * (DP + 4);
+    float* Y0 = X1 + SA_M * (DP + 4);
+    float* Y1 = Y0 + SA_N * (DP + 4);
+    float* Ps = Y1 + SA_N * (DP + 4);
+    float* Ds = Ps + SA_M * SA_LDP;
+    __shared__ int s_red[2];
+    __shared__ float s_lse[64], s_delta[64];             // of the queries: this CTA's rows, or the stream's
+    const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16, group = a.H / a.KV;
+    const int hx = blockIdx.y, b = blockIdx.z, off = a.Tk - a.Tq, rows = KEYS ? a.Tk : a.Tq, cols = KEYS ? a.Tq : a.Tk;
+    const int r0 = blockIdx.x * SA_M;
+    const int hk = KEYS ? hx : hx / group;
+    const long long os = (long long)a.H * a.D;           // of o and dout: contiguous
+    const T* kb = k + b * a.ks[0] + hk * a.ks[2];
+    const T* vb = v + b * a.vs[0] + hk * a.vs[2];
+    if constexpr (KEYS) {
+        load_tile<DP>(X0, kb, a.ks[1], r0, rows, a.D);
+        load_tile<DP>(X1, vb, a.vs[1], r0, rows, a.D);
+    } else {
+        load_tile<DP>(X0, q + b * a.qs[0] + hx * a.qs[2], a.qs[1], r0, rows, a.D);
+        load_tile<DP>(X1, dout + (size_t)b * a.Tq * os + hx * a.D, os, r0, rows, a.D);
+    }
+    auto span = [&](int r) { return r >= rows ? Span{0, 0} : KEYS ? queries_of(a, b, r) : keys_of(a, b, r); };
+    Span sp[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) sp[r] = span(r0 + 4 * ty + r);
+    const Span all = cta_span(tid < SA_M ? span(r0 + tid) : Span{0, 0}, tid < SA_M, s_red);
+    if constexpr (!KEYS) {
+        // delta of a row by four lanes; the products of a row are a sum over its channels, so it needs no other row
+        const int r = tid / 4, i = r0 + r;
+        float s = 0.f;
+        if (i < a.Tq) {
+            const T* ob = o + (((size_t)b * a.Tq + i) * a.H + hx) * a.D;
+            for (int d = (tid % 4) * 4; d < a.D; d += 16) s += dot4(ld4(ob + d), ld4(X1 + r * (DP + 4) + d));
+        }
+        s += __shfl_xor_sync(FULL, s, 1);
+        s += __shfl_xor_sync(FULL, s, 2);
+        if (tid % 4 == 0) {
+            const size_t at = ((size_t)b * a.H + hx) * a.Tq + i;
+            s_delta[r] = s;
+            s_lse[r] = i < a.Tq ? lse[at] : 0.f;
+            if (i < a.Tq) delta[at] = s;
+        }
+    }
+    float acc0[4][DP / 16], acc1[4][DP / 16];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) acc0[r][c] = acc1[r][c] = 0.f;
+    for (int g = 0; g < (KEYS ? group : 1); g++) {
+        const int h = KEYS ? hk * group + g : hx;
+        const Score sc(a, h);
+        for (int y0 = all.lo; y0 < all.hi; y0 += SA_N) {
+            __syncthreads();
+            if constexpr (KEYS) {
+                load_tile<DP>(Y0, q + b * a.qs[0] + h * a.qs[2], a.qs[1], y0, cols, a.D);
+                load_tile<DP>(Y1, dout + (size_t)b * a.Tq * os + h * a.D, os, y0, cols, a.D);
+                if (tid < SA_N) {
+                    const bool in = y0 + tid < a.Tq;
+                    const size_t at = ((size_t)b * a.H + h) * a.Tq + y0 + tid;
+                    s_lse[tid] = in ? lse[at] : 0.f;
+                    s_delta[tid] = in ? delta[at] : 0.f;
+                }
+            } else {
+                load_tile<DP>(Y0, kb, a.ks[1], y0, cols, a.D);
+                load_tile<DP>(Y1, vb, a.vs[1], y0, cols, a.D);
+            }
+            __syncthreads();
+            float s[4][4], dp[4][4];
+            dot_block<DP>(s, X0, Y0, ty, tx);
+            dot_block<DP>(dp, X1, Y1, ty, tx);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int x = r0 + 4 * ty + r;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int yl = tx + 16 * c, y = y0 + yl, ql = KEYS ? yl : 4 * ty + r;
+                    float p = 0.f, ds = 0.f;
+                    if (y >= sp[r].lo && y < sp[r].hi) {
+                        float f;
+                        const float z = score2(sc, s[r][c], KEYS ? abs(y + off - x) : abs(x + off - y), f);
+                        const bool single = s_lse[ql] == INFINITY;
+                        p = single ? 1.f : exp2f(z - s_lse[ql]);
+                        ds = single ? 0.f : p * (dp[r][c] - s_delta[ql]) * f;
+                    }
+                    if constexpr (KEYS) Ps[(4 * ty + r) * SA_LDP + yl] = p;
+                    Ds[(4 * ty + r) * SA_LDP + yl] = ds;
+                }
+            }
+            __syncthreads();
+            if constexpr (KEYS) product_block<DP>(acc0, Ps, Y1, ty, tx);
+            product_block<DP>(acc1, Ds, Y0, ty, tx);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int x = r0 + 4 * ty + r;
+        if (x >= rows) continue;
+        const size_t at = (((size_t)b * rows + x) * (KEYS ? a.KV : a.H) + hx) * a.D;
+#pragma unroll
+        for (int c = 0; c < DP / 64; c++) {
+            const int d = tx * 4 + 64 * c;
+            if (d >= a.D) continue;
+            if constexpr (KEYS) st4(d0 + at + d, make_float4(acc0[r][4 * c], acc0[r][4 * c + 1], acc0[r][4 * c + 2], acc0[r][4 * c + 3]));
+            st4(d1 + at + d, make_float4(acc1[r][4 * c] * a.scale, acc1[r][4 * c + 1] * a.scale, acc1[r][4 * c + 2] * a.scale, acc1[r][4 * c + 3] * a.scale));
+        }
+    }
+}
+
+template <int DP, typename T>
+static cudaError_t fwd_cores(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
+    const size_t sm = sizeof(float) * (2 * SA_M * (DP + 4) + SA_M * SA_LDP);
+    auto kern = attn_fwd_cores_kernel<DP, T>;
+    const cudaError_t e = opt_in_smem(kern, sm);
+    if (e != cudaSuccess) return e;
+    kern<<<dim3((a.Tq + SA_M - 1) / SA_M, a.H, a.B), SA_THREADS, sm, st>>>(a, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse);
+    return cudaGetLastError();
+}
+template <int DP, typename T>
+static cudaError_t bwd_cores(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                             float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    const size_t sm = sizeof(float) * (4 * SA_M * (DP + 4) + 2 * SA_M * SA_LDP);
+    auto rows_q = attn_bwd_cores_kernel<DP, false, T>;
+    auto rows_k = attn_bwd_cores_kernel<DP, true, T>;
+    cudaError_t e = opt_in_smem(rows_q, sm);
+    if (e == cudaSuccess) e = opt_in_smem(rows_k, sm);
+    if (e != cudaSuccess) return e;
+    rows_q<<<dim3((a.Tq + SA_M - 1) / SA_M, a.H, a.B), SA_THREADS, sm, st>>>(a, (const T*)q, (const T*)k, (const T*)v, (const T*)o, lse,
+                                                                            (const T*)dout, delta, nullptr, (T*)dq);
+    rows_k<<<dim3((a.Tk + SA_M - 1) / SA_M, a.KV, a.B), SA_THREADS, sm, st>>>(a, (const T*)q, (const T*)k, (const T*)v, (const T*)o, lse,
+                                                                             (const T*)dout, delta, (T*)dv, (T*)dk);
+    return cudaGetLastError();
+}
+
+cudaError_t run_attn_fwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
+    return a.D <= 64 ? fwd_cores<64, float>(a, q, k, v, o, lse, st) : fwd_cores<128, float>(a, q, k, v, o, lse, st);
+}
+cudaError_t run_attn_bwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                             float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    return a.D <= 64 ? bwd_cores<64, float>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st)
+                     : bwd_cores<128, float>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st);
+}
+cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
+    return a.D <= 64 ? fwd_cores<64, bf16>(a, q, k, v, o, lse, st) : fwd_cores<128, bf16>(a, q, k, v, o, lse, st);
+}
+cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                              float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    return a.D <= 64 ? bwd_cores<64, bf16>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st)
+                     : bwd_cores<128, bf16>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st);
+}
+
+}  // namespace slotscan

@@ -6,3 +6,4 @@ from ._lib import kernel_attrs  # noqa: F401
 from .epilogue import E4M3, fq, quantize_mem, writer_epilogue  # noqa: F401
 from .read import read_snapshots  # noqa: F401
 from .keyless import slot_scan_v  # noqa: F401
+from .tokens import document_bounds, norm_rope, norm_rope_append, rope_table, token_attention, token_attention_step  # noqa: F401

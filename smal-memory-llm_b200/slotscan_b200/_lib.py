@@ -57,6 +57,32 @@ class ReadParams(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("B", "T", "H", "NQ", "N", "DK", "DV", "G", "q_dtype", "snap_dtype")]
 
 
+_Strides = ctypes.c_int64 * 3
+
+
+class NormParams(ctypes.Structure):
+    """slotscan_norm_params of include/slotscan.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "T", "H", "KV", "D", "R", "table_len", "dtype")] + \
+               [("eps", ctypes.c_float), ("q_stride", _Strides), ("k_stride", _Strides)]
+
+
+class AppendParams(ctypes.Structure):
+    """slotscan_append_params of include/slotscan.h."""
+    _fields_ = [("base", NormParams), ("L", ctypes.c_int32), ("v_stride", _Strides), ("kc_stride", _Strides), ("vc_stride", _Strides)]
+
+
+class AttnParams(ctypes.Structure):
+    """slotscan_attn_params of include/slotscan.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "Tq", "Tk", "H", "KV", "D", "window", "dtype")] + \
+               [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_stride", _Strides), ("k_stride", _Strides), ("v_stride", _Strides)]
+
+
+class AttnStepParams(ctypes.Structure):
+    """slotscan_attn_step_params of include/slotscan.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "H", "KV", "D", "L", "window", "dtype")] + \
+               [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_stride", ctypes.c_int64 * 2), ("k_stride", _Strides), ("v_stride", _Strides)]
+
+
 class KernelAttr(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 48), ("regs", ctypes.c_int32), ("local_bytes", ctypes.c_int32),
                 ("static_smem", ctypes.c_int32), ("max_threads", ctypes.c_int32)]
@@ -126,6 +152,14 @@ def lib():
         L.slotscan_read_fwd.restype = ci
         L.slotscan_read_bwd.argtypes = [ctypes.POINTER(ReadParams)] + [vp] * 13
         L.slotscan_read_bwd.restype = ci
+        NP, TP, SP_ = ctypes.POINTER(NormParams), ctypes.POINTER(AttnParams), ctypes.POINTER(AttnStepParams)
+        for name, args, res in (
+                ("norm_rope_check", [NP], ci), ("norm_rope_fwd", [NP] + [vp] * 9, ci), ("norm_rope_bwd_scratch_bytes", [NP], sz),
+                ("norm_rope_bwd", [NP] + [vp] * 13 + [sz, vp], ci), ("norm_rope_append", [ctypes.POINTER(AppendParams)] + [vp] * 11, ci),
+                ("attn_check", [TP], ci), ("attn_fwd", [TP] + [vp] * 9, ci), ("attn_bwd", [TP] + [vp] * 14, ci),
+                ("attn_step_check", [SP_], ci), ("attn_step_scratch_bytes", [SP_], sz), ("attn_step", [SP_] + [vp] * 8 + [sz, vp], ci)):
+            f = getattr(L, "slotscan_" + name)
+            f.argtypes, f.restype = args, res
         L.slotscan_device_status.restype = ci
         L.slotscan_query_attrs.argtypes = [ctypes.POINTER(KernelAttr), ci]
         L.slotscan_profile_enable.argtypes = [ci]
