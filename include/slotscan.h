@@ -331,7 +331,9 @@ int slotscan_norm_rope_append(const slotscan_append_params* p, const void* q, co
  *   intervals, and padding stands in one of no length at its own place;  prefix (B) int32 or NULL
  *   o (B,Tq,H,D) contiguous;  lse (B,H,Tq) fp32 or NULL: what the backward needs of the softmax (base-2 logarithm of its sum;
  *   minus infinity for an empty row, plus infinity for a row of a single key, whose weight is 1 and whose scores have no gradient)
- * D a multiple of 8 up to 128.
+ *   rest  like o, for bf16 with lse (else NULL): what the rounding of o left, for the backward's <do, o>, whose error every
+ *   gradient of the row would carry
+ * D a multiple of 8 up to 128; scale > 0.
  * slotscan_attn_bwd: gradient dout (contiguous like o) to dq, dk, dv, contiguous.  delta: (B,H,Tq) fp32 scratch.  No atomics: the
  * results are equal from run to run. */
 typedef struct {
@@ -341,10 +343,10 @@ typedef struct {
 } slotscan_attn_params;
 int slotscan_attn_check(const slotscan_attn_params* p);
 int slotscan_attn_fwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
-                      const int32_t* docs, const int32_t* prefix, void* o, float* lse, void* stream);
+                      const int32_t* docs, const int32_t* prefix, void* o, void* rest, float* lse, void* stream);
 int slotscan_attn_bwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
-                      const int32_t* docs, const int32_t* prefix, const void* o, const float* lse, const void* dout, float* delta,
-                      void* dq, void* dk, void* dv, void* stream);
+                      const int32_t* docs, const int32_t* prefix, const void* o, const void* rest, const float* lse,
+                      const void* dout, float* delta, void* dq, void* dk, void* dv, void* stream);
 /* One query for each sequence over ring caches (B,L,KV,D) whose row j mod L holds position j: the query stands at pos[b] and sees
  * the positions from max(start[b], pos[b] - min(window, L) + 1, 0) to pos[b] (start NULL: 0).  q strides: of a sequence and a
  * head.  o (B,H,D) contiguous.  scratch: slotscan_attn_step_scratch_bytes, which depends on p alone. */

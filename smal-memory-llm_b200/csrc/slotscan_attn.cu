@@ -12,7 +12,7 @@ extern "C" int slotscan_attn_check(const slotscan_attn_params* p) {
     if (p->B < 0 || p->B > 65535 || p->Tq < 0 || p->Tk < p->Tq || p->Tk > (1 << 29) || p->H < 1 || p->H > 65535 || p->KV < 1 || p->H % p->KV ||
         p->D < 8 || p->D > 128 || p->D % 8)
         return SLOTSCAN_E_SHAPE;
-    if (p->window < 0 || !(p->cap >= 0.f) || !(p->cap < INFINITY)) return SLOTSCAN_E_MODE;
+    if (p->window < 0 || !(p->cap >= 0.f) || !(p->cap < INFINITY) || !(p->scale > 0.f) || !(p->scale < INFINITY)) return SLOTSCAN_E_MODE;
     const int e = p->dtype == SLOTSCAN_BF16 ? 2 : 4;
     for (int i = 0; i < 3; i++)
         if (p->q_stride[i] * e % 16 || p->k_stride[i] * e % 16 || p->v_stride[i] * e % 16) return SLOTSCAN_E_ALIGN;
@@ -30,20 +30,20 @@ static AttnArgs attn_args(const slotscan_attn_params& p, const float* slopes, co
 }
 
 extern "C" int slotscan_attn_fwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
-                                 const int32_t* docs, const int32_t* prefix, void* o, float* lse, void* stream) {
+                                 const int32_t* docs, const int32_t* prefix, void* o, void* rest, float* lse, void* stream) {
     const int rc = slotscan_attn_check(p);
     if (rc != SLOTSCAN_OK) return rc;
     if ((int64_t)p->B * p->Tq == 0) return SLOTSCAN_OK;
-    if (!q || !k || !v || !o) return SLOTSCAN_E_NULL;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || ((uintptr_t)docs & 7)) return SLOTSCAN_E_ALIGN;
+    if (!q || !k || !v || !o || (lse && p->dtype == SLOTSCAN_BF16 && !rest)) return SLOTSCAN_E_NULL;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest) || ((uintptr_t)docs & 7)) return SLOTSCAN_E_ALIGN;
     const AttnArgs a = attn_args(*p, slopes, docs, prefix);
-    return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_fwd_bf16(a, q, k, v, o, lse, (cudaStream_t)stream)
+    return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_fwd_bf16(a, q, k, v, o, rest, lse, (cudaStream_t)stream)
                                            : run_attn_fwd_f32(a, q, k, v, o, lse, (cudaStream_t)stream));
 }
 
 extern "C" int slotscan_attn_bwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
-                                 const int32_t* docs, const int32_t* prefix, const void* o, const float* lse, const void* dout, float* delta,
-                                 void* dq, void* dk, void* dv, void* stream) {
+                                 const int32_t* docs, const int32_t* prefix, const void* o, const void* rest, const float* lse, const void* dout,
+                                 float* delta, void* dq, void* dk, void* dv, void* stream) {
     const int rc = slotscan_attn_check(p);
     if (rc != SLOTSCAN_OK) return rc;
     if ((int64_t)p->B * p->Tk == 0) return SLOTSCAN_OK;
@@ -54,11 +54,11 @@ extern "C" int slotscan_attn_bwd(const slotscan_attn_params* p, const void* q, c
         if (e == cudaSuccess) e = cudaMemsetAsync(dv, 0, n, (cudaStream_t)stream);
         return (int)e;
     }
-    if (!q || !k || !v || !o || !lse || !dout || !delta || !dq || !dk || !dv) return SLOTSCAN_E_NULL;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+    if (!q || !k || !v || !o || (p->dtype == SLOTSCAN_BF16 && !rest) || !lse || !dout || !delta || !dq || !dk || !dv) return SLOTSCAN_E_NULL;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
         ((uintptr_t)docs & 7))
         return SLOTSCAN_E_ALIGN;
     const AttnArgs a = attn_args(*p, slopes, docs, prefix);
-    return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_bwd_bf16(a, q, k, v, o, lse, dout, delta, dq, dk, dv, (cudaStream_t)stream)
+    return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_bwd_bf16(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, (cudaStream_t)stream)
                                            : run_attn_bwd_f32(a, q, k, v, o, lse, dout, delta, dq, dk, dv, (cudaStream_t)stream));
 }

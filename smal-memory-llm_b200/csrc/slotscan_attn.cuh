@@ -43,6 +43,19 @@ __device__ __forceinline__ Span queries_of(const AttnArgs& a, int b, int j) {
     return {max(max(max(d.x, from), j - a.window + 1) - off, 0), min(min(d.y, a.Tk), j + a.window) - off};
 }
 
+// spans of the 128 rows of a tile
+struct TileSpan { int lo_min, lo_max, hi_min, hi_max; };
+__device__ __forceinline__ void tile_span_reset(TileSpan* s) { *s = {BIGI, 0, BIGI, 0}; }
+// by all 32 lanes; rows that do not exist do not count, and empty rows keep every tile masked
+__device__ __forceinline__ void tile_span_add(TileSpan* s, Span r, bool counts) {
+    const bool some = counts && r.hi > r.lo, none = counts && r.hi <= r.lo;
+    const int a = __reduce_min_sync(FULL, some ? r.lo : BIGI), b = __reduce_max_sync(FULL, none ? BIGI : some ? r.lo : 0);
+    const int c = __reduce_min_sync(FULL, none ? 0 : some ? r.hi : BIGI), d = __reduce_max_sync(FULL, some ? r.hi : 0);
+    if ((threadIdx.x & 31) == 0) {
+        atomicMin(&s->lo_min, a); atomicMax(&s->lo_max, b); atomicMin(&s->hi_min, c); atomicMax(&s->hi_max, d);
+    }
+}
+
 // a score as the base-2 exponent of its weight, before the softmax's shift.  Of the cap, t = tanh(scale <q, k> / cap), whose
 // derivative is 1 - t^2.
 struct Score {
@@ -59,8 +72,8 @@ struct Score {
 cudaError_t run_attn_fwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st);
 cudaError_t run_attn_bwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
                              float* delta, void* dq, void* dk, void* dv, cudaStream_t st);
-cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st);
-cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
-                              float* delta, void* dq, void* dk, void* dv, cudaStream_t st);
+cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st);
+cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const void* rest,
+                              const float* lse, const void* dout, float* delta, void* dq, void* dk, void* dv, cudaStream_t st);
 
 }  // namespace slotscan

@@ -1,0 +1,317 @@
+// Attention over tokens on the tensor cores, bf16: backward.
+//
+// The walk of the forward twice: with rows of queries (dq, and delta = <do, o>), then with rows of keys over the queries of all
+// heads that share the key head (dk, dv).  Five products would do for both, with sums of dq by atomics; two walks take seven, have
+// no atomics, and give the same bits from run to run.
+//   rows X0, X1 / stream Y0, Y1:   queries: q, do / k, v      keys: k, v / q, do
+//   s = X0 Y0^T, dp = X1 Y1^T, p = exp2(s - lse), ds = p (dp - delta) (1 - tanh^2),   out1 += ds Y0,  keys also out0 += p Y1
+// A CTA holds 128 rows; the stream comes 64 at a time.  Scores and dp have two buffers in tensor memory, one for each group of 128
+// threads, which form the weights of every other step (a thread has a row) and write p and ds, as bf16, over them, where the
+// products read them as their first operand.  So the products of a step run while the other group forms the next one's weights.
+#include "slotscan_attn.cuh"
+#include "slotscan_launch.h"
+#include "slotscan_tensor.cuh"
+
+namespace slotscan {
+
+static __device__ int g_attn_bwd_status = 0;             // a bounded wait gave up (slotscan_device_status)
+
+constexpr int AB_N = 64;                                 // rows of a step of the stream
+
+template <int DP>
+struct BwdShape {
+    static constexpr int STAGES = 4;
+    static constexpr int SUBS = DP / 64;
+    static constexpr int XTILE = 128 * DP * 2, YTILE = AB_N * DP * 2;
+    static constexpr int THREADS = 384;
+    static constexpr int SMEM = 2 * XTILE + STAGES * 2 * YTILE + 1024;
+};
+struct BwdMaps { CUtensorMap x0, x1, y0, y1, d0, d1; };
+
+template <int DP, bool KEYS, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(384, 1)
+attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const bf16* o, const bf16* rest, const bf16* dout, const float* lse,
+                       float* delta, int tiles, int tile_major) {
+    typedef BwdShape<DP> Sh;
+    extern __shared__ char smem_raw[];
+    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    char *X0 = smem, *X1 = smem + Sh::XTILE, *Ys = smem + 2 * Sh::XTILE;
+    __shared__ uint64_t x_full, done, s_full[2], p_full[2], full[Sh::STAGES], empty[Sh::STAGES];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_fail;
+    __shared__ TileSpan s_span;
+    __shared__ __align__(16) float s_stat[2][2][2][AB_N];              // group, buffer, lse / delta
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, group = a.H / a.KV;
+    const int heads = (KEYS ? a.KV : a.H) * a.B, rows = KEYS ? a.Tk : a.Tq, off = a.Tk - a.Tq;
+    const int at_tile = (int)(tile_major ? blockIdx.x / heads : blockIdx.x % tiles), tile = KEYS ? at_tile : tiles - 1 - at_tile;   // long ones first
+    const int hb = (int)(tile_major ? blockIdx.x % heads : blockIdx.x / tiles);
+    const int hx = hb % (heads / a.B), b = hb / (heads / a.B), hk = KEYS ? hx : hx / group, x0 = tile * 128;
+    if (tid == 0) {
+        mbar_init(&x_full, 1); mbar_init(&done, 1);
+        for (int w = 0; w < 2; w++) { mbar_init(&s_full[w], 1); mbar_init(&p_full[w], 4); }
+        for (int s = 0; s < Sh::STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_fence_init();
+        tile_span_reset(&s_span);
+        s_fail = 0;
+    }
+    if (warp == 8) tmem_alloc(&s_tmem, 512);
+    __syncthreads();
+    const int r = tid % 128, row = x0 + r;               // of the threads that form weights: two groups, the same rows
+    Span sp = {0, 0};
+    if (warp < 8) {
+        if (row < rows) sp = KEYS ? queries_of(a, b, row) : keys_of(a, b, row);
+        if (warp < 4) tile_span_add(&s_span, sp, row < rows);
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = s_tmem;
+    const TileSpan ts = s_span;
+    const int y_first = ts.hi_max > 0 ? ts.lo_min / AB_N : 0, y_tiles = ts.hi_max > 0 ? (ts.hi_max + AB_N - 1) / AB_N - y_first : 0;
+    const int steps = y_tiles * (KEYS ? group : 1);
+    if (warp < 8) {                                      // ---- weights ----
+        const int w = warp / 4;
+        const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
+        const uint32_t S = tmem + w * 128 + lane_at, P = S + 64;
+        const float at = (float)(KEYS ? row - off : row + off);                    // this row's place among the stream's
+        bool ok = true;
+        float my_lse = 0.f, my_delta = 0.f;
+        if constexpr (!KEYS) {
+            // delta of the row, half of its channels to each group
+            if (row < rows) my_lse = lse[((size_t)b * a.H + hx) * a.Tq + row];
+            float s = 0.f;
+            if (row < rows) {
+                const size_t at_o = (((size_t)b * a.Tq + row) * a.H + hx) * a.D;
+                for (int d = w * (DP / 2); d < (w + 1) * (DP / 2) && d < a.D; d += 8) {
+                    float x[8], y[8], z[8];
+                    ld8(x, o + at_o + d); ld8(y, rest + at_o + d); ld8(z, dout + at_o + d);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s = fmaf(x[i] + y[i], z[i], s);
+                }
+            }
+            float* ex = &s_stat[0][0][0][0];             // used here only, before the first step
+            ex[w * 128 + r] = s;
+            sync_group(3, 256);
+            my_delta = ex[r] + ex[128 + r];
+            if (w == 0 && row < rows) delta[((size_t)b * a.H + hx) * a.Tq + row] = my_delta;
+        }
+        auto stat_at = [&](int s, int c) {               // lse or delta of a query of step s
+            const int h = hk * group + s / y_tiles, i = (y_first + s % y_tiles) * AB_N + c % AB_N;
+            return i < a.Tq ? (c < AB_N ? lse : delta)[((size_t)b * a.H + h) * a.Tq + i] : 0.f;
+        };
+        float next = KEYS && w < steps ? stat_at(w, r) : 0.f;
+        for (int s = w, turn = 0; s < steps; s += 2, turn++) {
+            const int y0 = (y_first + (KEYS ? s % y_tiles : s)) * AB_N;
+            const Score sc(a, KEYS ? hk * group + s / y_tiles : hx);
+            const bool masked = y0 < ts.lo_max || y0 + AB_N > ts.hi_min;
+            if constexpr (KEYS) {
+                s_stat[w][turn & 1][r / AB_N][r % AB_N] = next;
+                if (s + 2 < steps) next = stat_at(s + 2, r);
+                sync_group(1 + w, 128);
+            }
+            if (!(ok = __all_sync(FULL, wait_soon(&s_full[w], turn & 1)))) break;
+            tmem_fence_after();
+#pragma unroll
+            for (int c = 0; c < AB_N / 32; c++) {
+                uint32_t xs[32], xd[32], wp[16], wd[16];
+                tmem_ld(S + c * 32, xs);
+                tmem_ld(P + c * 32, xd);
+                tmem_ld_wait(xs);
+                tmem_ld_wait(xd);
+                const int lo = sp.lo - y0 - c * 32, hi = sp.hi - y0 - c * 32;
+                const float ahead = at - (float)(y0 + c * 32);
+                const float4* ls = reinterpret_cast<const float4*>(&s_stat[w][turn & 1][0][c * 32]);
+                const float4* de = reinterpret_cast<const float4*>(&s_stat[w][turn & 1][1][c * 32]);
+#pragma unroll
+                for (int i4 = 0; i4 < 8; i4++) {
+                    float l4[4], d4[4], p[4], ds[4];
+                    if constexpr (KEYS) {
+                        const float4 lv = ls[i4], dv = de[i4];
+                        l4[0] = lv.x; l4[1] = lv.y; l4[2] = lv.z; l4[3] = lv.w;
+                        d4[0] = dv.x; d4[1] = dv.y; d4[2] = dv.z; d4[3] = dv.w;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int i = i4 * 4 + e;
+                        const float x = __uint_as_float(xs[i]), L = KEYS ? l4[e] : my_lse, dl = KEYS ? d4[e] : my_delta;
+                        float z, f = 1.f;
+                        if constexpr (CAP) {             // tanh x = 1 - 2 r, 1 - tanh^2 = 4 r (1 - r),  r = 1 / (e^2x + 1)
+                            const float rr = rcp_fast(exp2_fast(x * (2.f * LOG2E * sc.cap_in)) + 1.f);
+                            z = fmaf(-2.f * sc.cap_out, rr, sc.cap_out) - L;
+                            f = 4.f * fmaf(-rr, rr, rr);
+                        } else z = fmaf(x, sc.lin, -L);
+                        if constexpr (BIAS) z = fmaf(-sc.slope, fabsf(ahead - (float)i), z);
+                        p[e] = exp2_fast(z);
+                        ds[e] = p[e] * (__uint_as_float(xd[i]) - dl);
+                        if constexpr (CAP) ds[e] *= f;
+                        if (masked) {
+                            const bool in = i >= lo && i < hi, alone = L == INFINITY;
+                            p[e] = in ? (alone ? 1.f : p[e]) : 0.f;
+                            ds[e] = in && !alone ? ds[e] : 0.f;
+                        }
+                    }
+                    wp[i4 * 2] = pack_bf16(p[0], p[1]); wp[i4 * 2 + 1] = pack_bf16(p[2], p[3]);
+                    wd[i4 * 2] = pack_bf16(ds[0], ds[1]); wd[i4 * 2 + 1] = pack_bf16(ds[2], ds[3]);
+                }
+                if constexpr (KEYS) tmem_st(S + c * 16, wp);
+                tmem_st(P + c * 16, wd);
+            }
+            tmem_st_wait();
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(&p_full[w]);
+        }
+        if (ok && steps > 0) ok = wait_soon(&done, 0);
+        tmem_fence_after();
+        if (!ok) s_fail = 1;
+        // results through the tiles of the rows, whose products are done: of keys, dv by one group and dk by the other; of queries half the
+        // columns each, where there are two sub-tiles
+        const bool mine = KEYS || DP == 128 || w == 0;
+        const int c0 = KEYS || DP == 64 ? 0 : w, c1 = KEYS || DP == 64 ? Sh::SUBS : w + 1;
+        const uint32_t from = tmem + 256 + lane_at + (KEYS && w == 0 ? DP : 0);
+        const float mul = KEYS && w == 0 ? 1.f : a.scale;
+        char* out = KEYS && w == 1 ? X1 : X0;
+        if (mine) {
+            for (int c = c0 * 2; c < c1 * 2; c++) {
+                uint32_t x[32];
+                if (steps > 0) { tmem_ld(from + c * 32, x); tmem_ld_wait(x); }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        y[e] = steps > 0 ? pack_bf16(__uint_as_float(x[i + 2 * e]) * mul, __uint_as_float(x[i + 2 * e + 1]) * mul) : 0u;
+                    *reinterpret_cast<uint4*>(out + (c / 2) * 128 * 128 + swizzled(r, (c % 2) * 4 + i / 8)) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            sync_group(1 + w, 128);
+            if (r == 0) {
+                for (int c = c0; c < c1; c++) tile_s2g(KEYS && w == 0 ? &maps.d0 : &maps.d1, c * 64, x0, hx, b, out + c * 128 * 128);
+                bulk_commit();
+                bulk_wait_read<0>();
+            }
+        }
+    } else if (warp == 9) {                              // ---- copies ----
+        if (lane == 0 && steps > 0) {
+            bool ok = true;
+            mbar_arrive_expect_tx(&x_full, 2 * Sh::XTILE);
+            for (int c = 0; c < Sh::SUBS; c++) {
+                tile_g2s(X0 + c * 128 * 128, &maps.x0, c * 64, x0, hx, b, &x_full);
+                tile_g2s(X1 + c * 128 * 128, &maps.x1, c * 64, x0, hx, b, &x_full);
+            }
+            for (int s = 0; s < steps; s++) {
+                const int st = s % Sh::STAGES, turn = s / Sh::STAGES;
+                if (turn > 0 && !(ok = wait_soon(&empty[st], (turn - 1) & 1))) break;
+                const int head = KEYS ? hk * group + s / y_tiles : hk, y0 = (y_first + (KEYS ? s % y_tiles : s)) * AB_N;
+                char* y = Ys + st * 2 * Sh::YTILE;
+                mbar_arrive_expect_tx(&full[st], 2 * Sh::YTILE);
+                for (int c = 0; c < Sh::SUBS; c++) {
+                    tile_g2s(y + c * AB_N * 128, &maps.y0, c * 64, y0, head, b, &full[st]);
+                    tile_g2s(y + Sh::YTILE + c * AB_N * 128, &maps.y1, c * 64, y0, head, b, &full[st]);
+                }
+            }
+            if (!ok) s_fail = 1;
+        }
+    } else if (warp == 8) {                              // ---- products ----
+        if (lane == 0 && steps > 0) {
+            bool ok = wait_soon(&x_full, 0);
+            const uint64_t x0d = tile_desc(smem_u32(X0), 16), x1d = tile_desc(smem_u32(X1), 16);
+            auto scores = [&](int s) {                   // s and dp of a step
+                const int w = s & 1, st = s % Sh::STAGES;
+                if (!wait_soon(&full[st], (s / Sh::STAGES) & 1)) return false;
+                const uint64_t yd = tile_desc(smem_u32(Ys + st * 2 * Sh::YTILE), 16);
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++)
+                    mma_ss(tmem + w * 128, x0d + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, yd + ((k / 4) * AB_N * 128 + (k % 4) * 32) / 16,
+                           mma_shape(AB_N, false), k > 0);
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++)
+                    mma_ss(tmem + w * 128 + 64, x1d + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16,
+                           yd + (Sh::YTILE + (k / 4) * AB_N * 128 + (k % 4) * 32) / 16, mma_shape(AB_N, false), k > 0);
+                mma_commit(&s_full[w]);
+                return true;
+            };
+            ok = ok && scores(0);
+            if (steps > 1) ok = ok && scores(1);
+            for (int s = 0; s < steps && ok; s++) {
+                const int w = s & 1, st = s % Sh::STAGES;
+                if (!(ok = wait_soon(&p_full[w], (s / 2) & 1))) break;
+                tmem_fence_after();
+                const uint64_t yd = tile_desc(smem_u32(Ys + st * 2 * Sh::YTILE), AB_N * 128);
+                if constexpr (KEYS) {
+#pragma unroll
+                    for (int k = 0; k < AB_N / 16; k++)
+                        mma_ts(tmem + 256 + DP, tmem + w * 128 + k * 8, yd + (Sh::YTILE + k * 2048) / 16, mma_shape(DP, true), s > 0 || k > 0);
+                }
+#pragma unroll
+                for (int k = 0; k < AB_N / 16; k++)
+                    mma_ts(tmem + 256, tmem + w * 128 + 64 + k * 8, yd + k * 2048 / 16, mma_shape(DP, true), s > 0 || k > 0);
+                mma_commit(&empty[st]);
+                if (s + 2 < steps) ok = scores(s + 2);
+            }
+            mma_commit(&done);
+            if (!ok) s_fail = 1;
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (s_fail != 0) {                                   // report, and give copies and products in flight time to land
+        if (tid == 0) atomicExch(&g_attn_bwd_status, 1);
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    }
+    if (warp == 8) { tmem_fence_after(); tmem_free(tmem, 512); }
+}
+
+template <int DP, bool CAP, bool BIAS>
+static cudaError_t bwd_tensor(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const void* rest, const float* lse,
+                              const void* dout, float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    typedef BwdShape<DP> Sh;
+    const long long os[3] = {(long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D}, gs[3] = {(long long)a.Tk * a.KV * a.D, (long long)a.KV * a.D, a.D};
+    BwdMaps mq, mk;
+    if (!tile_map(&mq.x0, q, a.B, a.Tq, a.H, a.D, a.qs, 128) || !tile_map(&mq.x1, dout, a.B, a.Tq, a.H, a.D, os, 128) ||
+        !tile_map(&mq.y0, k, a.B, a.Tk, a.KV, a.D, a.ks, AB_N) || !tile_map(&mq.y1, v, a.B, a.Tk, a.KV, a.D, a.vs, AB_N) ||
+        !tile_map(&mq.d1, dq, a.B, a.Tq, a.H, a.D, os, 128))
+        return cudaErrorInvalidValue;
+    mq.d0 = mq.d1;
+    if (!tile_map(&mk.x0, k, a.B, a.Tk, a.KV, a.D, a.ks, 128) || !tile_map(&mk.x1, v, a.B, a.Tk, a.KV, a.D, a.vs, 128) ||
+        !tile_map(&mk.y0, q, a.B, a.Tq, a.H, a.D, a.qs, AB_N) || !tile_map(&mk.y1, dout, a.B, a.Tq, a.H, a.D, os, AB_N) ||
+        !tile_map(&mk.d0, dv, a.B, a.Tk, a.KV, a.D, gs, 128) || !tile_map(&mk.d1, dk, a.B, a.Tk, a.KV, a.D, gs, 128))
+        return cudaErrorInvalidValue;
+    auto rows_q = attn_bwd_tensor_kernel<DP, false, CAP, BIAS>;
+    auto rows_k = attn_bwd_tensor_kernel<DP, true, CAP, BIAS>;
+    cudaError_t e = opt_in_smem(rows_q, Sh::SMEM);
+    if (e == cudaSuccess) e = opt_in_smem(rows_k, Sh::SMEM);
+    if (e != cudaSuccess) return e;
+    const int tq = (a.Tq + 127) / 128, tk = (a.Tk + 127) / 128;
+    const long long cq = (long long)tq * a.H * a.B, ck = (long long)tk * a.KV * a.B;
+    if (cq > 0x7fffffffll || ck > 0x7fffffffll) return cudaErrorInvalidValue;
+    rows_q<<<(unsigned)cq, Sh::THREADS, Sh::SMEM, st>>>(a, mq, (const bf16*)o, (const bf16*)rest, (const bf16*)dout, lse, delta, tq, cq < 148 * 8);
+    rows_k<<<(unsigned)ck, Sh::THREADS, Sh::SMEM, st>>>(a, mk, nullptr, nullptr, nullptr, lse, delta, tk, ck < 148 * 8);
+    return cudaGetLastError();
+}
+template <int DP>
+static cudaError_t bwd_tensor_score(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const void* rest, const float* lse,
+                                    const void* dout, float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    if (a.cap > 0.f)
+        return a.slopes != nullptr ? bwd_tensor<DP, true, true>(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, st)
+                                   : bwd_tensor<DP, true, false>(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, st);
+    return a.slopes != nullptr ? bwd_tensor<DP, false, true>(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, st)
+                               : bwd_tensor<DP, false, false>(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, st);
+}
+
+cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const void* rest, const float* lse,
+                              const void* dout, float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    return a.D <= 64 ? bwd_tensor_score<64>(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, st)
+                     : bwd_tensor_score<128>(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, st);
+}
+
+int attn_bwd_mma_status() {
+    int v = 0;
+    const int z = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attn_bwd_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) cudaMemcpyToSymbol(g_attn_bwd_status, &z, sizeof(int));
+    return v;
+}
+
+}  // namespace slotscan

@@ -321,13 +321,4 @@ cudaError_t run_attn_bwd_f32(const AttnArgs& a, const void* q, const void* k, co
     return a.D <= 64 ? bwd_cores<64, float>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st)
                      : bwd_cores<128, float>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st);
 }
-cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
-    return a.D <= 64 ? fwd_cores<64, bf16>(a, q, k, v, o, lse, st) : fwd_cores<128, bf16>(a, q, k, v, o, lse, st);
-}
-cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
-                              float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
-    return a.D <= 64 ? bwd_cores<64, bf16>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st)
-                     : bwd_cores<128, bf16>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st);
-}
-
 }  // namespace slotscan

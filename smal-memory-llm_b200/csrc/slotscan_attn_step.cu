@@ -202,7 +202,7 @@ extern "C" int slotscan_attn_step_check(const slotscan_attn_step_params* p) {
     if (p->B < 0 || p->B > 65535 || p->H < 1 || p->KV < 1 || p->H > 65535 || p->H % p->KV || p->D < 8 || p->D > 128 || p->D % 8 || p->L < 1 ||
         p->L > (1 << 29))
         return SLOTSCAN_E_SHAPE;
-    if (p->window < 0 || !(p->cap >= 0.f) || !(p->cap < INFINITY)) return SLOTSCAN_E_MODE;
+    if (p->window < 0 || !(p->cap >= 0.f) || !(p->cap < INFINITY) || !(p->scale > 0.f) || !(p->scale < INFINITY)) return SLOTSCAN_E_MODE;
     const int e = p->dtype == SLOTSCAN_BF16 ? 2 : 4;
     for (int i = 0; i < 3; i++)
         if ((i < 2 && p->q_stride[i] * e % 16) || p->k_stride[i] * e % 16 || p->v_stride[i] * e % 16) return SLOTSCAN_E_ALIGN;

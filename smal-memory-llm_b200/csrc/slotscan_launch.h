@@ -82,6 +82,8 @@ bool read_bwd_mma_try(const slotscan_read_params& p, const void* qr, const float
                       const float* kinv, const uint8_t* valid, const void* drd, void* dqr, float* dsharp, void* dkbuf,
                       void* dvbuf, float* dkinv, cudaStream_t st, cudaError_t* err);
 int read_mma_status();
+int attn_mma_status();
+int attn_bwd_mma_status();
 int gather_status_f32();
 int gather_status_bf16();
 int rows_bwd_status_f32();

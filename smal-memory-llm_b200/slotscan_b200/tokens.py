@@ -25,7 +25,7 @@ def _laid(t):
     for x in (t, None):
         x = t.clone(memory_format=torch.contiguous_format) if x is None else x
         s = tuple(0 if n == 1 else st for n, st in zip(x.shape[:-1], x.stride()))
-        if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not any(st * size % 16 for st in s):
+        if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not any(st * size % 16 or (st == 0 and n > 1) for st, n in zip(s, x.shape)):
             return x, s
     raise ValueError("slotscan_b200: %s channels of %s do not fill 16 bytes" % (t.shape[-1], t.dtype))
 
@@ -263,8 +263,10 @@ def _attn_call(q, k, v, window, cap, scale):
 
 
 def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optional[torch.Tensor], docs: Optional[torch.Tensor],
-              prefix: Optional[torch.Tensor], window: int, cap: float, scale: float, want_lse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """o and, when asked for, lse (B,H,Tq); it has no elements otherwise."""
+              prefix: Optional[torch.Tensor], window: int, cap: float, scale: float, for_bwd: bool
+              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """o and what the backward needs besides (without elements unless asked for): lse (B,H,Tq), and for bfloat16 what the rounding
+    of o left."""
     _require_cuda(q, k, v, slopes, docs, prefix)
     _same("token_attention", q, k, v)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
@@ -283,35 +285,37 @@ def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optiona
     q, k, v, p, ref = _attn_call(q, k, v, window, cap, scale)
     slopes, docs, prefix = _f32(slopes), _i32(docs), _i32(prefix)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Tq) if want_lse else (0,), dtype=torch.float32, device=q.device)
+    lse = torch.empty((B, H, Tq) if for_bwd else (0,), dtype=torch.float32, device=q.device)
+    rest = torch.empty(q.shape if for_bwd and q.dtype == torch.bfloat16 else (0,), dtype=q.dtype, device=q.device)
     with _Here(q.device):
-        rc = _lib.lib().slotscan_attn_fwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(lse),
-                                          _stream(q.device))
+        rc = _lib.lib().slotscan_attn_fwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest),
+                                          _ptr(lse), _stream(q.device))
     _lib.check(rc, "slotscan_attn_fwd")
-    return o, lse
+    return o, lse, rest
 
 
 _attn_op = torch.library.custom_op("slotscan::attn_fwd", mutates_args=())(_attn_fwd)
 
 
 @_attn_op.register_fake
-def _(q, k, v, slopes, docs, prefix, window, cap, scale, want_lse):
-    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if want_lse else (0,), dtype=torch.float32)
+def _(q, k, v, slopes, docs, prefix, window, cap, scale, for_bwd):
+    return (q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if for_bwd else (0,), dtype=torch.float32),
+            q.new_empty(q.shape if for_bwd and q.dtype == torch.bfloat16 else (0,)))
 
 
 def _attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optional[torch.Tensor], docs: Optional[torch.Tensor],
-              prefix: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor, do: torch.Tensor, window: int, cap: float, scale: float
-              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    _require_cuda(q, k, v, slopes, docs, prefix, o, lse, do)
+              prefix: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor, rest: torch.Tensor, do: torch.Tensor, window: int, cap: float,
+              scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _require_cuda(q, k, v, slopes, docs, prefix, o, lse, rest, do)
     q, k, v, p, ref = _attn_call(q, k, v, window, cap, scale)
     slopes, docs, prefix = _f32(slopes), _i32(docs), _i32(prefix)
-    do, o, lse = _whole(do, q.dtype), _whole(o, q.dtype), lse.contiguous()
+    do, o, rest, lse = _whole(do, q.dtype), _whole(o, q.dtype), _whole(rest, q.dtype), lse.contiguous()
     dev = q.device
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
     delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
     with _Here(dev):
-        rc = _lib.lib().slotscan_attn_bwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(lse),
-                                          _ptr(do), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv), _stream(dev))
+        rc = _lib.lib().slotscan_attn_bwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest),
+                                          _ptr(lse), _ptr(do), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv), _stream(dev))
     _lib.check(rc, "slotscan_attn_bwd")
     return dq, dk, dv
 
@@ -320,17 +324,17 @@ _attn_bwd_op = torch.library.custom_op("slotscan::attn_bwd", mutates_args=())(_a
 
 
 @_attn_bwd_op.register_fake
-def _(q, k, v, slopes, docs, prefix, o, lse, do, window, cap, scale):
+def _(q, k, v, slopes, docs, prefix, o, lse, rest, do, window, cap, scale):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
 def _attn_setup(ctx, inputs, output):
     *ts, ctx.window, ctx.cap, ctx.scale, _ = inputs
     ctx.save_for_backward(*ts, *output)
-    ctx.mark_non_differentiable(output[1])
+    ctx.mark_non_differentiable(*output[1:])
 
 
-def _attn_backward(ctx, do, _, bwd=None):
+def _attn_backward(ctx, do, _, __, bwd=None):
     dq, dk, dv = (bwd or _attn_bwd_op)(*ctx.saved_tensors, do, ctx.window, ctx.cap, ctx.scale)
     return dq, dk, dv, None, None, None, None, None, None, None
 
@@ -349,8 +353,8 @@ class _Attn(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, do, _):
-        return _attn_backward(ctx, do, None, bwd=_attn_bwd if plain_grads(do) else None)
+    def backward(ctx, do, _, __):
+        return _attn_backward(ctx, do, None, None, bwd=_attn_bwd if plain_grads(do) else None)
 
 
 def _numbers(what, D, window, cap, scale, slopes):
