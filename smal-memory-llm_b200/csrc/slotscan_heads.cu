@@ -21,7 +21,7 @@ namespace slotscan {
 
 typedef __nv_bfloat16 bf16;
 constexpr int NR_THREADS = 256;
-constexpr int NR_MAX_CTAS = 148 * 4;                     // of the backward, which sums the weights' gradients per CTA
+constexpr int NR_MAX_CTAS = 148 * 2;                     // of the backward, which sums the weights' gradients per CTA: those of one wave
 
 struct NormArgs {
     int T, H, KV, D, R, table_len, slices, per_slice;    // per_slice heads (queries, keys, then values) to a group
@@ -36,6 +36,19 @@ struct AppendArgs {                                      // L 0: no caches
     int L;
     long long vs[3], kcs[3], vcs[3];
 };
+
+// 8 channels as they lie in memory: what a row in flight costs a thread in registers
+template <typename T>
+struct Raw8 { uint4 v[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ Raw8<T> raw8(const T* p, bool in) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.v[i] = in ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void widen(float (&x)[8], const Raw8<T>& r) { ld8(x, reinterpret_cast<const T*>(&r)); }
 
 // cosines and sines of this lane's 8 channels; NaN where the position lies outside the table
 __device__ __forceinline__ void load_turn(const NormArgs& a, long long at, int half, int c, float (&cs)[8], float (&sn)[8]) {
@@ -68,7 +81,7 @@ __device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[8], const 
 
 // T: bf16 or float.  CACHE: the keys and the values go into the caches.
 template <typename T, int LPG, bool CACHE>
-__global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
+__global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
     const int c = threadIdx.x % LPG;
     const long long unit = (long long)blockIdx.x * (NR_THREADS / LPG) + threadIdx.x / LPG;
@@ -78,46 +91,46 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(NormArgs a, Appen
     const long long b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
     const long long at = CACHE ? (long long)a.pos[b] + t : a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t;
     const int half = a.R / 16;
-    float cs[8], sn[8], w[2][8];
+    float cs[8], sn[8], w[8];
     if (half) load_turn(a, at, half, c, cs, sn);
-#pragma unroll
-    for (int i = 0; i < 8; i++) w[0][i] = w[1][i] = 1.f;
-    if (live && a.qw != nullptr) ld8(w[0], a.qw + c * 8);
-    if (live && a.kw != nullptr) ld8(w[1], a.kw + c * 8);
     const long long row = CACHE && at >= 0 ? at % ap.L : 0;
     const float inv_d = 1.f / a.D;
-    constexpr int U = 4;                                 // rows in flight to a group
+    constexpr int U = sizeof(T) == 2 ? 6 : 4;            // rows in flight to a group
     for (int u0 = 0; u0 < a.per_slice; u0 += U) {
-        float x[U][8];
+        Raw8<T> in[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int h = h0 + u0 + u;
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[u][i] = 0.f;
-            if (live && u0 + u < a.per_slice && h < all) {
-                if (h < a.H) ld8(x[u], q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + c * 8);
-                else if (!CACHE || h < a.H + a.KV) ld8(x[u], k + b * a.ks[0] + t * a.ks[1] + (h - a.H) * a.ks[2] + c * 8);
-                else ld8(x[u], v + b * ap.vs[0] + t * ap.vs[1] + (h - a.H - a.KV) * ap.vs[2] + c * 8);
-            }
+            const T* from = h < a.H ? q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2]
+                            : !CACHE || h < a.H + a.KV ? k + b * a.ks[0] + t * a.ks[1] + (h - a.H) * a.ks[2]
+                                                       : v + b * ap.vs[0] + t * ap.vs[1] + (h - a.H - a.KV) * ap.vs[2];
+            in[u] = raw8(from + c * 8, live && u0 + u < a.per_slice && h < all);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int h = h0 + u0 + u;
             if (u0 + u >= a.per_slice) break;            // the same in every lane of the CTA
             const bool is_v = CACHE && h >= a.H + a.KV, is_q = h < a.H;
-            float ss = 0.f, y[8];
+            if (h == a.H || u0 + u == 0) {               // the queries' weights, then the keys'
+                const float* from = is_q ? a.qw : a.kw;
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(x[u][i], x[u][i], ss);
+                for (int i = 0; i < 8; i++) w[i] = 1.f;
+                if (live && from != nullptr) ld8(w, from + c * 8);
+            }
+            float ss = 0.f, x[8], y[8];
+            widen(x, in[u]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
             const float r = rsqrtf(fmaf(group_sum<LPG>(ss), inv_d, a.eps));
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = x[u][i] * r * (is_q ? w[0][i] : w[1][i]);
+            for (int i = 0; i < 8; i++) y[i] = x[i] * r * w[i];
             if (half) turn<1>(y, cs, sn, half, c, LPG);
             if (!live || h >= all) continue;
             if (is_q) st8(qo + (tok * a.H + h) * a.D + c * 8, y);
             else if constexpr (!CACHE) st8(ko + (tok * a.KV + (h - a.H)) * a.D + c * 8, y);
             else if (at >= 0) {
                 if (!is_v) st8(kc + b * ap.kcs[0] + row * ap.kcs[1] + (h - a.H) * ap.kcs[2] + c * 8, y);
-                else st8(vc + b * ap.vcs[0] + row * ap.vcs[1] + (h - a.H - a.KV) * ap.vcs[2] + c * 8, x[u]);
+                else st8(vc + b * ap.vcs[0] + row * ap.vcs[1] + (h - a.H - a.KV) * ap.vcs[2] + c * 8, x);
             }
         }
     }
@@ -125,18 +138,16 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(NormArgs a, Appen
 
 // grid-stride over (token, slice of heads); part: (CTAs, 2, D) sums of the weights' gradients, or NULL
 template <typename T, int LPG>
-__global__ void __launch_bounds__(NR_THREADS) norm_rope_bwd_kernel(NormArgs a, const T* q, const T* k, const T* gq, const T* gk, T* dq, T* dk,
+__global__ void __launch_bounds__(NR_THREADS, 2) norm_rope_bwd_kernel(NormArgs a, const T* q, const T* k, const T* gq, const T* gk, T* dq, T* dk,
                                                                    float* part) {
     constexpr int GROUPS = NR_THREADS / LPG;
     __shared__ float s_part[GROUPS][LPG * 8];
     const int c = threadIdx.x % LPG, grp = threadIdx.x / LPG;
     const int half = a.R / 16;
     const float inv_d = 1.f / a.D;
-    float w[2][8], acc[2][8];
+    float w[8], acc[2][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) { w[0][i] = w[1][i] = 1.f; acc[0][i] = acc[1][i] = 0.f; }
-    if (c * 8 < a.D && a.qw != nullptr) ld8(w[0], a.qw + c * 8);
-    if (c * 8 < a.D && a.kw != nullptr) ld8(w[1], a.kw + c * 8);
+    for (int i = 0; i < 8; i++) acc[0][i] = acc[1][i] = 0.f;
     const long long units = a.tokens * a.slices;
     for (long long u0 = (long long)blockIdx.x * GROUPS; u0 < units; u0 += (long long)gridDim.x * GROUPS) {
         const long long unit = u0 + grp, tok = unit / a.slices;
@@ -145,36 +156,35 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_bwd_kernel(NormArgs a, c
         const long long b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
         float cs[8], sn[8];
         if (half) load_turn(a, a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t, half, c, cs, sn);
-        constexpr int U = 2;
+        constexpr int U = sizeof(T) == 2 ? 3 : 2;
         for (int v0 = 0; v0 < a.per_slice; v0 += U) {
-            float x[U][8], g[U][8];
+            Raw8<T> in[U], up[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int h = h0 + v0 + u;
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[u][i] = g[u][i] = 0.f;
-                if (live && v0 + u < a.per_slice && h < a.H + a.KV) {
-                    if (h < a.H) {
-                        ld8(x[u], q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] + c * 8);
-                        ld8(g[u], gq + (tok * a.H + h) * a.D + c * 8);
-                    } else {
-                        ld8(x[u], k + b * a.ks[0] + t * a.ks[1] + (h - a.H) * a.ks[2] + c * 8);
-                        ld8(g[u], gk + (tok * a.KV + (h - a.H)) * a.D + c * 8);
-                    }
-                }
+                const bool ok = live && v0 + u < a.per_slice && h < a.H + a.KV;
+                in[u] = raw8((h < a.H ? q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] : k + b * a.ks[0] + t * a.ks[1] + (h - a.H) * a.ks[2]) + c * 8, ok);
+                up[u] = raw8((h < a.H ? gq + (tok * a.H + h) * a.D : gk + (tok * a.KV + (h - a.H)) * a.D) + c * 8, ok);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int h = h0 + v0 + u;
                 if (v0 + u >= a.per_slice) break;        // the same in every lane of the CTA
                 const bool is_q = h < a.H;
-                if (half) turn<-1>(g[u], cs, sn, half, c, LPG);
-                float s1 = 0.f, s2 = 0.f, hh[8];
+                if (h == a.H || v0 + u == 0) {           // the queries' weights, then the keys'
+                    const float* from = is_q ? a.qw : a.kw;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) w[i] = 1.f;
+                    if (c * 8 < a.D && from != nullptr) ld8(w, from + c * 8);
+                }
+                float x[8], g[8], s1 = 0.f, s2 = 0.f;
+                widen(x, in[u]);
+                widen(g, up[u]);
+                if (half) turn<-1>(g, cs, sn, half, c, LPG);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    hh[i] = g[u][i] * (is_q ? w[0][i] : w[1][i]);
-                    s1 = fmaf(x[u][i], x[u][i], s1);
-                    s2 = fmaf(hh[i], x[u][i], s2);
+                    s1 = fmaf(x[i], x[i], s1);
+                    s2 = fmaf(g[i] * w[i], x[i], s2);
                 }
                 const float r = rsqrtf(fmaf(group_sum<LPG>(s1), inv_d, a.eps));
                 const float m = group_sum<LPG>(s2) * r * r * inv_d;
@@ -182,8 +192,8 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_bwd_kernel(NormArgs a, c
                 float dx[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    dx[i] = r * fmaf(-x[u][i], m, hh[i]);
-                    const float gx = g[u][i] * x[u][i] * r;
+                    dx[i] = r * fmaf(-x[i], m, g[i] * w[i]);
+                    const float gx = g[i] * x[i] * r;
                     if (is_q) acc[0][i] += gx; else acc[1][i] += gx;
                 }
                 if (is_q) st8(dq + (tok * a.H + h) * a.D + c * 8, dx);

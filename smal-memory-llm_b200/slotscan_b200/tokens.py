@@ -12,30 +12,44 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _Here, _ptr, _require_cuda, _stream, plain_call, plain_grads, wants_grad
+from .ops import _Here, _require_cuda, _stream, plain_call, plain_grads, wants_grad
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _SIZE = {torch.float32: 4, torch.bfloat16: 2}
 
 
+@functools.lru_cache(maxsize=512)
+def _strides(shape, stride, size):
+    """The strides of all dimensions but the channels', 0 where a dimension has one element; None where the kernels cannot read such a
+    tensor in place: adjacent channels, everything else on 16-byte boundaries, no dimension expanded."""
+    s = tuple(0 if n == 1 else st for n, st in zip(shape[:-1], stride))
+    return None if stride[-1] != 1 or any(n > 1 and (st == 0 or st * size % 16) for n, st in zip(shape[:-1], stride)) else s
+
+
 def _laid(t):
-    """`t` and its strides (the channels' apart) where the kernels can read it in place: adjacent channels, everything else on 16-byte
-    boundaries.  A tensor that is laid out otherwise is copied.  The stride of a dimension of one element does not matter: 0."""
+    """`t` and its strides where the kernels can read it; a tensor that is laid out otherwise is copied."""
     size = _SIZE[t.dtype]
-    for x in (t, None):
-        x = t.clone(memory_format=torch.contiguous_format) if x is None else x
-        s = tuple(0 if n == 1 else st for n, st in zip(x.shape[:-1], x.stride()))
-        if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not any(st * size % 16 or (st == 0 and n > 1) for st, n in zip(s, x.shape)):
-            return x, s
-    raise ValueError("slotscan_b200: %s channels of %s do not fill 16 bytes" % (t.shape[-1], t.dtype))
+    s = _strides(t.shape, t.stride(), size)
+    if s is not None and t.data_ptr() % 16 == 0:
+        return t, s
+    t = t.clone(memory_format=torch.contiguous_format)
+    s = _strides(t.shape, t.stride(), size)
+    if s is None:
+        raise ValueError("slotscan_b200: %d channels of %s do not fill 16 bytes" % (t.shape[-1], t.dtype))
+    return t, s
 
 
 def _f32(t):
-    return None if t is None else t.float().contiguous()
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.float().contiguous()
 
 
 def _i32(t):
-    return None if t is None else t.to(torch.int32).contiguous()
+    return t if t is None or (t.dtype is torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+
+
+def _ptr(t):
+    """A device address for a `c_void_p` argument; an empty tensor has none."""
+    return None if t is None else t.data_ptr() or None
 
 
 def _same(what, *ts):
@@ -108,30 +122,24 @@ def _norm_bwd(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], p
     dqo, dko = _whole(dqo, q.dtype), _whole(dko, k.dtype)
     dev, weights = q.device, qw is not None or kw is not None
     dq, dk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
-    dw = torch.empty(2, q.shape[3] if weights else 0, dtype=torch.float32, device=dev)
+    n = q.shape[3] if weights else 0
+    dqw, dkw = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
     scratch = torch.empty(scratch_bytes if weights else 0, dtype=torch.uint8, device=dev)
     with _Here(dev):
         rc = _lib.lib().slotscan_norm_rope_bwd(ref, _ptr(q), _ptr(k), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(dqo), _ptr(dko),
-                                               _ptr(dq), _ptr(dk), _ptr(dw[0]), _ptr(dw[1]), _ptr(scratch), scratch.numel(), _stream(dev))
+                                               _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(scratch), scratch.numel(), _stream(dev))
     _lib.check(rc, "slotscan_norm_rope_bwd")
-    return dq, dk, dw[0], dw[1]
+    return dq, dk, dqw, dkw
 
 
 def _whole(g, dtype):
     """An upstream gradient, contiguous and on a 16-byte boundary."""
-    g = g.to(dtype).contiguous()
+    if g.dtype is not dtype or not g.is_contiguous():
+        g = g.to(dtype).contiguous()
     return g if g.data_ptr() % 16 == 0 else g.clone()
 
 
-def _norm_bwd_apart(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], pos: Optional[torch.Tensor],
-                    q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], dqo: torch.Tensor, dko: torch.Tensor, eps: float
-                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """_norm_bwd for the registered op, none of whose outputs may share memory with another."""
-    dq, dk, dqw, dkw = _norm_bwd(q, k, table, pos, q_weight, k_weight, dqo, dko, eps)
-    return dq, dk, dqw, dkw.clone()
-
-
-_norm_bwd_op = torch.library.custom_op("slotscan::norm_rope_bwd", mutates_args=())(_norm_bwd_apart)
+_norm_bwd_op = torch.library.custom_op("slotscan::norm_rope_bwd", mutates_args=())(_norm_bwd)
 
 
 @_norm_bwd_op.register_fake
