@@ -5,9 +5,14 @@
 // no atomics, and give the same bits from run to run.
 //   rows X0, X1 / stream Y0, Y1:   queries: q, do / k, v      keys: k, v / q, do
 //   s = X0 Y0^T, dp = X1 Y1^T, p = exp2(s - lse), ds = p (dp - delta) (1 - tanh^2),   out1 += ds Y0,  keys also out0 += p Y1
-// A CTA holds 128 rows; the stream comes 64 at a time.  Scores and dp have two buffers in tensor memory, one for each group of 128
-// threads, which form the weights of every other step (a thread has a row) and write p and ds, as bf16, over them, where the
-// products read them as their first operand.  So the products of a step run while the other group forms the next one's weights.
+// A CTA holds 128 rows; the stream comes 64 at a time.  Scores and dp have two buffers in tensor memory.  256 threads form the
+// weights of a step, a thread half a row, and write p and ds, as bf16, over scores and dp, where the products read them as their first
+// operand.  Meanwhile the products run the last step's sums and the next one's scores.
+// A product of 128 x 64 with both operands in shared memory is bound by reading them (6 KB, 48 cycles, for 32 cycles of sums).  With
+// rows of queries there is room in tensor memory for the rows, so they are copied there once and only the stream is read; with
+// rows of keys the two results fill it.
+#include <type_traits>
+
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_tensor.cuh"
@@ -36,19 +41,19 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     char *X0 = smem, *X1 = smem + Sh::XTILE, *Ys = smem + 2 * Sh::XTILE;
-    __shared__ uint64_t x_full, done, s_full[2], p_full[2], full[Sh::STAGES], empty[Sh::STAGES];
+    __shared__ uint64_t x_full, x_moved, done, s_full[2], p_full[2], full[Sh::STAGES], empty[Sh::STAGES];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     __shared__ TileSpan s_span;
-    __shared__ __align__(16) float s_stat[2][2][2][AB_N];              // group, buffer, lse / delta
+    __shared__ __align__(16) float s_stat[8][2][2][AB_N / 2];          // warp, buffer, lse / delta
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, group = a.H / a.KV;
     const int heads = (KEYS ? a.KV : a.H) * a.B, rows = KEYS ? a.Tk : a.Tq, off = a.Tk - a.Tq;
     const int at_tile = (int)(tile_major ? blockIdx.x / heads : blockIdx.x % tiles), tile = KEYS ? at_tile : tiles - 1 - at_tile;   // long ones first
     const int hb = (int)(tile_major ? blockIdx.x % heads : blockIdx.x / tiles);
     const int hx = hb % (heads / a.B), b = hb / (heads / a.B), hk = KEYS ? hx : hx / group, x0 = tile * 128;
     if (tid == 0) {
-        mbar_init(&x_full, 1); mbar_init(&done, 1);
-        for (int w = 0; w < 2; w++) { mbar_init(&s_full[w], 1); mbar_init(&p_full[w], 4); }
+        mbar_init(&x_full, 1); mbar_init(&x_moved, 8); mbar_init(&done, 1);
+        for (int w = 0; w < 2; w++) { mbar_init(&s_full[w], 1); mbar_init(&p_full[w], 8); }
         for (int s = 0; s < Sh::STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_fence_init();
         tile_span_reset(&s_span);
@@ -56,7 +61,7 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
     }
     if (warp == 8) tmem_alloc(&s_tmem, 512);
     __syncthreads();
-    const int r = tid % 128, row = x0 + r;               // of the threads that form weights: two groups, the same rows
+    const int r = tid % 128, row = x0 + r;               // of the threads that form weights: two groups, half a row each
     Span sp = {0, 0};
     if (warp < 8) {
         if (row < rows) sp = KEYS ? queries_of(a, b, row) : keys_of(a, b, row);
@@ -72,11 +77,29 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
     if (warp < 8) {                                      // ---- weights ----
         const int w = warp / 4;
         const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
-        const uint32_t S = tmem + w * 128 + lane_at, P = S + 64;
         const float at = (float)(KEYS ? row - off : row + off);                    // this row's place among the stream's
         bool ok = true;
         float my_lse = 0.f, my_delta = 0.f;
         if constexpr (!KEYS) {
+            // the rows into tensor memory, q by one group and do by the other
+            if (steps > 0) {
+                ok = __all_sync(FULL, wait_soon(&x_full, 0));
+                const char* x = w ? X1 : X0;
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    uint32_t y[16];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(x + (c / 2) * 128 * 128 + swizzled(r, (c % 2) * 4 + i));
+                        y[4 * i] = u.x; y[4 * i + 1] = u.y; y[4 * i + 2] = u.z; y[4 * i + 3] = u.w;
+                    }
+                    tmem_st(tmem + 384 + w * 64 + lane_at + c * 16, y);
+                }
+                tmem_st_wait();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(&x_moved);
+            }
             // delta of the row, half of its channels to each group
             if (row < rows) my_lse = lse[((size_t)b * a.H + hx) * a.Tq + row];
             float s = 0.f;
@@ -95,71 +118,99 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
             my_delta = ex[r] + ex[128 + r];
             if (w == 0 && row < rows) delta[((size_t)b * a.H + hx) * a.Tq + row] = my_delta;
         }
-        auto stat_at = [&](int s, int c) {               // lse or delta of a query of step s
-            const int h = hk * group + s / y_tiles, i = (y_first + s % y_tiles) * AB_N + c % AB_N;
-            return i < a.Tq ? (c < AB_N ? lse : delta)[((size_t)b * a.H + h) * a.Tq + i] : 0.f;
+        // lse and delta of the step's queries that this thread's columns belong to: a lane fetches one of each, a step ahead
+        int head = KEYS ? hk * group : hx, y_at = 0;     // of the step: head, tile of the stream
+        float next_lse = 0.f, next_delta = 0.f;
+        auto fetch = [&](int h, int y) {
+            const int i = (y_first + y) * AB_N + w * 32 + lane;
+            const size_t from = ((size_t)b * a.H + h) * a.Tq + i;
+            next_lse = i < a.Tq ? lse[from] : 0.f;
+            next_delta = i < a.Tq ? delta[from] : 0.f;
         };
-        float next = KEYS && w < steps ? stat_at(w, r) : 0.f;
-        for (int s = w, turn = 0; s < steps; s += 2, turn++) {
-            const int y0 = (y_first + (KEYS ? s % y_tiles : s)) * AB_N;
-            const Score sc(a, KEYS ? hk * group + s / y_tiles : hx);
-            const bool masked = y0 < ts.lo_max || y0 + AB_N > ts.hi_min;
+        if (KEYS && steps > 0) fetch(head, 0);
+        for (int s = 0; s < steps; s++) {
+            const int buf = s & 1, y0 = (y_first + y_at) * AB_N + w * 32;
+            const uint32_t S = tmem + buf * 128 + w * 32 + lane_at, P = S + 64;
+            const Score sc(a, head);
+            const bool masked = y0 < ts.lo_max || y0 + 32 > ts.hi_min;
+            float* stat = &s_stat[warp][buf][0][0];
+            if (++y_at == y_tiles) { y_at = 0; head++; }
             if constexpr (KEYS) {
-                s_stat[w][turn & 1][r / AB_N][r % AB_N] = next;
-                if (s + 2 < steps) next = stat_at(s + 2, r);
-                sync_group(1 + w, 128);
+                stat[lane] = next_lse;
+                stat[32 + lane] = next_delta;
+                __syncwarp();
+                if (s + 1 < steps) fetch(head, y_at);
             }
-            if (!(ok = __all_sync(FULL, wait_soon(&s_full[w], turn & 1)))) break;
+            if (!(ok = __all_sync(FULL, ok && wait_soon(&s_full[buf], (s / 2) & 1)))) break;
             tmem_fence_after();
+            uint32_t xs[32], xd[32], wp[16], wd[16];
+            tmem_ld(S, xs);
+            tmem_ld(P, xd);
+            tmem_ld_wait(xs);
+            tmem_ld_wait(xd);
+            const int lo = sp.lo - y0, hi = sp.hi - y0;
+            const float ahead = at - (float)y0;
+            bool small = true;                           // the capped scores' polynomial serves this warp's block
+            if constexpr (CAP) {
+                float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-            for (int c = 0; c < AB_N / 32; c++) {
-                uint32_t xs[32], xd[32], wp[16], wd[16];
-                tmem_ld(S + c * 32, xs);
-                tmem_ld(P + c * 32, xd);
-                tmem_ld_wait(xs);
-                tmem_ld_wait(xd);
-                const int lo = sp.lo - y0 - c * 32, hi = sp.hi - y0 - c * 32;
-                const float ahead = at - (float)(y0 + c * 32);
-                const float4* ls = reinterpret_cast<const float4*>(&s_stat[w][turn & 1][0][c * 32]);
-                const float4* de = reinterpret_cast<const float4*>(&s_stat[w][turn & 1][1][c * 32]);
-#pragma unroll
-                for (int i4 = 0; i4 < 8; i4++) {
-                    float l4[4], d4[4], p[4], ds[4];
-                    if constexpr (KEYS) {
-                        const float4 lv = ls[i4], dv = de[i4];
-                        l4[0] = lv.x; l4[1] = lv.y; l4[2] = lv.z; l4[3] = lv.w;
-                        d4[0] = dv.x; d4[1] = dv.y; d4[2] = dv.z; d4[3] = dv.w;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int i = i4 * 4 + e;
-                        const float x = __uint_as_float(xs[i]), L = KEYS ? l4[e] : my_lse, dl = KEYS ? d4[e] : my_delta;
-                        float z, f = 1.f;
-                        if constexpr (CAP) {             // tanh x = 1 - 2 r, 1 - tanh^2 = 4 r (1 - r),  r = 1 / (e^2x + 1)
-                            const float rr = rcp_fast(exp2_fast(x * (2.f * LOG2E * sc.cap_in)) + 1.f);
-                            z = fmaf(-2.f * sc.cap_out, rr, sc.cap_out) - L;
-                            f = 4.f * fmaf(-rr, rr, rr);
-                        } else z = fmaf(x, sc.lin, -L);
-                        if constexpr (BIAS) z = fmaf(-sc.slope, fabsf(ahead - (float)i), z);
-                        p[e] = exp2_fast(z);
-                        ds[e] = p[e] * (__uint_as_float(xd[i]) - dl);
-                        if constexpr (CAP) ds[e] *= f;
-                        if (masked) {
-                            const bool in = i >= lo && i < hi, alone = L == INFINITY;
-                            p[e] = in ? (alone ? 1.f : p[e]) : 0.f;
-                            ds[e] = in && !alone ? ds[e] : 0.f;
-                        }
-                    }
-                    wp[i4 * 2] = pack_bf16(p[0], p[1]); wp[i4 * 2 + 1] = pack_bf16(p[2], p[3]);
-                    wd[i4 * 2] = pack_bf16(ds[0], ds[1]); wd[i4 * 2 + 1] = pack_bf16(ds[2], ds[3]);
+                for (int i = 0; i < 32; i += 2) {
+                    m0 = fmaxf(m0, fabsf(__uint_as_float(xs[i])));
+                    m1 = fmaxf(m1, fabsf(__uint_as_float(xs[i + 1])));
                 }
-                if constexpr (KEYS) tmem_st(S + c * 16, wp);
-                tmem_st(P + c * 16, wd);
+                small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= 1.f);
             }
+            auto weights = [&](auto poly) {
+                const CapPoly cp(sc);
+                const f32x2 lin = pack2(sc.lin, sc.lin), steep = pack2(-sc.slope, -sc.slope), one = pack2(1.f, 1.f);
+                const f32x2 k2 = pack2(-1.f / (sc.cap_out * sc.cap_out), -1.f / (sc.cap_out * sc.cap_out));
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float L[2] = {my_lse, my_lse}, dl[2] = {my_delta, my_delta};
+                    if constexpr (KEYS) {
+                        const float2 u = *reinterpret_cast<const float2*>(stat + i), v = *reinterpret_cast<const float2*>(stat + 32 + i);
+                        L[0] = u.x; L[1] = u.y; dl[0] = v.x; dl[1] = v.y;
+                    }
+                    const f32x2 x = pack2(__uint_as_float(xs[i]), __uint_as_float(xs[i + 1]));
+                    f32x2 z, f = one;
+                    if constexpr (CAP && decltype(poly)::value) {
+                        const f32x2 y = mul2(x, cp.slope(x));
+                        z = add2(y, pack2(-L[0], -L[1]));
+                        f = fma2(mul2(y, y), k2, one);
+                    } else if constexpr (CAP) {          // tanh x = 1 - 2 r, 1 - tanh^2 = 4 r (1 - r),  r = 1 / (e^2x + 1)
+                        float zz[2], ff[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float rr = rcp_fast(exp2_fast(__uint_as_float(xs[i + e]) * (2.f * LOG2E * sc.cap_in)) + 1.f);
+                            zz[e] = fmaf(-2.f * sc.cap_out, rr, sc.cap_out) - L[e];
+                            ff[e] = 4.f * fmaf(-rr, rr, rr);
+                        }
+                        z = pack2(zz[0], zz[1]);
+                        f = pack2(ff[0], ff[1]);
+                    } else z = fma2(x, lin, pack2(-L[0], -L[1]));
+                    if constexpr (BIAS) z = fma2(pack2(fabsf(ahead - (float)i), fabsf(ahead - (float)(i + 1))), steep, z);
+                    const float2 zf = unpack2(z);
+                    float2 p = make_float2(exp2_fast(zf.x), exp2_fast(zf.y));
+                    f32x2 d = mul2(pack2(p.x, p.y), add2(pack2(__uint_as_float(xd[i]), __uint_as_float(xd[i + 1])), pack2(-dl[0], -dl[1])));
+                    if constexpr (CAP) d = mul2(d, f);
+                    float2 ds = unpack2(d);
+                    if (masked) {
+                        const bool in0 = i >= lo && i < hi, in1 = i + 1 >= lo && i + 1 < hi, alone0 = L[0] == INFINITY, alone1 = L[1] == INFINITY;
+                        p = make_float2(in0 ? (alone0 ? 1.f : p.x) : 0.f, in1 ? (alone1 ? 1.f : p.y) : 0.f);
+                        ds = make_float2(in0 && !alone0 ? ds.x : 0.f, in1 && !alone1 ? ds.y : 0.f);
+                    }
+                    wp[i / 2] = pack_bf16(p.x, p.y);
+                    wd[i / 2] = pack_bf16(ds.x, ds.y);
+                }
+            };
+            if (small) weights(std::true_type{});
+            else if constexpr (CAP) weights(std::false_type{});
+            if constexpr (KEYS) tmem_st(S, wp);
+            tmem_st(P, wd);
             tmem_st_wait();
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) arrive(&p_full[w]);
+            if (lane == 0) arrive(&p_full[buf]);
         }
         if (ok && steps > 0) ok = wait_soon(&done, 0);
         tmem_fence_after();
@@ -215,20 +266,21 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
         }
     } else if (warp == 8) {                              // ---- products ----
         if (lane == 0 && steps > 0) {
-            bool ok = wait_soon(&x_full, 0);
+            bool ok = wait_soon(KEYS ? &x_full : &x_moved, 0);
+            tmem_fence_after();
             const uint64_t x0d = tile_desc(smem_u32(X0), 16), x1d = tile_desc(smem_u32(X1), 16);
             auto scores = [&](int s) {                   // s and dp of a step
                 const int w = s & 1, st = s % Sh::STAGES;
                 if (!wait_soon(&full[st], (s / Sh::STAGES) & 1)) return false;
                 const uint64_t yd = tile_desc(smem_u32(Ys + st * 2 * Sh::YTILE), 16);
 #pragma unroll
-                for (int k = 0; k < DP / 16; k++)
-                    mma_ss(tmem + w * 128, x0d + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, yd + ((k / 4) * AB_N * 128 + (k % 4) * 32) / 16,
-                           mma_shape(AB_N, false), k > 0);
+                for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int k = 0; k < DP / 16; k++)
-                    mma_ss(tmem + w * 128 + 64, x1d + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16,
-                           yd + (Sh::YTILE + (k / 4) * AB_N * 128 + (k % 4) * 32) / 16, mma_shape(AB_N, false), k > 0);
+                    for (int k = 0; k < DP / 16; k++) {
+                        const uint64_t y = yd + (x * Sh::YTILE + (k / 4) * AB_N * 128 + (k % 4) * 32) / 16;
+                        if constexpr (KEYS) mma_ss(tmem + w * 128 + x * 64, (x ? x1d : x0d) + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, y, mma_shape(AB_N, false), k > 0);
+                        else mma_ts(tmem + w * 128 + x * 64, tmem + 384 + x * 64 + k * 8, y, mma_shape(AB_N, false), k > 0);
+                    }
                 mma_commit(&s_full[w]);
                 return true;
             };
@@ -242,11 +294,11 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
                 if constexpr (KEYS) {
 #pragma unroll
                     for (int k = 0; k < AB_N / 16; k++)
-                        mma_ts(tmem + 256 + DP, tmem + w * 128 + k * 8, yd + (Sh::YTILE + k * 2048) / 16, mma_shape(DP, true), s > 0 || k > 0);
+                        mma_ts(tmem + 256 + DP, tmem + w * 128 + (k / 2) * 32 + (k % 2) * 8, yd + (Sh::YTILE + k * 2048) / 16, mma_shape(DP, true), s > 0 || k > 0);
                 }
 #pragma unroll
                 for (int k = 0; k < AB_N / 16; k++)
-                    mma_ts(tmem + 256, tmem + w * 128 + 64 + k * 8, yd + k * 2048 / 16, mma_shape(DP, true), s > 0 || k > 0);
+                    mma_ts(tmem + 256, tmem + w * 128 + 64 + (k / 2) * 32 + (k % 2) * 8, yd + k * 2048 / 16, mma_shape(DP, true), s > 0 || k > 0);
                 mma_commit(&empty[st]);
                 if (s + 2 < steps) ok = scores(s + 2);
             }

@@ -9,6 +9,8 @@
 // when a row's maximum has grown by more than 2^8: until then the weights are taken relative to the old one, which
 // float32 sums and the relative precision of bf16 bear.
 // p is rounded to bf16 for its product, as its operand type asks; the sum of the softmax takes it unrounded.
+#include <type_traits>
+
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_tensor.cuh"
@@ -34,17 +36,35 @@ struct FwdMaps { CUtensorMap q, k, v, o, rest; };
 // not see them
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ void scores32(float (&s)[32], const Score& sc, float ahead, bool masked, int lo, int hi) {
-    if constexpr (CAP || BIAS) {
+    bool small = true;                                   // the capped scores' polynomial serves this warp's block
+    if constexpr (CAP) {
+        float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            float z;
-            if constexpr (CAP) {
-                const float u = exp2_fast(s[i] * (2.f * LOG2E * sc.cap_in));                   // tanh x = 1 - 2 / (e^2x + 1)
-                z = fmaf(-2.f * sc.cap_out, rcp_fast(u + 1.f), sc.cap_out);
-            } else z = s[i] * sc.lin;
-            if constexpr (BIAS) z = fmaf(-sc.slope, fabsf(ahead - (float)i), z);
-            s[i] = z;
-        }
+        for (int i = 0; i < 32; i += 2) { m0 = fmaxf(m0, fabsf(s[i])); m1 = fmaxf(m1, fabsf(s[i + 1])); }
+        small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= 1.f);
+    }
+    if constexpr (CAP || BIAS) {
+        auto whole = [&](auto poly) {
+            const CapPoly cp(sc);
+            const f32x2 lin = pack2(sc.lin, sc.lin), steep = pack2(-sc.slope, -sc.slope);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const f32x2 x = pack2(s[i], s[i + 1]);
+                f32x2 z;
+                if constexpr (CAP && decltype(poly)::value) z = mul2(x, cp.slope(x));
+                else if constexpr (CAP) {                                                      // tanh x = 1 - 2 / (e^2x + 1)
+                    const float in = 2.f * LOG2E * sc.cap_in;
+                    z = pack2(fmaf(-2.f * sc.cap_out, rcp_fast(exp2_fast(s[i] * in) + 1.f), sc.cap_out),
+                              fmaf(-2.f * sc.cap_out, rcp_fast(exp2_fast(s[i + 1] * in) + 1.f), sc.cap_out));
+                } else z = mul2(x, lin);
+                if constexpr (BIAS) z = fma2(pack2(fabsf(ahead - (float)i), fabsf(ahead - (float)(i + 1))), steep, z);
+                const float2 u = unpack2(z);
+                s[i] = u.x;
+                s[i + 1] = u.y;
+            }
+        };
+        if (small) whole(std::true_type{});
+        else if constexpr (CAP) whole(std::false_type{});
     }
     if (masked) {
 #pragma unroll
@@ -151,22 +171,23 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                 l *= f;
             }
             const float base = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+            const f32x2 lin = pack2(sc.lin, sc.lin), back = pack2(-base, -base);
 #pragma unroll
             for (int c = 0; c < KT / 32; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
-                    const float x = __uint_as_float(raw[c][i]), y = __uint_as_float(raw[c][i + 1]);
-                    const float p0 = exp2_fast(CAP || BIAS ? x - base : fmaf(x, sc.lin, -base));
-                    const float p1 = exp2_fast(CAP || BIAS ? y - base : fmaf(y, sc.lin, -base));
-                    sum[i % 4] += p0;
-                    sum[i % 4 + 1] += p1;
+                    const f32x2 x = pack2(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1]));
+                    const float2 z = unpack2(CAP || BIAS ? add2(x, back) : fma2(x, lin, back));
+                    const float p0 = exp2_fast(z.x), p1 = exp2_fast(z.y);
+                    sum[(i / 2) % 2] = add2(sum[(i / 2) % 2], pack2(p0, p1));
                     w[i / 2] = pack_bf16(p0, p1);
                 }
                 tmem_st(S + c * 16, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const float2 total = unpack2(add2(sum[0], sum[1]));
+            l += total.x + total.y;
             tmem_st_wait();
             tmem_fence_before();
             __syncwarp();
