@@ -254,10 +254,10 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                 if (!ok) s_fail = 1;
             }
         } else if (warp == NT * 4) {                         // ---- products ----
-            if (lane == 0 && n0 < n1) {
+            if (n0 < n1) {
                 bool ok = true;
                 auto stage = [](int x) { return x % Sh::STAGES; };
-                auto arrived = [&](int x) { return wait_soon(&full[stage(x)], (x / Sh::STAGES) & 1); };
+                auto arrived = [&](int x) { return wait_soon_warp(&full[stage(x)], (x / Sh::STAGES) & 1); };
                 auto scores = [&](int t, int x) {            // s = q k^T
                     const uint64_t qd = tile_desc(smem_u32(Qs + t * Sh::QTILE), 16), kd = tile_desc(smem_u32(Ks + stage(x) * Sh::KTILE), 16);
     #pragma unroll
@@ -265,7 +265,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                         mma_ss(tmem + t * KT, qd + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, kd + ((k / 4) * KT * 128 + (k % 4) * 32) / 16, mma_shape(KT, false), k > 0);
                     mma_commit(&s_full[t]);
                 };
-                for (int t = 0; t < NT && ok; t++) ok = wait_soon(&q_full[t], 0);
+                for (int t = 0; t < NT && ok; t++) ok = wait_soon_warp(&q_full[t], 0);
                 ok = ok && arrived(0);
                 for (int t = 0; t < NT && ok; t++)
                     if (first[t] == n0 && last[t] > first[t]) scores(t, 0);
@@ -275,7 +275,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                     const uint64_t vd = tile_desc(smem_u32(Ks + stage(x + 1) * Sh::KTILE), KT * 128);
                     for (int t = 0; t < NT && ok; t++) {
                         if (n >= first[t] && n < last[t]) {
-                            ok = wait_soon(&p_full[t], (n - first[t]) & 1);
+                            ok = wait_soon_warp(&p_full[t], (n - first[t]) & 1);
                             tmem_fence_after();
     #pragma unroll
                             for (int k = 0; k < KT / 16; k++)
