@@ -110,7 +110,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = Sh::COLUMNS == 512 ? 0 : s_tmem;   // all 512 columns begin at the first
     int first[NT], last[NT], n0 = BIGI, n1 = 0;          // key tiles of each query tile, and of all
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -256,36 +256,47 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
         } else if (warp == NT * 4) {                         // ---- products ----
             if (n0 < n1) {
                 bool ok = true;
+                const bool lead = elected();
                 auto stage = [](int x) { return x % Sh::STAGES; };
                 auto arrived = [&](int x) { return wait_soon_warp(&full[stage(x)], (x / Sh::STAGES) & 1); };
                 auto scores = [&](int t, int x) {            // s = q k^T
-                    const uint64_t qd = tile_desc(smem_u32(Qs + t * Sh::QTILE), 16), kd = tile_desc(smem_u32(Ks + stage(x) * Sh::KTILE), 16);
-    #pragma unroll
-                    for (int k = 0; k < DP / 16; k++)
-                        mma_ss(tmem + t * KT, qd + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, kd + ((k / 4) * KT * 128 + (k % 4) * 32) / 16, mma_shape(KT, false), k > 0);
-                    mma_commit(&s_full[t]);
+                    const uint32_t qd = tile_desc(smem_u32(Qs + t * Sh::QTILE), 16), kd = tile_desc(smem_u32(Ks + stage(x) * Sh::KTILE), 16);
+                    if (lead) {
+#pragma unroll
+                        for (int k = 0; k < DP / 16; k++)
+                            mma_ss(tmem + t * KT, qd + ((k / 4) * 128 * 128 + (k % 4) * 32) / 16, kd + ((k / 4) * KT * 128 + (k % 4) * 32) / 16, mma_shape(KT, false), k > 0);
+                        mma_commit(&s_full[t]);
+                    }
+                    __syncwarp();
                 };
                 for (int t = 0; t < NT && ok; t++) ok = wait_soon_warp(&q_full[t], 0);
                 ok = ok && arrived(0);
                 for (int t = 0; t < NT && ok; t++)
                     if (first[t] == n0 && last[t] > first[t]) scores(t, 0);
-                mma_commit(&empty[0]);
+                if (lead) mma_commit(&empty[0]);
+                __syncwarp();
                 for (int n = n0, x = 0; n < n1 && ok; n++, x += 2) {
                     ok = arrived(x + 1) && (n + 1 == n1 || arrived(x + 2));
-                    const uint64_t vd = tile_desc(smem_u32(Ks + stage(x + 1) * Sh::KTILE), KT * 128);
+                    const uint32_t vd = tile_desc(smem_u32(Ks + stage(x + 1) * Sh::KTILE), KT * 128);
                     for (int t = 0; t < NT && ok; t++) {
                         if (n >= first[t] && n < last[t]) {
                             ok = wait_soon_warp(&p_full[t], (n - first[t]) & 1);
                             tmem_fence_after();
-    #pragma unroll
-                            for (int k = 0; k < KT / 16; k++)
-                                mma_ts(tmem + NT * KT + t * DP, tmem + t * KT + k * 8, vd + k * 2048 / 16, mma_shape(DP, true), n > first[t] || k > 0);
-                            mma_commit(&o_full[t]);
+                            if (lead) {
+#pragma unroll
+                                for (int k = 0; k < KT / 16; k++)
+                                    mma_ts(tmem + NT * KT + t * DP, tmem + t * KT + k * 8, vd + k * 2048 / 16, mma_shape(DP, true), n > first[t] || k > 0);
+                                mma_commit(&o_full[t]);
+                            }
+                            __syncwarp();
                         }
                         if (n + 1 >= first[t] && n + 1 < last[t]) scores(t, x + 2);
                     }
-                    mma_commit(&empty[stage(x + 1)]);
-                    if (n + 1 < n1) mma_commit(&empty[stage(x + 2)]);
+                    if (lead) {
+                        mma_commit(&empty[stage(x + 1)]);
+                        if (n + 1 < n1) mma_commit(&empty[stage(x + 2)]);
+                    }
+                    __syncwarp();
                 }
                 if (!ok) s_fail = 1;
             }
@@ -297,7 +308,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
         if (tid == 0) atomicExch(&g_attn_status, 1);
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
     }
-    if (warp == NT * 4) { tmem_fence_after(); tmem_free(tmem, Sh::COLUMNS); }
+    if (warp == NT * 4) { tmem_fence_after(); tmem_free(s_tmem, Sh::COLUMNS); }
 }
 
 template <int DP, int NT, int KT, bool CAP, bool BIAS>

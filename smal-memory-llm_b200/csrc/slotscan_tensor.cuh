@@ -65,28 +65,35 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[8]) {
                  ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
                  : "memory");
 }
-// ---- products: D (128 x N, float32 in tensor memory) = A B^T (+ D), bf16 operands.  Called by a whole warp, whose addresses are then
-// known to be the same in every lane and need no moves; one lane issues ----
-// shared-memory operand with the 128-byte swizzle; lead: bytes from sub-tile to sub-tile (used where rows run along the sum)
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// ---- products: D (128 x N, float32 in tensor memory) = A B^T (+ D), bf16 operands ----
+// The warp runs to them as a whole, so that addresses are known to be the same in every lane, and its elected lane issues.
+// The operands' descriptors are built from their lower halves, the upper one being a constant, so that a product takes
+// few instructions: with 64-bit sums and an election each the issue was slower than the products.
+// shared-memory operand with the 128-byte swizzle: lower half.  lead: bytes from sub-tile to sub-tile (used where rows run along
+// the sum); add bytes / 16 to move on
+__device__ __forceinline__ uint32_t tile_desc(uint32_t addr, uint32_t lead) { return ((addr >> 4) & 0x3fff) | ((lead >> 4) & 0x3fff) << 16; }
+constexpr uint32_t TILE_DESC_HIGH = (1024 >> 4) | 1u << 14 | 2u << 29;              // eight rows 1,024 bytes apart, version, swizzle
 // float32 sums of bf16 products, 128 x N; bT: B's rows run along the sum
 __host__ __device__ constexpr uint32_t mma_shape(int n, bool bT) { return 1u << 4 | 1u << 7 | 1u << 10 | (bT ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24; }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-    asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.u32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
-                 "r"(shape), "r"((uint32_t)add)
+__device__ __forceinline__ bool elected() {
+    uint32_t e;
+    asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\nsetp.ne.u32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(shape), "r"((uint32_t)add), "r"(TILE_DESC_HIGH)
                  : "memory");
 }
 // A in tensor memory: two bf16 to a column
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
-    asm volatile("{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.u32 p, %4, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
-                 "r"(shape), "r"((uint32_t)add)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 y;\nmov.b64 y, {%2, %5};\nsetp.ne.u32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(shape), "r"((uint32_t)add), "r"(TILE_DESC_HIGH)
                  : "memory");
 }
-// one arrival at `bar` when all products issued so far by the electing lane (the same each time) are done
+// one arrival at `bar` when all products issued so far by the elected lane (the same each time) are done; called by that lane
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // ---- tiled copies of a (sequence, head, token, channel) tensor ----
