@@ -29,14 +29,22 @@ static AttnArgs attn_args(const slotscan_attn_params& p, const float* slopes, co
     return a;
 }
 
+extern "C" int slotscan_attn_keeps(const slotscan_attn_params* p, int with_prefix) {
+    if (slotscan_attn_check(p) != SLOTSCAN_OK) return 0;
+    const int32_t none = 0;
+    return !(p->dtype == SLOTSCAN_BF16 && attn_narrow(attn_args(*p, nullptr, nullptr, with_prefix ? &none : nullptr)));
+}
+
 extern "C" int slotscan_attn_fwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
                                  const int32_t* docs, const int32_t* prefix, void* o, void* rest, float* lse, void* stream) {
     const int rc = slotscan_attn_check(p);
     if (rc != SLOTSCAN_OK) return rc;
     if ((int64_t)p->B * p->Tq == 0) return SLOTSCAN_OK;
-    if (!q || !k || !v || !o || (lse && p->dtype == SLOTSCAN_BF16 && !rest)) return SLOTSCAN_E_NULL;
+    if (!q || !k || !v || !o) return SLOTSCAN_E_NULL;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest) || ((uintptr_t)docs & 7)) return SLOTSCAN_E_ALIGN;
     const AttnArgs a = attn_args(*p, slopes, docs, prefix);
+    if (p->dtype == SLOTSCAN_BF16 && attn_narrow(a)) return (int)run_attn_fwd_narrow(a, q, k, v, o, (cudaStream_t)stream);
+    if (p->dtype == SLOTSCAN_BF16 && lse && !rest) return SLOTSCAN_E_NULL;
     return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_fwd_bf16(a, q, k, v, o, rest, lse, (cudaStream_t)stream)
                                            : run_attn_fwd_f32(a, q, k, v, o, lse, (cudaStream_t)stream));
 }
@@ -54,11 +62,13 @@ extern "C" int slotscan_attn_bwd(const slotscan_attn_params* p, const void* q, c
         if (e == cudaSuccess) e = cudaMemsetAsync(dv, 0, n, (cudaStream_t)stream);
         return (int)e;
     }
-    if (!q || !k || !v || !o || (p->dtype == SLOTSCAN_BF16 && !rest) || !lse || !dout || !delta || !dq || !dk || !dv) return SLOTSCAN_E_NULL;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
-        ((uintptr_t)docs & 7))
+    if (!q || !k || !v || !dout || !dq || !dk || !dv) return SLOTSCAN_E_NULL;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) ||
+        !aligned16(dv) || ((uintptr_t)docs & 7))
         return SLOTSCAN_E_ALIGN;
     const AttnArgs a = attn_args(*p, slopes, docs, prefix);
+    if (p->dtype == SLOTSCAN_BF16 && attn_narrow(a)) return (int)run_attn_bwd_narrow(a, q, k, v, dout, dq, dk, dv, (cudaStream_t)stream);
+    if (!o || !lse || !delta || (p->dtype == SLOTSCAN_BF16 && !rest)) return SLOTSCAN_E_NULL;
     return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_bwd_bf16(a, q, k, v, o, rest, lse, dout, delta, dq, dk, dv, (cudaStream_t)stream)
                                            : run_attn_bwd_f32(a, q, k, v, o, lse, dout, delta, dq, dk, dv, (cudaStream_t)stream));
 }

@@ -97,4 +97,12 @@ cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, c
 cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const void* rest,
                               const float* lse, const void* dout, float* delta, void* dq, void* dk, void* dv, cudaStream_t st);
 
+// bf16 with a window of up to NARROW_WINDOW tokens, as many queries as keys and no prefix: kernels of their own, whose backward needs
+// nothing of the forward
+constexpr int NARROW_WINDOW = 33;
+bool attn_narrow(const AttnArgs& a);
+cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st);
+cudaError_t run_attn_bwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv,
+                                cudaStream_t st);
+
 }  // namespace slotscan

@@ -456,9 +456,13 @@ extern "C" int slotscan_query_attrs(slotscan_kernel_attr* out, int cap) {
 
 extern "C" int slotscan_device_status(void) {
     if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-    const int a = rows_bwd_status_f32(), b = rows_bwd_status_bf16(), c = read_mma_status();
-    const int d = gather_status_f32(), e = gather_status_bf16(), f = replay_status(), g = attn_mma_status(), h = attn_bwd_mma_status();
-    return (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0 || g < 0 || h < 0) ? -1 : (a | b | c | d | e | f | g | h);
+    int all = 0;
+    for (int (*status)() : {rows_bwd_status_f32, rows_bwd_status_bf16, read_mma_status, gather_status_f32, gather_status_bf16, replay_status,
+                            attn_mma_status, attn_bwd_mma_status, attn_narrow_status}) {
+        const int one = status();
+        all = one < 0 || all < 0 ? -1 : all | one;
+    }
+    return all;
 }
 
 extern "C" int slotscan_profile_enable(int on) {

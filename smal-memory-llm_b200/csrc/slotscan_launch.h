@@ -84,6 +84,7 @@ bool read_bwd_mma_try(const slotscan_read_params& p, const void* qr, const float
 int read_mma_status();
 int attn_mma_status();
 int attn_bwd_mma_status();
+int attn_narrow_status();
 int gather_status_f32();
 int gather_status_bf16();
 int rows_bwd_status_f32();

@@ -156,7 +156,7 @@ def lib():
         for name, args, res in (
                 ("norm_rope_check", [NP], ci), ("norm_rope_fwd", [NP] + [vp] * 9, ci), ("norm_rope_bwd_scratch_bytes", [NP], sz),
                 ("norm_rope_bwd", [NP] + [vp] * 13 + [sz, vp], ci), ("norm_rope_append", [ctypes.POINTER(AppendParams)] + [vp] * 11, ci),
-                ("attn_check", [TP], ci), ("attn_fwd", [TP] + [vp] * 10, ci), ("attn_bwd", [TP] + [vp] * 15, ci),
+                ("attn_check", [TP], ci), ("attn_keeps", [TP, ci], ci), ("attn_fwd", [TP] + [vp] * 10, ci), ("attn_bwd", [TP] + [vp] * 15, ci),
                 ("attn_step_check", [SP_], ci), ("attn_step_scratch_bytes", [SP_], sz), ("attn_step", [SP_] + [vp] * 8 + [sz, vp], ci)):
             f = getattr(L, "slotscan_" + name)
             f.argtypes, f.restype = args, res

@@ -258,23 +258,24 @@ def norm_rope_append(q, k, v, k_cache, v_cache, pos, table, q_weight=None, k_wei
 # ---------------------------------------------------------------------------------------- attention
 
 @functools.lru_cache(maxsize=256)
-def _attn_params(B, Tq, Tk, H, KV, D, window, dtype, scale, cap, qs, ks, vs):
+def _attn_params(B, Tq, Tk, H, KV, D, window, dtype, scale, cap, prefix, qs, ks, vs):
+    """The parameters of a call of this shape, checked, and whether its backward needs what the forward can keep."""
     p = _lib.AttnParams(B, Tq, Tk, H, KV, D, window, dtype, scale, cap, qs, ks, vs)
     _lib.check(_lib.lib().slotscan_attn_check(ctypes.byref(p)), "slotscan_attn_check")
-    return p, ctypes.byref(p)
+    return p, ctypes.byref(p), bool(_lib.lib().slotscan_attn_keeps(ctypes.byref(p), prefix))
 
 
-def _attn_call(q, k, v, window, cap, scale):
+def _attn_call(q, k, v, prefix, window, cap, scale):
     (q, qs), (k, ks), (v, vs) = _laid(q), _laid(k), _laid(v)
     B, Tq, H, D = q.shape
-    return (q, k, v) + _attn_params(B, Tq, k.shape[1], H, k.shape[2], D, window, _CODE[q.dtype], scale, cap, qs, ks, vs)
+    return (q, k, v) + _attn_params(B, Tq, k.shape[1], H, k.shape[2], D, window, _CODE[q.dtype], scale, cap, prefix is not None, qs, ks, vs)
 
 
 def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optional[torch.Tensor], docs: Optional[torch.Tensor],
               prefix: Optional[torch.Tensor], window: int, cap: float, scale: float, for_bwd: bool
               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """o and what the backward needs besides (without elements unless asked for): lse (B,H,Tq), and for bfloat16 what the rounding
-    of o left."""
+    """o and what the backward needs besides (without elements where it needs nothing, or unless asked for): lse (B,H,Tq), and for
+    bfloat16 what the rounding of o left."""
     _require_cuda(q, k, v, slopes, docs, prefix)
     _same("token_attention", q, k, v)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
@@ -290,11 +291,12 @@ def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optiona
         raise ValueError("token_attention: document bounds (B, Tk, 2) from document_bounds, got %s" % (tuple(docs.shape),))
     if prefix is not None and prefix.shape != (B,):
         raise ValueError("token_attention: one prefix length for each sequence, got %s" % (tuple(prefix.shape),))
-    q, k, v, p, ref = _attn_call(q, k, v, window, cap, scale)
+    q, k, v, p, ref, keeps = _attn_call(q, k, v, prefix, window, cap, scale)
+    keeps = keeps and for_bwd
     slopes, docs, prefix = _f32(slopes), _i32(docs), _i32(prefix)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Tq) if for_bwd else (0,), dtype=torch.float32, device=q.device)
-    rest = torch.empty(q.shape if for_bwd and q.dtype == torch.bfloat16 else (0,), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Tq) if keeps else (0,), dtype=torch.float32, device=q.device)
+    rest = torch.empty(q.shape if keeps and q.dtype == torch.bfloat16 else (0,), dtype=q.dtype, device=q.device)
     with _Here(q.device):
         rc = _lib.lib().slotscan_attn_fwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest),
                                           _ptr(lse), _stream(q.device))
@@ -307,15 +309,18 @@ _attn_op = torch.library.custom_op("slotscan::attn_fwd", mutates_args=())(_attn_
 
 @_attn_op.register_fake
 def _(q, k, v, slopes, docs, prefix, window, cap, scale, for_bwd):
-    return (q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if for_bwd else (0,), dtype=torch.float32),
-            q.new_empty(q.shape if for_bwd and q.dtype == torch.bfloat16 else (0,)))
+    B, Tq, H, D = (int(n) for n in q.shape)
+    keeps = for_bwd and _attn_params(B, Tq, int(k.shape[1]), H, int(k.shape[2]), D, window, _CODE[q.dtype], scale, cap, prefix is not None,
+                                     *((0, 0, 0),) * 3)[2]
+    return (q.new_empty(q.shape), q.new_empty((B, H, Tq) if keeps else (0,), dtype=torch.float32),
+            q.new_empty(q.shape if keeps and q.dtype == torch.bfloat16 else (0,)))
 
 
 def _attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optional[torch.Tensor], docs: Optional[torch.Tensor],
               prefix: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor, rest: torch.Tensor, do: torch.Tensor, window: int, cap: float,
               scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     _require_cuda(q, k, v, slopes, docs, prefix, o, lse, rest, do)
-    q, k, v, p, ref = _attn_call(q, k, v, window, cap, scale)
+    q, k, v, p, ref, _ = _attn_call(q, k, v, prefix, window, cap, scale)
     slopes, docs, prefix = _f32(slopes), _i32(docs), _i32(prefix)
     do, o, rest, lse = _whole(do, q.dtype), _whole(o, q.dtype), _whole(rest, q.dtype), lse.contiguous()
     dev = q.device
@@ -338,7 +343,8 @@ def _(q, k, v, slopes, docs, prefix, o, lse, rest, do, window, cap, scale):
 
 def _attn_setup(ctx, inputs, output):
     *ts, ctx.window, ctx.cap, ctx.scale, _ = inputs
-    ctx.save_for_backward(*ts, *output)
+    o, lse, rest = output
+    ctx.save_for_backward(*ts, o if lse.numel() else lse, lse, rest)
     ctx.mark_non_differentiable(*output[1:])
 
 
