@@ -203,8 +203,10 @@ struct NarrowBwd {
     static constexpr int SMEM = 2 * QT + 2 * KT + WARPS * 2 * PT;
 };
 
-template <int DP, int NB>
-__global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32) attn_bwd_narrow_kernel(AttnArgs a, const __grid_constant__ NarrowBwdMaps maps) {
+// GROUP: several query heads share a key head, whose dk and dv stay in registers over them; one CTA to an SM.  Without, dv is done before dk is
+// begun, and two CTAs fit (286 against @@ONE@@ us for 64 x 1,024 tokens, window 16).
+template <int DP, int NB, bool GROUP>
+__global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP ? 1 : 2) attn_bwd_narrow_kernel(AttnArgs a, const __grid_constant__ NarrowBwdMaps maps) {
     typedef NarrowBwd<DP, NB> Sh;
     constexpr int HB = Sh::HB, SUBS = DP / 64;
     extern __shared__ __align__(1024) char smem[];
@@ -228,13 +230,38 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32) attn_bwd_narrow
         at[r] = x0 + warp * 16 + lane / 4 + 8 * r;
         sp[r] = at[r] < a.Tq ? keys_of(a, b, at[r]) : Span{0, 0};
     }
-    float dk[DP / 8][4], dv[DP / 8][4];                  // of the warp's 16 keys
+    float sums[GROUP ? 2 : 1][DP / 8][4];                // of the warp's 16 keys: dv, dk
+    auto clear = [](float (&x)[DP / 8][4]) {
 #pragma unroll
-    for (int c = 0; c < DP / 8; c++)
+        for (int c = 0; c < DP / 8; c++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) dk[c][i] = dv[c][i] = 0.f;
+            for (int i = 0; i < 4; i++) x[c][i] = 0.f;
+    };
+    // += p^T do (which 0) or ds^T q: the queries of block warp + n see these keys in their block HB - n
+    auto gather = [&](float (&x)[DP / 8][4], int which) {
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            uint32_t w[4];
+            ldsm_t(w, Pm + ((warp + n) * 2 + which) * Sh::PT + ((lane / 16) * 8 + lane % 8) * Sh::PLD + (HB - n) * 32 + ((lane / 8) % 2) * 16);
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) {
+                uint32_t y[4];
+                rows_as_bt(y, which ? Q : G, Sh::QROWS, (warp + n) * 16, c, lane);
+                mma(x[2 * c], w, y[0], y[1]);
+                mma(x[2 * c + 1], w, y[2], y[3]);
+            }
+        }
+    };
+    // dv over v, dk over k, which all have read
+    auto put = [&](const float (&x)[DP / 8][4], int which) {
+        const float mul = which ? a.scale : 1.f;
+#pragma unroll
+        for (int c = 0; c < DP / 8; c++)
+            put_rows<DP>(which ? K : V, Sh::KROWS, warp * 16, c, lane, pack_bf16(x[c][0] * mul, x[c][1] * mul), pack_bf16(x[c][2] * mul, x[c][3] * mul));
+    };
+    if constexpr (GROUP) { clear(sums[0]); clear(sums[1]); }
     const uint32_t P = Pm + warp * 2 * Sh::PT, D = P + Sh::PT;
-    for (int g = 0; g < group; g++) {
+    for (int g = 0; g < (GROUP ? group : 1); g++) {
         const int h = hk * group + g;
         if (tid == 0) {
             mbar_arrive_expect_tx(&q_full, 2 * Sh::QT);
@@ -301,21 +328,12 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32) attn_bwd_narrow
         __syncthreads();                                 // p and ds of all queries are there
         if (warp < 4) {
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                // queries of block warp + n see these keys in their block HB - n
-                const uint32_t from = Pm + (warp + n) * 2 * Sh::PT + ((lane / 16) * 8 + lane % 8) * Sh::PLD + (HB - n) * 32 + ((lane / 8) % 2) * 16;
-                uint32_t pt[4], dt[4];
-                ldsm_t(pt, from);
-                ldsm_t(dt, from + Sh::PT);
-#pragma unroll
-                for (int c = 0; c < DP / 16; c++) {
-                    uint32_t y[4];
-                    rows_as_bt(y, G, Sh::QROWS, (warp + n) * 16, c, lane);
-                    mma(dv[2 * c], pt, y[0], y[1]);
-                    mma(dv[2 * c + 1], pt, y[2], y[3]);
-                    rows_as_bt(y, Q, Sh::QROWS, (warp + n) * 16, c, lane);
-                    mma(dk[2 * c], dt, y[0], y[1]);
-                    mma(dk[2 * c + 1], dt, y[2], y[3]);
+            for (int which = 0; which < 2; which++) {
+                if constexpr (GROUP) gather(sums[which], which);
+                else {
+                    clear(sums[0]);
+                    gather(sums[0], which);
+                    put(sums[0], which);
                 }
             }
         }
@@ -331,14 +349,10 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32) attn_bwd_narrow
                 bulk_wait_read<0>();
             }
         }
-        if (g + 1 < group) __syncthreads();              // before the next head's queries come in
+        if (GROUP && g + 1 < group) __syncthreads();     // before the next head's queries come in
     }
-    if (warp < 4) {                                      // dk over k, dv over v: all have read them
-#pragma unroll
-        for (int c = 0; c < DP / 8; c++) {
-            put_rows<DP>(K, Sh::KROWS, warp * 16, c, lane, pack_bf16(dk[c][0] * a.scale, dk[c][1] * a.scale), pack_bf16(dk[c][2] * a.scale, dk[c][3] * a.scale));
-            put_rows<DP>(V, Sh::KROWS, warp * 16, c, lane, pack_bf16(dv[c][0], dv[c][1]), pack_bf16(dv[c][2], dv[c][3]));
-        }
+    if (warp < 4) {
+        if constexpr (GROUP) { put(sums[0], 0); put(sums[1], 1); }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0 && x0 + warp * 16 < a.Tk) {
@@ -376,7 +390,7 @@ static cudaError_t bwd_narrow(const AttnArgs& a, const void* q, const void* k, c
         !tile_map(&m.dq, dq, a.B, a.Tq, a.H, a.D, os, 16) || !tile_map(&m.dk, dk, a.B, a.Tk, a.KV, a.D, gs, 16) ||
         !tile_map(&m.dv, dv, a.B, a.Tk, a.KV, a.D, gs, 16))
         return cudaErrorInvalidValue;
-    auto kern = attn_bwd_narrow_kernel<DP, NB>;
+    auto kern = a.H > a.KV ? attn_bwd_narrow_kernel<DP, NB, true> : attn_bwd_narrow_kernel<DP, NB, false>;
     const cudaError_t e = opt_in_smem(kern, Sh::SMEM);
     if (e != cudaSuccess) return e;
     kern<<<dim3((a.Tk + NA_ROWS - 1) / NA_ROWS, a.KV, a.B), Sh::WARPS * 32, Sh::SMEM, st>>>(a, m);
