@@ -99,7 +99,7 @@ cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, c
 
 // bf16 with a window of up to NARROW_WINDOW tokens, as many queries as keys and no prefix: kernels of their own, whose backward needs
 // nothing of the forward
-constexpr int NARROW_WINDOW = 33;
+constexpr int NARROW_WINDOW = 65;
 bool attn_narrow(const AttnArgs& a);
 cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st);
 cudaError_t run_attn_bwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv,

@@ -365,6 +365,11 @@ template <int DP, bool CAP, bool BIAS>
 static cudaError_t bwd_tensor(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const void* rest, const float* lse,
                               const void* dout, float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
     typedef BwdShape<DP> Sh;
+    auto rows_q = attn_bwd_tensor_kernel<DP, false, CAP, BIAS>;
+    auto rows_k = attn_bwd_tensor_kernel<DP, true, CAP, BIAS>;
+    cudaError_t e = opt_in_smem(rows_q, Sh::SMEM);       // before the maps: a thread's first runtime call makes the context current for them
+    if (e == cudaSuccess) e = opt_in_smem(rows_k, Sh::SMEM);
+    if (e != cudaSuccess) return e;
     const long long os[3] = {(long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D}, gs[3] = {(long long)a.Tk * a.KV * a.D, (long long)a.KV * a.D, a.D};
     BwdMaps mq, mk;
     if (!tile_map(&mq.x0, q, a.B, a.Tq, a.H, a.D, a.qs, 128) || !tile_map(&mq.x1, dout, a.B, a.Tq, a.H, a.D, os, 128) ||
@@ -376,11 +381,6 @@ static cudaError_t bwd_tensor(const AttnArgs& a, const void* q, const void* k, c
         !tile_map(&mk.y0, q, a.B, a.Tq, a.H, a.D, a.qs, AB_N) || !tile_map(&mk.y1, dout, a.B, a.Tq, a.H, a.D, os, AB_N) ||
         !tile_map(&mk.d0, dv, a.B, a.Tk, a.KV, a.D, gs, 128) || !tile_map(&mk.d1, dk, a.B, a.Tk, a.KV, a.D, gs, 128))
         return cudaErrorInvalidValue;
-    auto rows_q = attn_bwd_tensor_kernel<DP, false, CAP, BIAS>;
-    auto rows_k = attn_bwd_tensor_kernel<DP, true, CAP, BIAS>;
-    cudaError_t e = opt_in_smem(rows_q, Sh::SMEM);
-    if (e == cudaSuccess) e = opt_in_smem(rows_k, Sh::SMEM);
-    if (e != cudaSuccess) return e;
     const int tq = (a.Tq + 127) / 128, tk = (a.Tk + 127) / 128;
     const long long cq = (long long)tq * a.H * a.B, ck = (long long)tk * a.KV * a.B;
     if (cq > 0x7fffffffll || ck > 0x7fffffffll) return cudaErrorInvalidValue;

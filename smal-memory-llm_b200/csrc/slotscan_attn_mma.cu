@@ -314,15 +314,15 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
 template <int DP, int NT, int KT, bool CAP, bool BIAS>
 static cudaError_t fwd_tensor(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st) {
     typedef FwdShape<DP, NT, KT> Sh;
+    auto kern = attn_fwd_tensor_kernel<DP, NT, KT, CAP, BIAS>;
+    const cudaError_t e = opt_in_smem(kern, Sh::SMEM);   // before the maps: a thread's first runtime call makes the context current for them
+    if (e != cudaSuccess) return e;
     FwdMaps maps;
     const long long os[3] = {(long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D};
     if (!tile_map(&maps.q, q, a.B, a.Tq, a.H, a.D, a.qs, 128) || !tile_map(&maps.k, k, a.B, a.Tk, a.KV, a.D, a.ks, KT) ||
         !tile_map(&maps.v, v, a.B, a.Tk, a.KV, a.D, a.vs, KT) || !tile_map(&maps.o, o, a.B, a.Tq, a.H, a.D, os, 128) ||
         !tile_map(&maps.rest, lse != nullptr ? rest : o, a.B, a.Tq, a.H, a.D, os, 128))
         return cudaErrorInvalidValue;
-    auto kern = attn_fwd_tensor_kernel<DP, NT, KT, CAP, BIAS>;
-    const cudaError_t e = opt_in_smem(kern, Sh::SMEM);
-    if (e != cudaSuccess) return e;
     const int tiles = (a.Tq + NT * 128 - 1) / (NT * 128);
     const long long ctas = (long long)tiles * a.H * a.B;
     if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;

@@ -206,7 +206,7 @@ struct NarrowBwd {
 // GROUP: several query heads share a key head, whose dk and dv stay in registers over them; one CTA to an SM.  Without, dv is done before dk is
 // begun, and two CTAs fit (286 against @@ONE@@ us for 64 x 1,024 tokens, window 16).
 template <int DP, int NB, bool GROUP>
-__global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP ? 1 : 2) attn_bwd_narrow_kernel(AttnArgs a, const __grid_constant__ NarrowBwdMaps maps) {
+__global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3 ? 1 : 2) attn_bwd_narrow_kernel(AttnArgs a, const __grid_constant__ NarrowBwdMaps maps) {
     typedef NarrowBwd<DP, NB> Sh;
     constexpr int HB = Sh::HB, SUBS = DP / 64;
     extern __shared__ __align__(1024) char smem[];
@@ -370,13 +370,13 @@ template <int DP, int NB>
 static cudaError_t fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st) {
     constexpr int KEYS = NA_ROWS + 16 * (NB - 1), SMEM = (NA_ROWS + 2 * KEYS) * DP * 2;
     const long long os[3] = {(long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D};
+    auto kern = attn_fwd_narrow_kernel<DP, NB>;
+    const cudaError_t e = opt_in_smem(kern, SMEM);       // before the maps: a thread's first runtime call makes the context current for them
+    if (e != cudaSuccess) return e;
     NarrowMaps m;
     if (!tile_map(&m.q, q, a.B, a.Tq, a.H, a.D, a.qs, NA_ROWS) || !tile_map(&m.k, k, a.B, a.Tk, a.KV, a.D, a.ks, KEYS) ||
         !tile_map(&m.v, v, a.B, a.Tk, a.KV, a.D, a.vs, KEYS) || !tile_map(&m.o, o, a.B, a.Tq, a.H, a.D, os, 16))
         return cudaErrorInvalidValue;
-    auto kern = attn_fwd_narrow_kernel<DP, NB>;
-    const cudaError_t e = opt_in_smem(kern, SMEM);
-    if (e != cudaSuccess) return e;
     kern<<<dim3((a.Tq + NA_ROWS - 1) / NA_ROWS, a.H, a.B), 128, SMEM, st>>>(a, m);
     return cudaGetLastError();
 }
@@ -384,15 +384,15 @@ template <int DP, int NB>
 static cudaError_t bwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv, cudaStream_t st) {
     typedef NarrowBwd<DP, NB> Sh;
     const long long os[3] = {(long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D}, gs[3] = {(long long)a.Tk * a.KV * a.D, (long long)a.KV * a.D, a.D};
+    auto kern = a.H > a.KV ? attn_bwd_narrow_kernel<DP, NB, true> : attn_bwd_narrow_kernel<DP, NB, false>;
+    const cudaError_t e = opt_in_smem(kern, Sh::SMEM);      // before the maps
+    if (e != cudaSuccess) return e;
     NarrowBwdMaps m;
     if (!tile_map(&m.q, q, a.B, a.Tq, a.H, a.D, a.qs, Sh::QROWS) || !tile_map(&m.d, dout, a.B, a.Tq, a.H, a.D, os, Sh::QROWS) ||
         !tile_map(&m.k, k, a.B, a.Tk, a.KV, a.D, a.ks, Sh::KROWS) || !tile_map(&m.v, v, a.B, a.Tk, a.KV, a.D, a.vs, Sh::KROWS) ||
         !tile_map(&m.dq, dq, a.B, a.Tq, a.H, a.D, os, 16) || !tile_map(&m.dk, dk, a.B, a.Tk, a.KV, a.D, gs, 16) ||
         !tile_map(&m.dv, dv, a.B, a.Tk, a.KV, a.D, gs, 16))
         return cudaErrorInvalidValue;
-    auto kern = a.H > a.KV ? attn_bwd_narrow_kernel<DP, NB, true> : attn_bwd_narrow_kernel<DP, NB, false>;
-    const cudaError_t e = opt_in_smem(kern, Sh::SMEM);
-    if (e != cudaSuccess) return e;
     kern<<<dim3((a.Tk + NA_ROWS - 1) / NA_ROWS, a.KV, a.B), Sh::WARPS * 32, Sh::SMEM, st>>>(a, m);
     return cudaGetLastError();
 }
@@ -401,12 +401,14 @@ bool attn_narrow(const AttnArgs& a) { return a.prefix == nullptr && a.Tq == a.Tk
 
 cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st) {
     if (a.window <= 17) return a.D <= 64 ? fwd_narrow<64, 2>(a, q, k, v, o, st) : fwd_narrow<128, 2>(a, q, k, v, o, st);
-    return a.D <= 64 ? fwd_narrow<64, 3>(a, q, k, v, o, st) : fwd_narrow<128, 3>(a, q, k, v, o, st);
+    if (a.window <= 33) return a.D <= 64 ? fwd_narrow<64, 3>(a, q, k, v, o, st) : fwd_narrow<128, 3>(a, q, k, v, o, st);
+    return a.D <= 64 ? fwd_narrow<64, 5>(a, q, k, v, o, st) : fwd_narrow<128, 5>(a, q, k, v, o, st);
 }
 cudaError_t run_attn_bwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv,
                                 cudaStream_t st) {
     if (a.window <= 17) return a.D <= 64 ? bwd_narrow<64, 2>(a, q, k, v, dout, dq, dk, dv, st) : bwd_narrow<128, 2>(a, q, k, v, dout, dq, dk, dv, st);
-    return a.D <= 64 ? bwd_narrow<64, 3>(a, q, k, v, dout, dq, dk, dv, st) : bwd_narrow<128, 3>(a, q, k, v, dout, dq, dk, dv, st);
+    if (a.window <= 33) return a.D <= 64 ? bwd_narrow<64, 3>(a, q, k, v, dout, dq, dk, dv, st) : bwd_narrow<128, 3>(a, q, k, v, dout, dq, dk, dv, st);
+    return a.D <= 64 ? bwd_narrow<64, 5>(a, q, k, v, dout, dq, dk, dv, st) : bwd_narrow<128, 5>(a, q, k, v, dout, dq, dk, dv, st);
 }
 
 int attn_narrow_status() {

@@ -436,6 +436,35 @@ def test_another_stream_and_copied_layouts():
     assert torch.equal(S.token_attention(q, one, one), S.token_attention(q, one.contiguous(), one.contiguous()))
 
 
+@pytest.mark.parametrize("window", [0, 16])
+def test_first_call_of_a_thread(window):
+    """A thread that has made no CUDA call before (as the worker of a backward) gets the same bits."""
+    import threading
+    S = _S()
+    g, q, k, v, do = _attn_inputs("bf16", 1, 150, 150, 2, 1, 128, seed=25)
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = S.token_attention(*x, window=window)
+    want = (o, *torch.autograd.grad(o, x, do))
+    got = []
+
+    def work():
+        from slotscan_b200 import tokens
+        out = tokens._attn_fwd(q, k, v, None, None, None, window, 0.0, 128 ** -0.5, True)
+        got.append(out[0])
+
+    def back():
+        from slotscan_b200 import tokens
+        out = tokens._attn_fwd(q, k, v, None, None, None, window, 0.0, 128 ** -0.5, True)
+        again = threading.Thread(target=lambda: got.extend(tokens._attn_bwd(q, k, v, None, None, None, *out, do, window, 0.0, 128 ** -0.5)))
+        again.start()
+        again.join()
+    for f in (work, back):
+        t = threading.Thread(target=f)
+        t.start()
+        t.join()
+    assert len(got) == 4 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_registered_ops_give_the_same():
     """Under a profiler the registered ops run instead of the plain calls; batched gradients take their backward."""
     from torch.profiler import ProfilerActivity, profile
