@@ -56,6 +56,20 @@ __device__ __forceinline__ void tile_span_add(TileSpan* s, Span r, bool counts) 
     }
 }
 
+// spans of the 32 rows of a warp: which of its blocks of 32 columns are hidden from all of them, and which are seen whole by all
+struct WarpSpan {
+    int lo_min, lo_max, hi_min, hi_max;
+    __device__ __forceinline__ explicit WarpSpan(Span r) {
+        const bool some = r.hi > r.lo;
+        lo_min = __reduce_min_sync(FULL, some ? r.lo : BIGI);
+        lo_max = __reduce_max_sync(FULL, some ? r.lo : BIGI);
+        hi_min = __reduce_min_sync(FULL, some ? r.hi : 0);
+        hi_max = __reduce_max_sync(FULL, some ? r.hi : 0);
+    }
+    __device__ __forceinline__ bool dead(int j) const { return j + 32 <= lo_min || j >= hi_max; }
+    __device__ __forceinline__ bool clear(int j, int n = 32) const { return j >= lo_max && j + n <= hi_min; }
+};
+
 // a score as the base-2 exponent of its weight, before the softmax's shift.  Of the cap, t = tanh(scale <q, k> / cap), whose
 // derivative is 1 - t^2.
 struct Score {

@@ -1,11 +1,13 @@
 // Attention over tokens on the tensor cores, bf16: forward.
 //
-// A CTA holds NT tiles of 128 queries of a head, passes over their keys KT at a time, and keeps scores and outputs in tensor memory.
+// A CTA holds two tiles of 128 queries of a head, passes over their keys 128 at a time, and keeps scores and outputs in tensor
+// memory (two of each fill its 512 columns).
 //   copy warp    tiles of q once, then k, v, k, v, ... through a ring of stages
-//   product warp one thread: s = q k^T into columns S, o += p v with p read from the same columns
+//   product warp s = q k^T into columns S, o += p v with p read from the same columns
 //   128 threads to a query tile: a thread owns a row, so maximum and sum of its softmax need no other lane.  It reads its scores,
 //                writes the weights p (bf16) over them, and hands them to the product warp
-// With NT = 2 the products of one tile run while the other tile's weights are formed.  The outputs are rescaled in place, and only
+// The products of one tile run while the other tile's weights are formed.  (One tile to a CTA, two CTAs to an SM: 597 us against
+// 375 for one sequence of 16,384, and no better for short ones.)  The outputs are rescaled in place, and only
 // when a row's maximum has grown by more than 2^8: until then the weights are taken relative to the old one, which
 // float32 sums and the relative precision of bf16 bear.
 // p is rounded to bf16 for its product, as its operand type asks; the sum of the softmax takes it unrounded.
@@ -20,15 +22,16 @@ namespace slotscan {
 static __device__ int g_attn_status = 0;                 // a bounded wait gave up (slotscan_device_status)
 
 constexpr float GROWN = 8.f;                             // in powers of two
+constexpr int NT = 2;                                    // tiles of 128 queries of a CTA
+constexpr int KT = 128;                                  // keys of a tile
 
-template <int DP, int NT, int KT>
+template <int DP>
 struct FwdShape {
-    static constexpr int STAGES = 4;
+    static constexpr int STAGES = 4;                     // tiles of the ring, keys and values in turn
     static constexpr int SUBS = DP / 64;                 // 64-column sub-tiles of a tile
     static constexpr int QTILE = 128 * DP * 2, KTILE = KT * DP * 2;                // bytes
     static constexpr int THREADS = NT * 128 + 128;
     static constexpr int SMEM = NT * QTILE + STAGES * KTILE + 1024;
-    static constexpr int COLUMNS = NT * (KT + DP) <= 256 ? 256 : 512;
 };
 struct FwdMaps { CUtensorMap q, k, v, o, rest; };
 
@@ -72,10 +75,10 @@ __device__ __forceinline__ void scores32(float (&s)[32], const Score& sc, float 
     }
 }
 
-template <int DP, int NT, int KT, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NT * 128 + 128, NT == 1 ? 2 : 1)
+template <int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(NT * 128 + 128, 1)
 attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* lse, int tiles, int tile_major) {
-    typedef FwdShape<DP, NT, KT> Sh;
+    typedef FwdShape<DP> Sh;
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     char* Qs = smem;
@@ -99,7 +102,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
         mbar_fence_init();
         s_fail = 0;
     }
-    if (warp == NT * 4) tmem_alloc(&s_tmem, Sh::COLUMNS);
+    if (warp == NT * 4) tmem_alloc(&s_tmem, 512);
     __syncthreads();
     const int my_t = tid / 128, row = i0 + tid;          // of the softmax threads
     Span sp = {0, 0};
@@ -110,7 +113,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = Sh::COLUMNS == 512 ? 0 : s_tmem;   // all 512 columns begin at the first
+    constexpr uint32_t tmem = 0;                         // all 512 columns are this CTA's, so they begin at the first
     int first[NT], last[NT], n0 = BIGI, n1 = 0;          // key tiles of each query tile, and of all
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -119,12 +122,12 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
         last[t] = s.hi_max > 0 ? (s.hi_max + KT - 1) / KT : 0;
         if (last[t] > first[t]) { n0 = min(n0, first[t]); n1 = max(n1, last[t]); }
     }
-    // NT = 2: 3 x 128 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72; a row of 128 scores stays in registers
+    // 3 x 128 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72; a row of 128 scores stays in registers
     if (warp < NT * 4) {                                 // ---- softmax of a tile ----
-        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int t = my_t;
         const int f0 = t == 0 ? first[0] : first[NT - 1], l0 = t == 0 ? last[0] : last[NT - 1];
-        const TileSpan ts = s_span[t];
+        const WarpSpan ws(sp);
         const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
         const uint32_t S = tmem + t * KT + lane_at, O = tmem + NT * KT + t * DP + lane_at;
         const Score sc(a, h);
@@ -133,8 +136,8 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
         bool ok = true;
         for (int n = f0; n < l0; n++) {
             const int j0 = n * KT;
-            const bool masked = j0 < ts.lo_max || j0 + KT > ts.hi_min;
-            if (!(ok = __all_sync(FULL, wait_soon(&s_full[t], (n - f0) & 1)))) break;
+            const bool masked = !ws.clear(j0, KT);
+            if (!(ok = wait_soon_warp(&s_full[t], (n - f0) & 1))) break;
             tmem_fence_after();
             uint32_t raw[KT / 32][32];
 #pragma unroll
@@ -151,11 +154,13 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                 top = fmaxf(top, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
             }
             if constexpr (!CAP && !BIAS) top *= sc.lin;
-            const bool grown = top > m + GROWN || (m == -INFINITY && top > m);
+            // a row that has seen nothing so far has only zeros to rescale
+            const bool grown = top > m + GROWN && m != -INFINITY;
+            if (m == -INFINITY) m = top;
             if (__any_sync(FULL, grown)) {
                 const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_fast(m - to);
                 if (n > f0) {
-                    if (!(ok = __all_sync(FULL, wait_soon(&o_full[t], (n - f0 - 1) & 1)))) break;
+                    if (!(ok = wait_soon_warp(&o_full[t], (n - f0 - 1) & 1))) break;
                     tmem_fence_after();
 #pragma unroll
                     for (int c = 0; c < DP / 32; c++) {
@@ -234,7 +239,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
             lse[((size_t)b * a.H + h) * a.Tq + row] = none ? -INFINITY : sp.hi - sp.lo == 1 ? INFINITY : m + log2f(l);
         if (r == 0) bulk_wait_read<0>();
     } else {
-        if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == NT * 4 + 1) {                            // ---- copies ----
             if (lane == 0 && n0 < n1) {
                 bool ok = true;
@@ -308,13 +313,13 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
         if (tid == 0) atomicExch(&g_attn_status, 1);
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
     }
-    if (warp == NT * 4) { tmem_fence_after(); tmem_free(s_tmem, Sh::COLUMNS); }
+    if (warp == NT * 4) { tmem_fence_after(); tmem_free(s_tmem, 512); }
 }
 
-template <int DP, int NT, int KT, bool CAP, bool BIAS>
+template <int DP, bool CAP, bool BIAS>
 static cudaError_t fwd_tensor(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st) {
-    typedef FwdShape<DP, NT, KT> Sh;
-    auto kern = attn_fwd_tensor_kernel<DP, NT, KT, CAP, BIAS>;
+    typedef FwdShape<DP> Sh;
+    auto kern = attn_fwd_tensor_kernel<DP, CAP, BIAS>;
     const cudaError_t e = opt_in_smem(kern, Sh::SMEM);   // before the maps: a thread's first runtime call makes the context current for them
     if (e != cudaSuccess) return e;
     FwdMaps maps;
@@ -329,16 +334,16 @@ static cudaError_t fwd_tensor(const AttnArgs& a, const void* q, const void* k, c
     kern<<<(unsigned)ctas, Sh::THREADS, Sh::SMEM, st>>>(a, maps, lse, tiles, ctas < 148 * 8);
     return cudaGetLastError();
 }
-template <int DP, int NT, int KT>
+template <int DP>
 static cudaError_t fwd_tensor_score(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st) {
-    if (a.cap > 0.f) return a.slopes != nullptr ? fwd_tensor<DP, NT, KT, true, true>(a, q, k, v, o, rest, lse, st)
-                                                : fwd_tensor<DP, NT, KT, true, false>(a, q, k, v, o, rest, lse, st);
-    return a.slopes != nullptr ? fwd_tensor<DP, NT, KT, false, true>(a, q, k, v, o, rest, lse, st)
-                               : fwd_tensor<DP, NT, KT, false, false>(a, q, k, v, o, rest, lse, st);
+    if (a.cap > 0.f) return a.slopes != nullptr ? fwd_tensor<DP, true, true>(a, q, k, v, o, rest, lse, st)
+                                                : fwd_tensor<DP, true, false>(a, q, k, v, o, rest, lse, st);
+    return a.slopes != nullptr ? fwd_tensor<DP, false, true>(a, q, k, v, o, rest, lse, st)
+                               : fwd_tensor<DP, false, false>(a, q, k, v, o, rest, lse, st);
 }
 
 cudaError_t run_attn_fwd_bf16(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st) {
-    return a.D <= 64 ? fwd_tensor_score<64, 2, 128>(a, q, k, v, o, rest, lse, st) : fwd_tensor_score<128, 2, 128>(a, q, k, v, o, rest, lse, st);
+    return a.D <= 64 ? fwd_tensor_score<64>(a, q, k, v, o, rest, lse, st) : fwd_tensor_score<128>(a, q, k, v, o, rest, lse, st);
 }
 
 int attn_mma_status() {
