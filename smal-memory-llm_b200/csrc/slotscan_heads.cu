@@ -84,16 +84,22 @@ template <typename T, int LPG, bool CACHE>
 __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
     const int c = threadIdx.x % LPG;
-    const long long unit = (long long)blockIdx.x * (NR_THREADS / LPG) + threadIdx.x / LPG;
-    const long long tok = unit / a.slices;
+    const unsigned unit = blockIdx.x * (NR_THREADS / LPG) + threadIdx.x / LPG, tok = unit / a.slices;            // fewer than 2^31
     const int h0 = (int)(unit % a.slices) * a.per_slice, all = a.H + a.KV + (CACHE ? a.KV : 0);
     const bool live = tok < a.tokens && c * 8 < a.D;
-    const long long b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
+    const unsigned b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
     const long long at = CACHE ? (long long)a.pos[b] + t : a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t;
+    const T* qt = q + b * a.qs[0] + t * a.qs[1] + c * 8;                           // of the token
+    const T* kt = k + b * a.ks[0] + t * a.ks[1] + c * 8;
+    const T* vt = CACHE ? v + b * ap.vs[0] + t * ap.vs[1] + c * 8 : nullptr;
+    T* qot = qo + (size_t)tok * a.H * a.D + c * 8;
     const int half = a.R / 16;
     float cs[8], sn[8], w[8];
     if (half) load_turn(a, at, half, c, cs, sn);
-    const long long row = CACHE && at >= 0 ? at % ap.L : 0;
+    const long long row = CACHE && at >= 0 ? (unsigned)at % (unsigned)ap.L : 0;
+    T* kot = CACHE ? kc + b * ap.kcs[0] + row * ap.kcs[1] + c * 8 : ko + (size_t)tok * a.KV * a.D + c * 8;
+    T* vot = CACHE ? vc + b * ap.vcs[0] + row * ap.vcs[1] + c * 8 : nullptr;
+    const long long kos = CACHE ? ap.kcs[2] : a.D;
     const float inv_d = 1.f / a.D;
     constexpr int U = sizeof(T) == 2 ? 6 : 4;            // rows in flight to a group
     for (int u0 = 0; u0 < a.per_slice; u0 += U) {
@@ -101,10 +107,8 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, Ap
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int h = h0 + u0 + u;
-            const T* from = h < a.H ? q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2]
-                            : !CACHE || h < a.H + a.KV ? k + b * a.ks[0] + t * a.ks[1] + (h - a.H) * a.ks[2]
-                                                       : v + b * ap.vs[0] + t * ap.vs[1] + (h - a.H - a.KV) * ap.vs[2];
-            in[u] = raw8(from + c * 8, live && u0 + u < a.per_slice && h < all);
+            const T* from = h < a.H ? qt + h * a.qs[2] : !CACHE || h < a.H + a.KV ? kt + (h - a.H) * a.ks[2] : vt + (h - a.H - a.KV) * ap.vs[2];
+            in[u] = raw8(from, live && u0 + u < a.per_slice && h < all);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -126,11 +130,10 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, Ap
             for (int i = 0; i < 8; i++) y[i] = x[i] * r * w[i];
             if (half) turn<1>(y, cs, sn, half, c, LPG);
             if (!live || h >= all) continue;
-            if (is_q) st8(qo + (tok * a.H + h) * a.D + c * 8, y);
-            else if constexpr (!CACHE) st8(ko + (tok * a.KV + (h - a.H)) * a.D + c * 8, y);
-            else if (at >= 0) {
-                if (!is_v) st8(kc + b * ap.kcs[0] + row * ap.kcs[1] + (h - a.H) * ap.kcs[2] + c * 8, y);
-                else st8(vc + b * ap.vcs[0] + row * ap.vcs[1] + (h - a.H - a.KV) * ap.vcs[2] + c * 8, x);
+            if (is_q) st8(qot + h * a.D, y);
+            else if (!CACHE || at >= 0) {
+                if (!is_v) st8(kot + (h - a.H) * kos, y);
+                else st8(vot + (h - a.H - a.KV) * ap.vcs[2], x);
             }
         }
     }
@@ -148,12 +151,15 @@ __global__ void __launch_bounds__(NR_THREADS, 2) norm_rope_bwd_kernel(NormArgs a
     float w[8], acc[2][8];
 #pragma unroll
     for (int i = 0; i < 8; i++) acc[0][i] = acc[1][i] = 0.f;
-    const long long units = a.tokens * a.slices;
-    for (long long u0 = (long long)blockIdx.x * GROUPS; u0 < units; u0 += (long long)gridDim.x * GROUPS) {
-        const long long unit = u0 + grp, tok = unit / a.slices;
+    const unsigned units = (unsigned)a.tokens * a.slices;                          // fewer than 2^31
+    for (unsigned u0 = blockIdx.x * GROUPS; u0 < units; u0 += gridDim.x * GROUPS) {
+        const unsigned unit = u0 + grp, tok = unit / a.slices;
         const int h0 = (int)(unit % a.slices) * a.per_slice;
         const bool live = unit < units && c * 8 < a.D;
-        const long long b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
+        const unsigned b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
+        const T* qt = q + b * a.qs[0] + t * a.qs[1] + c * 8;                       // of the token
+        const T* kt = k + b * a.ks[0] + t * a.ks[1] + c * 8;
+        const size_t qo = (size_t)tok * a.H * a.D + c * 8, ko = (size_t)tok * a.KV * a.D + c * 8;
         float cs[8], sn[8];
         if (half) load_turn(a, a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t, half, c, cs, sn);
         constexpr int U = sizeof(T) == 2 ? 3 : 2;
@@ -163,8 +169,8 @@ __global__ void __launch_bounds__(NR_THREADS, 2) norm_rope_bwd_kernel(NormArgs a
             for (int u = 0; u < U; u++) {
                 const int h = h0 + v0 + u;
                 const bool ok = live && v0 + u < a.per_slice && h < a.H + a.KV;
-                in[u] = raw8((h < a.H ? q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2] : k + b * a.ks[0] + t * a.ks[1] + (h - a.H) * a.ks[2]) + c * 8, ok);
-                up[u] = raw8((h < a.H ? gq + (tok * a.H + h) * a.D : gk + (tok * a.KV + (h - a.H)) * a.D) + c * 8, ok);
+                in[u] = raw8(h < a.H ? qt + h * a.qs[2] : kt + (h - a.H) * a.ks[2], ok);
+                up[u] = raw8(h < a.H ? gq + qo + h * a.D : gk + ko + (h - a.H) * a.D, ok);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -196,8 +202,8 @@ __global__ void __launch_bounds__(NR_THREADS, 2) norm_rope_bwd_kernel(NormArgs a
                     const float gx = g[i] * x[i] * r;
                     if (is_q) acc[0][i] += gx; else acc[1][i] += gx;
                 }
-                if (is_q) st8(dq + (tok * a.H + h) * a.D + c * 8, dx);
-                else st8(dk + (tok * a.KV + (h - a.H)) * a.D + c * 8, dx);
+                if (is_q) st8(dq + qo + h * a.D, dx);
+                else st8(dk + ko + (h - a.H) * a.D, dx);
             }
         }
     }
@@ -225,6 +231,7 @@ __global__ void norm_rope_weights_kernel(const float* part, int ctas, int D, flo
     if (lane == 0) (d < D ? dqw : dkw)[d < D ? d : d - D] = s;
 }
 
+static int lanes_of(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 static NormArgs norm_args(const slotscan_norm_params& p, const float* table, const int32_t* pos, const float* qw, const float* kw, int heads) {
     NormArgs a;
     a.T = p.T; a.H = p.H; a.KV = p.KV; a.D = p.D; a.R = p.R; a.table_len = p.table_len;
@@ -232,12 +239,13 @@ static NormArgs norm_args(const slotscan_norm_params& p, const float* table, con
     a.eps = p.eps;
     for (int i = 0; i < 3; i++) { a.qs[i] = p.q_stride[i]; a.ks[i] = p.k_stride[i]; }
     a.table = table; a.pos = pos; a.qw = qw; a.kw = kw;
-    // a group to a row while the rows leave lanes idle, whole tokens beyond, so that a token's table is read once
-    a.per_slice = a.tokens * heads <= 148 * 64 ? 1 : heads;
+    // fewer heads to a group while the groups would leave SMs idle (three CTAs each, two rounds); whole tokens beyond, whose table is
+    // then read once
+    const long long groups = 148ll * 6 * NR_THREADS / lanes_of(p.D), want = (a.tokens * heads + groups - 1) / groups;
+    a.per_slice = (int)(want < 1 ? 1 : want > heads ? heads : want);
     a.slices = (heads + a.per_slice - 1) / a.per_slice;
     return a;
 }
-static int lanes_of(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 static int bwd_ctas(const NormArgs& a) {
     const long long want = (a.tokens * a.slices + NR_THREADS / lanes_of(a.D) - 1) / (NR_THREADS / lanes_of(a.D));
     return (int)(want < NR_MAX_CTAS ? want : NR_MAX_CTAS);
@@ -285,7 +293,7 @@ extern "C" int slotscan_norm_rope_check(const slotscan_norm_params* p) {
     if (p->B < 0 || p->T < 0 || p->H < 1 || p->KV < 1 || p->D < 8 || p->D > 256 || p->D % 8 || p->R < 0 || p->R > p->D || p->R % 16 ||
         (p->R && p->table_len < 1))
         return SLOTSCAN_E_SHAPE;
-    if ((int64_t)p->B * p->T > (1ll << 31) || (int64_t)p->B * p->T * ((int64_t)p->H + 2ll * p->KV) > (1ll << 33)) return SLOTSCAN_E_SHAPE;
+    if ((int64_t)p->B * p->T >= (1ll << 31) || (int64_t)p->B * p->T * ((int64_t)p->H + 2ll * p->KV) > (1ll << 33)) return SLOTSCAN_E_SHAPE;
     if (!strides16(p->q_stride, 3, p->dtype) || !strides16(p->k_stride, 3, p->dtype)) return SLOTSCAN_E_ALIGN;
     return SLOTSCAN_OK;
 }

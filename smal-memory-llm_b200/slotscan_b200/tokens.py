@@ -345,7 +345,8 @@ def _attn_setup(ctx, inputs, output):
     *ts, ctx.window, ctx.cap, ctx.scale, _ = inputs
     o, lse, rest = output
     ctx.save_for_backward(*ts, o if lse.numel() else lse, lse, rest)
-    ctx.mark_non_differentiable(*output[1:])
+    ctx.mark_non_differentiable(lse, rest)
+    ctx.set_materialize_grads(False)                                   # no zeros for what has no gradient
 
 
 def _attn_backward(ctx, do, _, __, bwd=None):
