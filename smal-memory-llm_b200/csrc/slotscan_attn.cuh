@@ -82,6 +82,147 @@ struct Score {
     }
 };
 
+// base-2 exponent of a score, and 1 - tanh^2 of it
+__device__ __forceinline__ float score2(const Score& sc, float s, int dist, float& slope_of_cap) {
+    if (sc.cap_in != 0.f) {
+        const float t = tanhf(s * sc.cap_in);
+        slope_of_cap = 1.f - t * t;
+        return fmaf(-sc.slope, (float)dist, sc.cap_out * t);
+    }
+    slope_of_cap = 1.f;
+    return fmaf(-sc.slope, (float)dist, s * sc.lin);
+}
+
+// ---- A row at a time, by a warp, over the visible pairs alone ----
+// The tiles' products take hidden keys with weight zero, and zero times infinity or NaN is NaN.  Where a row's result is not finite, it is
+// done anew here: what a row does not see then cannot reach it, and what it sees does.  Costs nothing where all is finite.
+// A lane holds channels lane + 32 c.
+template <typename T>
+struct RowInputs { const T *q, *k, *v, *dout; };         // dout (B,Tq,H,D) contiguous
+
+template <typename T>
+__device__ __forceinline__ void lane_row(float (&x)[4], const T* row, int D) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) { const int d = (threadIdx.x & 31) + 32 * c; x[c] = d < D ? ld1(row + d) : 0.f; }
+}
+__device__ __forceinline__ float lane_dot(const float (&x)[4], const float (&y)[4]) {
+    return warp_sum(fmaf(x[0], y[0], fmaf(x[1], y[1], fmaf(x[2], y[2], x[3] * y[3]))));
+}
+template <typename T>
+__device__ __forceinline__ const T* query_row(const AttnArgs& a, const RowInputs<T>& in, int b, int h, int i) { return in.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2]; }
+template <typename T>
+__device__ __forceinline__ const T* key_row(const AttnArgs& a, const T* k, const long long (&s)[3], int b, int hk, int j) { return k + b * s[0] + j * s[1] + hk * s[2]; }
+template <typename T>
+__device__ __forceinline__ const T* dout_row(const AttnArgs& a, const RowInputs<T>& in, int b, int h, int i) {
+    return in.dout + (((size_t)b * a.Tq + i) * a.H + h) * a.D;
+}
+
+// o of a query, and the base-2 logarithm of its sum; with `dout` also delta = sum p <do, v>
+template <typename T>
+__device__ __forceinline__ void careful_query(const AttnArgs& a, const RowInputs<T>& in, int b, int h, int i, float (&o)[4], float& lse, float& delta) {
+    const Span sp = keys_of(a, b, i);
+    const Score sc(a, h);
+    const int hk = h / (a.H / a.KV), at = i + a.Tk - a.Tq;
+    float q[4], g[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f, d = 0.f, unused;
+    lane_row(q, query_row(a, in, b, h, i), a.D);
+    if (in.dout != nullptr) lane_row(g, dout_row(a, in, b, h, i), a.D);
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] = 0.f;
+    for (int j = sp.lo; j < sp.hi; j++) {
+        float x[4];
+        lane_row(x, key_row(a, in.k, a.ks, b, hk, j), a.D);
+        const float z = score2(sc, lane_dot(q, x), abs(at - j), unused);
+        const float top = fmaxf(m, z), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), p = exp2f(z - base);
+        lane_row(x, key_row(a, in.v, a.vs, b, hk, j), a.D);
+        l = fmaf(l, f, p);
+        d = d * f + (in.dout != nullptr && p != 0.f ? p * lane_dot(g, x) : 0.f);
+        bool gone = true;                                // NaN stays NaN
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            o[c] = p != 0.f ? fmaf(p, x[c], o[c] * f) : o[c] * f;
+            gone = gone && (isnan(o[c]) || (threadIdx.x & 31) + 32 * c >= a.D);
+        }
+        m = top;
+        if (__all_sync(FULL, gone)) break;
+    }
+    const float inv = sp.hi > sp.lo ? 1.f / l : 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] = sp.hi > sp.lo ? o[c] * inv : 0.f;
+    lse = sp.hi - sp.lo == 1 ? INFINITY : m + log2f(l);
+    delta = d * inv;
+}
+// weight and scaled gradient of the score of a visible pair
+__device__ __forceinline__ void careful_pair(const AttnArgs& a, const Score& sc, float s, float dp, int dist, float lse, float delta, float& p, float& ds) {
+    float f;
+    const float z = score2(sc, s, dist, f);
+    const bool alone = lse == INFINITY;
+    p = alone ? 1.f : exp2f(z - lse);
+    ds = alone ? 0.f : p * (dp - delta) * f * a.scale;
+}
+// dq of a query.  lse, delta: of all queries (B,H,Tq), or NULL: formed anew
+template <typename T>
+__device__ __forceinline__ void careful_dq(const AttnArgs& a, const RowInputs<T>& in, const float* lse, const float* delta, int b, int h, int i, float (&dq)[4]) {
+    const Span sp = keys_of(a, b, i);
+    const Score sc(a, h);
+    const int hk = h / (a.H / a.KV), at = i + a.Tk - a.Tq;
+    const size_t row = ((size_t)b * a.H + h) * a.Tq + i;
+    float q[4], g[4], o[4], L = 0.f, dl = 0.f;
+    if (lse != nullptr) { L = lse[row]; dl = delta[row]; }
+    else careful_query(a, in, b, h, i, o, L, dl);
+    lane_row(q, query_row(a, in, b, h, i), a.D);
+    lane_row(g, dout_row(a, in, b, h, i), a.D);
+#pragma unroll
+    for (int c = 0; c < 4; c++) dq[c] = 0.f;
+    for (int j = sp.lo; j < sp.hi; j++) {
+        float k[4], v[4], p, ds;
+        lane_row(k, key_row(a, in.k, a.ks, b, hk, j), a.D);
+        lane_row(v, key_row(a, in.v, a.vs, b, hk, j), a.D);
+        careful_pair(a, sc, lane_dot(q, k), lane_dot(g, v), abs(at - j), L, dl, p, ds);
+        bool gone = true;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if (ds != 0.f) dq[c] = fmaf(ds, k[c], dq[c]);
+            gone = gone && (isnan(dq[c]) || (threadIdx.x & 31) + 32 * c >= a.D);
+        }
+        if (__all_sync(FULL, gone)) break;
+    }
+}
+// dk and dv of a key, over the queries of all heads that share it
+template <typename T>
+__device__ __forceinline__ void careful_dkv(const AttnArgs& a, const RowInputs<T>& in, const float* lse, const float* delta, int b, int hk, int j, float (&dk)[4],
+                                         float (&dv)[4]) {
+    const Span sp = queries_of(a, b, j);
+    const int group = a.H / a.KV;
+    float k[4], v[4];
+    lane_row(k, key_row(a, in.k, a.ks, b, hk, j), a.D);
+    lane_row(v, key_row(a, in.v, a.vs, b, hk, j), a.D);
+#pragma unroll
+    for (int c = 0; c < 4; c++) dk[c] = dv[c] = 0.f;
+    for (int g = 0; g < group; g++) {
+        const int h = hk * group + g;
+        const Score sc(a, h);
+        for (int i = sp.lo; i < sp.hi; i++) {
+            const size_t row = ((size_t)b * a.H + h) * a.Tq + i;
+            float q[4], x[4], o[4], L = 0.f, dl = 0.f, p, ds;
+            if (lse != nullptr) { L = lse[row]; dl = delta[row]; }
+            else careful_query(a, in, b, h, i, o, L, dl);
+            lane_row(q, query_row(a, in, b, h, i), a.D);
+            lane_row(x, dout_row(a, in, b, h, i), a.D);
+            careful_pair(a, sc, lane_dot(q, k), lane_dot(x, v), abs(i + a.Tk - a.Tq - j), L, dl, p, ds);
+            bool gone = true;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (ds != 0.f) dk[c] = fmaf(ds, q[c], dk[c]);
+                if (p != 0.f) dv[c] = fmaf(p, x[c], dv[c]);
+                gone = gone && ((isnan(dk[c]) && isnan(dv[c])) || (threadIdx.x & 31) + 32 * c >= a.D);
+            }
+            if (__all_sync(FULL, gone)) return;
+        }
+    }
+}
+// 0 while all values added are finite, NaN from the first that is not
+__device__ __forceinline__ void watch(float& w, float x) { w = fmaf(x, 0.f, w); }
+
 // The capped score as a polynomial, for |x| <= 1 (x = scale <q, k> / cap): tanh x = x sum_k a_k x^2k, the a_k fitted here for the least
 // greatest error of tanh (iteratively reweighted least squares on Chebyshev nodes): 2.4e-7.  Three and a half instructions a score,
 // two scores to an instruction, where the exponential form takes two of the special function unit's, eight cycles a warp each; a

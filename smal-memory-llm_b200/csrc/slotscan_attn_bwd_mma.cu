@@ -39,7 +39,7 @@ struct BwdMaps { CUtensorMap x0, x1, y0, y1, d0, d1; };
 
 template <int DP, bool KEYS, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(AB_WARPS * 32 + 128, 1)
-attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const bf16* o, const bf16* rest, const float* lse, float* delta, int tiles,
+attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ BwdMaps maps, const bf16* o, const bf16* rest, const float* lse, float* delta, int tiles,
                        int tile_major) {
     typedef BwdShape<DP> Sh;
     extern __shared__ __align__(1024) char smem[];
@@ -162,7 +162,7 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
                 const CapPoly cp(sc);
                 const f32x2 lin = pack2(sc.lin, sc.lin), steep = pack2(-sc.slope, -sc.slope), one = pack2(1.f, 1.f);
                 const float in2 = -1.f / (sc.cap_out * sc.cap_out);
-                uint32_t wp[16];
+                [[maybe_unused]] uint32_t wp[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                     float L[2] = {my_lse, my_lse};
@@ -249,16 +249,33 @@ attn_bwd_tensor_kernel(AttnArgs a, const __grid_constant__ BwdMaps maps, const b
         const float mul = KEYS && cg == 0 ? 1.f : a.scale;
         char* out = KEYS && cg == 1 ? X1 : X0;
         if (mine) {
+            float seen = 0.f;
             for (int c = c0 * 2; c < c1 * 2; c++) {
                 uint32_t x[32];
                 if (steps > 0) { tmem_ld(from + c * 32, x); tmem_ld_wait(x); }
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     uint32_t y[4];
+                    if (steps > 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) watch(seen, __uint_as_float(x[i + e]));
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         y[e] = steps > 0 ? pack_bf16(__uint_as_float(x[i + 2 * e]) * mul, __uint_as_float(x[i + 2 * e + 1]) * mul) : 0u;
                     *reinterpret_cast<uint4*>(out + (c / 2) * 128 * 128 + swizzled(r, (c % 2) * 4 + i / 8)) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            for (unsigned bad = __ballot_sync(FULL, seen != seen && row < rows); bad != 0; bad &= bad - 1) {
+                const int n = __ffs(bad) - 1, nr = r - lane + n;
+                float x[4], y[4];
+                if constexpr (KEYS) careful_dkv(a, in, lse, delta, b, hx, row - lane + n, x, y);
+                else careful_dq(a, in, lse, delta, b, hx, row - lane + n, x);
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    const int d = lane + 32 * c;
+                    if (d / 64 >= c0 && d / 64 < c1)
+                        *reinterpret_cast<bf16*>(out + (d / 64) * 128 * 128 + swizzled(nr, d % 64 / 8) + d % 8 * 2) = __float2bfloat16_rn(KEYS && cg == 0 ? y[c] : x[c]);
                 }
             }
             fence_proxy_async_smem();
@@ -381,11 +398,12 @@ static cudaError_t bwd_tensor(const AttnArgs& a, const void* q, const void* k, c
         !tile_map(&mk.y0, q, a.B, a.Tq, a.H, a.D, a.qs, AB_N) || !tile_map(&mk.y1, dout, a.B, a.Tq, a.H, a.D, os, AB_N) ||
         !tile_map(&mk.d0, dv, a.B, a.Tk, a.KV, a.D, gs, 128) || !tile_map(&mk.d1, dk, a.B, a.Tk, a.KV, a.D, gs, 128))
         return cudaErrorInvalidValue;
+    const RowInputs<bf16> in = {(const bf16*)q, (const bf16*)k, (const bf16*)v, (const bf16*)dout};
     const int tq = (a.Tq + 127) / 128, tk = (a.Tk + 127) / 128;
     const long long cq = (long long)tq * a.H * a.B, ck = (long long)tk * a.KV * a.B;
     if (cq > 0x7fffffffll || ck > 0x7fffffffll) return cudaErrorInvalidValue;
-    rows_q<<<(unsigned)cq, Sh::THREADS, Sh::SMEM, st>>>(a, mq, (const bf16*)o, (const bf16*)rest, lse, delta, tq, cq < 148 * 8);
-    rows_k<<<(unsigned)ck, Sh::THREADS, Sh::SMEM, st>>>(a, mk, nullptr, nullptr, lse, delta, tk, ck < 148 * 8);
+    rows_q<<<(unsigned)cq, Sh::THREADS, Sh::SMEM, st>>>(a, in, mq, (const bf16*)o, (const bf16*)rest, lse, delta, tq, cq < 148 * 8);
+    rows_k<<<(unsigned)ck, Sh::THREADS, Sh::SMEM, st>>>(a, in, mk, nullptr, nullptr, lse, delta, tk, ck < 148 * 8);
     return cudaGetLastError();
 }
 template <int DP>

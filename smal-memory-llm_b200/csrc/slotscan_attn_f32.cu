@@ -75,16 +75,6 @@ __device__ __forceinline__ float max16(float v) {        // over the 16 lanes of
     for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, off));
     return v;
 }
-// base-2 exponent of a score and the factor of its derivative (1 - tanh^2)
-__device__ __forceinline__ float score2(const Score& sc, float s, int dist, float& slope_of_cap) {
-    if (sc.cap_in != 0.f) {
-        const float t = tanhf(s * sc.cap_in);
-        slope_of_cap = 1.f - t * t;
-        return fmaf(-sc.slope, (float)dist, sc.cap_out * t);
-    }
-    slope_of_cap = 1.f;
-    return fmaf(-sc.slope, (float)dist, s * sc.lin);
-}
 // least lo and greatest hi of the CTA's 64 rows (the rows that do not exist have an empty span)
 __device__ __forceinline__ Span cta_span(Span mine, bool counts, int* s_red) {
     if (threadIdx.x == 0) { s_red[0] = BIGI; s_red[1] = 0; }
@@ -92,6 +82,27 @@ __device__ __forceinline__ Span cta_span(Span mine, bool counts, int* s_red) {
     if (counts && mine.hi > mine.lo) { atomicMin(&s_red[0], mine.lo); atomicMax(&s_red[1], mine.hi); }
     __syncthreads();
     return {s_red[0], s_red[1]};
+}
+
+template <typename T>
+__device__ __forceinline__ void put_lane_row(T* row, const float (&x)[4], int D) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) { const int d = (threadIdx.x & 31) + 32 * c; if (d < D) st1(row + d, x[c]); }
+}
+// `again(r)`, by the whole warp, for each of its eight rows r of the CTA whose sums `bad` says not to be finite; after the rows are stored
+template <int N, typename Bad, typename Again>
+__device__ __forceinline__ void again_where_not_finite(const float (&acc)[4][N], Bad bad, Again again) {
+    const int ty = threadIdx.x / 16, warp = threadIdx.x / 32;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        float w = 0.f;
+#pragma unroll
+        for (int c = 0; c < N; c++) watch(w, acc[r][c]);
+        const unsigned hit = __ballot_sync(FULL, bad(4 * ty + r, w));
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+            if (hit >> (16 * half) & 0xffffu) { __syncwarp(); again(4 * (2 * warp + half) + r); }
+    }
 }
 
 template <int DP, typename T>
@@ -172,6 +183,11 @@ __global__ void __launch_bounds__(SA_THREADS) attn_fwd_cores_kernel(AttnArgs a, 
         if (lse != nullptr && tx == 0)
             lse[((size_t)b * a.H + h) * a.Tq + i] = empty ? -INFINITY : sp[r].hi - sp[r].lo == 1 ? INFINITY : m[r] + log2f(l[r]);
     }
+    again_where_not_finite(acc, [&](int r, float w) { return i0 + r < a.Tq && w != w; }, [&](int r) {
+        float x[4], unused0, unused1;
+        careful_query(a, RowInputs<T>{q, k, v, nullptr}, b, h, i0 + r, x, unused0, unused1);
+        put_lane_row(o + (((size_t)b * a.Tq + i0 + r) * a.H + h) * a.D, x, a.D);
+    });
 }
 
 // KEYS: rows of keys (dk, dv); else rows of queries (dq, and delta)
@@ -286,6 +302,19 @@ __global__ void __launch_bounds__(SA_THREADS) attn_bwd_cores_kernel(AttnArgs a, 
             st4(d1 + at + d, make_float4(acc1[r][4 * c] * a.scale, acc1[r][4 * c + 1] * a.scale, acc1[r][4 * c + 2] * a.scale, acc1[r][4 * c + 3] * a.scale));
         }
     }
+    auto again = [&](int r) {
+        const RowInputs<T> in = {q, k, v, dout};
+        const size_t at = (((size_t)b * rows + r0 + r) * (KEYS ? a.KV : a.H) + hx) * a.D;
+        float x[4], y[4];
+        if constexpr (KEYS) {
+            careful_dkv(a, in, lse, delta, b, hx, r0 + r, x, y);
+            put_lane_row(d0 + at, y, a.D);
+        } else careful_dq(a, in, lse, delta, b, hx, r0 + r, x);
+        put_lane_row(d1 + at, x, a.D);
+    };
+    auto bad = [&](int r, float w) { return r0 + r < rows && w != w; };
+    if constexpr (KEYS) again_where_not_finite(acc0, bad, again);
+    again_where_not_finite(acc1, bad, again);
 }
 
 template <int DP, typename T>

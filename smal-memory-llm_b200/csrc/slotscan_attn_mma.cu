@@ -77,7 +77,7 @@ __device__ __forceinline__ void scores32(float (&s)[32], const Score& sc, float 
 
 template <int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(NT * 128 + 128, 1)
-attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* lse, int tiles, int tile_major) {
+attn_fwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ FwdMaps maps, float* lse, int tiles, int tile_major) {
     typedef FwdShape<DP> Sh;
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -212,6 +212,7 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                 if (r == 0) bulk_wait_read<0>();
                 sync_group(1 + t, 128);
             }
+            float seen = 0.f;
 #pragma unroll
             for (int c = 0; c < DP / 32; c++) {
                 uint32_t o[32];
@@ -223,9 +224,22 @@ attn_fwd_tensor_kernel(AttnArgs a, const __grid_constant__ FwdMaps maps, float* 
                     for (int e = 0; e < 4; e++) {
                         const float x = none ? 0.f : __uint_as_float(o[i + 2 * e]) * inv, y = none ? 0.f : __uint_as_float(o[i + 2 * e + 1]) * inv;
                         w[e] = pack_bf16(x, y);
+                        watch(seen, x);
+                        watch(seen, y);
                         if (pass) w[e] = pack_bf16(x - __uint_as_float(w[e] << 16), y - __uint_as_float(w[e] & 0xffff0000u));
                     }
                     *reinterpret_cast<uint4*>(out + (c / 2) * 128 * 128 + swizzled(r, (c % 2) * 4 + i / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            for (unsigned bad = __ballot_sync(FULL, seen != seen && row < a.Tq); bad != 0; bad &= bad - 1) {
+                const int x = __ffs(bad) - 1, xr = r - lane + x;
+                float v[4], unused0, unused1;
+                careful_query(a, in, b, h, row - lane + x, v, unused0, unused1);
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++) {
+                    const bf16 hi = __float2bfloat16_rn(v[c]);
+                    const int d = lane + 32 * c;
+                    *reinterpret_cast<bf16*>(out + (d / 64) * 128 * 128 + swizzled(xr, d % 64 / 8) + d % 8 * 2) = pass ? __float2bfloat16_rn(v[c] - __bfloat162float(hi)) : hi;
                 }
             }
             fence_proxy_async_smem();
@@ -331,7 +345,7 @@ static cudaError_t fwd_tensor(const AttnArgs& a, const void* q, const void* k, c
     const int tiles = (a.Tq + NT * 128 - 1) / (NT * 128);
     const long long ctas = (long long)tiles * a.H * a.B;
     if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
-    kern<<<(unsigned)ctas, Sh::THREADS, Sh::SMEM, st>>>(a, maps, lse, tiles, ctas < 148 * 8);
+    kern<<<(unsigned)ctas, Sh::THREADS, Sh::SMEM, st>>>(a, RowInputs<bf16>{(const bf16*)q, (const bf16*)k, (const bf16*)v, nullptr}, maps, lse, tiles, ctas < 148 * 8);
     return cudaGetLastError();
 }
 template <int DP>

@@ -53,6 +53,12 @@ __device__ __forceinline__ void put_rows(uint32_t tile, int rows, int row0, int 
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(piece_at(tile, rows, row0 + lane / 4 + 8, c) + at), "r"(hi) : "memory");
 }
 
+// a row's channels lane + 32 c
+__device__ __forceinline__ void put_lane_row(bf16* row, const float (&x)[4], int D) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) { const int d = (threadIdx.x & 31) + 32 * c; if (d < D) row[d] = __float2bfloat16_rn(x[c]); }
+}
+
 // 16 x 16 NB scores of a warp's queries (rows `row0` of the tile Q, keys from `key0` of the tile K)
 template <int DP, int NB>
 __device__ __forceinline__ void band(float (&s)[2 * NB][4], uint32_t Q, int q_rows, int row0, uint32_t K, int k_rows, int key0, int lane) {
@@ -132,7 +138,7 @@ __device__ __forceinline__ void give_up() {              // report, and give the
 }
 
 template <int DP, int NB>
-__global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, const __grid_constant__ NarrowMaps maps) {
+__global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, RowInputs<bf16> in, bf16* out, const __grid_constant__ NarrowMaps maps) {
     constexpr int KEYS = NA_ROWS + 16 * (NB - 1), SUBS = DP / 64;
     extern __shared__ __align__(1024) char smem[];
     const uint32_t Q = smem_u32(smem), K = Q + NA_ROWS * DP * 2, V = K + KEYS * DP * 2;
@@ -172,6 +178,7 @@ __global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, const 
         p[n][3] = pack_bf16(s[2 * n + 1][2], s[2 * n + 1][3]);
     }
     __syncwarp();                                        // the warp's queries are read: its outputs go over them
+    float seen = 0.f;
 #pragma unroll
     for (int c = 0; c < DP / 16; c++) {
         float o[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -183,8 +190,11 @@ __global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, const 
             mma(o[1], p[n], y[2], y[3]);
         }
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < 2; t++) {
             put_rows<DP>(Q, NA_ROWS, warp * 16, 2 * c + t, lane, pack_bf16(o[t][0] * inv[0], o[t][1] * inv[0]), pack_bf16(o[t][2] * inv[1], o[t][3] * inv[1]));
+#pragma unroll
+            for (int i = 0; i < 4; i++) watch(seen, o[t][i]);
+        }
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -192,6 +202,15 @@ __global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, const 
         for (int c = 0; c < SUBS; c++) tile_s2g(&maps.o, c * 64, i0 + warp * 16, h, b, smem + c * NA_ROWS * 128 + warp * 16 * 128);
         bulk_commit();
         bulk_wait_read<0>();
+    }
+    if (__any_sync(FULL, seen != seen)) {                // some row is not finite: the warp's rows anew, over what they see alone
+        if (lane == 0) bulk_wait<0>();
+        __syncwarp();
+        for (int i = i0 + warp * 16; i < min(i0 + warp * 16 + 16, a.Tq); i++) {
+            float x[4], unused0, unused1;
+            careful_query(a, in, b, h, i, x, unused0, unused1);
+            put_lane_row(out + (((size_t)b * a.Tq + i) * a.H + h) * a.D, x, a.D);
+        }
     }
 }
 
@@ -206,7 +225,7 @@ struct NarrowBwd {
 // GROUP: several query heads share a key head, whose dk and dv stay in registers over them; one CTA to an SM.  Without, dv is done before dk is
 // begun, and two CTAs fit (286 against @@ONE@@ us for 64 x 1,024 tokens, window 16).
 template <int DP, int NB, bool GROUP>
-__global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3 ? 1 : 2) attn_bwd_narrow_kernel(AttnArgs a, const __grid_constant__ NarrowBwdMaps maps) {
+__global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3 ? 1 : 2) attn_bwd_narrow_kernel(AttnArgs a, RowInputs<bf16> in, bf16* dq_out, bf16* dk_out, bf16* dv_out, const __grid_constant__ NarrowBwdMaps maps) {
     typedef NarrowBwd<DP, NB> Sh;
     constexpr int HB = Sh::HB, SUBS = DP / 64;
     extern __shared__ __align__(1024) char smem[];
@@ -252,12 +271,17 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3
             }
         }
     };
+    float seen_keys = 0.f;                               // NaN where dk or dv is not finite
+    unsigned bad_heads = 0;                              // of the group, whose dq is not: bit 31 for all from the 32nd on
     // dv over v, dk over k, which all have read
     auto put = [&](const float (&x)[DP / 8][4], int which) {
         const float mul = which ? a.scale : 1.f;
 #pragma unroll
-        for (int c = 0; c < DP / 8; c++)
+        for (int c = 0; c < DP / 8; c++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) watch(seen_keys, x[c][i]);
             put_rows<DP>(which ? K : V, Sh::KROWS, warp * 16, c, lane, pack_bf16(x[c][0] * mul, x[c][1] * mul), pack_bf16(x[c][2] * mul, x[c][3] * mul));
+        }
     };
     if constexpr (GROUP) { clear(sums[0]); clear(sums[1]); }
     const uint32_t P = Pm + warp * 2 * Sh::PT, D = P + Sh::PT;
@@ -309,6 +333,7 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3
         }
         // dq = scale ds k, kept packed until k and v are no longer needed as they are
         uint32_t dq[DP / 8][2];
+        float seen = 0.f;
 #pragma unroll
         for (int c = 0; c < DP / 16; c++) {
             float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -321,10 +346,13 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3
             }
 #pragma unroll
             for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) watch(seen, x[t][i]);
                 dq[2 * c + t][0] = pack_bf16(x[t][0] * a.scale, x[t][1] * a.scale);
                 dq[2 * c + t][1] = pack_bf16(x[t][2] * a.scale, x[t][3] * a.scale);
             }
         }
+        if (__any_sync(FULL, seen != seen)) bad_heads |= 1u << min(g, 31);
         __syncthreads();                                 // p and ds of all queries are there
         if (warp < 4) {
 #pragma unroll
@@ -363,6 +391,23 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3
             bulk_commit();
             bulk_wait_read<0>();
         }
+        if (bad_heads != 0 || __any_sync(FULL, seen_keys != seen_keys)) {          // some row is not finite: anew, over what sees what alone
+            const bool keys = __any_sync(FULL, seen_keys != seen_keys);
+            if (lane == 0) bulk_wait<0>();
+            __syncwarp();
+            for (int x = x0 + warp * 16; x < min(x0 + warp * 16 + 16, a.Tk); x++) {
+                float dk[4], dv[4];
+                for (int g = 0; g < group; g++) {
+                    if (!(bad_heads >> min(g, 31) & 1)) continue;
+                    careful_dq(a, in, nullptr, nullptr, b, hk * group + g, x, dk);
+                    put_lane_row(dq_out + (((size_t)b * a.Tq + x) * a.H + hk * group + g) * a.D, dk, a.D);
+                }
+                if (!keys) continue;
+                careful_dkv(a, in, nullptr, nullptr, b, hk, x, dk, dv);
+                put_lane_row(dk_out + (((size_t)b * a.Tk + x) * a.KV + hk) * a.D, dk, a.D);
+                put_lane_row(dv_out + (((size_t)b * a.Tk + x) * a.KV + hk) * a.D, dv, a.D);
+            }
+        }
     }
 }
 
@@ -377,7 +422,7 @@ static cudaError_t fwd_narrow(const AttnArgs& a, const void* q, const void* k, c
     if (!tile_map(&m.q, q, a.B, a.Tq, a.H, a.D, a.qs, NA_ROWS) || !tile_map(&m.k, k, a.B, a.Tk, a.KV, a.D, a.ks, KEYS) ||
         !tile_map(&m.v, v, a.B, a.Tk, a.KV, a.D, a.vs, KEYS) || !tile_map(&m.o, o, a.B, a.Tq, a.H, a.D, os, 16))
         return cudaErrorInvalidValue;
-    kern<<<dim3((a.Tq + NA_ROWS - 1) / NA_ROWS, a.H, a.B), 128, SMEM, st>>>(a, m);
+    kern<<<dim3((a.Tq + NA_ROWS - 1) / NA_ROWS, a.H, a.B), 128, SMEM, st>>>(a, RowInputs<bf16>{(const bf16*)q, (const bf16*)k, (const bf16*)v, nullptr}, (bf16*)o, m);
     return cudaGetLastError();
 }
 template <int DP, int NB>
@@ -393,7 +438,7 @@ static cudaError_t bwd_narrow(const AttnArgs& a, const void* q, const void* k, c
         !tile_map(&m.dq, dq, a.B, a.Tq, a.H, a.D, os, 16) || !tile_map(&m.dk, dk, a.B, a.Tk, a.KV, a.D, gs, 16) ||
         !tile_map(&m.dv, dv, a.B, a.Tk, a.KV, a.D, gs, 16))
         return cudaErrorInvalidValue;
-    kern<<<dim3((a.Tk + NA_ROWS - 1) / NA_ROWS, a.KV, a.B), Sh::WARPS * 32, Sh::SMEM, st>>>(a, m);
+    kern<<<dim3((a.Tk + NA_ROWS - 1) / NA_ROWS, a.KV, a.B), Sh::WARPS * 32, Sh::SMEM, st>>>(a, RowInputs<bf16>{(const bf16*)q, (const bf16*)k, (const bf16*)v, (const bf16*)dout}, (bf16*)dq, (bf16*)dk, (bf16*)dv, m);
     return cudaGetLastError();
 }
 

@@ -12,7 +12,6 @@
 // p is split into two bf16 (p = hi + lo, off by 2^-17): the second product costs nothing here and keeps the float32 weights' precision.
 //
 // float32: the CUDA cores.  A row is read by LPG lanes, 8 channels each, and every group of lanes goes its own way through the split.
-#include <cstdlib>
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_tensor.cuh"
@@ -361,8 +360,9 @@ static StepArgs step_args(const slotscan_attn_step_params& p) {
     for (int i = 0; i < 3; i++) { a.ks[i] = p.k_stride[i]; a.vs[i] = p.v_stride[i]; }
     const int group = p.H / p.KV, G = heads_at_once(group, p.dtype);
     a.chunks = (group + G - 1) / G;
-    // bf16: two CTAs for each SM at a time (their rings), four in turn; float32 eight; 128 rows at least
-    const long long ctas = (long long)p.B * p.KV * a.chunks, want = 148 * (p.dtype == SLOTSCAN_BF16 ? (getenv("SW") ? atoi(getenv("SW")) : 8) : 8);
+    // 128 rows at least; bf16: two CTAs for each SM at a time (their rings), six rounds of them (8 x 131,072 rows: two rounds 384 us, four
+    // 363, six 341, eight 351); float32: eight for each SM
+    const long long ctas = (long long)p.B * p.KV * a.chunks, want = 148 * (p.dtype == SLOTSCAN_BF16 ? 12 : 8);
     long long s = (want + ctas - 1) / (ctas > 0 ? ctas : 1);
     if (s > (a.window + 127) / 128) s = (a.window + 127) / 128;
     a.splits = (int)(s < 1 ? 1 : s > ST_MAX_SPLITS ? ST_MAX_SPLITS : s);

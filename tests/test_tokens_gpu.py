@@ -279,6 +279,41 @@ def test_attention(case, dtype):
     assert all(torch.equal(a, got[n]) for a, n in zip(again, ("dq", "dk", "dv")))
 
 
+@pytest.mark.parametrize("dtype,window,H,KV,D,cap", [("f32", 0, 2, 1, 64, 0.0), ("f32", 16, 2, 2, 96, 5.0), ("bf16", 0, 2, 1, 128, 0.0), ("bf16", 0, 2, 2, 64, 6.0),
+                                                     ("bf16", 16, 2, 2, 128, 0.0), ("bf16", 30, 4, 2, 64, 6.0), ("bf16", 60, 2, 2, 40, 0.0), ("bf16", 200, 2, 2, 128, 0.0)])
+def test_hidden_values_do_not_reach_anything(dtype, window, H, KV, D, cap):
+    """Padding that holds infinities and NaN, in queries, keys, values and upstream gradients, and a token of NaN that only later ones
+    see."""
+    S = _S()
+    B, T = 2, 300
+    g, q, k, v, do = _attn_inputs(dtype, B, T, T, H, KV, D, seed=31)
+    docs = _docs(B, T, 8, 40)
+    docs[:, -7:] = -1
+    pad = docs < 0
+    kw = dict(window=window, cap=cap)
+    ref = _attn_ref(q, k, v, do, window, cap, None, docs, None, dtype)
+    x = [t.clone() for t in (q, k, v, do)]
+    for t, bad in zip(x, (math.nan, math.inf, -math.inf, math.nan)):
+        t[pad] = bad
+        t[pad & (torch.arange(T, device="cuda") % 2 == 0)] = math.nan
+    leaves = [t.requires_grad_() for t in x[:3]]
+    o = S.token_attention(*leaves, docs=S.document_bounds(docs), **kw)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, x[3]))))
+    for name, (want, allowed) in ref.items():
+        want, allowed = want.clone(), allowed.clone()
+        want[pad], allowed[pad] = 0, 0
+        within(got[name], want, allowed, name)
+    ref = _attn_ref(q, k, v, None, window, cap, None, None, None, dtype)["o"]
+    k2, v2 = k.clone(), v.clone()
+    k2[:, 150], v2[:, 151] = math.nan, math.inf
+    with torch.no_grad():
+        o = S.token_attention(q, k2, v2, **kw)
+    within(o[:, :150], ref[0][:, :150], ref[1][:, :150], "before")
+    behind = 151 + (window or T)
+    assert o[:, 150:min(T, 150 + (window or T))].isnan().all() and not o[:, 151].isfinite().any()
+    within(o[:, behind:], ref[0][:, behind:], ref[1][:, behind:], "behind the window")
+
+
 def test_attention_gradients_against_differences():
     """Central differences of sum(o * do) in float32 kernels' own values: step h, error h^2 / 6 of the third derivative and 2^-23 / h of
     the value; with inputs of order one and h = 2^-7 both stay below 2e-3 of the gradients' scale."""
