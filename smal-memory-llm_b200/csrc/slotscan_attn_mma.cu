@@ -199,6 +199,7 @@ attn_fwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ F
             if (lane == 0) arrive(&p_full[t]);
         }
         if (ok && l0 > f0) ok = wait_soon(&o_full[t], (l0 - f0 - 1) & 1);
+        else if (ok && n0 < n1) ok = wait_soon(&q_full[t], 0);                     // a tile that sees nothing: its queries still come in where its outputs go
         tmem_fence_after();
         if (!ok) s_fail = 1;
         const bool none = sp.hi <= sp.lo;

@@ -314,6 +314,24 @@ def test_hidden_values_do_not_reach_anything(dtype, window, H, KV, D, cap):
     within(o[:, behind:], ref[0][:, behind:], ref[1][:, behind:], "behind the window")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_whole_tile_of_padding_beside_a_full_one(dtype):
+    """Many sequences whose first 128 tokens are a document and whose others are padding, and the other way round."""
+    S = _S()
+    g, q, k, v, do = _attn_inputs(dtype, 96, 256, 256, 4, 2, 64, seed=33)
+    docs = torch.full((96, 256), -1, device="cuda")
+    docs[::2, :128] = 1
+    docs[1::2, 128:] = 1
+    pad = docs < 0
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    for _ in range(5):
+        o = S.token_attention(*x, docs=S.document_bounds(docs))
+        got = torch.autograd.grad(o, x, do)
+        assert not o[pad].any() and all(not t[pad].any() for t in got)
+        want = S.token_attention(q[::2, :128], k[::2, :128], v[::2, :128])
+        assert torch.equal(o[::2, :128], want)
+
+
 def test_attention_gradients_against_differences():
     """Central differences of sum(o * do) in float32 kernels' own values: step h, error h^2 / 6 of the third derivative and 2^-23 / h of
     the value; with inputs of order one and h = 2^-7 both stay below 2e-3 of the gradients' scale."""
