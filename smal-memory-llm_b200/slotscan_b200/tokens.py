@@ -57,6 +57,11 @@ def _same(what, *ts):
         raise TypeError("%s: float32 or bfloat16 tensors, all of one type" % what)
 
 
+def _first_order(*grads):
+    """Whether a backward may go round the registered op: ordinary gradients, and none of a higher order wanted, which the op refuses."""
+    return not torch.is_grad_enabled() and plain_grads(*grads)
+
+
 # ---------------------------------------------------------------------------------------- norms and rotation
 
 @functools.lru_cache(maxsize=256)
@@ -124,10 +129,10 @@ def _norm_bwd(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], p
     dq, dk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
     n = q.shape[3] if weights else 0
     dqw, dkw = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
-    scratch = torch.empty(scratch_bytes if weights else 0, dtype=torch.uint8, device=dev)
+    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev) if weights else None
     with _Here(dev):
         rc = _lib.lib().slotscan_norm_rope_bwd(ref, _ptr(q), _ptr(k), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(dqo), _ptr(dko),
-                                               _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(scratch), scratch.numel(), _stream(dev))
+                                               _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(scratch), scratch_bytes if weights else 0, _stream(dev))
     _lib.check(rc, "slotscan_norm_rope_bwd")
     return dq, dk, dqw, dkw
 
@@ -148,6 +153,10 @@ def _(q, k, table, pos, q_weight, k_weight, dqo, dko, eps):
     return q.new_empty(q.shape), k.new_empty(k.shape), *(q.new_empty((n,), dtype=torch.float32) for _ in range(2))
 
 
+def _as(grad, weight):
+    return None if weight is None else grad if grad.dtype is weight.dtype else grad.to(weight.dtype)
+
+
 def _norm_setup(ctx, inputs, output):
     *ts, ctx.eps = inputs
     ctx.save_for_backward(*ts)
@@ -156,7 +165,7 @@ def _norm_setup(ctx, inputs, output):
 def _norm_backward(ctx, dqo, dko, bwd=None):
     q, k, table, pos, qw, kw = ctx.saved_tensors
     dq, dk, dqw, dkw = (bwd or _norm_bwd_op)(q, k, table, pos, qw, kw, dqo, dko, ctx.eps)
-    return dq, dk, None, None, None if qw is None else dqw.to(qw.dtype), None if kw is None else dkw.to(kw.dtype), None
+    return dq, dk, None, None, _as(dqw, qw), _as(dkw, kw), None
 
 
 _norm_op.register_autograd(_norm_backward, setup_context=_norm_setup)
@@ -172,9 +181,8 @@ class _Norm(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dqo, dko):
-        return _norm_backward(ctx, dqo, dko, bwd=_norm_bwd if plain_grads(dqo, dko) else None)
+        return _norm_backward(ctx, dqo, dko, bwd=_norm_bwd if _first_order(dqo, dko) else None)
 
 
 def rope_table(length, rot, theta=10000.0, device=None):
@@ -367,9 +375,8 @@ class _Attn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do, _, __):
-        return _attn_backward(ctx, do, None, None, bwd=_attn_bwd if plain_grads(do) else None)
+        return _attn_backward(ctx, do, None, None, bwd=_attn_bwd if _first_order(do) else None)
 
 
 def _numbers(what, D, window, cap, scale, slopes):

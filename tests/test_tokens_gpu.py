@@ -518,6 +518,17 @@ def test_first_call_of_a_thread(window):
     assert len(got) == 4 and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_gradients_of_gradients_are_refused():
+    S = _S()
+    g, q, k, v, do = _attn_inputs("f32", 1, 20, 20, 1, 1, 32, seed=27)
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    table = S.rope_table(20, 32, device="cuda")
+    for y in (S.token_attention(*x, window=4), S.norm_rope(x[0], x[1], table)[0]):
+        first = torch.autograd.grad(y, x[0], torch.ones_like(y), create_graph=True)[0]
+        with pytest.raises(RuntimeError):
+            first.sum().backward()
+
+
 def test_registered_ops_give_the_same():
     """Under a profiler the registered ops run instead of the plain calls; batched gradients take their backward."""
     from torch.profiler import ProfilerActivity, profile
