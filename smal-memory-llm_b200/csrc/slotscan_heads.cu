@@ -8,7 +8,10 @@
 //
 // Layout: a group of LPG lanes (a power of two, 8 channels to a lane: one 16-byte load of bf16, two of float32) takes a token and walks
 // over a slice of its heads, queries first, with the token's cosines and sines in registers: the table of a position has the bytes of
-// two bf16 rows, and is read once for all its heads.  A pair's two channels lie R/16 lanes apart: one shuffle.
+// two bf16 rows, and is read once for all its heads.  A pair's two channels lie R/16 lanes apart: one shuffle.  What hides a row's
+// chain of load, two sums and store is the other warps: two rows in flight to a group and four CTAs to an SM took 101 us for
+// 64 x 1,024 tokens of 6 + 6 heads of 128 (4.0 TB/s), six rows and three CTAs 113; the backward, with more to keep, 150 us (4.0 TB/s)
+// with four rows and two CTAs, 164 with three, 186 with two, 256 with two rows and three CTAs.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -21,7 +24,8 @@ namespace slotscan {
 
 typedef __nv_bfloat16 bf16;
 constexpr int NR_THREADS = 256;
-constexpr int NR_MAX_CTAS = 148 * 2;                     // of the backward, which sums the weights' gradients per CTA: those of one wave
+constexpr int NR_FWD_CTAS = 4, NR_BWD_CTAS = 2;         // of an SM
+constexpr int NR_MAX_CTAS = 148 * NR_BWD_CTAS;                     // of the backward, which sums the weights' gradients per CTA: those of one wave
 
 struct NormArgs {
     int T, H, KV, D, R, table_len, slices, per_slice;    // per_slice heads (queries, keys, then values) to a group
@@ -81,7 +85,7 @@ __device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[8], const 
 
 // T: bf16 or float.  CACHE: the keys and the values go into the caches.
 template <typename T, int LPG, bool CACHE>
-__global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
+__global__ void __launch_bounds__(NR_THREADS, NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
     const int c = threadIdx.x % LPG;
     const unsigned unit = blockIdx.x * (NR_THREADS / LPG) + threadIdx.x / LPG, tok = unit / a.slices;            // fewer than 2^31
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, Ap
     T* vot = CACHE ? vc + b * ap.vcs[0] + row * ap.vcs[1] + c * 8 : nullptr;
     const long long kos = CACHE ? ap.kcs[2] : a.D;
     const float inv_d = 1.f / a.D;
-    constexpr int U = sizeof(T) == 2 ? 6 : 4;            // rows in flight to a group
+    constexpr int U = sizeof(T) == 2 ? 2 : 4;            // rows in flight to a group
     for (int u0 = 0; u0 < a.per_slice; u0 += U) {
         Raw8<T> in[U];
 #pragma unroll
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(NormArgs a, Ap
 
 // grid-stride over (token, slice of heads); part: (CTAs, 2, D) sums of the weights' gradients, or NULL
 template <typename T, int LPG>
-__global__ void __launch_bounds__(NR_THREADS, 2) norm_rope_bwd_kernel(NormArgs a, const T* q, const T* k, const T* gq, const T* gk, T* dq, T* dk,
+__global__ void __launch_bounds__(NR_THREADS, NR_BWD_CTAS) norm_rope_bwd_kernel(NormArgs a, const T* q, const T* k, const T* gq, const T* gk, T* dq, T* dk,
                                                                    float* part) {
     constexpr int GROUPS = NR_THREADS / LPG;
     __shared__ float s_part[GROUPS][LPG * 8];
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(NR_THREADS, 2) norm_rope_bwd_kernel(NormArgs a
         const size_t qo = (size_t)tok * a.H * a.D + c * 8, ko = (size_t)tok * a.KV * a.D + c * 8;
         float cs[8], sn[8];
         if (half) load_turn(a, a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t, half, c, cs, sn);
-        constexpr int U = sizeof(T) == 2 ? 3 : 2;
+        constexpr int U = sizeof(T) == 2 ? 4 : 2;
         for (int v0 = 0; v0 < a.per_slice; v0 += U) {
             Raw8<T> in[U], up[U];
 #pragma unroll
