@@ -44,7 +44,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
     typedef BwdShape<DP> Sh;
     extern __shared__ __align__(1024) char smem[];
     char *X0 = smem, *X1 = smem + Sh::TILE, *Y0 = X1 + Sh::TILE, *Y1 = Y0 + AB_R0 * Sh::TILE;
-    float2* s_stat = reinterpret_cast<float2*>(Y1 + AB_R1 * Sh::TILE);             // [2][128] -lse, -delta of the stream's queries
+    float* s_stat = reinterpret_cast<float*>(Y1 + AB_R1 * Sh::TILE);               // [2][2][128] -lse, -delta of the stream's queries
     __shared__ uint64_t x_full, done, s_full, d_full, s_read, d_read, p_full, ds_full, full0[AB_R0], full1[AB_R1], empty0[AB_R0], empty1[AB_R1];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
@@ -110,7 +110,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                     for (int e = 0; e < 8; e++) s = fmaf(x[e] + y[e], z[e], s);
                 }
             }
-            float* ex = reinterpret_cast<float*>(s_stat);
+            float* ex = s_stat;
             ex[cg * 128 + r] = s;
             sync_group(1, AB_WARPS * 32);
             my_delta = (ex[r] + ex[128 + r]) + (ex[256 + r] + ex[384 + r]);
@@ -129,10 +129,10 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
             const int y0 = (y_first + y_at) * AB_N + cg * 32;
             const Score sc(a, head);
             const bool masked = y0 < ts.lo_max || y0 + 32 > ts.hi_min;
-            const float2* stat = s_stat + (s & 1) * AB_N + cg * 32;
+            float* stat = s_stat + (s & 1) * 2 * AB_N + cg * 32;
             if (++y_at == y_tiles) { y_at = 0; head++; }
             if constexpr (KEYS) {
-                if (r < 64) reinterpret_cast<float*>(s_stat + (s & 1) * AB_N + cg * 32 + r % 32)[r / 32] = next;
+                if (r < 64) stat[r / 32 * AB_N + r % 32] = next;
                 if (s + 1 < steps) fetch();
                 sync_group(2 + cg, 128);
             }
@@ -163,10 +163,14 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                 const f32x2 lin = pack2(sc.lin, sc.lin), steep = pack2(-sc.slope, -sc.slope), one = pack2(1.f, 1.f);
                 const float in2 = -1.f / (sc.cap_out * sc.cap_out);
                 [[maybe_unused]] uint32_t wp[16];
+                [[maybe_unused]] float4 four;
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                     float L[2] = {my_lse, my_lse};
-                    if constexpr (KEYS) { L[0] = stat[i].x; L[1] = stat[i + 1].x; }
+                    if constexpr (KEYS) {                // four at a time: the products want the shared memory's cycles
+                        if (i % 4 == 0) four = ld4(stat + i);
+                        L[0] = i % 4 ? four.z : four.x; L[1] = i % 4 ? four.w : four.y;
+                    }
                     const f32x2 x = pack2(__uint_as_float(xs[i]), __uint_as_float(xs[i + 1]));
                     f32x2 z, f = one;
                     if constexpr (CAP && decltype(poly)::value) {
@@ -214,6 +218,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
             if (!(ok = wait_soon_warp(&d_full, s & 1))) break;
             tmem_fence_after();
             uint32_t xd[32], wd[16];
+            [[maybe_unused]] float4 four;
             tmem_ld(S + 128, xd);
             tmem_ld_wait(xd);
             if constexpr (!KEYS) {
@@ -224,7 +229,10 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
                 float dl[2] = {my_delta, my_delta};
-                if constexpr (KEYS) { dl[0] = stat[i].y; dl[1] = stat[i + 1].y; }
+                if constexpr (KEYS) {
+                    if (i % 4 == 0) four = ld4(stat + AB_N + i);
+                    dl[0] = i % 4 ? four.z : four.x; dl[1] = i % 4 ? four.w : four.y;
+                }
                 float2 ds = unpack2(mul2(pack2(__uint_as_float(xs[i]), __uint_as_float(xs[i + 1])),
                                          add2(pack2(__uint_as_float(xd[i]), __uint_as_float(xd[i + 1])), pack2(dl[0], dl[1]))));
                 if (masked) {                            // nothing of a hidden dp, infinities and NaN among them

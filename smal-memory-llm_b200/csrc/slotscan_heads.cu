@@ -85,7 +85,7 @@ __device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[8], const 
 
 // T: bf16 or float.  CACHE: the keys and the values go into the caches.
 template <typename T, int LPG, bool CACHE>
-__global__ void __launch_bounds__(NR_THREADS, NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
+__global__ void __launch_bounds__(NR_THREADS, CACHE ? 3 : NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
     const int c = threadIdx.x % LPG;
     const unsigned unit = blockIdx.x * (NR_THREADS / LPG) + threadIdx.x / LPG, tok = unit / a.slices;            // fewer than 2^31
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(NR_THREADS, NR_FWD_CTAS) norm_rope_kernel(Norm
     T* vot = CACHE ? vc + b * ap.vcs[0] + row * ap.vcs[1] + c * 8 : nullptr;
     const long long kos = CACHE ? ap.kcs[2] : a.D;
     const float inv_d = 1.f / a.D;
-    constexpr int U = sizeof(T) == 2 ? 2 : 4;            // rows in flight to a group
+    constexpr int U = 2;                                 // rows in flight to a group
     for (int u0 = 0; u0 < a.per_slice; u0 += U) {
         Raw8<T> in[U];
 #pragma unroll
