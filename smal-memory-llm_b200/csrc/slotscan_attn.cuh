@@ -223,24 +223,24 @@ __device__ __forceinline__ void careful_dkv(const AttnArgs& a, const RowInputs<T
 // 0 while all values added are finite, NaN from the first that is not
 __device__ __forceinline__ void watch(float& w, float x) { w = fmaf(x, 0.f, w); }
 
-// The capped score as a polynomial, for |x| <= 1 (x = scale <q, k> / cap): tanh x = x sum_k a_k x^2k, the a_k fitted here for the least
-// greatest error of tanh (iteratively reweighted least squares on Chebyshev nodes): 2.4e-7.  Three and a half instructions a score,
+// The capped score as a polynomial, for |x| <= 0.6 (x = scale <q, k> / cap): tanh x = x sum_k a_k x^2k, the a_k fitted here for the
+// least greatest error of tanh (iteratively reweighted least squares on Chebyshev nodes): 6e-7.  Two and a half instructions a score,
 // two scores to an instruction, where the exponential form takes two of the special function unit's, eight cycles a warp each; a
-// block with a larger score takes that form.  The coefficients carry cap and scale: base-2 exponent = s sum_k c_k s^2k.
+// block of a warp with a larger score takes that form.  (Six terms for |x| <= 1 and its two registers a term: 626 + 1,575 us for one capped
+// sequence of 16,384, forward + backward; @@CAP@@ so.)  The coefficients carry cap and scale: base-2 exponent = s sum_k c_k s^2k.
+constexpr float CAP_POLY_MOST = 0.6f;
 struct CapPoly {
-    f32x2 c[6];
-    float most;                                          // the greatest |s| it serves
+    f32x2 c[4];
     __device__ __forceinline__ explicit CapPoly(const Score& sc) {
-        const float a[6] = {0.9999968538152487f, -0.333240039679371f, 0.13253525772679928f, -0.050972871352707325f, 0.016114187219736308f, -0.002839467407190691f};
+        const float a[4] = {0.9999910176913201f, -0.33298974340939966f, 0.12974554465812582f, -0.03961128075861646f};
         float f = sc.cap_out * sc.cap_in;
 #pragma unroll
-        for (int k = 0; k < 6; k++) { c[k] = pack2(a[k] * f, a[k] * f); f *= sc.cap_in * sc.cap_in; }
-        most = 1.f / sc.cap_in;
+        for (int k = 0; k < 4; k++) { c[k] = pack2(a[k] * f, a[k] * f); f *= sc.cap_in * sc.cap_in; }
     }
     // two scores without their last factor: exponents = s * slope(s)
     __device__ __forceinline__ f32x2 slope(f32x2 s) const {
         const f32x2 w = mul2(s, s);
-        return fma2(w, fma2(w, fma2(w, fma2(w, fma2(w, c[5], c[4]), c[3]), c[2]), c[1]), c[0]);
+        return fma2(w, fma2(w, fma2(w, c[3], c[2]), c[1]), c[0]);
     }
 };
 

@@ -156,7 +156,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                     m0 = fmaxf(m0, fabsf(__uint_as_float(xs[i])));
                     m1 = fmaxf(m1, fabsf(__uint_as_float(xs[i + 1])));
                 }
-                small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= 1.f);
+                small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= CAP_POLY_MOST);
             }
             auto weights = [&](auto poly, auto some) {   // some: of the block's scores are masked
                 const CapPoly cp(sc);

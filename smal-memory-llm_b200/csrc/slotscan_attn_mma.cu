@@ -44,7 +44,7 @@ __device__ __forceinline__ void scores32(float (&s)[32], const Score& sc, float 
         float m0 = 0.f, m1 = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) { m0 = fmaxf(m0, fabsf(s[i])); m1 = fmaxf(m1, fabsf(s[i + 1])); }
-        small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= 1.f);
+        small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= CAP_POLY_MOST);
     }
     if constexpr (CAP || BIAS) {
         auto whole = [&](auto poly) {
