@@ -3,6 +3,9 @@ attention over the tokens themselves, for a training step, a prompt and single t
 
 The reference runs a 16-token causal window beside its memory and leaves it to library calls (gqa25/memlm_sh.py:349-359, the rotated
 queries and keys of memlm_kv.py); here each piece is a CUDA kernel of libslotscan.so with no other implementation behind it.
+
+Small calls are bound by their host side, so what depends on the arguments' shapes, strides and types alone -- the checks, the
+parameters of the C call, scratch sizes -- is worked out once per such signature (the `_..._plan` functions) and looked up after that.
 """
 import ctypes
 import functools
@@ -16,27 +19,30 @@ from .ops import _Here, _require_cuda, _stream, plain_call, plain_grads, wants_g
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _SIZE = {torch.float32: 4, torch.bfloat16: 2}
+_getDevice = torch._C._cuda_getDevice
 
 
-@functools.lru_cache(maxsize=512)
-def _strides(shape, stride, size):
+def _sig(t):
+    """What a plan depends on of a tensor."""
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _strides(sig):
     """The strides of all dimensions but the channels', 0 where a dimension has one element; None where the kernels cannot read such a
     tensor in place: adjacent channels, everything else on 16-byte boundaries, no dimension expanded."""
-    s = tuple(0 if n == 1 else st for n, st in zip(shape[:-1], stride))
-    return None if stride[-1] != 1 or any(n > 1 and (st == 0 or st * size % 16) for n, st in zip(shape[:-1], stride)) else s
+    shape, stride, dtype = sig
+    bad = stride[-1] != 1 or any(n > 1 and (st == 0 or st * _SIZE[dtype] % 16) for n, st in zip(shape[:-1], stride))
+    return None if bad else tuple(0 if n == 1 else st for n, st in zip(shape[:-1], stride))
 
 
 def _laid(t):
-    """`t` and its strides where the kernels can read it; a tensor that is laid out otherwise is copied."""
-    size = _SIZE[t.dtype]
-    s = _strides(t.shape, t.stride(), size)
-    if s is not None and t.data_ptr() % 16 == 0:
-        return t, s
+    """`t` where the kernels can read it, else a copy that they can."""
+    if _strides(_sig(t)) is not None and t.data_ptr() % 16 == 0:
+        return t
     t = t.clone(memory_format=torch.contiguous_format)
-    s = _strides(t.shape, t.stride(), size)
-    if s is None:
+    if _strides(_sig(t)) is None:
         raise ValueError("slotscan_b200: %d channels of %s do not fill 16 bytes" % (t.shape[-1], t.dtype))
-    return t, s
+    return t
 
 
 def _f32(t):
@@ -47,13 +53,32 @@ def _i32(t):
     return t if t is None or (t.dtype is torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
 
 
+def _whole(g, dtype):
+    """An upstream gradient, contiguous and on a 16-byte boundary."""
+    if g.dtype is not dtype or not g.is_contiguous():
+        g = g.to(dtype).contiguous()
+    return g if g.data_ptr() % 16 == 0 else g.clone()
+
+
 def _ptr(t):
     """A device address for a `c_void_p` argument; an empty tensor has none."""
     return None if t is None else t.data_ptr() or None
 
 
-def _same(what, *ts):
-    if any(t.dtype not in _CODE or t.dtype != ts[0].dtype for t in ts):
+def _launch(dev, name, *args):
+    """The C call on the current stream of `dev`, which is made current if it is not."""
+    f = getattr(_lib.lib(), name)
+    if _getDevice() == dev.index:
+        rc = f(*args, _stream(dev))
+    else:
+        with _Here(dev):
+            rc = f(*args, _stream(dev))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _type_check(what, *sigs):
+    if any(s[2] not in _CODE or s[2] != sigs[0][2] for s in sigs):
         raise TypeError("%s: float32 or bfloat16 tensors, all of one type" % what)
 
 
@@ -64,48 +89,50 @@ def _first_order(*grads):
 
 # ---------------------------------------------------------------------------------------- norms and rotation
 
-@functools.lru_cache(maxsize=256)
-def _norm_params(B, T, H, KV, D, R, table_len, dtype, eps, qs, ks):
-    """The parameters of a call of this shape, checked, and the scratch bytes of its backward."""
-    p = _lib.NormParams(B, T, H, KV, D, R, table_len, dtype, eps, qs, ks)
-    _lib.check(_lib.lib().slotscan_norm_rope_check(ctypes.byref(p)), "slotscan_norm_rope_check")
-    return p, ctypes.byref(p), _lib.lib().slotscan_norm_rope_bwd_scratch_bytes(ctypes.byref(p))
-
-
-def _norm_shapes(what, q, k, table, q_weight, k_weight):
-    _same(what, q, k)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ValueError("%s: queries (B, T, H, D) and keys (B, T, KV, D), got %s and %s" % (what, tuple(q.shape), tuple(k.shape)))
-    D = q.shape[3]
-    if table is not None and (table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32):
+def _norm_checked(what, q, k, table, q_weight, k_weight):
+    """(B, T, H, KV, D, R, positions) of signatures that fit together."""
+    _type_check(what, q, k)
+    qs, ks = q[0], k[0]
+    if len(qs) != 4 or len(ks) != 4 or qs[:2] != ks[:2] or qs[3] != ks[3]:
+        raise ValueError("%s: queries (B, T, H, D) and keys (B, T, KV, D), got %s and %s" % (what, tuple(qs), tuple(ks)))
+    if table is not None and (len(table[0]) != 3 or table[0][2] != 2 or table[2] != torch.float32):
         raise ValueError("%s: the table is float32 of shape (positions, R / 2, 2)" % what)
     for w in (q_weight, k_weight):
-        if w is not None and w.shape != (D,):
-            raise ValueError("%s: a weight has one entry for each of the %d channels, got %s" % (what, D, tuple(w.shape)))
+        if w is not None and w[0] != (qs[3],):
+            raise ValueError("%s: a weight has one entry for each of the %d channels, got %s" % (what, qs[3], tuple(w[0])))
+    return qs[0], qs[1], qs[2], ks[2], qs[3], 0 if table is None else 2 * table[0][1], 0 if table is None else table[0][0]
 
 
-def _norm_call(q, k, table, eps):
-    """q and k where the kernels can read them, and the call's parameters."""
-    (q, qs), (k, ks) = _laid(q), _laid(k)
-    B, T, H, D = q.shape
-    return (q, k) + _norm_params(B, T, H, k.shape[2], D, 0 if table is None else 2 * table.shape[1], 0 if table is None else table.shape[0],
-                                 _CODE[q.dtype], eps, qs, ks)
+@functools.lru_cache(maxsize=256)
+def _norm_plan(q, k, table, pos, q_weight, k_weight, eps):
+    """(reference to the parameters, scratch bytes of the backward, the parameters); the reference is None where q or k must be copied."""
+    sizes = _norm_checked("norm_rope", q, k, table, q_weight, k_weight)
+    if pos is not None and pos[0] != q[0][:2]:
+        raise ValueError("norm_rope: positions (B, T), got %s" % (tuple(pos[0]),))
+    if pos is None and table is not None and sizes[1] > sizes[6]:
+        raise ValueError("norm_rope: %d tokens, %d positions in the table" % (sizes[1], sizes[6]))
+    strides = _strides(q), _strides(k)
+    p = _lib.NormParams(*sizes, _CODE[q[2]], eps, *((0, 0, 0) if s is None else s for s in strides))
+    _lib.check(_lib.lib().slotscan_norm_rope_check(ctypes.byref(p)), "slotscan_norm_rope_check")
+    return None if None in strides else ctypes.byref(p), _lib.lib().slotscan_norm_rope_bwd_scratch_bytes(ctypes.byref(p)), p
+
+
+def _norm_call(q, k, table, pos, q_weight, k_weight, eps):
+    """The tensors as the kernels read them, and the plan of the call."""
+    plan = _norm_plan(_sig(q), _sig(k), _sig(table), _sig(pos), _sig(q_weight), _sig(k_weight), eps)
+    if plan[0] is None or (q.data_ptr() | k.data_ptr()) & 15:
+        q, k = _laid(q), _laid(k)
+        plan = _norm_plan(_sig(q), _sig(k), _sig(table), _sig(pos), _sig(q_weight), _sig(k_weight), eps)
+    return q, k, _f32(table), _i32(pos), _f32(q_weight), _f32(k_weight), plan
 
 
 def _norm_fwd(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], pos: Optional[torch.Tensor],
               q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
     _require_cuda(q, k, table, pos, q_weight, k_weight)
-    _norm_shapes("norm_rope", q, k, table, q_weight, k_weight)
-    if pos is not None and pos.shape != q.shape[:2]:
-        raise ValueError("norm_rope: positions (B, T), got %s" % (tuple(pos.shape),))
-    q, k, p, ref, _ = _norm_call(q, k, table, eps)
-    table, pos, qw, kw = _f32(table), _i32(pos), _f32(q_weight), _f32(k_weight)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    with _Here(q.device):
-        rc = _lib.lib().slotscan_norm_rope_fwd(ref, _ptr(q), _ptr(k), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(qo), _ptr(ko),
-                                               _stream(q.device))
-    _lib.check(rc, "slotscan_norm_rope_fwd")
+    q, k, table, pos, qw, kw, plan = _norm_call(q, k, table, pos, q_weight, k_weight, eps)
+    dev = q.device
+    qo, ko = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
+    _launch(dev, "slotscan_norm_rope_fwd", plan[0], _ptr(q), _ptr(k), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(qo), _ptr(ko))
     return qo, ko
 
 
@@ -122,26 +149,16 @@ def _norm_bwd(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], p
               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """dq, dk and the float32 gradients of the two weights (empty without weights)."""
     _require_cuda(q, k, table, pos, q_weight, k_weight, dqo, dko)
-    q, k, p, ref, scratch_bytes = _norm_call(q, k, table, eps)
-    table, pos, qw, kw = _f32(table), _i32(pos), _f32(q_weight), _f32(k_weight)
+    q, k, table, pos, qw, kw, plan = _norm_call(q, k, table, pos, q_weight, k_weight, eps)
     dqo, dko = _whole(dqo, q.dtype), _whole(dko, k.dtype)
     dev, weights = q.device, qw is not None or kw is not None
     dq, dk = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
-    n = q.shape[3] if weights else 0
+    n, scratch_bytes = (q.shape[3], plan[1]) if weights else (0, 0)
     dqw, dkw = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
-    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev) if weights else None
-    with _Here(dev):
-        rc = _lib.lib().slotscan_norm_rope_bwd(ref, _ptr(q), _ptr(k), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(dqo), _ptr(dko),
-                                               _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(scratch), scratch_bytes if weights else 0, _stream(dev))
-    _lib.check(rc, "slotscan_norm_rope_bwd")
+    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=dev) if scratch_bytes else None
+    _launch(dev, "slotscan_norm_rope_bwd", plan[0], _ptr(q), _ptr(k), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(dqo), _ptr(dko),
+            _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(scratch), scratch_bytes)
     return dq, dk, dqw, dkw
-
-
-def _whole(g, dtype):
-    """An upstream gradient, contiguous and on a 16-byte boundary."""
-    if g.dtype is not dtype or not g.is_contiguous():
-        g = g.to(dtype).contiguous()
-    return g if g.data_ptr() % 16 == 0 else g.clone()
 
 
 _norm_bwd_op = torch.library.custom_op("slotscan::norm_rope_bwd", mutates_args=())(_norm_bwd)
@@ -153,13 +170,13 @@ def _(q, k, table, pos, q_weight, k_weight, dqo, dko, eps):
     return q.new_empty(q.shape), k.new_empty(k.shape), *(q.new_empty((n,), dtype=torch.float32) for _ in range(2))
 
 
-def _as(grad, weight):
-    return None if weight is None else grad if grad.dtype is weight.dtype else grad.to(weight.dtype)
-
-
 def _norm_setup(ctx, inputs, output):
     *ts, ctx.eps = inputs
     ctx.save_for_backward(*ts)
+
+
+def _as(grad, weight):
+    return None if weight is None else grad if grad.dtype is weight.dtype else grad.to(weight.dtype)
 
 
 def _norm_backward(ctx, dqo, dko, bwd=None):
@@ -199,50 +216,57 @@ def norm_rope(q, k, table, q_weight=None, k_weight=None, pos=None, eps=1e-6):
     `rope_table`, or None for no rotation; `pos` (B,T) integer positions (None: 0 .. T-1).  Slices of a fused projection are read in
     place.  A position outside the table gives NaN.  Differentiable in q, k and the weights."""
     ts = (q, k, table, pos, q_weight, k_weight)
-    if pos is None and table is not None and q.dim() == 4 and q.shape[1] > table.shape[0]:
-        raise ValueError("norm_rope: %d tokens, %d positions in the table" % (q.shape[1], table.shape[0]))
     if not plain_call(*ts):
         return _norm_op(*ts, float(eps))
     return _Norm.apply(*ts, float(eps)) if wants_grad(*ts) else _norm_fwd(*ts, float(eps))
 
 
-@functools.lru_cache(maxsize=256)
-def _append_params(L, vs, kcs, vcs, *norm):
-    p = _lib.AppendParams(_lib.NormParams(*norm), L, vs, kcs, vcs)
-    return p, ctypes.byref(p)
-
-
 def _caches(what, k_cache, v_cache, dtype):
-    if k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-        raise ValueError("%s: caches (B, L, KV, D) of the queries' type, got %s and %s" % (what, tuple(k_cache.shape), tuple(v_cache.shape)))
-    (k, ks), (v, vs) = _laid(k_cache), _laid(v_cache)
-    if k is not k_cache or v is not v_cache:
+    """The strides of caches that the kernels can use in place."""
+    if k_cache[2] != dtype or v_cache[2] != dtype or len(k_cache[0]) != 4 or k_cache[0] != v_cache[0]:
+        raise ValueError("%s: caches (B, L, KV, D) of the queries' type, got %s and %s" % (what, tuple(k_cache[0]), tuple(v_cache[0])))
+    ks, vs = _strides(k_cache), _strides(v_cache)
+    if ks is None or vs is None:
         raise ValueError("%s: the caches must have adjacent channels and 16-byte aligned rows" % what)
     return ks, vs
+
+
+def _cache_bases(what, k_cache, v_cache):
+    if (k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        raise ValueError("%s: the caches must begin on a 16-byte boundary" % what)
+
+
+@functools.lru_cache(maxsize=256)
+def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps):
+    B, T, H, KV, D, R, length = sizes = _norm_checked("norm_rope_append", q, k, table, q_weight, k_weight)
+    _type_check("norm_rope_append", q, k, v)
+    kcs, vcs = _caches("norm_rope_append", k_cache, v_cache, q[2])
+    L = k_cache[0][1]
+    if v[0] != k[0] or k_cache[0] != (B, L, KV, D) or pos[0] != (B,):
+        raise ValueError("norm_rope_append: keys, values, caches and positions do not match: %s, %s, %s, %s"
+                         % (tuple(k[0]), tuple(v[0]), tuple(k_cache[0]), tuple(pos[0])))
+    if T > L:
+        raise ValueError("norm_rope_append: %d tokens at once into caches of %d rows" % (T, L))
+    qs, ks, vs = _strides(q), _strides(k), _strides(v)
+    if None in (qs, ks, vs):
+        return None, None
+    p = _lib.AppendParams(_lib.NormParams(*sizes, _CODE[q[2]], eps, qs, ks), L, vs, kcs, vcs)
+    return ctypes.byref(p), p
 
 
 def _append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor,
             table: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> torch.Tensor:
     _require_cuda(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
-    _norm_shapes("norm_rope_append", q, k, table, q_weight, k_weight)
-    _same("norm_rope_append", q, k, v)
-    B, T, H, D = q.shape
-    KV, L = k.shape[2], k_cache.shape[1] if k_cache.dim() == 4 else 0
-    kcs, vcs = _caches("norm_rope_append", k_cache, v_cache, q.dtype)
-    if v.shape != k.shape or k_cache.shape != (B, L, KV, D) or pos.shape != (B,):
-        raise ValueError("norm_rope_append: keys, values, caches and positions do not match: %s, %s, %s, %s"
-                         % (tuple(k.shape), tuple(v.shape), tuple(k_cache.shape), tuple(pos.shape)))
-    if T > L:
-        raise ValueError("norm_rope_append: %d tokens at once into caches of %d rows" % (T, L))
-    (q, qs), (k, ks), (v, vs) = _laid(q), _laid(k), _laid(v)
-    p, ref = _append_params(L, vs, kcs, vcs, B, T, H, KV, D, 0 if table is None else 2 * table.shape[1], 0 if table is None else table.shape[0],
-                            _CODE[q.dtype], eps, qs, ks)
+    rest = (_sig(k_cache), _sig(v_cache), _sig(pos), _sig(table), _sig(q_weight), _sig(k_weight), eps)
+    plan = _append_plan(_sig(q), _sig(k), _sig(v), *rest)
+    if plan[0] is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _laid(q), _laid(k), _laid(v)
+        plan = _append_plan(_sig(q), _sig(k), _sig(v), *rest)
+    _cache_bases("norm_rope_append", k_cache, v_cache)
     table, pos, qw, kw = _f32(table), _i32(pos), _f32(q_weight), _f32(k_weight)
     qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    with _Here(q.device):
-        rc = _lib.lib().slotscan_norm_rope_append(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(qo),
-                                                  _ptr(k_cache), _ptr(v_cache), _stream(q.device))
-    _lib.check(rc, "slotscan_norm_rope_append")
+    _launch(q.device, "slotscan_norm_rope_append", plan[0], _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(qo),
+            _ptr(k_cache), _ptr(v_cache))
     return qo
 
 
@@ -266,17 +290,38 @@ def norm_rope_append(q, k, v, k_cache, v_cache, pos, table, q_weight=None, k_wei
 # ---------------------------------------------------------------------------------------- attention
 
 @functools.lru_cache(maxsize=256)
-def _attn_params(B, Tq, Tk, H, KV, D, window, dtype, scale, cap, prefix, qs, ks, vs):
-    """The parameters of a call of this shape, checked, and whether its backward needs what the forward can keep."""
-    p = _lib.AttnParams(B, Tq, Tk, H, KV, D, window, dtype, scale, cap, qs, ks, vs)
+def _attn_plan(q, k, v, slopes, docs, prefix, window, cap, scale):
+    """(reference to the parameters, whether the backward needs what the forward can keep, the parameters); the reference is None
+    where q, k or v must be copied."""
+    _type_check("token_attention", q, k, v)
+    qs, ks = q[0], k[0]
+    if len(qs) != 4 or len(ks) != 4 or v[0] != ks or qs[0] != ks[0] or qs[3] != ks[3] or ks[2] == 0 or qs[2] % ks[2]:
+        raise ValueError("token_attention: queries (B, Tq, H, D), keys and values (B, Tk, KV, D) with H a multiple of KV, got %s, %s, %s"
+                         % (tuple(qs), tuple(ks), tuple(v[0])))
+    B, Tq, H, D = qs
+    Tk = ks[1]
+    if Tq > Tk:
+        raise ValueError("token_attention: %d queries over %d keys; the queries are the last tokens of the keys" % (Tq, Tk))
+    if slopes is not None and slopes[0] != (H,):
+        raise ValueError("token_attention: one slope for each of the %d heads, got %s" % (H, tuple(slopes[0])))
+    if docs is not None and docs[0] != (B, Tk, 2):
+        raise ValueError("token_attention: document bounds (B, Tk, 2) from document_bounds, got %s" % (tuple(docs[0]),))
+    if prefix is not None and prefix[0] != (B,):
+        raise ValueError("token_attention: one prefix length for each sequence, got %s" % (tuple(prefix[0]),))
+    strides = _strides(q), _strides(k), _strides(v)
+    p = _lib.AttnParams(B, Tq, Tk, H, ks[2], D, window, _CODE[q[2]], scale, cap, *((0, 0, 0) if s is None else s for s in strides))
     _lib.check(_lib.lib().slotscan_attn_check(ctypes.byref(p)), "slotscan_attn_check")
-    return p, ctypes.byref(p), bool(_lib.lib().slotscan_attn_keeps(ctypes.byref(p), prefix))
+    return None if None in strides else ctypes.byref(p), bool(_lib.lib().slotscan_attn_keeps(ctypes.byref(p), prefix is not None)), p
 
 
-def _attn_call(q, k, v, prefix, window, cap, scale):
-    (q, qs), (k, ks), (v, vs) = _laid(q), _laid(k), _laid(v)
-    B, Tq, H, D = q.shape
-    return (q, k, v) + _attn_params(B, Tq, k.shape[1], H, k.shape[2], D, window, _CODE[q.dtype], scale, cap, prefix is not None, qs, ks, vs)
+def _attn_call(q, k, v, slopes, docs, prefix, window, cap, scale):
+    """The tensors as the kernels read them, and the plan of the call."""
+    rest = (_sig(slopes), _sig(docs), _sig(prefix), window, cap, scale)
+    plan = _attn_plan(_sig(q), _sig(k), _sig(v), *rest)
+    if plan[0] is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _laid(q), _laid(k), _laid(v)
+        plan = _attn_plan(_sig(q), _sig(k), _sig(v), *rest)
+    return q, k, v, _f32(slopes), _i32(docs), _i32(prefix), plan
 
 
 def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optional[torch.Tensor], docs: Optional[torch.Tensor],
@@ -285,30 +330,12 @@ def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optiona
     """o and what the backward needs besides (without elements where it needs nothing, or unless asked for): lse (B,H,Tq), and for
     bfloat16 what the rounding of o left."""
     _require_cuda(q, k, v, slopes, docs, prefix)
-    _same("token_attention", q, k, v)
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or k.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError("token_attention: queries (B, Tq, H, D), keys and values (B, Tk, KV, D) with H a multiple of KV, got %s, %s, %s"
-                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    B, Tq, H, D = q.shape
-    Tk = k.shape[1]
-    if Tq > Tk:
-        raise ValueError("token_attention: %d queries over %d keys; the queries are the last tokens of the keys" % (Tq, Tk))
-    if slopes is not None and slopes.shape != (H,):
-        raise ValueError("token_attention: one slope for each of the %d heads, got %s" % (H, tuple(slopes.shape)))
-    if docs is not None and docs.shape != (B, Tk, 2):
-        raise ValueError("token_attention: document bounds (B, Tk, 2) from document_bounds, got %s" % (tuple(docs.shape),))
-    if prefix is not None and prefix.shape != (B,):
-        raise ValueError("token_attention: one prefix length for each sequence, got %s" % (tuple(prefix.shape),))
-    q, k, v, p, ref, keeps = _attn_call(q, k, v, prefix, window, cap, scale)
-    keeps = keeps and for_bwd
-    slopes, docs, prefix = _f32(slopes), _i32(docs), _i32(prefix)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Tq) if keeps else (0,), dtype=torch.float32, device=q.device)
-    rest = torch.empty(q.shape if keeps and q.dtype == torch.bfloat16 else (0,), dtype=q.dtype, device=q.device)
-    with _Here(q.device):
-        rc = _lib.lib().slotscan_attn_fwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest),
-                                          _ptr(lse), _stream(q.device))
-    _lib.check(rc, "slotscan_attn_fwd")
+    q, k, v, slopes, docs, prefix, plan = _attn_call(q, k, v, slopes, docs, prefix, window, cap, scale)
+    (B, Tq, H, _), dev, dtype, keeps = q.shape, q.device, q.dtype, plan[1] and for_bwd
+    o = torch.empty(q.shape, dtype=dtype, device=dev)
+    lse = torch.empty((B, H, Tq) if keeps else (0,), dtype=torch.float32, device=dev)
+    rest = torch.empty(q.shape if keeps and dtype is torch.bfloat16 else (0,), dtype=dtype, device=dev)
+    _launch(dev, "slotscan_attn_fwd", plan[0], _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest), _ptr(lse))
     return o, lse, rest
 
 
@@ -317,10 +344,9 @@ _attn_op = torch.library.custom_op("slotscan::attn_fwd", mutates_args=())(_attn_
 
 @_attn_op.register_fake
 def _(q, k, v, slopes, docs, prefix, window, cap, scale, for_bwd):
-    B, Tq, H, D = (int(n) for n in q.shape)
-    keeps = for_bwd and _attn_params(B, Tq, int(k.shape[1]), H, int(k.shape[2]), D, window, _CODE[q.dtype], scale, cap, prefix is not None,
-                                     *((0, 0, 0),) * 3)[2]
-    return (q.new_empty(q.shape), q.new_empty((B, H, Tq) if keeps else (0,), dtype=torch.float32),
+    sig = lambda t: None if t is None else (tuple(int(n) for n in t.shape), (0,) * (t.dim() - 1) + (1,), t.dtype)   # noqa: E731
+    keeps = for_bwd and _attn_plan(*(sig(t) for t in (q, k, v, slopes, docs, prefix)), window, cap, scale)[1]
+    return (q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if keeps else (0,), dtype=torch.float32),
             q.new_empty(q.shape if keeps and q.dtype == torch.bfloat16 else (0,)))
 
 
@@ -328,16 +354,17 @@ def _attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optiona
               prefix: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor, rest: torch.Tensor, do: torch.Tensor, window: int, cap: float,
               scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     _require_cuda(q, k, v, slopes, docs, prefix, o, lse, rest, do)
-    q, k, v, p, ref, _ = _attn_call(q, k, v, prefix, window, cap, scale)
-    slopes, docs, prefix = _f32(slopes), _i32(docs), _i32(prefix)
-    do, o, rest, lse = _whole(do, q.dtype), _whole(o, q.dtype), _whole(rest, q.dtype), lse.contiguous()
-    dev = q.device
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-    delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
-    with _Here(dev):
-        rc = _lib.lib().slotscan_attn_bwd(ref, _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest),
-                                          _ptr(lse), _ptr(do), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv), _stream(dev))
-    _lib.check(rc, "slotscan_attn_bwd")
+    q, k, v, slopes, docs, prefix, plan = _attn_call(q, k, v, slopes, docs, prefix, window, cap, scale)
+    dev, dtype = q.device, q.dtype
+    do = _whole(do, dtype)
+    dq, dk, dv = torch.empty(q.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev), torch.empty(k.shape, dtype=dtype, device=dev)
+    if plan[1]:
+        o, rest, lse = _whole(o, dtype), _whole(rest, dtype), lse.contiguous()
+        delta = torch.empty(lse.shape, dtype=torch.float32, device=dev)
+    else:
+        o = lse = rest = delta = None
+    _launch(dev, "slotscan_attn_bwd", plan[0], _ptr(q), _ptr(k), _ptr(v), _ptr(slopes), _ptr(docs), _ptr(prefix), _ptr(o), _ptr(rest), _ptr(lse),
+            _ptr(do), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv))
     return dq, dk, dv
 
 
@@ -408,44 +435,48 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
     last Tq tokens of the keys (Tq = Tk in training; fewer for a chunk of a prompt behind its window).
       scores   s = scale <q, k> (scale: D^-1/2), then cap * tanh(s / cap) if cap, then minus slopes[head] * |i - j| (constants)
       visible  j <= i, or j < prefix[b];  and |i - j| < window if window;  and the same document of `document_bounds`
-    A row that sees nothing gives zeros.  Differentiable in q, k and v; results and gradients are equal from run to run."""
+    A row that sees nothing gives zeros, and what a row does not see, infinities and NaN among it, does not reach it.  Differentiable
+    in q, k and v; results and gradients are equal from run to run."""
     window, cap, scale = _numbers("token_attention", q.shape[-1], window, cap, scale, slopes)
     ts = (q, k, v, slopes, docs, prefix)
-    grad = wants_grad(q, k, v)
     if not plain_call(*ts):
         return _attn_op(*ts, window, cap, scale, True)[0]
-    return _Attn.apply(*ts, window, cap, scale, True)[0] if grad else _attn_fwd(*ts, window, cap, scale, False)[0]
+    return _Attn.apply(*ts, window, cap, scale, True)[0] if wants_grad(q, k, v) else _attn_fwd(*ts, window, cap, scale, False)[0]
 
 
 @functools.lru_cache(maxsize=256)
-def _step_params(B, H, KV, D, L, window, dtype, scale, cap, qs, ks, vs):
-    p = _lib.AttnStepParams(B, H, KV, D, L, window, dtype, scale, cap, qs, ks, vs)
+def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
+    """(reference to the parameters, scratch bytes, the parameters); the reference is None where q must be copied."""
+    _type_check("token_attention_step", q)
+    if len(q[0]) != 4 or q[0][1] != 1:
+        raise ValueError("token_attention_step: one query for each sequence, (B, 1, H, D), got %s" % (tuple(q[0]),))
+    B, _, H, D = q[0]
+    ks, vs = _caches("token_attention_step", k_cache, v_cache, q[2])
+    _, L, KV, _ = k_cache[0]
+    if k_cache[0] != (B, L, KV, D) or KV == 0 or H % KV:
+        raise ValueError("token_attention_step: queries %s do not match caches %s" % (tuple(q[0]), tuple(k_cache[0])))
+    if pos[0] != (B,) or (start is not None and start[0] != (B,)) or (slopes is not None and slopes[0] != (H,)):
+        raise ValueError("token_attention_step: positions (B), starts (B) and slopes (H)")
+    qs = _strides(q)
+    p = _lib.AttnStepParams(B, H, KV, D, L, window, _CODE[q[2]], scale, cap, (0, 0) if qs is None else (qs[0], qs[2]), ks, vs)
     _lib.check(_lib.lib().slotscan_attn_step_check(ctypes.byref(p)), "slotscan_attn_step_check")
-    return p, ctypes.byref(p), _lib.lib().slotscan_attn_step_scratch_bytes(ctypes.byref(p))
+    return None if qs is None else ctypes.byref(p), _lib.lib().slotscan_attn_step_scratch_bytes(ctypes.byref(p)), p
 
 
 def _step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor],
           start: Optional[torch.Tensor], window: int, cap: float, scale: float) -> torch.Tensor:
     _require_cuda(q, k_cache, v_cache, pos, slopes, start)
-    _same("token_attention_step", q)
-    if q.dim() != 4 or q.shape[1] != 1:
-        raise ValueError("token_attention_step: one query for each sequence, (B, 1, H, D), got %s" % (tuple(q.shape),))
-    B, _, H, D = q.shape
-    ks, vs = _caches("token_attention_step", k_cache, v_cache, q.dtype)
-    L, KV = k_cache.shape[1], k_cache.shape[2]
-    if k_cache.shape != (B, L, KV, D) or KV == 0 or H % KV:
-        raise ValueError("token_attention_step: queries %s do not match caches %s" % (tuple(q.shape), tuple(k_cache.shape)))
-    if pos.shape != (B,) or (start is not None and start.shape != (B,)) or (slopes is not None and slopes.shape != (H,)):
-        raise ValueError("token_attention_step: positions (B), starts (B) and slopes (H)")
-    q, qs = _laid(q)
-    p, ref, scratch_bytes = _step_params(B, H, KV, D, L, window, _CODE[q.dtype], scale, cap, (qs[0], qs[2]), ks, vs)
+    rest = (_sig(k_cache), _sig(v_cache), _sig(pos), _sig(slopes), _sig(start), window, cap, scale)
+    plan = _step_plan(_sig(q), *rest)
+    if plan[0] is None or q.data_ptr() & 15:
+        q = _laid(q)
+        plan = _step_plan(_sig(q), *rest)
+    _cache_bases("token_attention_step", k_cache, v_cache)
     pos, start, slopes = _i32(pos), _i32(start), _f32(slopes)
-    o = torch.empty((B, 1, H, D), dtype=q.dtype, device=q.device)
-    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=q.device) if scratch_bytes else None
-    with _Here(q.device):
-        rc = _lib.lib().slotscan_attn_step(ref, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(pos), _ptr(start), _ptr(slopes), _ptr(o),
-                                           _ptr(scratch), scratch_bytes, _stream(q.device))
-    _lib.check(rc, "slotscan_attn_step")
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    scratch = torch.empty(plan[1], dtype=torch.uint8, device=q.device) if plan[1] else None
+    _launch(q.device, "slotscan_attn_step", plan[0], _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(pos), _ptr(start), _ptr(slopes), _ptr(o),
+            _ptr(scratch), plan[1])
     return o
 
 
