@@ -227,7 +227,7 @@ __device__ __forceinline__ void watch(float& w, float x) { w = fmaf(x, 0.f, w); 
 // least greatest error of tanh (iteratively reweighted least squares on Chebyshev nodes): 6e-7.  Two and a half instructions a score,
 // two scores to an instruction, where the exponential form takes two of the special function unit's, eight cycles a warp each; a
 // block of a warp with a larger score takes that form.  (Six terms for |x| <= 1 and its two registers a term: 626 + 1,575 us for one capped
-// sequence of 16,384, forward + backward; @@CAP@@ so.)  The coefficients carry cap and scale: base-2 exponent = s sum_k c_k s^2k.
+// sequence of 16,384, forward + backward; 538 + 1,470 so.)  The coefficients carry cap and scale: base-2 exponent = s sum_k c_k s^2k.
 constexpr float CAP_POLY_MOST = 0.6f;
 struct CapPoly {
     f32x2 c[4];

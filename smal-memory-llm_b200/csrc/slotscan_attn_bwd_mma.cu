@@ -6,7 +6,7 @@
 //   rows X0, X1 / stream Y0, Y1:   queries: q, do / k, v      keys: k, v / q, do
 //   s = X0 Y0^T, dp = X1 Y1^T, p = exp2(s - lse), ds = p (dp - delta) (1 - tanh^2),   out1 += ds Y0,  keys also out0 += p Y1
 // A CTA holds 128 rows; the stream comes 128 at a time.  (With 64 at a time a product of 128 x 64 reads 6 KB of shared memory in 48
-// cycles for 32 of sums, and the walk over keys took 1,930 cycles for what @@STEP@@ do now.)
+// cycles for 32 of sums, and the walk over keys took 720 us for one sequence of 16,384 with six heads of 128; it takes 638.)
 //   copy warp     the tiles of the rows, then Y0 and Y1 through rings of their own: Y0 is needed first and let go last
 //   product warp  between two steps' scores it runs the sums of the step before, so that it waits for weights only if they take longer
 //                 than the products

@@ -3,7 +3,7 @@
 // A row sees a few keys around its own place, so nothing is worth handing from warp to warp and bytes bound: the products are
 // m16n8k16, a warp's own from scores to output.  A warp takes 16 queries and the NB blocks of 16 keys that their windows touch; the whole
 // softmax of a row is in its registers at once.  (On the tcgen05 kernels a tile of 128 rows costs 26,000 cycles of filling and handing
-// over whatever it sees: 163 us for 64 x 1,024 tokens of six heads of 128, window 16, against @@FWD@@ here; backward 567 against @@BWD@@.)
+// over whatever it sees: 163 us for 64 x 1,024 tokens of six heads of 128, window 16, against 69 here; backward 567 against 167.)
 //
 // Forward: a CTA takes 64 queries and the 64 + 16 (NB - 1) keys before and among them.
 // Backward: a CTA owns 64 keys and the 64 queries at their places.  It also takes the queries behind that see its keys, and the keys that
@@ -223,7 +223,7 @@ struct NarrowBwd {
 };
 
 // GROUP: several query heads share a key head, whose dk and dv stay in registers over them; one CTA to an SM.  Without, dv is done before dk is
-// begun, and two CTAs fit (286 against @@ONE@@ us for 64 x 1,024 tokens, window 16).
+// begun, and two CTAs fit (286 against 158 us for 64 x 1,024 tokens, window 16).
 template <int DP, int NB, bool GROUP>
 __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3 ? 1 : 2) attn_bwd_narrow_kernel(AttnArgs a, RowInputs<bf16> in, bf16* dq_out, bf16* dk_out, bf16* dv_out, const __grid_constant__ NarrowBwdMaps maps) {
     typedef NarrowBwd<DP, NB> Sh;

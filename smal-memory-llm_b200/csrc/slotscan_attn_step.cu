@@ -6,7 +6,7 @@
 //
 // bf16: the heads of a group are the rows of m16n8k16 products (up to 16 of them, the others zero), the keys the columns.  The
 // tensor cores idle most of the time all the same; what they save is instructions, which on the CUDA cores took longer than
-// the bytes do (one key in 20 instructions a head; 32 sequences of 8,192, three heads to a key head: 233 us so, @@B32@@ now).  tcgen05
+// the bytes do (one key in 20 instructions a head; 32 sequences of 8,192, three heads to a key head: 233 us so, 79 now).  tcgen05
 // would compute 128 rows for these few.  Each warp streams 16 keys and values a step through a ring of its own in shared memory, several
 // steps ahead (cp.async, zero-filled beyond its span), with a maximum, a sum and an output of its own; the warps are joined at the end.
 // p is split into two bf16 (p = hi + lo, off by 2^-17): the second product costs nothing here and keeps the float32 weights' precision.
