@@ -4,8 +4,9 @@ attention over the tokens themselves, for a training step, a prompt and single t
 The reference runs a 16-token causal window beside its memory and leaves it to library calls (gqa25/memlm_sh.py:349-359, the rotated
 queries and keys of memlm_kv.py); here each piece is a CUDA kernel of libslotscan.so with no other implementation behind it.
 
-Small calls are bound by their host side, so what depends on the arguments' shapes, strides and types alone -- the checks, the
-parameters of the C call, scratch sizes -- is worked out once per such signature (the `_..._plan` functions) and looked up after that.
+Small calls are bound by their host side, so an ordinary eager call whose tensors the kernels take as they are goes through
+`_tokens_host` (csrc/slotscan_tokens_host.cpp): checks, outputs, launch and autograd in C++ over the same C ABI.  What that hands back as
+None is checked here, with the errors, converted, and given to it once more.  Tracing, compiling and other modes take the registered ops.
 """
 import ctypes
 import functools
@@ -15,11 +16,32 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _Here, _require_cuda, _stream, plain_call, plain_grads, wants_grad
+from .ops import _Here, _require_cuda, _stream, plain_call, wants_grad
 
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _SIZE = {torch.float32: 4, torch.bfloat16: 2}
 _getDevice = torch._C._cuda_getDevice
+_host_module = None
+
+
+def _host():
+    """The C++ host module; an exception if it is not built."""
+    global _host_module
+    if _host_module is None:
+        _lib.lib()                                                     # the C-ABI library first: its errors name what is missing
+        try:
+            from . import _tokens_host
+        except ImportError as e:
+            raise RuntimeError("_tokens_host.so is not built or not loadable (%s): build it with `make -C smal-memory-llm_b200`" % e) from e
+        _host_module = _tokens_host
+    return _host_module
+
+
+def _taken(what, out):
+    """What a call through the host module gave; the only causes left of a second None are these."""
+    if out is None:
+        raise ValueError("%s: all tensors must be on one device, and no size may pass 2^31 - 1" % what)
+    return out
 
 
 def _sig(t):
@@ -46,11 +68,17 @@ def _laid(t):
 
 
 def _f32(t):
-    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.float().contiguous()
+    if t is None:
+        return None
+    t = t.float().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _i32(t):
-    return t if t is None or (t.dtype is torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+    if t is None:
+        return None
+    t = t.to(torch.int32).contiguous()
+    return t if t.data_ptr() % 8 == 0 or t.dim() < 3 else t.clone()    # document bounds are read in pairs
 
 
 def _whole(g, dtype):
@@ -80,11 +108,6 @@ def _launch(dev, name, *args):
 def _type_check(what, *sigs):
     if any(s[2] not in _CODE or s[2] != sigs[0][2] for s in sigs):
         raise TypeError("%s: float32 or bfloat16 tensors, all of one type" % what)
-
-
-def _first_order(*grads):
-    """Whether a backward may go round the registered op: ordinary gradients, and none of a higher order wanted, which the op refuses."""
-    return not torch.is_grad_enabled() and plain_grads(*grads)
 
 
 # ---------------------------------------------------------------------------------------- norms and rotation
@@ -179,27 +202,13 @@ def _as(grad, weight):
     return None if weight is None else grad if grad.dtype is weight.dtype else grad.to(weight.dtype)
 
 
-def _norm_backward(ctx, dqo, dko, bwd=None):
+def _norm_backward(ctx, dqo, dko):
     q, k, table, pos, qw, kw = ctx.saved_tensors
-    dq, dk, dqw, dkw = (bwd or _norm_bwd_op)(q, k, table, pos, qw, kw, dqo, dko, ctx.eps)
+    dq, dk, dqw, dkw = _norm_bwd_op(q, k, table, pos, qw, kw, dqo, dko, ctx.eps)
     return dq, dk, None, None, _as(dqw, qw), _as(dkw, kw), None
 
 
 _norm_op.register_autograd(_norm_backward, setup_context=_norm_setup)
-
-
-class _Norm(torch.autograd.Function):
-    """norm_rope_fwd and its backward for a plain_call."""
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        out = _norm_fwd(*inputs)
-        _norm_setup(ctx, inputs, out)
-        return out
-
-    @staticmethod
-    def backward(ctx, dqo, dko):
-        return _norm_backward(ctx, dqo, dko, bwd=_norm_bwd if _first_order(dqo, dko) else None)
 
 
 def rope_table(length, rot, theta=10000.0, device=None):
@@ -218,7 +227,12 @@ def norm_rope(q, k, table, q_weight=None, k_weight=None, pos=None, eps=1e-6):
     ts = (q, k, table, pos, q_weight, k_weight)
     if not plain_call(*ts):
         return _norm_op(*ts, float(eps))
-    return _Norm.apply(*ts, float(eps)) if wants_grad(*ts) else _norm_fwd(*ts, float(eps))
+    out = _host().norm_rope(q, k, table, q_weight, k_weight, pos, eps)
+    if out is None:
+        _require_cuda(*ts)
+        q, k, table, pos, q_weight, k_weight, _ = _norm_call(*ts, float(eps))
+        out = _taken("norm_rope", _host().norm_rope(q, k, table, q_weight, k_weight, pos, eps))
+    return out
 
 
 def _caches(what, k_cache, v_cache, dtype):
@@ -254,8 +268,8 @@ def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps)
     return ctypes.byref(p), p
 
 
-def _append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor,
-            table: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> torch.Tensor:
+def _append_call(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps):
+    """The tensors as the kernel reads them, and the plan of the call."""
     _require_cuda(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
     rest = (_sig(k_cache), _sig(v_cache), _sig(pos), _sig(table), _sig(q_weight), _sig(k_weight), eps)
     plan = _append_plan(_sig(q), _sig(k), _sig(v), *rest)
@@ -263,7 +277,12 @@ def _append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Te
         q, k, v = _laid(q), _laid(k), _laid(v)
         plan = _append_plan(_sig(q), _sig(k), _sig(v), *rest)
     _cache_bases("norm_rope_append", k_cache, v_cache)
-    table, pos, qw, kw = _f32(table), _i32(pos), _f32(q_weight), _f32(k_weight)
+    return q, k, v, k_cache, v_cache, _i32(pos), _f32(table), _f32(q_weight), _f32(k_weight), plan
+
+
+def _append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor,
+            table: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> torch.Tensor:
+    q, k, v, k_cache, v_cache, pos, table, qw, kw, plan = _append_call(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps)
     qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _launch(q.device, "slotscan_norm_rope_append", plan[0], _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(pos), _ptr(qw), _ptr(kw), _ptr(qo),
             _ptr(k_cache), _ptr(v_cache))
@@ -284,7 +303,13 @@ def norm_rope_append(q, k, v, k_cache, v_cache, pos, table, q_weight=None, k_wei
     ts = (q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
     if wants_grad(*ts):
         raise ValueError("norm_rope_append: forward only; use norm_rope where a gradient is wanted")
-    return (_append if plain_call(*ts) else _append_op)(*ts, float(eps))
+    if not plain_call(*ts):
+        return _append_op(*ts, float(eps))
+    out = _host().norm_rope_append(*ts, eps)
+    if out is None:
+        *ts, _ = _append_call(*ts, float(eps))
+        out = _taken("norm_rope_append", _host().norm_rope_append(*ts, eps))
+    return out
 
 
 # ---------------------------------------------------------------------------------------- attention
@@ -384,26 +409,12 @@ def _attn_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)                                   # no zeros for what has no gradient
 
 
-def _attn_backward(ctx, do, _, __, bwd=None):
-    dq, dk, dv = (bwd or _attn_bwd_op)(*ctx.saved_tensors, do, ctx.window, ctx.cap, ctx.scale)
+def _attn_backward(ctx, do, _, __):
+    dq, dk, dv = _attn_bwd_op(*ctx.saved_tensors, do, ctx.window, ctx.cap, ctx.scale)
     return dq, dk, dv, None, None, None, None, None, None, None
 
 
 _attn_op.register_autograd(_attn_backward, setup_context=_attn_setup)
-
-
-class _Attn(torch.autograd.Function):
-    """attn_fwd and its backward for a plain_call."""
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        out = _attn_fwd(*inputs)
-        _attn_setup(ctx, inputs, out)
-        return out
-
-    @staticmethod
-    def backward(ctx, do, _, __):
-        return _attn_backward(ctx, do, None, None, bwd=_attn_bwd if _first_order(do) else None)
 
 
 def _numbers(what, D, window, cap, scale, slopes):
@@ -411,7 +422,8 @@ def _numbers(what, D, window, cap, scale, slopes):
         raise ValueError("%s: a window of %s and a cap of %s: both are 0 (none) or positive" % (what, window, cap))
     if slopes is not None and slopes.requires_grad:
         raise ValueError("%s: the slopes of the distance bias are constants; they have no gradient" % what)
-    return int(window), float(cap), float(D ** -0.5 if scale is None else scale)
+    window = int(window) if window < 2 ** 31 - 1 else 0                # further than any two tokens can be apart
+    return window, float(cap), float(D ** -0.5 if scale is None else scale)
 
 
 def document_bounds(doc):
@@ -441,7 +453,12 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
     ts = (q, k, v, slopes, docs, prefix)
     if not plain_call(*ts):
         return _attn_op(*ts, window, cap, scale, True)[0]
-    return _Attn.apply(*ts, window, cap, scale, True)[0] if wants_grad(q, k, v) else _attn_fwd(*ts, window, cap, scale, False)[0]
+    out = _host().token_attention(*ts, window, cap, scale)
+    if out is None:
+        _require_cuda(*ts)
+        *ts, _ = _attn_call(*ts, window, cap, scale)
+        out = _taken("token_attention", _host().token_attention(*ts, window, cap, scale))
+    return out
 
 
 @functools.lru_cache(maxsize=256)
@@ -463,8 +480,8 @@ def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
     return None if qs is None else ctypes.byref(p), _lib.lib().slotscan_attn_step_scratch_bytes(ctypes.byref(p)), p
 
 
-def _step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor],
-          start: Optional[torch.Tensor], window: int, cap: float, scale: float) -> torch.Tensor:
+def _step_call(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
+    """The tensors as the kernel reads them, and the plan of the call."""
     _require_cuda(q, k_cache, v_cache, pos, slopes, start)
     rest = (_sig(k_cache), _sig(v_cache), _sig(pos), _sig(slopes), _sig(start), window, cap, scale)
     plan = _step_plan(_sig(q), *rest)
@@ -472,7 +489,12 @@ def _step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: to
         q = _laid(q)
         plan = _step_plan(_sig(q), *rest)
     _cache_bases("token_attention_step", k_cache, v_cache)
-    pos, start, slopes = _i32(pos), _i32(start), _f32(slopes)
+    return q, k_cache, v_cache, _i32(pos), _f32(slopes), _i32(start), plan
+
+
+def _step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor],
+          start: Optional[torch.Tensor], window: int, cap: float, scale: float) -> torch.Tensor:
+    q, k_cache, v_cache, pos, slopes, start, plan = _step_call(q, k_cache, v_cache, pos, slopes, start, window, cap, scale)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     scratch = torch.empty(plan[1], dtype=torch.uint8, device=q.device) if plan[1] else None
     _launch(q.device, "slotscan_attn_step", plan[0], _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(pos), _ptr(start), _ptr(slopes), _ptr(o),
@@ -496,4 +518,10 @@ def token_attention_step(q, k_cache, v_cache, pos, window=0, cap=0.0, slopes=Non
     ts = (q, k_cache, v_cache, pos, slopes, start)
     if wants_grad(*ts):
         raise ValueError("token_attention_step: forward only; use token_attention where a gradient is wanted")
-    return (_step if plain_call(*ts) else _step_op)(*ts, window, cap, scale)
+    if not plain_call(*ts):
+        return _step_op(*ts, window, cap, scale)
+    out = _host().token_attention_step(*ts, window, cap, scale)
+    if out is None:
+        *ts, _ = _step_call(*ts, window, cap, scale)
+        out = _taken("token_attention_step", _host().token_attention_step(*ts, window, cap, scale))
+    return out

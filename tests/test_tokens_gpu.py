@@ -559,3 +559,71 @@ def test_registered_ops_give_the_same():
         b = S.token_attention_step(a, kc, vc, pos, window=1)
     assert torch.equal(kc[:, 3], S.norm_rope(d[0][:, :1], d[1][:, :1], table, pos=pos.view(1, 1))[1][:, 0])
     assert torch.equal(b, S.token_attention_step(a, kc, vc, pos, window=1)) and (b[0, 0] - d[2][0, 0]).abs().max() < 1e-6
+
+
+def test_converted_arguments():
+    """bf16 weights and wider integers are converted with their gradients, unaligned small tensors are copied; weights that bf16 holds exactly
+    give the same bits, and their gradients the same numbers rounded once."""
+    S = _S()
+    g = _gen(31)
+    x, kx = [_rand(g, 2, 33, H, 64).bfloat16().requires_grad_() for H in (4, 2)]
+    w16 = (1 + 0.1 * _rand(g, 64)).bfloat16()
+    w = [w16.float().requires_grad_(), w16.clone().requires_grad_()]
+    table = S.rope_table(40, 64, device="cuda")
+    odd = torch.cat((table.flatten()[:1], table.flatten()))[1:].view(table.shape)
+    pos = torch.arange(7, 40, device="cuda").expand(2, -1)
+    go, gk = torch.randn_like(x), torch.randn_like(kx)
+    out = [S.norm_rope(x, kx, t, y, y, p) for t, y, p in ((table, w[0], pos.int().contiguous()), (odd, w[1], pos))]
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    grads = [torch.autograd.grad(o, (x, kx, y), (go, gk)) for o, y in zip(out, w)]
+    assert all(torch.equal(a, b) for a, b in zip(grads[0][:2], grads[1][:2]))
+    # the one weight stands for two: each use is converted by itself, so its two gradients are rounded and then added
+    two = [w16.float().requires_grad_() for _ in range(2)]
+    dw = torch.autograd.grad(S.norm_rope(x, kx, table, *two, pos.int().contiguous()), two, (go, gk))
+    assert torch.equal(grads[0][2], dw[0] + dw[1]) and torch.equal(grads[1][2], dw[0].bfloat16() + dw[1].bfloat16())
+
+    q, k, v = [_rand(g, 2, 50, H, 64).bfloat16().requires_grad_() for H in (4, 2, 2)]
+    docs = S.document_bounds((torch.arange(50, device="cuda") // 20).expand(2, -1).contiguous())
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625], device="cuda")
+    do = torch.randn_like(q)
+    a = S.token_attention(q, k, v, docs=docs, slopes=slopes)
+    b = S.token_attention(q, k, v, docs=docs.long(), slopes=slopes.double())
+    shifted = torch.cat((docs.flatten()[:1], docs.flatten()))[1:].view(docs.shape)
+    c = S.token_attention(q, k, v, docs=shifted, slopes=slopes.bfloat16())
+    assert torch.equal(a, b) and torch.equal(a, c)
+    want = torch.autograd.grad(a, (q, k, v), do)
+    assert all(torch.equal(m, n) for m, n in zip(want, torch.autograd.grad(c, (q, k, v), do.transpose(1, 2).contiguous().transpose(1, 2))))
+    huge = S.token_attention(q, k, v, window=2 ** 40)
+    assert torch.equal(huge, S.token_attention(q, k, v))
+
+    kc, vc = [torch.zeros(2, 16, 2, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    kd, vd = kc.clone(), vc.clone()
+    at = torch.tensor([3, 30], device="cuda")
+    with torch.no_grad():
+        p = S.norm_rope_append(q[:, :5], k[:, :5], v[:, :5], kc, vc, at.int(), table, w[0], w[0])
+        r = S.norm_rope_append(q[:, :5], k[:, :5], v[:, :5], kd, vd, at, odd, w16, w16)
+        assert torch.equal(p, r) and torch.equal(kc, kd) and torch.equal(vc, vd)
+        s = S.token_attention_step(p[:, :1], kc, vc, at.int(), slopes=slopes)
+        assert torch.equal(s, S.token_attention_step(p[:, :1].transpose(1, 2).contiguous().transpose(1, 2), kc, vc, at, slopes=slopes.double()))
+
+
+def test_saved_tensors_are_watched():
+    """A tensor that the backward reads may not change in between; hooks of saved tensors see what is kept; unused outputs need no gradient."""
+    S = _S()
+    g, q, k, v, do = _attn_inputs("bf16", 1, 90, 90, 2, 1, 64, seed=33)
+    x = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    o = S.token_attention(*x)
+    want = torch.autograd.grad(o, x, do, retain_graph=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        got = torch.autograd.grad(S.token_attention(*x), x, do)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with torch.no_grad():
+        x[1].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o, x, do)
+    table = S.rope_table(90, 64, device="cuda")
+    y = [t.detach().requires_grad_() for t in (q, k)]
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    only_q = S.norm_rope(*y, table, w, None)[0]
+    dq, dk, dw = torch.autograd.grad(only_q, (*y, w), do)
+    assert not dk.any() and dq.abs().max() > 0 and dw.abs().max() > 0
