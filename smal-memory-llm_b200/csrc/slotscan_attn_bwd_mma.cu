@@ -11,6 +11,9 @@
 //   product warp  between two steps' scores it runs the sums of the step before, so that it waits for weights only if they take longer
 //                 than the products
 //   16 warps      form the weights, a thread 32 columns of a row: p as soon as s is there, ds when dp is
+// A barrier serves every step where its next round needs what the warp that waits on it does after the wait.  With rows of queries that
+// does not hold for ds: both scores of a step are issued before the ds of the step before are waited for, so warps may hand over two
+// steps' ds before the product warp looks at the first.  ds has two barriers in turn; the third step's needs the wait for the first.
 // Tensor memory, 512 columns:  rows of queries:  s | dp | dq | 2 x ds;   rows of keys:  s, p written over it | dp, ds over it | dk | dv
 // Weights are bf16 where the sums' products read them as their first operand; a group of 32 columns' weights lie where its scores
 // lay, which its own threads have read.
@@ -45,7 +48,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
     extern __shared__ __align__(1024) char smem[];
     char *X0 = smem, *X1 = smem + Sh::TILE, *Y0 = X1 + Sh::TILE, *Y1 = Y0 + AB_R0 * Sh::TILE;
     float* s_stat = reinterpret_cast<float*>(Y1 + AB_R1 * Sh::TILE);               // [2][2][128] -lse, -delta of the stream's queries
-    __shared__ uint64_t x_full, done, s_full, d_full, s_read, d_read, p_full, ds_full, full0[AB_R0], full1[AB_R1], empty0[AB_R0], empty1[AB_R1];
+    __shared__ uint64_t x_full, done, s_full, d_full, s_read, d_read, p_full, ds_full[2], full0[AB_R0], full1[AB_R1], empty0[AB_R0], empty1[AB_R1];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     __shared__ TileSpan s_span;
@@ -56,7 +59,8 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
     const int hx = hb % (heads / a.B), b = hb / (heads / a.B), hk = KEYS ? hx : hx / group, x0 = tile * 128;
     if (tid == 0) {
         mbar_init(&x_full, 1); mbar_init(&done, 1); mbar_init(&s_full, 1); mbar_init(&d_full, 1);
-        mbar_init(&s_read, AB_WARPS); mbar_init(&d_read, AB_WARPS); mbar_init(&p_full, AB_WARPS); mbar_init(&ds_full, AB_WARPS);
+        mbar_init(&s_read, AB_WARPS); mbar_init(&d_read, AB_WARPS); mbar_init(&p_full, AB_WARPS);
+        for (int i = 0; i < 2; i++) mbar_init(&ds_full[i], AB_WARPS);
         for (int i = 0; i < AB_R0; i++) { mbar_init(&full0[i], 1); mbar_init(&empty0[i], 1); }
         for (int i = 0; i < AB_R1; i++) { mbar_init(&full1[i], 1); mbar_init(&empty1[i], 1); }
         mbar_fence_init();
@@ -245,7 +249,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
             tmem_st_wait();
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) arrive(&ds_full);
+            if (lane == 0) arrive(&ds_full[s & 1]);
         }
         if (ok && steps > 0) ok = wait_soon(&done, 0);
         tmem_fence_after();
@@ -354,7 +358,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                     tmem_fence_after();
                     sums(s, 1);
                     if (more && !(ok = scores(s + 1, 0))) break;
-                    if (!(ok = wait_soon_warp(&ds_full, s & 1))) break;
+                    if (!(ok = wait_soon_warp(&ds_full[s & 1], (s >> 1) & 1))) break;
                     tmem_fence_after();
                     sums(s, 0);
                     if (more && !(ok = scores(s + 1, 1))) break;
@@ -367,7 +371,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                         tmem_fence_after();
                         if (!(ok = scores(s + 1, 1))) break;
                     }
-                    if (!(ok = wait_soon_warp(&ds_full, s & 1))) break;
+                    if (!(ok = wait_soon_warp(&ds_full[s & 1], (s >> 1) & 1))) break;
                     tmem_fence_after();
                     sums(s, 0);
                 }

@@ -627,3 +627,23 @@ def test_saved_tensors_are_watched():
     only_q = S.norm_rope(*y, table, w, None)[0]
     dq, dk, dw = torch.autograd.grad(only_q, (*y, w), do)
     assert not dk.any() and dq.abs().max() > 0 and dw.abs().max() > 0
+
+
+def test_long_runs_hand_over_every_step():
+    """The warps of the backward pass thousands of steps' weights to each other; with some luck of the timing they run two steps apart.  No
+    wait gives up and every run has the same bits (a hand-over lost once in some thousand calls)."""
+    from slotscan_b200 import _lib
+    S = _S()
+    g, q, k, v, do = _attn_inputs("bf16", 1, 8192, 8192, 6, 6, 128, seed=35)
+    cuts = [0, 700, 2900, 3000, 4700, 4701, 6900, 8192]
+    doc = torch.cat([torch.full((b - a,), i if i != 3 else -1) for i, (a, b) in enumerate(zip(cuts, cuts[1:]))]).cuda()[None]
+    docs, slopes = S.document_bounds(doc), torch.linspace(0.02, 0.5, 6, device="cuda")
+    x = [t.detach().requires_grad_() for t in (q, k, v)]
+    _lib.lib().slotscan_device_status()
+    first, off = None, torch.zeros((), dtype=torch.long, device="cuda")
+    for _ in range(2000):
+        got = torch.autograd.grad(S.token_attention(*x, docs=docs, slopes=slopes), x, do)
+        first = first or got
+        for a, b in zip(got, first):
+            off += (a != b).any()
+    assert int(off) == 0 and _lib.lib().slotscan_device_status() == 0
