@@ -1,26 +1,30 @@
 // Attention over tokens on the CUDA cores: float32, whose products the tensor cores would round to 11 bits or fewer.
 //
-// Forward: a CTA holds 64 queries of a head and passes over their keys 64 at a time, with the running maximum and sum of each
+// Forward: a CTA holds 64 or 32 queries of a head and passes over their keys 64 at a time, with the running maximum and sum of each
 // row's softmax.  Backward: the same walk twice, once with rows of queries (dq, and delta = <do, o> for the other), once with
 // rows of keys over the queries of all heads that share the key head (dk, dv): one more pair of products than a single walk with
 // atomic sums would take, and the same bits from run to run.
 //   rows X0, X1 / stream Y0, Y1:   queries: q, do / k, v      keys: k, v / q, do
 //   s = X0 Y0^T, dp = X1 Y1^T, p = exp(s - lse), ds = p (dp - delta) (1 - tanh^2),  out1 += ds Y0,  keys also out0 += p Y1
-// Bound by shared memory: two 16-byte reads for 8 multiply-adds of a thread's 4 x 4 block.
+// Bound by shared memory and its latency: a thread's 4 x 4 block takes eight 16-byte reads for 32 paired multiply-adds, with 8 warps on
+// an SM in the backward.  One sequence of 4,096 with six heads of 128: 33 TFLOP/s forward, 33 of its seven products backward.
+// Blocks of 2 x 4 with twice the warps took 1.4 times as long, unpaired multiply-adds 1.1 times.
+// All heads' long rows first: of the CTAs of one head after the other a third of the SMs' time was lost at the end.
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 
 namespace slotscan {
 
-constexpr int SA_THREADS = 256, SA_M = 64, SA_N = 64, SA_LDP = SA_N + 4;
+constexpr int SA_N = 64, SA_LDP = SA_N + 4;              // rows of a step of the stream
+constexpr int SA_SMS = 148;
 
 template <typename T>
 __device__ __forceinline__ float4 ld4or0(const T* p, bool ok) { return ok ? ld4(p) : make_float4(0.f, 0.f, 0.f, 0.f); }
 
-// rows [r0, r0 + 64) of a strided matrix into shared memory, zeros beyond `rows` and beyond D channels
-template <int DP, typename T>
+// rows [r0, r0 + N) of a strided matrix into shared memory, zeros beyond `rows` and beyond D channels
+template <int DP, int N, int THREADS, typename T>
 __device__ __forceinline__ void load_tile(float* dst, const T* src, long long stride, int r0, int rows, int D) {
-    for (int i = threadIdx.x; i < SA_M * (DP / 4); i += SA_THREADS) {
+    for (int i = threadIdx.x; i < N * (DP / 4); i += THREADS) {
         const int r = i / (DP / 4), c = i % (DP / 4) * 4;
         st4(dst + r * (DP + 4) + c, ld4or0(src + (long long)(r0 + r) * stride + c, r0 + r < rows && c < D));
     }
@@ -28,23 +32,30 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, long long st
 // C[r][c] = <A row 4 ty + r, B row tx + 16 c>
 template <int DP>
 __device__ __forceinline__ void dot_block(float (&C)[4][4], const float* A, const float* Bm, int ty, int tx) {
+    f32x2 sum[4][4];                                     // of the even and of the odd channels
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) C[r][c] = 0.f;
+        for (int c = 0; c < 4; c++) sum[r][c] = pack2(0.f, 0.f);
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
-        float4 x[4], y[4];
+        f32x4 x[4], y[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) x[r] = ld4(A + (4 * ty + r) * (DP + 4) + d);
+        for (int r = 0; r < 4; r++) x[r] = pack4(ld4(A + (4 * ty + r) * (DP + 4) + d));
 #pragma unroll
-        for (int c = 0; c < 4; c++) y[c] = ld4(Bm + (tx + 16 * c) * (DP + 4) + d);
+        for (int c = 0; c < 4; c++) y[c] = pack4(ld4(Bm + (tx + 16 * c) * (DP + 4) + d));
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                C[r][c] = fmaf(x[r].x, y[c].x, fmaf(x[r].y, y[c].y, fmaf(x[r].z, y[c].z, fmaf(x[r].w, y[c].w, C[r][c]))));
+            for (int c = 0; c < 4; c++) sum[r][c] = fma2(x[r].b, y[c].b, fma2(x[r].a, y[c].a, sum[r][c]));
     }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float2 t = unpack2(sum[r][c]);
+            C[r][c] = t.x + t.y;
+        }
 }
 // acc[r][8 channels of tx] += sum_j P[4 ty + r][j] Y[j]
 template <int DP>
@@ -57,14 +68,17 @@ __device__ __forceinline__ void product_block(float (&acc)[4][DP / 16], const fl
         for (int jj = 0; jj < 4; jj++) {
 #pragma unroll
             for (int c = 0; c < DP / 64; c++) {
-                const float4 y = ld4(Y + (j + jj) * (DP + 4) + tx * 4 + 64 * c);
+                const f32x4 y = pack4(ld4(Y + (j + jj) * (DP + 4) + tx * 4 + 64 * c));
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float w = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
-                    acc[r][4 * c] = fmaf(w, y.x, acc[r][4 * c]);
-                    acc[r][4 * c + 1] = fmaf(w, y.y, acc[r][4 * c + 1]);
-                    acc[r][4 * c + 2] = fmaf(w, y.z, acc[r][4 * c + 2]);
-                    acc[r][4 * c + 3] = fmaf(w, y.w, acc[r][4 * c + 3]);
+                    const f32x2 w2 = pack2(w, w);
+                    const float2 lo = unpack2(fma2(w2, y.a, pack2(acc[r][4 * c], acc[r][4 * c + 1])));
+                    const float2 hi = unpack2(fma2(w2, y.b, pack2(acc[r][4 * c + 2], acc[r][4 * c + 3])));
+                    acc[r][4 * c] = lo.x;
+                    acc[r][4 * c + 1] = lo.y;
+                    acc[r][4 * c + 2] = hi.x;
+                    acc[r][4 * c + 3] = hi.y;
                 }
             }
         }
@@ -105,23 +119,23 @@ __device__ __forceinline__ void again_where_not_finite(const float (&acc)[4][N],
     }
 }
 
-template <int DP, typename T>
-__global__ void __launch_bounds__(SA_THREADS) attn_fwd_cores_kernel(AttnArgs a, const T* q, const T* k, const T* v, T* o, float* lse) {
+template <int DP, int M, typename T>
+__global__ void __launch_bounds__(4 * M, M == 64 ? 2 : 3) attn_fwd_cores_kernel(AttnArgs a, const T* q, const T* k, const T* v, T* o, float* lse) {
     extern __shared__ float4 smem4[];
     float* Qs = reinterpret_cast<float*>(smem4);
-    float* Ys = Qs + SA_M * (DP + 4);                    // keys, then values
+    float* Ys = Qs + M * (DP + 4);                    // keys, then values
     float* Ps = Ys + SA_N * (DP + 4);
     __shared__ int s_red[2];
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-    const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.KV);
-    const int i0 = (gridDim.x - 1 - blockIdx.x) * SA_M;                            // the long rows first
+    const int heads = a.H * a.B, h = blockIdx.x % heads % a.H, b = blockIdx.x % heads / a.H, hk = h / (a.H / a.KV);
+    const int i0 = ((a.Tq + M - 1) / M - 1 - (int)(blockIdx.x / heads)) * M;       // the long rows of all heads first
     const T* kb = k + b * a.ks[0] + hk * a.ks[2];
     const T* vb = v + b * a.vs[0] + hk * a.vs[2];
-    load_tile<DP>(Qs, q + b * a.qs[0] + h * a.qs[2], a.qs[1], i0, a.Tq, a.D);
+    load_tile<DP, M, 4 * M>(Qs, q + b * a.qs[0] + h * a.qs[2], a.qs[1], i0, a.Tq, a.D);
     Span sp[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) sp[r] = i0 + 4 * ty + r < a.Tq ? keys_of(a, b, i0 + 4 * ty + r) : Span{0, 0};
-    const Span all = cta_span(i0 + tid < a.Tq && tid < SA_M ? keys_of(a, b, i0 + tid) : Span{0, 0}, tid < SA_M, s_red);
+    const Span all = cta_span(i0 + tid < a.Tq && tid < M ? keys_of(a, b, i0 + tid) : Span{0, 0}, tid < M, s_red);
     const Score sc(a, h);
     float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
@@ -132,7 +146,7 @@ __global__ void __launch_bounds__(SA_THREADS) attn_fwd_cores_kernel(AttnArgs a, 
     }
     for (int j0 = all.lo; j0 < all.hi; j0 += SA_N) {
         __syncthreads();
-        load_tile<DP>(Ys, kb, a.ks[1], j0, a.Tk, a.D);
+        load_tile<DP, SA_N, 4 * M>(Ys, kb, a.ks[1], j0, a.Tk, a.D);
         __syncthreads();
         float s[4][4];
         dot_block<DP>(s, Qs, Ys, ty, tx);
@@ -163,7 +177,7 @@ __global__ void __launch_bounds__(SA_THREADS) attn_fwd_cores_kernel(AttnArgs a, 
             for (int c = 0; c < DP / 16; c++) acc[r][c] *= shrink[r];
         }
         __syncthreads();
-        load_tile<DP>(Ys, vb, a.vs[1], j0, a.Tk, a.D);
+        load_tile<DP, SA_N, 4 * M>(Ys, vb, a.vs[1], j0, a.Tk, a.D);
         __syncthreads();
         product_block<DP>(acc, Ps, Ys, ty, tx);
     }
@@ -191,37 +205,38 @@ __global__ void __launch_bounds__(SA_THREADS) attn_fwd_cores_kernel(AttnArgs a, 
 }
 
 // KEYS: rows of keys (dk, dv); else rows of queries (dq, and delta)
-template <int DP, bool KEYS, typename T>
-__global__ void __launch_bounds__(SA_THREADS) attn_bwd_cores_kernel(AttnArgs a, const T* q, const T* k, const T* v, const T* o, const float* lse,
+template <int DP, int M, bool KEYS, typename T>
+__global__ void __launch_bounds__(4 * M, DP == 64 ? 2 : 1) attn_bwd_cores_kernel(AttnArgs a, const T* q, const T* k, const T* v, const T* o, const float* lse,
                                                                     const T* dout, float* delta, T* d0, T* d1) {
     extern __shared__ float4 smem4[];
     float* X0 = reinterpret_cast<float*>(smem4);
-    float* X1 = X0 + SA_M * (DP + 4);
-    float* Y0 = X1 + SA_M * (DP + 4);
+    float* X1 = X0 + M * (DP + 4);
+    float* Y0 = X1 + M * (DP + 4);
     float* Y1 = Y0 + SA_N * (DP + 4);
     float* Ps = Y1 + SA_N * (DP + 4);
-    float* Ds = Ps + SA_M * SA_LDP;
+    float* Ds = Ps + M * SA_LDP;
     __shared__ int s_red[2];
     __shared__ float s_lse[64], s_delta[64];             // of the queries: this CTA's rows, or the stream's
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16, group = a.H / a.KV;
-    const int hx = blockIdx.y, b = blockIdx.z, off = a.Tk - a.Tq, rows = KEYS ? a.Tk : a.Tq, cols = KEYS ? a.Tq : a.Tk;
-    const int r0 = blockIdx.x * SA_M;
+    const int hs = KEYS ? a.KV : a.H, heads = hs * a.B, hx = blockIdx.x % heads % hs, b = blockIdx.x % heads / hs;
+    const int off = a.Tk - a.Tq, rows = KEYS ? a.Tk : a.Tq, cols = KEYS ? a.Tq : a.Tk, tile = (int)(blockIdx.x / heads);
+    const int r0 = (KEYS ? tile : (a.Tq + M - 1) / M - 1 - tile) * M;              // the long rows of all heads first
     const int hk = KEYS ? hx : hx / group;
     const long long os = (long long)a.H * a.D;           // of o and dout: contiguous
     const T* kb = k + b * a.ks[0] + hk * a.ks[2];
     const T* vb = v + b * a.vs[0] + hk * a.vs[2];
     if constexpr (KEYS) {
-        load_tile<DP>(X0, kb, a.ks[1], r0, rows, a.D);
-        load_tile<DP>(X1, vb, a.vs[1], r0, rows, a.D);
+        load_tile<DP, M, 4 * M>(X0, kb, a.ks[1], r0, rows, a.D);
+        load_tile<DP, M, 4 * M>(X1, vb, a.vs[1], r0, rows, a.D);
     } else {
-        load_tile<DP>(X0, q + b * a.qs[0] + hx * a.qs[2], a.qs[1], r0, rows, a.D);
-        load_tile<DP>(X1, dout + (size_t)b * a.Tq * os + hx * a.D, os, r0, rows, a.D);
+        load_tile<DP, M, 4 * M>(X0, q + b * a.qs[0] + hx * a.qs[2], a.qs[1], r0, rows, a.D);
+        load_tile<DP, M, 4 * M>(X1, dout + (size_t)b * a.Tq * os + hx * a.D, os, r0, rows, a.D);
     }
     auto span = [&](int r) { return r >= rows ? Span{0, 0} : KEYS ? queries_of(a, b, r) : keys_of(a, b, r); };
     Span sp[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) sp[r] = span(r0 + 4 * ty + r);
-    const Span all = cta_span(tid < SA_M ? span(r0 + tid) : Span{0, 0}, tid < SA_M, s_red);
+    const Span all = cta_span(tid < M ? span(r0 + tid) : Span{0, 0}, tid < M, s_red);
     if constexpr (!KEYS) {
         // delta of a row by four lanes; the products of a row are a sum over its channels, so it needs no other row
         const int r = tid / 4, i = r0 + r;
@@ -250,8 +265,8 @@ __global__ void __launch_bounds__(SA_THREADS) attn_bwd_cores_kernel(AttnArgs a, 
         for (int y0 = all.lo; y0 < all.hi; y0 += SA_N) {
             __syncthreads();
             if constexpr (KEYS) {
-                load_tile<DP>(Y0, q + b * a.qs[0] + h * a.qs[2], a.qs[1], y0, cols, a.D);
-                load_tile<DP>(Y1, dout + (size_t)b * a.Tq * os + h * a.D, os, y0, cols, a.D);
+                load_tile<DP, SA_N, 4 * M>(Y0, q + b * a.qs[0] + h * a.qs[2], a.qs[1], y0, cols, a.D);
+                load_tile<DP, SA_N, 4 * M>(Y1, dout + (size_t)b * a.Tq * os + h * a.D, os, y0, cols, a.D);
                 if (tid < SA_N) {
                     const bool in = y0 + tid < a.Tq;
                     const size_t at = ((size_t)b * a.H + h) * a.Tq + y0 + tid;
@@ -259,8 +274,8 @@ __global__ void __launch_bounds__(SA_THREADS) attn_bwd_cores_kernel(AttnArgs a, 
                     s_delta[tid] = in ? delta[at] : 0.f;
                 }
             } else {
-                load_tile<DP>(Y0, kb, a.ks[1], y0, cols, a.D);
-                load_tile<DP>(Y1, vb, a.vs[1], y0, cols, a.D);
+                load_tile<DP, SA_N, 4 * M>(Y0, kb, a.ks[1], y0, cols, a.D);
+                load_tile<DP, SA_N, 4 * M>(Y1, vb, a.vs[1], y0, cols, a.D);
             }
             __syncthreads();
             float s[4][4], dp[4][4];
@@ -317,37 +332,58 @@ __global__ void __launch_bounds__(SA_THREADS) attn_bwd_cores_kernel(AttnArgs a, 
     again_where_not_finite(acc1, bad, again);
 }
 
-template <int DP, typename T>
+template <int DP, int M>
 static cudaError_t fwd_cores(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
-    const size_t sm = sizeof(float) * (2 * SA_M * (DP + 4) + SA_M * SA_LDP);
-    auto kern = attn_fwd_cores_kernel<DP, T>;
+    const size_t sm = sizeof(float) * ((M + SA_N) * (DP + 4) + M * SA_LDP);
+    auto kern = attn_fwd_cores_kernel<DP, M, float>;
     const cudaError_t e = opt_in_smem(kern, sm);
     if (e != cudaSuccess) return e;
-    kern<<<dim3((a.Tq + SA_M - 1) / SA_M, a.H, a.B), SA_THREADS, sm, st>>>(a, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse);
+    const long long ctas = (long long)((a.Tq + M - 1) / M) * a.H * a.B;
+    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+    kern<<<(unsigned)ctas, 4 * M, sm, st>>>(a, (const float*)q, (const float*)k, (const float*)v, (float*)o, lse);
     return cudaGetLastError();
 }
-template <int DP, typename T>
+template <int DP, int M, bool KEYS>
 static cudaError_t bwd_cores(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
-                             float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
-    const size_t sm = sizeof(float) * (4 * SA_M * (DP + 4) + 2 * SA_M * SA_LDP);
-    auto rows_q = attn_bwd_cores_kernel<DP, false, T>;
-    auto rows_k = attn_bwd_cores_kernel<DP, true, T>;
-    cudaError_t e = opt_in_smem(rows_q, sm);
-    if (e == cudaSuccess) e = opt_in_smem(rows_k, sm);
+                             float* delta, void* d0, void* d1, cudaStream_t st) {
+    const size_t sm = sizeof(float) * (2 * (M + SA_N) * (DP + 4) + 2 * M * SA_LDP);
+    auto kern = attn_bwd_cores_kernel<DP, M, KEYS, float>;
+    const cudaError_t e = opt_in_smem(kern, sm);
     if (e != cudaSuccess) return e;
-    rows_q<<<dim3((a.Tq + SA_M - 1) / SA_M, a.H, a.B), SA_THREADS, sm, st>>>(a, (const T*)q, (const T*)k, (const T*)v, (const T*)o, lse,
-                                                                            (const T*)dout, delta, nullptr, (T*)dq);
-    rows_k<<<dim3((a.Tk + SA_M - 1) / SA_M, a.KV, a.B), SA_THREADS, sm, st>>>(a, (const T*)q, (const T*)k, (const T*)v, (const T*)o, lse,
-                                                                             (const T*)dout, delta, (T*)dv, (T*)dk);
+    const long long ctas = (long long)(((KEYS ? a.Tk : a.Tq) + M - 1) / M) * (KEYS ? a.KV : a.H) * a.B;
+    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+    kern<<<(unsigned)ctas, 4 * M, sm, st>>>(a, (const float*)q, (const float*)k, (const float*)v, (const float*)o, lse, (const float*)dout, delta,
+                                            (float*)d0, (float*)d1);
     return cudaGetLastError();
+}
+// 32 rows to a CTA where 64 would leave SMs without one.  The forward and the walk over queries of 64 channels, of whose CTAs
+// several fit an SM, take 32 up to three of 64 for each SM.  With 64 rows against 32, us, forward + queries + keys:
+//   2 x 1,881 tokens, one head of 128    288 + 389 + 485     222 + 281 + 339
+//   4 x 1,024 tokens, four heads of 64   128 + 168 + 365     105 + 127 + 315
+//   1 x 4,096 tokens, six heads of 128   864 + 1,234 + 1,527     792 + 1,618 + 1,951
+//   34 x 494 tokens, twelve heads of 128     853 + 1,663 + 1,835     941 + 2,657 + 2,815
+static bool few(int rows, int heads, int B, int each) { return (long long)((rows + 63) / 64) * heads * B < each * SA_SMS; }
+
+template <int DP>
+static cudaError_t fwd_cores_rows(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
+    return few(a.Tq, a.H, a.B, 3) ? fwd_cores<DP, 32>(a, q, k, v, o, lse, st) : fwd_cores<DP, 64>(a, q, k, v, o, lse, st);
+}
+template <int DP>
+static cudaError_t bwd_cores_rows(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                                  float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
+    const cudaError_t e = few(a.Tq, a.H, a.B, DP == 64 ? 3 : 1) ? bwd_cores<DP, 32, false>(a, q, k, v, o, lse, dout, delta, nullptr, dq, st)
+                                              : bwd_cores<DP, 64, false>(a, q, k, v, o, lse, dout, delta, nullptr, dq, st);
+    if (e != cudaSuccess) return e;
+    return few(a.Tk, a.KV, a.B, 1) ? bwd_cores<DP, 32, true>(a, q, k, v, o, lse, dout, delta, dv, dk, st)
+                                : bwd_cores<DP, 64, true>(a, q, k, v, o, lse, dout, delta, dv, dk, st);
 }
 
 cudaError_t run_attn_fwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
-    return a.D <= 64 ? fwd_cores<64, float>(a, q, k, v, o, lse, st) : fwd_cores<128, float>(a, q, k, v, o, lse, st);
+    return a.D <= 64 ? fwd_cores_rows<64>(a, q, k, v, o, lse, st) : fwd_cores_rows<128>(a, q, k, v, o, lse, st);
 }
 cudaError_t run_attn_bwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
                              float* delta, void* dq, void* dk, void* dv, cudaStream_t st) {
-    return a.D <= 64 ? bwd_cores<64, float>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st)
-                     : bwd_cores<128, float>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st);
+    return a.D <= 64 ? bwd_cores_rows<64>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st)
+                     : bwd_cores_rows<128>(a, q, k, v, o, lse, dout, delta, dq, dk, dv, st);
 }
 }  // namespace slotscan
