@@ -6,12 +6,13 @@
 // A row's two sums are its only reductions, so each element is read once and written once: two rows of traffic forward, three
 // backward, and some ten operations an element.  Bandwidth bounds it.
 //
-// Layout: a group of LPG lanes (a power of two, 8 channels to a lane: one 16-byte load of bf16, two of float32) takes a token and walks
-// over a slice of its heads, queries first, with the token's cosines and sines in registers: the table of a position has the bytes of
-// two bf16 rows, and is read once for all its heads.  A pair's two channels lie R/16 lanes apart: one shuffle.  What hides a row's
-// chain of load, two sums and store is the other warps: two rows in flight to a group and four CTAs to an SM took 101 us for
-// 64 x 1,024 tokens of 6 + 6 heads of 128 (4.0 TB/s), six rows and three CTAs 113; the backward, with more to keep, 150 us (4.0 TB/s)
-// with four rows and two CTAs, 164 with three, 186 with two, 256 with two rows and three CTAs.
+// Layout: a group of LPG lanes (a power of two, 8 channels to a lane) takes a token and walks over a slice of its heads, queries first,
+// with the token's cosines and sines in registers: the table of a position has the bytes of two bf16 rows, and is read once for all its
+// heads.  A lane owns both sides of four pairs, so that a turn is its own.  Rows come ahead through shared memory, which takes no
+// registers: 4 in flight to a group and four CTAs to an SM, backward 5 rows with their gradients and two CTAs.  64 x 1,024 tokens of
+// 6 + 6 heads of 128, bf16: 76 us (5.3 TB/s), backward 120 us (5.0 TB/s).  Before: 101 and 150 us with rows in registers and a pair's
+// sides 8 lanes apart; 80 and 129 with the ring alone.  Three, five or six CTAs: 78, 85, 84 us; backward three CTAs 129, four 204.
+// float32 is as fast either way (8 x 4,096 tokens of 12 + 4 heads of 64: 44 + 71 us, 6.1 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -25,6 +26,9 @@ namespace slotscan {
 typedef __nv_bfloat16 bf16;
 constexpr int NR_THREADS = 256;
 constexpr int NR_FWD_CTAS = 4, NR_BWD_CTAS = 2;         // of an SM
+// slots of a thread's ring, one more than the rows in flight
+template <typename T> constexpr int NR_FWD_SLOTS = 5;
+template <typename T> constexpr int NR_BWD_SLOTS = sizeof(T) == 2 ? 6 : 3;
 constexpr int NR_MAX_CTAS = 148 * NR_BWD_CTAS;                     // of the backward, which sums the weights' gradients per CTA: those of one wave
 
 struct NormArgs {
@@ -41,45 +45,89 @@ struct AppendArgs {                                      // L 0: no caches
     long long vs[3], kcs[3], vcs[3];
 };
 
-// 8 channels as they lie in memory: what a row in flight costs a thread in registers
-template <typename T>
-struct Raw8 { uint4 v[sizeof(T) / 2]; };
-template <typename T>
-__device__ __forceinline__ Raw8<T> raw8(const T* p, bool in) {
-    Raw8<T> r;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.v[i] = in ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
-    return r;
+// The two pieces of four adjacent channels that a lane owns.  In the rotated part they are the two sides of four pairs, so that a turn
+// needs no other lane; beyond it they lie side by side.
+struct Pieces {
+    int at[2];
+    __device__ __forceinline__ Pieces(int c, int R) {
+        const bool rot = c * 8 < R;
+        at[0] = rot ? 4 * c : 8 * c;
+        at[1] = rot ? R / 2 + 4 * c : 8 * c + 4;
+    }
+};
+__device__ __forceinline__ void ld4x(float* x, const float* p) { const float4 v = ld4(p); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+__device__ __forceinline__ void ld4x(float* x, const bf16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u); x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void st4x(float* p, const float* x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void st4x(bf16* p, const float* x) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 template <typename T>
-__device__ __forceinline__ void widen(float (&x)[8], const Raw8<T>& r) { ld8(x, reinterpret_cast<const T*>(&r)); }
+__device__ __forceinline__ void ld_pieces(float (&x)[8], const T* row, const Pieces& pc) { ld4x(x, row + pc.at[0]); ld4x(x + 4, row + pc.at[1]); }
+template <typename T>
+__device__ __forceinline__ void st_pieces(T* row, const float (&x)[8], const Pieces& pc) { st4x(row + pc.at[0], x); st4x(row + pc.at[1], x + 4); }
 
-// cosines and sines of this lane's 8 channels; NaN where the position lies outside the table
-__device__ __forceinline__ void load_turn(const NormArgs& a, long long at, int half, int c, float (&cs)[8], float (&sn)[8]) {
-    const bool in = at >= 0 && at < a.table_len;
-    const float* t = a.table + ((size_t)(in ? at : 0) * (a.R / 2) + (c % half) * 8) * 2;
+// Rows fetched ahead into S slots of shared memory, X of them to a slot, 16-byte pieces in their own order: a group's lanes read
+// each other's.  A slot is fetched again only after the warp has met at the next one's arrival.
+template <typename T, int LPG, int X, int S>
+struct Ahead {
+    static constexpr int P = sizeof(T) / 2, BYTES = S * X * P * NR_THREADS * 16;
+    uint4* rows;                                         // the group's rows of the first slot
+    int put, get;
+    __device__ __forceinline__ explicit Ahead(uint4* ring) : rows(ring + threadIdx.x / LPG * LPG * P), put(0), get(0) {}
+    __device__ __forceinline__ uint4* row(int slot, int x) const { return rows + (slot * X + x) * P * NR_THREADS; }
+    // piece c of a row; zeros unless `in`; `from` (the row) is an address of the tensor all the same
+    __device__ __forceinline__ void fetch(int x, const T* from, int c, bool in, int D) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < P; i++) {
+            const bool piece = in && (c + i * LPG) * 16 < D * (int)sizeof(T);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(row(put, x) + c + i * LPG)),
+                         "l"(reinterpret_cast<const uint4*>(from) + (piece ? c + i * LPG : 0)), "r"(piece ? 16 : 0)
+                         : "memory");
+        }
+    }
+    __device__ __forceinline__ void fetched() {          // the slot is complete
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        put = put + 1 == S ? 0 : put + 1;
+    }
+    __device__ __forceinline__ void arrived() {          // of S - 1 fetched, the oldest
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        __syncwarp();
+    }
+    __device__ __forceinline__ void rest() {             // before the ring serves something else
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    __device__ __forceinline__ void read(int x, float (&y)[8], const Pieces& pc) const { ld_pieces(y, reinterpret_cast<const T*>(row(get, x)), pc); }
+    __device__ __forceinline__ void used() { get = get + 1 == S ? 0 : get + 1; }
+};
+
+// cosines and sines of this lane's four pairs; NaN where the position lies outside the table
+__device__ __forceinline__ void load_turn(const NormArgs& a, long long at, int c, float (&cs)[4], float (&sn)[4]) {
+    if (c * 8 >= a.R) return;
+    const bool in = at >= 0 && at < a.table_len;
+    const float* t = a.table + ((size_t)(in ? at : 0) * (a.R / 2) + c * 4) * 2;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
         const float4 u = ld4(t + 4 * i);
         cs[2 * i] = u.x; sn[2 * i] = u.y; cs[2 * i + 1] = u.z; sn[2 * i + 1] = u.w;
     }
     if (!in) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) cs[i] = sn[i] = __int_as_float(0x7fffffff);
+        for (int i = 0; i < 4; i++) cs[i] = sn[i] = __int_as_float(0x7fffffff);
     }
 }
 
-// y turned by the angle (DIR 1) or back (DIR -1); lanes c < half hold the first of each pair, [half, 2 half) the second
+// y turned by the angle (DIR 1) or back (DIR -1)
 template <int DIR>
-__device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[8], const float (&sn)[8], int half, int c, int LPG) {
-    const int lane = threadIdx.x & 31;
-    const bool first = c < half, rot = c < 2 * half;
-    const int partner = rot ? (lane & ~(LPG - 1)) + (first ? c + half : c - half) : lane;
-    const bool minus = first == (DIR > 0);
+__device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[4], const float (&sn)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float o = __shfl_sync(FULL, y[i], partner);
-        if (rot) y[i] = fmaf(y[i], cs[i], minus ? -o * sn[i] : o * sn[i]);
+    for (int i = 0; i < 4; i++) {
+        const float a = y[i], b = y[4 + i], s = DIR > 0 ? sn[i] : -sn[i];
+        y[i] = fmaf(a, cs[i], -b * s);
+        y[4 + i] = fmaf(b, cs[i], a * s);
     }
 }
 
@@ -87,135 +135,158 @@ __device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[8], const 
 template <typename T, int LPG, bool CACHE>
 __global__ void __launch_bounds__(NR_THREADS, CACHE ? 3 : NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
+    constexpr int SLOTS = NR_FWD_SLOTS<T>;
+    __shared__ uint4 ring[Ahead<T, LPG, 1, SLOTS>::BYTES / 16];
+    Ahead<T, LPG, 1, SLOTS> rows(ring);
     const int c = threadIdx.x % LPG;
     const unsigned unit = blockIdx.x * (NR_THREADS / LPG) + threadIdx.x / LPG, tok = unit / a.slices;            // fewer than 2^31
     const int h0 = (int)(unit % a.slices) * a.per_slice, all = a.H + a.KV + (CACHE ? a.KV : 0);
-    const bool live = tok < a.tokens && c * 8 < a.D;
-    const unsigned b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
-    const long long at = CACHE ? (long long)a.pos[b] + t : a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t;
-    const T* qt = q + b * a.qs[0] + t * a.qs[1] + c * 8;                           // of the token
-    const T* kt = k + b * a.ks[0] + t * a.ks[1] + c * 8;
-    const T* vt = CACHE ? v + b * ap.vs[0] + t * ap.vs[1] + c * 8 : nullptr;
-    T* qot = qo + (size_t)tok * a.H * a.D + c * 8;
-    const int half = a.R / 16;
-    float cs[8], sn[8], w[8];
-    if (half) load_turn(a, at, half, c, cs, sn);
+    const bool token = tok < a.tokens, live = token && c * 8 < a.D;                // a lane without channels still fetches for the others
+    const unsigned b = token ? tok / a.T : 0, t = token ? tok % a.T : 0;
+    const long long at = CACHE ? (long long)a.pos[b] + t : a.pos != nullptr ? (long long)a.pos[token ? tok : 0] : t;
+    const T* qt = q + b * a.qs[0] + t * a.qs[1];         // of the token
+    const T* kt = k + b * a.ks[0] + t * a.ks[1];
+    const T* vt = CACHE ? v + b * ap.vs[0] + t * ap.vs[1] : nullptr;
+    // a row's 16-byte pieces are shared out over the lanes in order: in float32 lane c also takes piece LPG + c
+    auto fetch = [&](int u) {
+        const int h = h0 + u;
+        const T* from = h < a.H ? qt + h * a.qs[2] : !CACHE || h < a.H + a.KV ? kt + (h - a.H) * a.ks[2] : vt + (h - a.H - a.KV) * ap.vs[2];
+        const bool in = token && u < a.per_slice && h < all;
+        rows.fetch(0, in ? from : q, c, in, a.D);
+        rows.fetched();
+    };
+#pragma unroll
+    for (int u = 0; u < SLOTS - 1; u++) fetch(u);
+    const Pieces pc(c, a.R);
+    T* qot = qo + (size_t)tok * a.H * a.D;
+    const bool rot = c * 8 < a.R;
+    float cs[4], sn[4], w[8];
+    load_turn(a, at, c, cs, sn);
     const long long row = CACHE && at >= 0 ? (unsigned)at % (unsigned)ap.L : 0;
-    T* kot = CACHE ? kc + b * ap.kcs[0] + row * ap.kcs[1] + c * 8 : ko + (size_t)tok * a.KV * a.D + c * 8;
-    T* vot = CACHE ? vc + b * ap.vcs[0] + row * ap.vcs[1] + c * 8 : nullptr;
+    T* kot = CACHE ? kc + b * ap.kcs[0] + row * ap.kcs[1] : ko + (size_t)tok * a.KV * a.D;
+    T* vot = CACHE ? vc + b * ap.vcs[0] + row * ap.vcs[1] : nullptr;
     const long long kos = CACHE ? ap.kcs[2] : a.D;
     const float inv_d = 1.f / a.D;
-    constexpr int U = 2;                                 // rows in flight to a group
-    for (int u0 = 0; u0 < a.per_slice; u0 += U) {
-        Raw8<T> in[U];
+    for (int u = 0; u < a.per_slice; u++) {
+        const int h = h0 + u;
+        const bool is_v = CACHE && h >= a.H + a.KV, is_q = h < a.H;
+        rows.arrived();
+        fetch(u + SLOTS - 1);
+        if (h == a.H || u == 0) {                        // the queries' weights, then the keys'
+            const float* from = is_q ? a.qw : a.kw;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int h = h0 + u0 + u;
-            const T* from = h < a.H ? qt + h * a.qs[2] : !CACHE || h < a.H + a.KV ? kt + (h - a.H) * a.ks[2] : vt + (h - a.H - a.KV) * ap.vs[2];
-            in[u] = raw8(from, live && u0 + u < a.per_slice && h < all);
+            for (int i = 0; i < 8; i++) w[i] = 1.f;
+            if (live && from != nullptr) ld_pieces(w, from, pc);
         }
+        float ss = 0.f, x[8], y[8];
+        rows.read(0, x, pc);
+        rows.used();
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int h = h0 + u0 + u;
-            if (u0 + u >= a.per_slice) break;            // the same in every lane of the CTA
-            const bool is_v = CACHE && h >= a.H + a.KV, is_q = h < a.H;
-            if (h == a.H || u0 + u == 0) {               // the queries' weights, then the keys'
-                const float* from = is_q ? a.qw : a.kw;
+        for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+        const float r = rsqrtf(fmaf(group_sum<LPG>(ss), inv_d, a.eps));
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = 1.f;
-                if (live && from != nullptr) ld8(w, from + c * 8);
-            }
-            float ss = 0.f, x[8], y[8];
-            widen(x, in[u]);
-#pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-            const float r = rsqrtf(fmaf(group_sum<LPG>(ss), inv_d, a.eps));
-#pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = x[i] * r * w[i];
-            if (half) turn<1>(y, cs, sn, half, c, LPG);
-            if (!live || h >= all) continue;
-            if (is_q) st8(qot + h * a.D, y);
-            else if (!CACHE || at >= 0) {
-                if (!is_v) st8(kot + (h - a.H) * kos, y);
-                else st8(vot + (h - a.H - a.KV) * ap.vcs[2], x);
-            }
+        for (int i = 0; i < 8; i++) y[i] = x[i] * r * w[i];
+        if (rot) turn<1>(y, cs, sn);
+        if (!live || h >= all) continue;
+        if (is_q) st_pieces(qot + h * a.D, y, pc);
+        else if (!CACHE || at >= 0) {
+            if (!is_v) st_pieces(kot + (h - a.H) * kos, y, pc);
+            else st_pieces(vot + (h - a.H - a.KV) * ap.vcs[2], x, pc);
         }
     }
+    rows.rest();
 }
 
 // grid-stride over (token, slice of heads); part: (CTAs, 2, D) sums of the weights' gradients, or NULL
 template <typename T, int LPG>
 __global__ void __launch_bounds__(NR_THREADS, NR_BWD_CTAS) norm_rope_bwd_kernel(NormArgs a, const T* q, const T* k, const T* gq, const T* gk, T* dq, T* dk,
                                                                    float* part) {
-    constexpr int GROUPS = NR_THREADS / LPG;
-    __shared__ float s_part[GROUPS][LPG * 8];
+    constexpr int GROUPS = NR_THREADS / LPG, SLOTS = NR_BWD_SLOTS<T>;              // a slot: a row and its gradient
+    __shared__ uint4 ring[Ahead<T, LPG, 2, SLOTS>::BYTES / 16];
+    float(*s_part)[LPG * 8] = reinterpret_cast<float(*)[LPG * 8]>(ring);           // after the last row
     const int c = threadIdx.x % LPG, grp = threadIdx.x / LPG;
-    const int half = a.R / 16;
+    const Pieces pc(c, a.R);
+    const bool rot = c * 8 < a.R;
     const float inv_d = 1.f / a.D;
     float w[8], acc[2][8];
 #pragma unroll
     for (int i = 0; i < 8; i++) acc[0][i] = acc[1][i] = 0.f;
-    const unsigned units = (unsigned)a.tokens * a.slices;                          // fewer than 2^31
-    for (unsigned u0 = blockIdx.x * GROUPS; u0 < units; u0 += gridDim.x * GROUPS) {
-        const unsigned unit = u0 + grp, tok = unit / a.slices;
-        const int h0 = (int)(unit % a.slices) * a.per_slice;
-        const bool live = unit < units && c * 8 < a.D;
-        const unsigned b = live ? tok / a.T : 0, t = live ? tok % a.T : 0;
-        const T* qt = q + b * a.qs[0] + t * a.qs[1] + c * 8;                       // of the token
-        const T* kt = k + b * a.ks[0] + t * a.ks[1] + c * 8;
-        const size_t qo = (size_t)tok * a.H * a.D + c * 8, ko = (size_t)tok * a.KV * a.D + c * 8;
-        float cs[8], sn[8];
-        if (half) load_turn(a, a.pos != nullptr ? (long long)a.pos[live ? tok : 0] : t, half, c, cs, sn);
-        constexpr int U = sizeof(T) == 2 ? 4 : 2;
-        for (int v0 = 0; v0 < a.per_slice; v0 += U) {
-            Raw8<T> in[U], up[U];
+    const unsigned units = (unsigned)a.tokens * a.slices, first = blockIdx.x * GROUPS + grp, stride = gridDim.x * GROUPS;      // fewer than 2^31
+    const int rounds = (int)((units - blockIdx.x * GROUPS + stride - 1) / stride); // the same in all groups of the CTA
+    struct Place { unsigned tok, b, t; int h0; bool live; };
+    auto place = [&](int round) {
+        const unsigned unit = first + round * stride, tok = unit / a.slices;
+        const bool live = round < rounds && unit < units;
+        return Place{tok, live ? tok / a.T : 0, live ? tok % a.T : 0, (int)(unit % a.slices) * a.per_slice, live};
+    };
+    Ahead<T, LPG, 2, SLOTS> rows(ring);
+    Place pf = place(0);                                 // of the rows to fetch next
+    const T *qt, *kt, *gqt, *gkt;
+    auto bases = [&] {
+        qt = q + pf.b * a.qs[0] + pf.t * a.qs[1];
+        kt = k + pf.b * a.ks[0] + pf.t * a.ks[1];
+        gqt = gq + (size_t)pf.tok * a.H * a.D;
+        gkt = gk + (size_t)pf.tok * a.KV * a.D;
+    };
+    bases();
+    int f_round = 0, f_u = 0;
+    auto fetch = [&] {
+        const int h = pf.h0 + f_u;
+        const bool in = pf.live && h < a.H + a.KV;
+        rows.fetch(0, !in ? q : h < a.H ? qt + h * a.qs[2] : kt + (h - a.H) * a.ks[2], c, in, a.D);
+        rows.fetch(1, !in ? gq : h < a.H ? gqt + h * a.D : gkt + (h - a.H) * a.D, c, in, a.D);
+        rows.fetched();
+        if (++f_u == a.per_slice) { f_u = 0; pf = place(++f_round); bases(); }
+    };
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int h = h0 + v0 + u;
-                const bool ok = live && v0 + u < a.per_slice && h < a.H + a.KV;
-                in[u] = raw8(h < a.H ? qt + h * a.qs[2] : kt + (h - a.H) * a.ks[2], ok);
-                up[u] = raw8(h < a.H ? gq + qo + h * a.D : gk + ko + (h - a.H) * a.D, ok);
+    for (int u = 0; u < SLOTS - 1; u++) fetch();
+    for (int round = 0; round < rounds; round++) {
+        const Place p = place(round);
+        const bool live = p.live && c * 8 < a.D;
+        const size_t qo = (size_t)p.tok * a.H * a.D, ko = (size_t)p.tok * a.KV * a.D;
+        float cs[4], sn[4];
+        load_turn(a, a.pos != nullptr ? (long long)a.pos[p.live ? p.tok : 0] : p.t, c, cs, sn);
+        for (int u = 0; u < a.per_slice; u++) {
+            const int h = p.h0 + u;
+            const bool is_q = h < a.H;
+            rows.arrived();
+            fetch();
+            if (h == a.H || u == 0) {                    // the queries' weights, then the keys'
+                const float* from = is_q ? a.qw : a.kw;
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] = 1.f;
+                if (c * 8 < a.D && from != nullptr) ld_pieces(w, from, pc);
             }
+            float x[8], g[8], s1 = 0.f, s2 = 0.f;
+            rows.read(0, x, pc);
+            rows.read(1, g, pc);
+            rows.used();
+            if (rot) turn<-1>(g, cs, sn);
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int h = h0 + v0 + u;
-                if (v0 + u >= a.per_slice) break;        // the same in every lane of the CTA
-                const bool is_q = h < a.H;
-                if (h == a.H || v0 + u == 0) {           // the queries' weights, then the keys'
-                    const float* from = is_q ? a.qw : a.kw;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) w[i] = 1.f;
-                    if (c * 8 < a.D && from != nullptr) ld8(w, from + c * 8);
-                }
-                float x[8], g[8], s1 = 0.f, s2 = 0.f;
-                widen(x, in[u]);
-                widen(g, up[u]);
-                if (half) turn<-1>(g, cs, sn, half, c, LPG);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    s1 = fmaf(x[i], x[i], s1);
-                    s2 = fmaf(g[i] * w[i], x[i], s2);
-                }
-                const float r = rsqrtf(fmaf(group_sum<LPG>(s1), inv_d, a.eps));
-                const float m = group_sum<LPG>(s2) * r * r * inv_d;
-                if (!live || h >= a.H + a.KV) continue;
-                float dx[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    dx[i] = r * fmaf(-x[i], m, g[i] * w[i]);
-                    const float gx = g[i] * x[i] * r;
-                    if (is_q) acc[0][i] += gx; else acc[1][i] += gx;
-                }
-                if (is_q) st8(dq + qo + h * a.D, dx);
-                else st8(dk + ko + (h - a.H) * a.D, dx);
+            for (int i = 0; i < 8; i++) {
+                s1 = fmaf(x[i], x[i], s1);
+                s2 = fmaf(g[i] * w[i], x[i], s2);
             }
+            const float r = rsqrtf(fmaf(group_sum<LPG>(s1), inv_d, a.eps));
+            const float m = group_sum<LPG>(s2) * r * r * inv_d;
+            if (!live || h >= a.H + a.KV) continue;
+            float dx[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                dx[i] = r * fmaf(-x[i], m, g[i] * w[i]);
+                const float gx = g[i] * x[i] * r;
+                if (is_q) acc[0][i] += gx; else acc[1][i] += gx;
+            }
+            if (is_q) st_pieces(dq + qo + h * a.D, dx, pc);
+            else st_pieces(dk + ko + (h - a.H) * a.D, dx, pc);
         }
     }
+    rows.rest();
     if (part == nullptr) return;
     for (int n = 0; n < 2; n++) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; i++) s_part[grp][c * 8 + i] = n ? acc[1][i] : acc[0][i];
+        for (int i = 0; i < 8; i++) s_part[grp][pc.at[i / 4] + i % 4] = n ? acc[1][i] : acc[0][i];
         __syncthreads();
         for (int d = threadIdx.x; d < a.D; d += NR_THREADS) {
             float s = 0.f;
