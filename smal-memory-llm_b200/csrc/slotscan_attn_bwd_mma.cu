@@ -16,7 +16,8 @@
 // steps' ds before the product warp looks at the first.  ds has two barriers in turn; the third step's needs the wait for the first.
 // Tensor memory, 512 columns:  rows of queries:  s | dp | dq | 2 x ds;   rows of keys:  s, p written over it | dp, ds over it | dk | dv
 // Weights are bf16 where the sums' products read them as their first operand; a group of 32 columns' weights lie where its scores
-// lay, which its own threads have read.
+// lay, which its own threads have read.  One rounding of ds to bf16 costs dq and dk about as much as their own rounding; ds as a sum of
+// two would take a fourth product of three, and a fifth of four.
 #include <type_traits>
 
 #include "slotscan_attn.cuh"

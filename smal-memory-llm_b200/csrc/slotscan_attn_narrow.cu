@@ -10,6 +10,8 @@
 // those see, forms the softmax of each row anew and sums delta = sum p dp of the row itself, so nothing but q, k, v and do is
 // read (the halo comes from the cache) and nothing is kept by the forward.  dq is done by the warp of its rows; p and ds go to
 // shared memory, where the warp of 16 keys gathers dk and dv from the NB blocks of queries that see them: no atomics.
+// p and ds are rounded once to bf16 for their products, as the operands' type asks: dq and dk are then off by about the root of two times
+// what their own rounding costs.
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_tensor.cuh"

@@ -12,7 +12,8 @@
 // registers: 4 in flight to a group and four CTAs to an SM, backward 5 rows with their gradients and two CTAs.  64 x 1,024 tokens of
 // 6 + 6 heads of 128, bf16: 76 us (5.3 TB/s), backward 120 us (5.0 TB/s).  Before: 101 and 150 us with rows in registers and a pair's
 // sides 8 lanes apart; 80 and 129 with the ring alone.  Three, five or six CTAs: 78, 85, 84 us; backward three CTAs 129, four 204.
-// float32 is as fast either way (8 x 4,096 tokens of 12 + 4 heads of 64: 44 + 71 us, 6.1 TB/s).
+// Now bound by the issue of instructions (84 % of the slots, backward 76 %); paired multiply-adds took 81 and 126: their operands
+// have to be moved into pairs.  float32 is as fast either way (8 x 4,096 tokens of 12 + 4 heads of 64: 44 + 71 us, 6.1 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
