@@ -85,6 +85,10 @@ variable_list registered(const char* name, std::vector<c10::IValue> args) {
 }
 c10::IValue or_none(const Tensor& t) { return t.defined() ? c10::IValue(t) : c10::IValue(); }
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
+// Written in place, past the dispatcher: a backward that has saved `t` must find out (tensors of inference mode are not counted)
+void changed(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // ---- norms and rotation ----
 bool norm_params(slotscan_norm_params& p, const Tensor& q, const Tensor& k, const Maybe& table, const Maybe& qw, const Maybe& kw, double eps) {
@@ -187,6 +191,8 @@ py::object norm_rope_append(const Tensor& q, const Tensor& k, const Tensor& v, c
     check(slotscan_norm_rope_append(&p, in(q), in(k), in(v), ptr<float>(table), ptr<int32_t>(pos), ptr<float>(qw), ptr<float>(kw), out(qo), out(kc), out(vc),
                                     stream_of(q)),
           "slotscan_norm_rope_append");
+    changed(kc);
+    changed(vc);
     return py::cast(qo);
 }
 
