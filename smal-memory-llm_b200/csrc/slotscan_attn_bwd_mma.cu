@@ -144,7 +144,8 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
             const int lo = sp.lo - y0, hi = sp.hi - y0;
             const float ahead = at - (float)y0;
             uint32_t xs[32];                             // s, then p (1 - tanh^2)
-            if (!(ok = ok && wait_soon_warp(&s_full, s & 1))) break;
+            // a warp that has given up stays with its group's barrier, at which the others would wait for it without a limit
+            if (!(ok = ok && wait_soon_warp(&s_full, s & 1))) continue;
             tmem_fence_after();
             tmem_ld(S, xs);
             tmem_ld_wait(xs);
@@ -220,7 +221,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                 __syncwarp();
                 if (lane == 0) arrive(&p_full);
             }
-            if (!(ok = wait_soon_warp(&d_full, s & 1))) break;
+            if (!(ok = wait_soon_warp(&d_full, s & 1))) continue;
             tmem_fence_after();
             uint32_t xd[32], wd[16];
             [[maybe_unused]] float4 four;
