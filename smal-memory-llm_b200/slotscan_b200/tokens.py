@@ -38,9 +38,9 @@ def _host():
 
 
 def _taken(what, out):
-    """What a call through the host module gave; the only causes left of a second None are these."""
+    """What a call through the host module gave; the only cause left of a second None is this."""
     if out is None:
-        raise ValueError("%s: all tensors must be on one device, and no size may pass 2^31 - 1" % what)
+        raise ValueError("%s: no size may pass 2^31 - 1" % what)
     return out
 
 
@@ -105,6 +105,13 @@ def _launch(dev, name, *args):
         _lib.check(rc, name)
 
 
+def _on_one_gpu(what, *ts):
+    """`ts[0]` is a tensor; the others are tensors or None."""
+    _require_cuda(*ts)
+    if any(t is not None and t.device != ts[0].device for t in ts):
+        raise ValueError("%s: all tensors must be on one device" % what)
+
+
 def _type_check(what, *sigs):
     if any(s[2] not in _CODE or s[2] != sigs[0][2] for s in sigs):
         raise TypeError("%s: float32 or bfloat16 tensors, all of one type" % what)
@@ -151,7 +158,7 @@ def _norm_call(q, k, table, pos, q_weight, k_weight, eps):
 
 def _norm_fwd(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], pos: Optional[torch.Tensor],
               q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
-    _require_cuda(q, k, table, pos, q_weight, k_weight)
+    _on_one_gpu("norm_rope", q, k, table, pos, q_weight, k_weight)
     q, k, table, pos, qw, kw, plan = _norm_call(q, k, table, pos, q_weight, k_weight, eps)
     dev = q.device
     qo, ko = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=k.dtype, device=dev)
@@ -171,7 +178,7 @@ def _norm_bwd(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor], p
               q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], dqo: torch.Tensor, dko: torch.Tensor, eps: float
               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """dq, dk and the float32 gradients of the two weights (empty without weights)."""
-    _require_cuda(q, k, table, pos, q_weight, k_weight, dqo, dko)
+    _on_one_gpu("norm_rope", q, k, table, pos, q_weight, k_weight, dqo, dko)
     q, k, table, pos, qw, kw, plan = _norm_call(q, k, table, pos, q_weight, k_weight, eps)
     dqo, dko = _whole(dqo, q.dtype), _whole(dko, k.dtype)
     dev, weights = q.device, qw is not None or kw is not None
@@ -229,7 +236,7 @@ def norm_rope(q, k, table, q_weight=None, k_weight=None, pos=None, eps=1e-6):
         return _norm_op(*ts, float(eps))
     out = _host().norm_rope(q, k, table, q_weight, k_weight, pos, eps)
     if out is None:
-        _require_cuda(*ts)
+        _on_one_gpu("norm_rope", *ts)
         q, k, table, pos, q_weight, k_weight, _ = _norm_call(*ts, float(eps))
         out = _taken("norm_rope", _host().norm_rope(q, k, table, q_weight, k_weight, pos, eps))
     return out
@@ -270,7 +277,7 @@ def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps)
 
 def _append_call(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps):
     """The tensors as the kernel reads them, and the plan of the call."""
-    _require_cuda(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
+    _on_one_gpu("norm_rope_append", q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
     rest = (_sig(k_cache), _sig(v_cache), _sig(pos), _sig(table), _sig(q_weight), _sig(k_weight), eps)
     plan = _append_plan(_sig(q), _sig(k), _sig(v), *rest)
     if plan[0] is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
@@ -354,7 +361,7 @@ def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optiona
               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """o and what the backward needs besides (without elements where it needs nothing, or unless asked for): lse (B,H,Tq), and for
     bfloat16 what the rounding of o left."""
-    _require_cuda(q, k, v, slopes, docs, prefix)
+    _on_one_gpu("token_attention", q, k, v, slopes, docs, prefix)
     q, k, v, slopes, docs, prefix, plan = _attn_call(q, k, v, slopes, docs, prefix, window, cap, scale)
     (B, Tq, H, _), dev, dtype, keeps = q.shape, q.device, q.dtype, plan[1] and for_bwd
     o = torch.empty(q.shape, dtype=dtype, device=dev)
@@ -378,7 +385,7 @@ def _(q, k, v, slopes, docs, prefix, window, cap, scale, for_bwd):
 def _attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optional[torch.Tensor], docs: Optional[torch.Tensor],
               prefix: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor, rest: torch.Tensor, do: torch.Tensor, window: int, cap: float,
               scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    _require_cuda(q, k, v, slopes, docs, prefix, o, lse, rest, do)
+    _on_one_gpu("token_attention", q, k, v, slopes, docs, prefix, o, lse, rest, do)
     q, k, v, slopes, docs, prefix, plan = _attn_call(q, k, v, slopes, docs, prefix, window, cap, scale)
     dev, dtype = q.device, q.dtype
     do = _whole(do, dtype)
@@ -455,7 +462,7 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
         return _attn_op(*ts, window, cap, scale, True)[0]
     out = _host().token_attention(*ts, window, cap, scale)
     if out is None:
-        _require_cuda(*ts)
+        _on_one_gpu("token_attention", *ts)
         *ts, _ = _attn_call(*ts, window, cap, scale)
         out = _taken("token_attention", _host().token_attention(*ts, window, cap, scale))
     return out
@@ -482,7 +489,7 @@ def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
 
 def _step_call(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
     """The tensors as the kernel reads them, and the plan of the call."""
-    _require_cuda(q, k_cache, v_cache, pos, slopes, start)
+    _on_one_gpu("token_attention_step", q, k_cache, v_cache, pos, slopes, start)
     rest = (_sig(k_cache), _sig(v_cache), _sig(pos), _sig(slopes), _sig(start), window, cap, scale)
     plan = _step_plan(_sig(q), *rest)
     if plan[0] is None or q.data_ptr() & 15:

@@ -3,6 +3,10 @@ import glob
 import os
 import re
 
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "smal-memory-llm_b200", "csrc")
 
@@ -36,3 +40,21 @@ def test_no_thread_leaves_a_loop_that_holds_a_barrier():
                 found += 1
                 assert "break;" not in body, (os.path.basename(path), body[:200])
     assert found >= 4
+
+
+def test_tensors_of_two_gpus_are_refused():
+    """The implementations of the registered ops refuse them too: a kernel would be given another GPU's addresses."""
+    from slotscan_b200 import tokens as K
+    with FakeTensorMode():
+        f = lambda *s, at=0, dt=torch.float32: torch.empty(*s, device="cuda:%d" % at, dtype=dt)             # noqa: E731
+        q, k, table, w, kc, one = f(2, 9, 2, 64), f(2, 9, 2, 64, at=1), f(9, 32, 2, at=1), f(64, at=1), f(2, 16, 2, 64), f(2, 1, 2, 64)
+        pos, far = f(2, dt=torch.int32), f(2, at=1, dt=torch.int32)
+        lse = f(2, 2, 9)
+        for call in (lambda: K._norm_fwd(q, k, None, None, None, None, 1e-6), lambda: K._norm_fwd(q, q, table, None, None, None, 1e-6),
+                     lambda: K._norm_fwd(q, q, None, None, w, None, 1e-6), lambda: K._norm_bwd(q, q, None, None, None, None, q, k, 1e-6),
+                     lambda: K._append(q, q, q, kc, kc, far, None, None, None, 1e-6), lambda: K._append(q, q, k, kc, kc, pos, None, None, None, 1e-6),
+                     lambda: K._attn_fwd(q, k, q, None, None, None, 0, 0.0, 0.1, True), lambda: K._attn_fwd(q, q, q, None, None, far, 0, 0.0, 0.1, True),
+                     lambda: K._attn_bwd(q, q, q, None, None, None, q, lse, q, k, 0, 0.0, 0.1), lambda: K._step(one, kc, kc, far, None, None, 0, 0.0, 0.1),
+                     lambda: K._step(one, kc, kc, pos, None, far, 0, 0.0, 0.1)):
+            with pytest.raises(ValueError, match="one device"):
+                call()
