@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <cstdint>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -90,6 +91,10 @@ void changed(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// int64 as the kernels read integers; what 32 bits cannot hold becomes the nearest that they can: beyond every table, bound and length
+Tensor in_32_bits(const Tensor& t) { return t.scalar_type() == at::kLong && t.is_cuda() ? t.clamp(INT32_MIN, INT32_MAX).to(at::kInt) : t; }
+Maybe in_32_bits(const Maybe& t) { return some(t) ? Maybe(in_32_bits(*t)) : t; }
+
 // ---- norms and rotation ----
 bool norm_params(slotscan_norm_params& p, const Tensor& q, const Tensor& k, const Maybe& table, const Maybe& qw, const Maybe& kw, double eps) {
     if (q.dim() != 4 || k.dim() != 4 || code(q) < 0 || code(q) != code(k) || !q.is_cuda() || q.device() != k.device()) return false;
@@ -155,8 +160,9 @@ struct NormRope : torch::autograd::Function<NormRope> {
     }
 };
 
-py::object norm_rope(const Tensor& q, const Tensor& k, const Maybe& table, const Maybe& qw, const Maybe& kw, const Maybe& pos, double eps) {
+py::object norm_rope(const Tensor& q, const Tensor& k, const Maybe& table, const Maybe& qw, const Maybe& kw, const Maybe& any_pos, double eps) {
     slotscan_norm_params p;
+    const Maybe pos = in_32_bits(any_pos);
     if (!norm_params(p, q, k, table, qw, kw, eps) || !fits(pos, at::kInt, {q.size(0), q.size(1)}, q)) return py::none();
     if (some(table) && !some(pos) && q.size(1) > table->size(0)) return py::none();
     if (some(table) && (uintptr_t)table->const_data_ptr() % 16) return py::none();
@@ -169,9 +175,10 @@ py::object norm_rope(const Tensor& q, const Tensor& k, const Maybe& table, const
     return py::cast(norm_fwd(p, q, k, table, pos, qw, kw));
 }
 
-py::object norm_rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& pos, const Maybe& table,
+py::object norm_rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& any_pos, const Maybe& table,
                             const Maybe& qw, const Maybe& kw, double eps) {
     slotscan_append_params p;
+    const Tensor pos = in_32_bits(any_pos);
     if (!norm_params(p.base, q, k, table, qw, kw, eps)) return py::none();
     const int64_t B = q.size(0), T = q.size(1), D = q.size(3), KV = k.size(2);
     if (v.sizes() != k.sizes() || v.scalar_type() != q.scalar_type() || v.device() != q.device() || kc.dim() != 4 || vc.sizes() != kc.sizes() ||
@@ -267,17 +274,20 @@ struct TokenAttention : torch::autograd::Function<TokenAttention> {
     }
 };
 
-py::object token_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& slopes, const Maybe& docs, const Maybe& prefix, int64_t window,
-                           double cap, double scale) {
+py::object token_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& slopes, const Maybe& any_docs, const Maybe& any_prefix,
+                           int64_t window, double cap, double scale) {
     slotscan_attn_params p;
+    const Maybe docs = in_32_bits(any_docs), prefix = in_32_bits(any_prefix);
     if (!attn_params(p, q, k, v, slopes, docs, prefix, window, cap, scale)) return py::none();
     const Maybe ts[] = {q, k, v};
     if (wants_grad({&ts[0], &ts[1], &ts[2]})) return py::cast(TokenAttention::apply(q, k, v, slopes, docs, prefix, window, cap, scale));
     return py::cast(attn_fwd(p, q, k, v, slopes, docs, prefix, false)[0]);
 }
 
-py::object token_attention_step(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& pos, const Maybe& slopes, const Maybe& start, int64_t window,
-                                double cap, double scale) {
+py::object token_attention_step(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& any_pos, const Maybe& slopes, const Maybe& any_start,
+                                int64_t window, double cap, double scale) {
+    const Tensor pos = in_32_bits(any_pos);
+    const Maybe start = in_32_bits(any_start);
     if (q.dim() != 4 || q.size(1) != 1 || kc.dim() != 4 || vc.sizes() != kc.sizes() || code(q) < 0 || code(kc) != code(q) || code(vc) != code(q) ||
         !q.is_cuda() || kc.device() != q.device() || vc.device() != q.device())
         return py::none();

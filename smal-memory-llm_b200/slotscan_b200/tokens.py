@@ -75,8 +75,11 @@ def _f32(t):
 
 
 def _i32(t):
+    """Integers as the kernels read them; what 32 bits cannot hold becomes the nearest that they can: beyond every table, bound and length."""
     if t is None:
         return None
+    if t.dtype is torch.int64:                                         # of the ordinary calls: in the host module
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
     t = t.to(torch.int32).contiguous()
     return t if t.data_ptr() % 8 == 0 or t.dim() < 3 else t.clone()    # document bounds are read in pairs
 
@@ -117,6 +120,14 @@ def _type_check(what, *sigs):
         raise TypeError("%s: float32 or bfloat16 tensors, all of one type" % what)
 
 
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def _integers(what, *sigs):
+    if any(s is not None and s[2] not in _INTEGERS for s in sigs):
+        raise TypeError("%s: positions, lengths and bounds are signed integers (or bytes), got %s" % (what, [s[2] for s in sigs if s is not None]))
+
+
 # ---------------------------------------------------------------------------------------- norms and rotation
 
 def _norm_checked(what, q, k, table, q_weight, k_weight):
@@ -139,6 +150,7 @@ def _norm_plan(q, k, table, pos, q_weight, k_weight, eps):
     sizes = _norm_checked("norm_rope", q, k, table, q_weight, k_weight)
     if pos is not None and pos[0] != q[0][:2]:
         raise ValueError("norm_rope: positions (B, T), got %s" % (tuple(pos[0]),))
+    _integers("norm_rope", pos)
     if pos is None and table is not None and sizes[1] > sizes[6]:
         raise ValueError("norm_rope: %d tokens, %d positions in the table" % (sizes[1], sizes[6]))
     strides = _strides(q), _strides(k)
@@ -268,6 +280,7 @@ def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps)
                          % (tuple(k[0]), tuple(v[0]), tuple(k_cache[0]), tuple(pos[0])))
     if T > L:
         raise ValueError("norm_rope_append: %d tokens at once into caches of %d rows" % (T, L))
+    _integers("norm_rope_append", pos)
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
     if None in (qs, ks, vs):
         return None, None
@@ -340,6 +353,7 @@ def _attn_plan(q, k, v, slopes, docs, prefix, window, cap, scale):
         raise ValueError("token_attention: document bounds (B, Tk, 2) from document_bounds, got %s" % (tuple(docs[0]),))
     if prefix is not None and prefix[0] != (B,):
         raise ValueError("token_attention: one prefix length for each sequence, got %s" % (tuple(prefix[0]),))
+    _integers("token_attention", docs, prefix)
     strides = _strides(q), _strides(k), _strides(v)
     p = _lib.AttnParams(B, Tq, Tk, H, ks[2], D, window, _CODE[q[2]], scale, cap, *((0, 0, 0) if s is None else s for s in strides))
     _lib.check(_lib.lib().slotscan_attn_check(ctypes.byref(p)), "slotscan_attn_check")
@@ -481,6 +495,7 @@ def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
         raise ValueError("token_attention_step: queries %s do not match caches %s" % (tuple(q[0]), tuple(k_cache[0])))
     if pos[0] != (B,) or (start is not None and start[0] != (B,)) or (slopes is not None and slopes[0] != (H,)):
         raise ValueError("token_attention_step: positions (B), starts (B) and slopes (H)")
+    _integers("token_attention_step", pos, start)
     qs = _strides(q)
     p = _lib.AttnStepParams(B, H, KV, D, L, window, _CODE[q[2]], scale, cap, (0, 0) if qs is None else (qs[0], qs[2]), ks, vs)
     _lib.check(_lib.lib().slotscan_attn_step_check(ctypes.byref(p)), "slotscan_attn_step_check")

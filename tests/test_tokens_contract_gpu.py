@@ -47,3 +47,42 @@ def test_append_in_inference_mode():
         got = kc.clone(), vc.clone()
         S.norm_rope_append(q, k, v, *got, pos, None)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_integers_beyond_32_bits_keep_their_meaning():
+    """A length that is longer than everything is everything; a position that no table has gives NaN, wherever its lower 32 bits point."""
+    S = _S()
+    q = _randn(5, 2, 30, 2, 64)
+    far = torch.tensor([2 ** 40, 2 ** 32 + 3], device="cuda")
+    assert torch.equal(S.token_attention(q, q, q, prefix=far), S.token_attention(q, q, q, prefix=torch.full_like(far, 30)))
+    assert torch.equal(S.token_attention(q, q, q, prefix=-far), S.token_attention(q, q, q))
+    docs = torch.stack((torch.full((2, 30), -2 ** 35, device="cuda"), torch.full((2, 30), 2 ** 33 + 4, device="cuda")), -1)
+    assert torch.equal(S.token_attention(q, q, q, docs=docs), S.token_attention(q, q, q))
+    table = S.rope_table(40, 64, device="cuda")
+    pos = torch.arange(30, device="cuda").repeat(2, 1)
+    want = S.norm_rope(q, q, table, pos=pos)[0]
+    pos[0, 7], pos[1, 9] = 2 ** 32 + 3, 3 - 2 ** 32
+    got = S.norm_rope(q, q, table, pos=pos)[0]
+    assert got[0, 7].isnan().all() and got[1, 9].isnan().all()
+    want[0, 7] = want[1, 9] = got[0, 7] = got[1, 9] = 0
+    assert torch.equal(got, want)
+    kc, vc, at = _randn(6, 2, 16, 2, 64), _randn(7, 2, 16, 2, 64), torch.tensor([20, 9], device="cuda")
+    keep = kc.clone()
+    S.norm_rope_append(q[:, :1], q[:, :1], q[:, :1], kc, vc, at - 2 ** 32, table)          # a negative position stores nothing
+    assert torch.equal(kc, keep)
+    assert not S.token_attention_step(q[:, :1], kc, vc, at, start=far).any()                # a start behind the query: nothing to see
+    assert torch.equal(S.token_attention_step(q[:, :1], kc, vc, at, start=-far), S.token_attention_step(q[:, :1], kc, vc, at))
+
+
+def test_positions_that_are_no_integers_are_refused():
+    S = _S()
+    q, kc = _randn(8, 2, 1, 2, 64), _randn(9, 2, 16, 2, 64)
+    table, f = S.rope_table(40, 64, device="cuda"), torch.tensor([2.7, 3.0], device="cuda")
+    for call in (lambda: S.norm_rope(q, q, table, pos=f.view(2, 1)), lambda: S.norm_rope_append(q, q, q, kc, kc.clone(), f, table),
+                 lambda: S.token_attention(q, q, q, prefix=f), lambda: S.token_attention(q, q, q, docs=f.view(2, 1, 1).expand(2, 1, 2)),
+                 lambda: S.token_attention_step(q, kc, kc, f), lambda: S.token_attention_step(q, kc, kc, f.int(), start=f.half()),
+                 lambda: S.token_attention(q, q, q, prefix=f > 2)):
+        with pytest.raises(TypeError, match="integers"):
+            call()
+    for dt in (torch.int8, torch.int16, torch.uint8, torch.int64):
+        assert torch.equal(S.token_attention_step(q, kc, kc, f.to(dt)), S.token_attention_step(q, kc, kc, f.int()))
