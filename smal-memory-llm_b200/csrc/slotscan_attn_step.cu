@@ -12,6 +12,8 @@
 // p is split into two bf16 (p = hi + lo, off by 2^-17): the second product costs nothing here and keeps the float32 weights' precision.
 //
 // float32: the CUDA cores.  A row is read by LPG lanes, 8 channels each, and every group of lanes goes its own way through the split.
+#include <cfloat>
+
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_tensor.cuh"
@@ -32,6 +34,8 @@ struct StepArgs {
 };
 
 struct Softmax { float m, l; };                          // running maximum (base-2 exponent) and sum
+// what a split hands to the join as its maximum: minus infinity says that the query sees nothing at all
+__device__ __forceinline__ float split_max(int visible, float top) { return visible == 0 ? -INFINITY : fmaxf(top, -FLT_MAX); }
 
 template <typename T, int LPG, int G>
 __global__ void __launch_bounds__(ST_THREADS) attn_step_kernel(StepArgs a, const T* q, const T* k, const T* v, T* o, float* part) {
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(ST_THREADS) attn_step_kernel(StepArgs a, const
         else {
             float* pp = part + (((size_t)b * a.H + h) * a.splits + split) * (a.D + 2);
             pp[d] = s;
-            if (d == 0) { pp[a.D] = top; pp[a.D + 1] = l; }
+            if (d == 0) { pp[a.D] = split_max(n, top); pp[a.D + 1] = l; }
         }
     }
 }
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
         else {
             float* pp = part + (((size_t)b * a.H + h) * a.splits + split) * (a.D + 2);
             pp[d] = sum;
-            if (d == 0) { pp[a.D] = top; pp[a.D + 1] = ll; }
+            if (d == 0) { pp[a.D] = split_max(n, top); pp[a.D + 1] = ll; }
         }
     }
 }
@@ -339,13 +343,13 @@ __global__ void __launch_bounds__(128) attn_step_join_kernel(const float* part, 
             l = fmaf(pp[(size_t)i * (D + 2) + D + 1], f, l);
         }
         l = warp_sum(l);
-        if (tid == 0) s_red[0] = l;
+        if (tid == 0) { s_red[0] = l; s_red[1] = top; }
     }
     __syncthreads();
     for (int d = tid; d < D; d += 128) {
         float s = 0.f;
         for (int i = 0; i < splits; i++) s = fmaf(pp[(size_t)i * (D + 2) + d], s_f[i], s);
-        st1(o + (size_t)blockIdx.x * D + d, s_red[0] == 0.f ? 0.f : s / s_red[0]);
+        st1(o + (size_t)blockIdx.x * D + d, s_red[1] == -INFINITY ? 0.f : s / s_red[0]);
     }
 }
 

@@ -86,3 +86,17 @@ def test_positions_that_are_no_integers_are_refused():
             call()
     for dt in (torch.int8, torch.int16, torch.uint8, torch.int64):
         assert torch.equal(S.token_attention_step(q, kc, kc, f.to(dt)), S.token_attention_step(q, kc, kc, f.int()))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("L", [16, 4096])
+def test_scores_of_minus_infinity_are_no_empty_row(dtype, L):
+    """A softmax over scores that are all minus infinity is NaN, in one CTA and joined from many; a row that sees nothing gives zeros."""
+    S = _S()
+    q, v = torch.ones(2, 1, 2, 64, device="cuda", dtype=DT[dtype]), torch.ones(2, L, 2, 64, device="cuda", dtype=DT[dtype])
+    k = torch.full_like(v, -torch.inf)
+    pos, start = torch.tensor([L - 1, L - 1], device="cuda"), torch.tensor([0, L], device="cuda")
+    o = S.token_attention_step(q, k, v, pos, start=start)
+    assert o[0].isnan().all() and not o[1].any()
+    k[0, L // 2] = 0                                                   # one that is not
+    assert torch.equal(S.token_attention_step(q, k, v, pos, start=start)[0], torch.ones_like(o[0]))
