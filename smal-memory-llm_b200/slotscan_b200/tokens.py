@@ -441,7 +441,7 @@ _attn_op.register_autograd(_attn_backward, setup_context=_attn_setup)
 def _numbers(what, D, window, cap, scale, slopes):
     if window < 0 or not 0 <= cap < math.inf:
         raise ValueError("%s: a window of %s and a cap of %s: both are 0 (none) or positive" % (what, window, cap))
-    if slopes is not None and slopes.requires_grad:
+    if wants_grad(slopes):
         raise ValueError("%s: the slopes of the distance bias are constants; they have no gradient" % what)
     window = int(window) if window < 2 ** 31 - 1 else 0                # further than any two tokens can be apart
     return window, float(cap), float(D ** -0.5 if scale is None else scale)

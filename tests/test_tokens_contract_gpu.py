@@ -100,3 +100,14 @@ def test_scores_of_minus_infinity_are_no_empty_row(dtype, L):
     assert o[0].isnan().all() and not o[1].any()
     k[0, L // 2] = 0                                                   # one that is not
     assert torch.equal(S.token_attention_step(q, k, v, pos, start=start)[0], torch.ones_like(o[0]))
+
+
+def test_slopes_that_are_a_parameter():
+    """Refused only where their gradient is wanted."""
+    S = _S()
+    q, kc, slopes, pos = _randn(11, 1, 20, 2, 64), _randn(12, 1, 20, 2, 64), torch.nn.Parameter(torch.tensor([0.5, 0.25], device="cuda")), torch.tensor([19], device="cuda")
+    for call in (lambda s: S.token_attention(q, q, q, slopes=s), lambda s: S.token_attention_step(q[:, :1], kc, kc, pos, slopes=s)):
+        with pytest.raises(ValueError, match="slopes"):
+            call(slopes)
+        with torch.no_grad():
+            assert torch.equal(call(slopes), call(slopes.detach().clone()))
