@@ -244,6 +244,8 @@ def norm_rope(q, k, table, q_weight=None, k_weight=None, pos=None, eps=1e-6):
     `rope_table`, or None for no rotation; `pos` (B,T) integer positions (None: 0 .. T-1).  Slices of a fused projection are read in
     place.  A position outside the table gives NaN.  Differentiable in q, k and the weights."""
     ts = (q, k, table, pos, q_weight, k_weight)
+    if wants_grad(table):
+        raise ValueError("norm_rope: the table is a constant; it has no gradient")
     if not plain_call(*ts):
         return _norm_op(*ts, float(eps))
     out = _host().norm_rope(q, k, table, q_weight, k_weight, pos, eps)

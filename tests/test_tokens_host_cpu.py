@@ -58,3 +58,13 @@ def test_tensors_of_two_gpus_are_refused():
                      lambda: K._step(one, kc, kc, pos, None, far, 0, 0.0, 0.1)):
             with pytest.raises(ValueError, match="one device"):
                 call()
+
+
+def test_a_table_whose_gradient_is_wanted_is_refused():
+    """It would get none, in silence."""
+    import slotscan_b200 as S
+    q, table = torch.zeros(1, 3, 2, 64), S.rope_table(9, 64).requires_grad_()
+    with pytest.raises(ValueError, match="table"):
+        S.norm_rope(q, q, table)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        S.norm_rope(q, q, table)
