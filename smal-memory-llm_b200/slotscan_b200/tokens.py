@@ -440,13 +440,14 @@ def _attn_backward(ctx, do, _, __):
 _attn_op.register_autograd(_attn_backward, setup_context=_attn_setup)
 
 
-def _numbers(what, D, window, cap, scale, slopes):
+def _numbers(what, q, window, cap, scale, slopes):
+    D = q.shape[-1] if q.dim() else 0                                  # without channels: refused for its shape, later
     if window < 0 or not 0 <= cap < math.inf:
         raise ValueError("%s: a window of %s and a cap of %s: both are 0 (none) or positive" % (what, window, cap))
     if wants_grad(slopes):
         raise ValueError("%s: the slopes of the distance bias are constants; they have no gradient" % what)
     window = int(window) if window < 2 ** 31 - 1 else 0                # further than any two tokens can be apart
-    return window, float(cap), float(D ** -0.5 if scale is None else scale)
+    return window, float(cap), float((D or 1) ** -0.5 if scale is None else scale)
 
 
 def document_bounds(doc):
@@ -472,7 +473,7 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
       visible  j <= i, or j < prefix[b];  and |i - j| < window if window;  and the same document of `document_bounds`
     A row that sees nothing gives zeros, and what a row does not see, infinities and NaN among it, does not reach it.  Differentiable
     in q, k and v; results and gradients are equal from run to run."""
-    window, cap, scale = _numbers("token_attention", q.shape[-1], window, cap, scale, slopes)
+    window, cap, scale = _numbers("token_attention", q, window, cap, scale, slopes)
     ts = (q, k, v, slopes, docs, prefix)
     if not plain_call(*ts):
         return _attn_op(*ts, window, cap, scale, True)[0]
@@ -538,7 +539,7 @@ def token_attention_step(q, k_cache, v_cache, pos, window=0, cap=0.0, slopes=Non
     """`token_attention` of one query for each sequence, (B,1,H,D), over ring caches (B,L,KV,D) that `norm_rope_append` fills, forward only.
     The query stands at pos[b] (its own key is in the caches) and sees the positions from start[b] on (None: 0), of the last
     min(window, L).  Rows outside are not read."""
-    window, cap, scale = _numbers("token_attention_step", q.shape[-1], window, cap, scale, slopes)
+    window, cap, scale = _numbers("token_attention_step", q, window, cap, scale, slopes)
     ts = (q, k_cache, v_cache, pos, slopes, start)
     if wants_grad(*ts):
         raise ValueError("token_attention_step: forward only; use token_attention where a gradient is wanted")

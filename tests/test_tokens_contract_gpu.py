@@ -111,3 +111,14 @@ def test_slopes_that_are_a_parameter():
             call(slopes)
         with torch.no_grad():
             assert torch.equal(call(slopes), call(slopes.detach().clone()))
+
+
+def test_heads_without_channels_are_refused():
+    S = _S()
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for shape in ((2, 1, 2, 0), (), (2,)):
+        q = torch.zeros(shape, device="cuda")
+        for call in (lambda: S.token_attention(q, q, q), lambda: S.token_attention_step(q, q, q, pos), lambda: S.norm_rope(q, q, None),
+                     lambda: S.norm_rope_append(q, q, q, q, q, pos, None)):
+            with pytest.raises(ValueError):
+                call()
