@@ -14,6 +14,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _Here, _require_cuda, _stream, plain_call, wants_grad
@@ -113,6 +114,12 @@ def _on_one_gpu(what, *ts):
     _require_cuda(*ts)
     if any(t is not None and t.device != ts[0].device for t in ts):
         raise ValueError("%s: all tensors must be on one device" % what)
+
+
+def _no_tangents(what, *ts):
+    """Forward-mode differentiation has no formula here; its tangents would be lost in silence."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("%s: forward-mode differentiation is not implemented" % what)
 
 
 def _type_check(what, *sigs):
@@ -246,6 +253,7 @@ def norm_rope(q, k, table, q_weight=None, k_weight=None, pos=None, eps=1e-6):
     ts = (q, k, table, pos, q_weight, k_weight)
     if wants_grad(table):
         raise ValueError("norm_rope: the table is a constant; it has no gradient")
+    _no_tangents("norm_rope", *ts)
     if not plain_call(*ts):
         return _norm_op(*ts, float(eps))
     out = _host().norm_rope(q, k, table, q_weight, k_weight, pos, eps)
@@ -325,6 +333,7 @@ def norm_rope_append(q, k, v, k_cache, v_cache, pos, table, q_weight=None, k_wei
     ts = (q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
     if wants_grad(*ts):
         raise ValueError("norm_rope_append: forward only; use norm_rope where a gradient is wanted")
+    _no_tangents("norm_rope_append", *ts)
     if not plain_call(*ts):
         return _append_op(*ts, float(eps))
     out = _host().norm_rope_append(*ts, eps)
@@ -475,6 +484,7 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
     in q, k and v; results and gradients are equal from run to run."""
     window, cap, scale = _numbers("token_attention", q, window, cap, scale, slopes)
     ts = (q, k, v, slopes, docs, prefix)
+    _no_tangents("token_attention", *ts)
     if not plain_call(*ts):
         return _attn_op(*ts, window, cap, scale, True)[0]
     out = _host().token_attention(*ts, window, cap, scale)
@@ -543,6 +553,7 @@ def token_attention_step(q, k_cache, v_cache, pos, window=0, cap=0.0, slopes=Non
     ts = (q, k_cache, v_cache, pos, slopes, start)
     if wants_grad(*ts):
         raise ValueError("token_attention_step: forward only; use token_attention where a gradient is wanted")
+    _no_tangents("token_attention_step", *ts)
     if not plain_call(*ts):
         return _step_op(*ts, window, cap, scale)
     out = _host().token_attention_step(*ts, window, cap, scale)

@@ -68,3 +68,20 @@ def test_a_table_whose_gradient_is_wanted_is_refused():
         S.norm_rope(q, q, table)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
         S.norm_rope(q, q, table)
+
+
+def test_forward_mode_is_refused():
+    """Tangents would be lost in silence; calls without one go on to the next check (here: no CUDA)."""
+    import torch.autograd.forward_ad as fa
+    import slotscan_b200 as S
+    q, kc, w, pos = torch.randn(1, 1, 2, 64), torch.zeros(1, 4, 2, 64), torch.ones(64), torch.zeros(1, dtype=torch.int32)
+    calls = (lambda x: S.norm_rope(x, q, None), lambda x: S.norm_rope(q, q, None, q_weight=x.flatten()[:64]), lambda x: S.norm_rope_append(q, x, q, kc, kc, pos, None),
+             lambda x: S.token_attention(q, q, x), lambda x: S.token_attention_step(x, kc, kc, pos))
+    for call in calls:
+        with fa.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(fa.make_dual(q, torch.ones_like(q)))
+            with pytest.raises(RuntimeError, match="CUDA"):
+                call(q)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (q,), (torch.ones_like(q),))
