@@ -71,6 +71,9 @@ class AppendParams(ctypes.Structure):
     _fields_ = [("base", NormParams), ("L", ctypes.c_int32), ("v_stride", _Strides), ("kc_stride", _Strides), ("vc_stride", _Strides)]
 
 
+NARROW_WINDOW = 65                                                     # csrc/slotscan_attn.cuh: bf16 windows with kernels of their own
+
+
 class AttnParams(ctypes.Structure):
     """slotscan_attn_params of include/slotscan.h."""
     _fields_ = [(n, ctypes.c_int32) for n in ("B", "Tq", "Tk", "H", "KV", "D", "window", "dtype")] + \

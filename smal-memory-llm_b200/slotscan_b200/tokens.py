@@ -399,10 +399,16 @@ def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slopes: Optiona
 _attn_op = torch.library.custom_op("slotscan::attn_fwd", mutates_args=())(_attn_fwd)
 
 
+def _keeps(q, k, prefix, window):
+    """slotscan_attn_keeps for sizes that may be symbols: asks of them no more than the choice of the kernels needs."""
+    if q.dtype != torch.bfloat16 or prefix is not None or q.shape[1] != k.shape[1]:
+        return True
+    return not (0 < window <= _lib.NARROW_WINDOW or k.shape[1] <= _lib.NARROW_WINDOW)
+
+
 @_attn_op.register_fake
 def _(q, k, v, slopes, docs, prefix, window, cap, scale, for_bwd):
-    sig = lambda t: None if t is None else (tuple(int(n) for n in t.shape), (0,) * (t.dim() - 1) + (1,), t.dtype)   # noqa: E731
-    keeps = for_bwd and _attn_plan(*(sig(t) for t in (q, k, v, slopes, docs, prefix)), window, cap, scale)[1]
+    keeps = for_bwd and _keeps(q, k, prefix, window)
     return (q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if keeps else (0,), dtype=torch.float32),
             q.new_empty(q.shape if keeps and q.dtype == torch.bfloat16 else (0,)))
 

@@ -122,3 +122,29 @@ def test_heads_without_channels_are_refused():
                      lambda: S.norm_rope_append(q, q, q, q, q, pos, None)):
             with pytest.raises(ValueError):
                 call()
+
+
+def test_a_compiled_block_serves_every_length():
+    from torch._dynamo.backends.debugging import aot_eager
+    S = _S()
+    graphs = []
+
+    def backend(gm, inputs):
+        graphs.append(gm)
+        return aot_eager(gm, inputs)
+
+    table = S.rope_table(400, 64, device="cuda")
+
+    def block(q, k, v):
+        q, k = S.norm_rope(q, k, table)
+        return S.token_attention(q, k, v)
+    torch._dynamo.reset()
+    f = torch.compile(block, backend=backend, dynamic=True, fullgraph=True)
+    for T in (100, 140, 230, 317):
+        x = [_randn(T + H, 2, T, H, 64).bfloat16().requires_grad_() for H in (4, 2, 2)]
+        do = _randn(T, 2, T, 4, 64).bfloat16()
+        a, b = f(*x), block(*x)
+        assert torch.equal(a, b) and all(torch.equal(m, n) for m, n in zip(torch.autograd.grad(a, x, do), torch.autograd.grad(b, x, do)))
+    assert len(graphs) == 1
+    with torch.no_grad():
+        assert torch.equal(f(*x), a)

@@ -85,3 +85,39 @@ def test_forward_mode_is_refused():
                 call(q)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(call, (q,), (torch.ones_like(q),))
+
+
+def _traced(f, *tensors):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    return make_fx(f, tracing_mode="symbolic")(*tensors)
+
+
+def _meta(*shape, dt=torch.bfloat16, grad=False):
+    return torch.empty(*shape, device="meta", dtype=dt, requires_grad=grad)
+
+
+@pytest.mark.parametrize("window", [0, 16, 200])
+def test_tracing_fixes_neither_batch_nor_length(window):
+    """A block that is compiled with symbolic sizes serves every batch and length: no guard names the traced ones."""
+    import slotscan_b200 as S
+    B, T = 37, 149
+
+    def block(q, k, v, table):
+        q, k = S.norm_rope(q, k, table)
+        return S.token_attention(q, k, v, window=window)
+    g = _traced(block, _meta(B, T, 4, 64), _meta(B, T, 2, 64), _meta(B, T, 2, 64), _meta(1000, 32, 2, dt=torch.float32))
+    guards = [str(x.expr) for x in g.shape_env.guards]
+    assert guards and not any(re.search(r"\b(%d|%d)\b" % (B, T), x) for x in guards), guards
+
+
+def test_the_fake_form_keeps_what_the_library_keeps():
+    import ctypes
+    from slotscan_b200 import _lib, tokens as K
+    L = _lib.lib()
+    for dt, code in ((torch.bfloat16, _lib.BF16), (torch.float32, _lib.F32)):
+        for Tq, Tk in ((1, 1), (64, 64), (65, 65), (66, 66), (300, 300), (20, 65), (20, 300)):
+            for window in (0, 1, 64, 65, 66, 299, 1000):
+                for prefix in (None, torch.zeros(2, device="meta", dtype=torch.int32)):
+                    p = _lib.AttnParams(2, Tq, Tk, 2, 2, 64, window, code, 0.125, 0.0)
+                    want = bool(L.slotscan_attn_keeps(ctypes.byref(p), prefix is not None))
+                    assert K._keeps(_meta(2, Tq, 2, 64, dt=dt), _meta(2, Tk, 2, 64, dt=dt), prefix, window) is want, (dt, Tq, Tk, window)
