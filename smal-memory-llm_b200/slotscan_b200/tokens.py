@@ -492,7 +492,7 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
     ts = (q, k, v, slopes, docs, prefix)
     _no_tangents("token_attention", *ts)
     if not plain_call(*ts):
-        return _attn_op(*ts, window, cap, scale, True)[0]
+        return _attn_op(*ts, window, cap, scale, wants_grad(q, k, v))[0]
     out = _host().token_attention(*ts, window, cap, scale)
     if out is None:
         _on_one_gpu("token_attention", *ts)

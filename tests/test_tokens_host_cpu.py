@@ -121,3 +121,12 @@ def test_the_fake_form_keeps_what_the_library_keeps():
                     p = _lib.AttnParams(2, Tq, Tk, 2, 2, 64, window, code, 0.125, 0.0)
                     want = bool(L.slotscan_attn_keeps(ctypes.byref(p), prefix is not None))
                     assert K._keeps(_meta(2, Tq, 2, 64, dt=dt), _meta(2, Tk, 2, 64, dt=dt), prefix, window) is want, (dt, Tq, Tk, window)
+
+
+@pytest.mark.parametrize("grad,mode", [(False, True), (True, True), (True, False)])
+def test_a_traced_call_without_gradients_keeps_nothing_for_them(grad, mode):
+    import slotscan_b200 as S
+    with torch.set_grad_enabled(mode):
+        g = _traced(lambda q, k: S.token_attention(q, k, k), _meta(2, 300, 4, 64, grad=grad), _meta(2, 300, 2, 64))
+    call, = (n for n in g.graph.nodes if "attn_fwd" in str(n.target))
+    assert call.args[-1] is (grad and mode)
