@@ -151,15 +151,27 @@ def _norm_checked(what, q, k, table, q_weight, k_weight):
     return qs[0], qs[1], qs[2], ks[2], qs[3], 0 if table is None else 2 * table[0][1], 0 if table is None else table[0][0]
 
 
-@functools.lru_cache(maxsize=256)
-def _norm_plan(q, k, table, pos, q_weight, k_weight, eps):
-    """(reference to the parameters, scratch bytes of the backward, the parameters); the reference is None where q or k must be copied."""
+def _norm_shapes(q, k, table, pos, q_weight, k_weight):
     sizes = _norm_checked("norm_rope", q, k, table, q_weight, k_weight)
     if pos is not None and pos[0] != q[0][:2]:
         raise ValueError("norm_rope: positions (B, T), got %s" % (tuple(pos[0]),))
     _integers("norm_rope", pos)
     if pos is None and table is not None and sizes[1] > sizes[6]:
         raise ValueError("norm_rope: %d tokens, %d positions in the table" % (sizes[1], sizes[6]))
+    return sizes
+
+
+def _norm_limits(sizes, dtype, eps):
+    """The library's limits on heads and channels, of sizes whose others may be symbols."""
+    _, _, H, KV, D, R, _ = sizes
+    p = _lib.NormParams(1, 1, int(H), int(KV), int(D), int(R), 1, _CODE[dtype], eps)
+    _lib.check(_lib.lib().slotscan_norm_rope_check(ctypes.byref(p)), "slotscan_norm_rope_check")
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_plan(q, k, table, pos, q_weight, k_weight, eps):
+    """(reference to the parameters, scratch bytes of the backward, the parameters); the reference is None where q or k must be copied."""
+    sizes = _norm_shapes(q, k, table, pos, q_weight, k_weight)
     strides = _strides(q), _strides(k)
     p = _lib.NormParams(*sizes, _CODE[q[2]], eps, *((0, 0, 0) if s is None else s for s in strides))
     _lib.check(_lib.lib().slotscan_norm_rope_check(ctypes.byref(p)), "slotscan_norm_rope_check")
@@ -190,6 +202,7 @@ _norm_op = torch.library.custom_op("slotscan::norm_rope_fwd", mutates_args=())(_
 
 @_norm_op.register_fake
 def _(q, k, table, pos, q_weight, k_weight, eps):
+    _norm_limits(_norm_shapes(*map(_sig, (q, k, table, pos, q_weight, k_weight))), q.dtype, eps)
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
@@ -279,9 +292,9 @@ def _cache_bases(what, k_cache, v_cache):
         raise ValueError("%s: the caches must begin on a 16-byte boundary" % what)
 
 
-@functools.lru_cache(maxsize=256)
-def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps):
-    B, T, H, KV, D, R, length = sizes = _norm_checked("norm_rope_append", q, k, table, q_weight, k_weight)
+def _append_shapes(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight):
+    """Sizes, and the caches' strides."""
+    B, T, _, KV, D, _, _ = sizes = _norm_checked("norm_rope_append", q, k, table, q_weight, k_weight)
     _type_check("norm_rope_append", q, k, v)
     kcs, vcs = _caches("norm_rope_append", k_cache, v_cache, q[2])
     L = k_cache[0][1]
@@ -291,10 +304,17 @@ def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps)
     if T > L:
         raise ValueError("norm_rope_append: %d tokens at once into caches of %d rows" % (T, L))
     _integers("norm_rope_append", pos)
+    return sizes, kcs, vcs
+
+
+@functools.lru_cache(maxsize=256)
+def _append_plan(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps):
+    """(reference to the parameters, the parameters); None where q, k or v must be copied."""
+    sizes, kcs, vcs = _append_shapes(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
     if None in (qs, ks, vs):
         return None, None
-    p = _lib.AppendParams(_lib.NormParams(*sizes, _CODE[q[2]], eps, qs, ks), L, vs, kcs, vcs)
+    p = _lib.AppendParams(_lib.NormParams(*sizes, _CODE[q[2]], eps, qs, ks), k_cache[0][1], vs, kcs, vcs)
     return ctypes.byref(p), p
 
 
@@ -324,6 +344,7 @@ _append_op = torch.library.custom_op("slotscan::norm_rope_append", mutates_args=
 
 @_append_op.register_fake
 def _(q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight, eps):
+    _norm_limits(_append_shapes(*map(_sig, (q, k, v, k_cache, v_cache, pos, table, q_weight, k_weight)))[0], q.dtype, eps)
     return q.new_empty(q.shape)
 
 
@@ -345,10 +366,8 @@ def norm_rope_append(q, k, v, k_cache, v_cache, pos, table, q_weight=None, k_wei
 
 # ---------------------------------------------------------------------------------------- attention
 
-@functools.lru_cache(maxsize=256)
-def _attn_plan(q, k, v, slopes, docs, prefix, window, cap, scale):
-    """(reference to the parameters, whether the backward needs what the forward can keep, the parameters); the reference is None
-    where q, k or v must be copied."""
+def _attn_shapes(q, k, v, slopes, docs, prefix):
+    """B, Tq, Tk, H, KV, D."""
     _type_check("token_attention", q, k, v)
     qs, ks = q[0], k[0]
     if len(qs) != 4 or len(ks) != 4 or v[0] != ks or qs[0] != ks[0] or qs[3] != ks[3] or ks[2] == 0 or qs[2] % ks[2]:
@@ -365,8 +384,16 @@ def _attn_plan(q, k, v, slopes, docs, prefix, window, cap, scale):
     if prefix is not None and prefix[0] != (B,):
         raise ValueError("token_attention: one prefix length for each sequence, got %s" % (tuple(prefix[0]),))
     _integers("token_attention", docs, prefix)
+    return B, Tq, Tk, H, ks[2], D
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_plan(q, k, v, slopes, docs, prefix, window, cap, scale):
+    """(reference to the parameters, whether the backward needs what the forward can keep, the parameters); the reference is None
+    where q, k or v must be copied."""
+    sizes = _attn_shapes(q, k, v, slopes, docs, prefix)
     strides = _strides(q), _strides(k), _strides(v)
-    p = _lib.AttnParams(B, Tq, Tk, H, ks[2], D, window, _CODE[q[2]], scale, cap, *((0, 0, 0) if s is None else s for s in strides))
+    p = _lib.AttnParams(*sizes, window, _CODE[q[2]], scale, cap, *((0, 0, 0) if s is None else s for s in strides))
     _lib.check(_lib.lib().slotscan_attn_check(ctypes.byref(p)), "slotscan_attn_check")
     return None if None in strides else ctypes.byref(p), bool(_lib.lib().slotscan_attn_keeps(ctypes.byref(p), prefix is not None)), p
 
@@ -408,6 +435,9 @@ def _keeps(q, k, prefix, window):
 
 @_attn_op.register_fake
 def _(q, k, v, slopes, docs, prefix, window, cap, scale, for_bwd):
+    _, _, _, H, KV, D = _attn_shapes(*map(_sig, (q, k, v, slopes, docs, prefix)))
+    p = _lib.AttnParams(1, 1, 1, int(H), int(KV), int(D), window, _CODE[q.dtype], scale, cap)
+    _lib.check(_lib.lib().slotscan_attn_check(ctypes.byref(p)), "slotscan_attn_check")
     keeps = for_bwd and _keeps(q, k, prefix, window)
     return (q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]) if keeps else (0,), dtype=torch.float32),
             q.new_empty(q.shape if keeps and q.dtype == torch.bfloat16 else (0,)))
@@ -501,9 +531,8 @@ def token_attention(q, k, v, window=0, cap=0.0, slopes=None, docs=None, prefix=N
     return out
 
 
-@functools.lru_cache(maxsize=256)
-def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
-    """(reference to the parameters, scratch bytes, the parameters); the reference is None where q must be copied."""
+def _step_shapes(q, k_cache, v_cache, pos, slopes, start):
+    """B, H, KV, D, L, and the caches' strides."""
     _type_check("token_attention_step", q)
     if len(q[0]) != 4 or q[0][1] != 1:
         raise ValueError("token_attention_step: one query for each sequence, (B, 1, H, D), got %s" % (tuple(q[0]),))
@@ -515,8 +544,15 @@ def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
     if pos[0] != (B,) or (start is not None and start[0] != (B,)) or (slopes is not None and slopes[0] != (H,)):
         raise ValueError("token_attention_step: positions (B), starts (B) and slopes (H)")
     _integers("token_attention_step", pos, start)
+    return (B, H, KV, D, L), ks, vs
+
+
+@functools.lru_cache(maxsize=256)
+def _step_plan(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
+    """(reference to the parameters, scratch bytes, the parameters); the reference is None where q must be copied."""
+    sizes, ks, vs = _step_shapes(q, k_cache, v_cache, pos, slopes, start)
     qs = _strides(q)
-    p = _lib.AttnStepParams(B, H, KV, D, L, window, _CODE[q[2]], scale, cap, (0, 0) if qs is None else (qs[0], qs[2]), ks, vs)
+    p = _lib.AttnStepParams(*sizes, window, _CODE[q[2]], scale, cap, (0, 0) if qs is None else (qs[0], qs[2]), ks, vs)
     _lib.check(_lib.lib().slotscan_attn_step_check(ctypes.byref(p)), "slotscan_attn_step_check")
     return None if qs is None else ctypes.byref(p), _lib.lib().slotscan_attn_step_scratch_bytes(ctypes.byref(p)), p
 
@@ -548,6 +584,9 @@ _step_op = torch.library.custom_op("slotscan::attn_step", mutates_args=())(_step
 
 @_step_op.register_fake
 def _(q, k_cache, v_cache, pos, slopes, start, window, cap, scale):
+    (_, H, KV, D, _), _, _ = _step_shapes(*map(_sig, (q, k_cache, v_cache, pos, slopes, start)))
+    p = _lib.AttnStepParams(1, int(H), int(KV), int(D), 1, window, _CODE[q.dtype], scale, cap)
+    _lib.check(_lib.lib().slotscan_attn_step_check(ctypes.byref(p)), "slotscan_attn_step_check")
     return q.new_empty(q.shape)
 
 

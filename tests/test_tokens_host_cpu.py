@@ -130,3 +130,37 @@ def test_a_traced_call_without_gradients_keeps_nothing_for_them(grad, mode):
         g = _traced(lambda q, k: S.token_attention(q, k, k), _meta(2, 300, 4, 64, grad=grad), _meta(2, 300, 2, 64))
     call, = (n for n in g.graph.nodes if "attn_fwd" in str(n.target))
     assert call.args[-1] is (grad and mode)
+
+
+def test_fake_forms_refuse_what_the_eager_forms_refuse():
+    """Shapes, types and limits, before anything is compiled; what is right passes, with the results' shapes and types."""
+    import slotscan_b200 as S
+    with FakeTensorMode():
+        f = lambda *s, dt=torch.bfloat16: _meta(*s, dt=dt)                                        # noqa: E731
+        i = lambda *s: _meta(*s, dt=torch.int32)                                                  # noqa: E731
+        q, k, kc, pos, one = f(2, 9, 4, 64), f(2, 9, 2, 64), f(2, 16, 2, 64), i(2), f(2, 1, 4, 64)
+        t = _meta(16, 32, 2, dt=torch.float32)
+        wide = [f(1, 4, 2, 136)] * 3
+        V, T = ValueError, TypeError
+        for err, call in [
+                (T, lambda: S.token_attention(q, k.float(), k)), (T, lambda: S.token_attention(q.half(), k.half(), k.half())), (V, lambda: S.token_attention(q, k, k[:, :8])),
+                (V, lambda: S.token_attention(f(2, 9, 3, 64), k, k)), (V, lambda: S.token_attention(q, k[:, :5], k[:, :5])), (V, lambda: S.token_attention(*wide)),
+                (V, lambda: S.token_attention(q, k, k, scale=-1.0)), (V, lambda: S.token_attention(q, k, k, slopes=f(3))), (T, lambda: S.token_attention(q, k, k, prefix=f(2))),
+                (V, lambda: S.token_attention(q, k, k, docs=i(2, 9))), (V, lambda: S.token_attention(q, k, k, prefix=i(1))),
+                (T, lambda: S.norm_rope(q, k.float(), t)), (V, lambda: S.norm_rope(q, k[:, :3], t)), (V, lambda: S.norm_rope(q, k, t[:4])), (V, lambda: S.norm_rope(q, k, t[..., :1])),
+                (V, lambda: S.norm_rope(q, k, f(16, 36, 2, dt=torch.float32))), (V, lambda: S.norm_rope(q, k, t, q_weight=f(32))), (V, lambda: S.norm_rope(q, k, t, pos=pos)),
+                (T, lambda: S.norm_rope(q, k, t, pos=f(2, 9))), (V, lambda: S.norm_rope(f(1, 2, 1, 264), f(1, 2, 1, 264), None)),
+                (V, lambda: S.norm_rope_append(q, k, k, kc[:, :8], kc[:, :8], pos, t)), (V, lambda: S.norm_rope_append(q, k, k, kc.float(), kc, pos, t)),
+                (V, lambda: S.norm_rope_append(q, k, k, kc[..., ::2], kc[..., ::2], pos, t)), (V, lambda: S.norm_rope_append(q, k, k, kc, kc, pos[:1], t)),
+                (V, lambda: S.token_attention_step(q, kc, kc, pos)), (V, lambda: S.token_attention_step(f(2, 1, 3, 64), kc, kc, pos)),
+                (V, lambda: S.token_attention_step(f(2, 1, 4, 32), kc, kc, pos)), (V, lambda: S.token_attention_step(one, kc, kc, pos, start=pos[:1])),
+                (T, lambda: S.token_attention_step(one, kc, kc, f(2)))]:
+            with pytest.raises(err):
+                call()
+        a, b = torch.ops.slotscan.norm_rope_fwd(q, k, t, None, None, None, 1e-6)
+        assert (a.shape, b.shape, a.dtype) == (q.shape, k.shape, q.dtype)
+        assert torch.ops.slotscan.norm_rope_append(q, k, k, kc, f(2, 16, 2, 64), pos, t, None, None, 1e-6).shape == q.shape
+        assert torch.ops.slotscan.attn_step(one, kc, kc, pos, None, None, 0, 0.0, 0.125).shape == one.shape
+        for dt, window, sizes in ((torch.bfloat16, 0, ((2, 4, 90), (2, 90, 4, 64))), (torch.bfloat16, 16, ((0,), (0,))), (torch.float32, 16, ((2, 4, 90), (0,)))):
+            o, lse, rest = torch.ops.slotscan.attn_fwd(f(2, 90, 4, 64, dt=dt), *[f(2, 90, 2, 64, dt=dt)] * 2, None, None, None, window, 0.0, 0.125, True)
+            assert o.shape == (2, 90, 4, 64) and o.dtype is dt and lse.dtype is torch.float32 and (tuple(lse.shape), tuple(rest.shape)) == sizes
