@@ -164,3 +164,13 @@ def test_fake_forms_refuse_what_the_eager_forms_refuse():
         for dt, window, sizes in ((torch.bfloat16, 0, ((2, 4, 90), (2, 90, 4, 64))), (torch.bfloat16, 16, ((0,), (0,))), (torch.float32, 16, ((2, 4, 90), (0,)))):
             o, lse, rest = torch.ops.slotscan.attn_fwd(f(2, 90, 4, 64, dt=dt), *[f(2, 90, 2, 64, dt=dt)] * 2, None, None, None, window, 0.0, 0.125, True)
             assert o.shape == (2, 90, 4, 64) and o.dtype is dt and lse.dtype is torch.float32 and (tuple(lse.shape), tuple(rest.shape)) == sizes
+
+
+def test_the_library_builds_without_torch():
+    """A user of the C ABI needs no torch: without it `make` builds the library alone, with it the host module too."""
+    import subprocess
+    import sys
+    for python, host in (("false", False), (sys.executable, True)):
+        r = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "smal-memory-llm_b200"), "PYTHON=" + python], capture_output=True, text=True)
+        assert r.returncode == 0 and "-o slotscan_b200/libslotscan.so" in r.stdout, r.stderr
+        assert ("-o slotscan_b200/_tokens_host.so" in r.stdout) is host
