@@ -342,7 +342,8 @@ typedef struct {
     int64_t q_stride[3], k_stride[3], v_stride[3];
 } slotscan_attn_params;
 int slotscan_attn_check(const slotscan_attn_params* p);
-/* Whether the backward of such a call needs o, lse and rest of the forward and delta; 0: they may be NULL. */
+/* Whether the backward of such a call needs o, lse and rest of the forward and delta; 0: they may be NULL, and lse and rest are written
+ * where they are given all the same. */
 int slotscan_attn_keeps(const slotscan_attn_params* p, int with_prefix);
 int slotscan_attn_fwd(const slotscan_attn_params* p, const void* q, const void* k, const void* v, const float* slopes,
                       const int32_t* docs, const int32_t* prefix, void* o, void* rest, float* lse, void* stream);

@@ -43,7 +43,7 @@ extern "C" int slotscan_attn_fwd(const slotscan_attn_params* p, const void* q, c
     if (!q || !k || !v || !o) return SLOTSCAN_E_NULL;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(rest) || ((uintptr_t)docs & 7)) return SLOTSCAN_E_ALIGN;
     const AttnArgs a = attn_args(*p, slopes, docs, prefix);
-    if (p->dtype == SLOTSCAN_BF16 && attn_narrow(a)) return (int)run_attn_fwd_narrow(a, q, k, v, o, (cudaStream_t)stream);
+    if (p->dtype == SLOTSCAN_BF16 && attn_narrow(a)) return (int)run_attn_fwd_narrow(a, q, k, v, o, lse ? rest : nullptr, lse, (cudaStream_t)stream);
     if (p->dtype == SLOTSCAN_BF16 && lse && !rest) return SLOTSCAN_E_NULL;
     return (int)(p->dtype == SLOTSCAN_BF16 ? run_attn_fwd_bf16(a, q, k, v, o, rest, lse, (cudaStream_t)stream)
                                            : run_attn_fwd_f32(a, q, k, v, o, lse, (cudaStream_t)stream));

@@ -256,7 +256,7 @@ cudaError_t run_attn_bwd_bf16(const AttnArgs& a, const void* q, const void* k, c
 // nothing of the forward
 constexpr int NARROW_WINDOW = 65;
 bool attn_narrow(const AttnArgs& a);
-cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st);
+cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st);
 cudaError_t run_attn_bwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv,
                                 cudaStream_t st);
 

@@ -83,10 +83,10 @@ __device__ __forceinline__ void band(float (&s)[2 * NB][4], uint32_t Q, int q_ro
 }
 
 // Scores to unnormalised weights exp2(z - max), in place, and the sum's reciprocal of the lane's two rows; F: also 1 - tanh^2 of each.
-// key0: position of the first key
+// key0: position of the first key; lse: the two rows' logarithms as slotscan_attn_fwd gives them, or NULL
 template <int NB, bool F>
 __device__ __forceinline__ void band_softmax(float (&s)[2 * NB][4], float (&f)[F ? 2 * NB : 1][4], float (&inv)[2], const Score& sc, const Span (&sp)[2],
-                                             const int (&at)[2], int key0, int lane) {
+                                             const int (&at)[2], int key0, int lane, float* lse = nullptr) {
     const bool capped = sc.cap_in != 0.f;
 #pragma unroll
     for (int r = 0; r < 2; r++) {
@@ -122,7 +122,9 @@ __device__ __forceinline__ void band_softmax(float (&s)[2 * NB][4], float (&f)[F
             }
         sum += __shfl_xor_sync(FULL, sum, 1);
         sum += __shfl_xor_sync(FULL, sum, 2);
-        inv[r] = sp[r].hi > sp[r].lo ? 1.f / sum : 0.f;
+        const int n = sp[r].hi - sp[r].lo;
+        inv[r] = n > 0 ? 1.f / sum : 0.f;
+        if (lse != nullptr) lse[r] = n <= 0 ? -INFINITY : n == 1 ? INFINITY : base + log2f(sum);
     }
 }
 
@@ -139,8 +141,10 @@ __device__ __forceinline__ void give_up() {              // report, and give the
     for (int i = 0; i < 1000; i++) __nanosleep(1000);
 }
 
-template <int DP, int NB>
-__global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, RowInputs<bf16> in, bf16* out, const __grid_constant__ NarrowMaps maps) {
+// KEEP: with lse, and rest where it is given.  The backward of these windows reads neither, so only callers of the C ABI ask for
+// them; a form of its own, since asking while running costs all others 5 us of 68 (64 x 1,024 tokens, window 16)
+template <int DP, int NB, bool KEEP>
+__global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, RowInputs<bf16> in, bf16* out, bf16* rest, float* lse, const __grid_constant__ NarrowMaps maps) {
     constexpr int KEYS = NA_ROWS + 16 * (NB - 1), SUBS = DP / 64;
     extern __shared__ __align__(1024) char smem[];
     const uint32_t Q = smem_u32(smem), K = Q + NA_ROWS * DP * 2, V = K + KEYS * DP * 2;
@@ -169,7 +173,14 @@ __global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, RowInp
     if (!all_arrived(&qk_full, 0)) { give_up(); return; }
     float s[2 * NB][4], none[1][4], inv[2];
     band<DP, NB>(s, Q, NA_ROWS, warp * 16, K, KEYS, warp * 16, lane);
-    band_softmax<NB, false>(s, none, inv, sc, sp, at, j0 + warp * 16, lane);
+    if constexpr (!KEEP) band_softmax<NB, false>(s, none, inv, sc, sp, at, j0 + warp * 16, lane);
+    else {
+        float x[2];
+        band_softmax<NB, false>(s, none, inv, sc, sp, at, j0 + warp * 16, lane, x);
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+            if (lane % 4 == 0 && at[r] < a.Tq) lse[((size_t)b * a.H + h) * a.Tq + at[r]] = x[r];
+    }
     if (!all_arrived(&v_full, 0)) { give_up(); return; }
     uint32_t p[NB][4];
 #pragma unroll
@@ -193,9 +204,18 @@ __global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, RowInp
         }
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            put_rows<DP>(Q, NA_ROWS, warp * 16, 2 * c + t, lane, pack_bf16(o[t][0] * inv[0], o[t][1] * inv[0]), pack_bf16(o[t][2] * inv[1], o[t][3] * inv[1]));
+            const uint32_t w[2] = {pack_bf16(o[t][0] * inv[0], o[t][1] * inv[0]), pack_bf16(o[t][2] * inv[1], o[t][3] * inv[1])};
+            put_rows<DP>(Q, NA_ROWS, warp * 16, 2 * c + t, lane, w[0], w[1]);
 #pragma unroll
             for (int i = 0; i < 4; i++) watch(seen, o[t][i]);
+            if (KEEP && rest != nullptr) {
+                const int d = c * 16 + t * 8 + (lane % 4) * 2;
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+                    if (d < a.D && at[r] < a.Tq)
+                        *reinterpret_cast<uint32_t*>(rest + (((size_t)b * a.Tq + at[r]) * a.H + h) * a.D + d) =
+                            pack_bf16(o[t][2 * r] * inv[r] - __uint_as_float(w[r] << 16), o[t][2 * r + 1] * inv[r] - __uint_as_float(w[r] & 0xffff0000u));
+            }
         }
     }
     fence_proxy_async_smem();
@@ -209,9 +229,16 @@ __global__ void __launch_bounds__(128) attn_fwd_narrow_kernel(AttnArgs a, RowInp
         if (lane == 0) bulk_wait<0>();
         __syncwarp();
         for (int i = i0 + warp * 16; i < min(i0 + warp * 16 + 16, a.Tq); i++) {
-            float x[4], unused0, unused1;
-            careful_query(a, in, b, h, i, x, unused0, unused1);
-            put_lane_row(out + (((size_t)b * a.Tq + i) * a.H + h) * a.D, x, a.D);
+            float x[4], l, unused;
+            const size_t to = (((size_t)b * a.Tq + i) * a.H + h) * a.D;
+            careful_query(a, in, b, h, i, x, l, unused);
+            put_lane_row(out + to, x, a.D);
+            if (KEEP && lane == 0) lse[((size_t)b * a.H + h) * a.Tq + i] = l;
+            if (KEEP && rest != nullptr) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[c] -= __bfloat162float(__float2bfloat16_rn(x[c]));
+                put_lane_row(rest + to, x, a.D);
+            }
         }
     }
 }
@@ -414,17 +441,17 @@ __global__ void __launch_bounds__(NarrowBwd<DP, NB>::WARPS * 32, GROUP || NB > 3
 }
 
 template <int DP, int NB>
-static cudaError_t fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st) {
+static cudaError_t fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st) {
     constexpr int KEYS = NA_ROWS + 16 * (NB - 1), SMEM = (NA_ROWS + 2 * KEYS) * DP * 2;
     const long long os[3] = {(long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D};
-    auto kern = attn_fwd_narrow_kernel<DP, NB>;
+    auto kern = lse != nullptr ? attn_fwd_narrow_kernel<DP, NB, true> : attn_fwd_narrow_kernel<DP, NB, false>;
     const cudaError_t e = opt_in_smem(kern, SMEM);       // before the maps: a thread's first runtime call makes the context current for them
     if (e != cudaSuccess) return e;
     NarrowMaps m;
     if (!tile_map(&m.q, q, a.B, a.Tq, a.H, a.D, a.qs, NA_ROWS) || !tile_map(&m.k, k, a.B, a.Tk, a.KV, a.D, a.ks, KEYS) ||
         !tile_map(&m.v, v, a.B, a.Tk, a.KV, a.D, a.vs, KEYS) || !tile_map(&m.o, o, a.B, a.Tq, a.H, a.D, os, 16))
         return cudaErrorInvalidValue;
-    kern<<<dim3((a.Tq + NA_ROWS - 1) / NA_ROWS, a.H, a.B), 128, SMEM, st>>>(a, RowInputs<bf16>{(const bf16*)q, (const bf16*)k, (const bf16*)v, nullptr}, (bf16*)o, m);
+    kern<<<dim3((a.Tq + NA_ROWS - 1) / NA_ROWS, a.H, a.B), 128, SMEM, st>>>(a, RowInputs<bf16>{(const bf16*)q, (const bf16*)k, (const bf16*)v, nullptr}, (bf16*)o, (bf16*)rest, lse, m);
     return cudaGetLastError();
 }
 template <int DP, int NB>
@@ -446,10 +473,10 @@ static cudaError_t bwd_narrow(const AttnArgs& a, const void* q, const void* k, c
 
 bool attn_narrow(const AttnArgs& a) { return a.prefix == nullptr && a.Tq == a.Tk && a.window <= NARROW_WINDOW; }
 
-cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, cudaStream_t st) {
-    if (a.window <= 17) return a.D <= 64 ? fwd_narrow<64, 2>(a, q, k, v, o, st) : fwd_narrow<128, 2>(a, q, k, v, o, st);
-    if (a.window <= 33) return a.D <= 64 ? fwd_narrow<64, 3>(a, q, k, v, o, st) : fwd_narrow<128, 3>(a, q, k, v, o, st);
-    return a.D <= 64 ? fwd_narrow<64, 5>(a, q, k, v, o, st) : fwd_narrow<128, 5>(a, q, k, v, o, st);
+cudaError_t run_attn_fwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, void* rest, float* lse, cudaStream_t st) {
+    if (a.window <= 17) return a.D <= 64 ? fwd_narrow<64, 2>(a, q, k, v, o, rest, lse, st) : fwd_narrow<128, 2>(a, q, k, v, o, rest, lse, st);
+    if (a.window <= 33) return a.D <= 64 ? fwd_narrow<64, 3>(a, q, k, v, o, rest, lse, st) : fwd_narrow<128, 3>(a, q, k, v, o, rest, lse, st);
+    return a.D <= 64 ? fwd_narrow<64, 5>(a, q, k, v, o, rest, lse, st) : fwd_narrow<128, 5>(a, q, k, v, o, rest, lse, st);
 }
 cudaError_t run_attn_bwd_narrow(const AttnArgs& a, const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk, void* dv,
                                 cudaStream_t st) {

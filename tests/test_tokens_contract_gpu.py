@@ -1,5 +1,8 @@
 """What callers of the token ops rely on beside the numbers: what is counted as changed, refused, converted and left unwritten (CUDA)."""
 
+import ctypes
+import math
+
 import pytest
 import torch
 
@@ -148,3 +151,48 @@ def test_a_compiled_block_serves_every_length():
     assert len(graphs) == 1
     with torch.no_grad():
         assert torch.equal(f(*x), a)
+
+
+@pytest.mark.parametrize("T,H,KV,D,window,cap,docs", [(100, 2, 2, 64, 16, 0.0, False), (150, 4, 2, 128, 1, 0.0, False), (65, 2, 1, 40, 0, 5.0, False), (200, 2, 2, 96, 30, 0.0, True),
+                                                      (129, 1, 1, 128, 65, 4.0, True)])
+def test_a_narrow_forward_writes_what_its_caller_asks_for(T, H, KV, D, window, cap, docs):
+    """The C call with lse and rest for a window whose backward needs neither: the logarithms against float64 (a score is off by (D + 16) 2^-24 of
+    its products' magnitudes, the fast exponentials by 2^-22 of the sum, the fast hyperbolic tangent by 2^-21 of the cap), and what the rounding of o left, at most half
+    a step of o.  o is the same with and without them."""
+    from slotscan_b200 import _lib
+    S = _S()
+    B, scale = 2, D ** -0.5
+    q, k, v = (2 * _randn(20 + n, B, T, n, D).bfloat16() for n in (H, KV, KV))
+    doc = torch.zeros(B, T, dtype=torch.int64, device="cuda")
+    if docs:
+        doc = torch.arange(T, device="cuda").div(23, rounding_mode="floor").repeat(B, 1)
+        doc[:, 40:50] = doc[1, 90:] = -1
+    bounds, pad = S.document_bounds(doc), doc < 0
+    for t in (q, k, v):
+        t[pad] = math.nan
+    want = S.token_attention(q, k, v, window=window, cap=cap, docs=bounds if docs else None)
+    st = lambda t: tuple(t.stride()[:3])                                                      # noqa: E731
+    p = _lib.AttnParams(B, T, T, H, KV, D, window, _lib.BF16, scale, cap, st(q), st(k), st(v))
+    assert not _lib.lib().slotscan_attn_keeps(ctypes.byref(p), 0)
+    o, rest, lse = torch.full_like(q, 7.0), torch.full_like(q, 7.0), torch.full((B, H, T), 7.0, device="cuda")
+    rc = _lib.lib().slotscan_attn_fwd(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), None, bounds.data_ptr() if docs else None, None, o.data_ptr(),
+                                      rest.data_ptr(), lse.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    i, j = torch.arange(T, device="cuda")[:, None], torch.arange(T, device="cuda")[None]
+    seen = (j <= i) & (i - j < (window or T)) & (doc[:, :, None] == doc[:, None]) & ~pad[:, None]
+    Q, K = q.double().transpose(1, 2), k.double().transpose(1, 2).repeat_interleave(H // KV, 1)
+    s, mag = Q @ K.transpose(-1, -2) * scale, Q.abs() @ K.abs().transpose(-1, -2) * scale
+    s = cap * torch.tanh(s / cap) if cap else s
+    hide = ~seen[:, None].expand_as(s)
+    ref = torch.logsumexp(s.masked_fill(hide, -math.inf), -1) / math.log(2)
+    off = ((D + 16) * 2.0 ** -24 * mag.masked_fill(hide, 0).amax(-1) + cap * 2.0 ** -21) / math.log(2) + 2.0 ** -21 + ref.abs().nan_to_num(posinf=0.0) * 2.0 ** -23
+    n = seen.sum(-1)[:, None].expand_as(ref)
+    assert (lse[n == 0] == -math.inf).all() and (lse[n == 1] == math.inf).all()
+    assert ((lse.double() - ref).abs() <= off)[n > 1].all()
+    keep = (~pad)[:, :, None, None].expand_as(o)
+    assert torch.equal(o[keep], want[keep]) and not o[~keep].any() and not rest[~keep].any()
+    step = torch.exp2(torch.floor(torch.log2(o.float().abs().clamp_min(2.0 ** -100))) - 8)
+    assert (rest.float().abs() <= step).all()
+    one = (n == 1).transpose(1, 2)[..., None].expand_as(o)
+    assert not rest[one].any()                                         # o is a row of v
+    assert bool(rest[keep & ~one].any()) == bool((keep & ~one).any())
