@@ -174,3 +174,39 @@ def test_the_library_builds_without_torch():
         r = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "smal-memory-llm_b200"), "PYTHON=" + python], capture_output=True, text=True)
         assert r.returncode == 0 and "-o slotscan_b200/libslotscan.so" in r.stdout, r.stderr
         assert ("-o slotscan_b200/_tokens_host.so" in r.stdout) is host
+
+
+def test_c_checks_need_no_gpu():
+    import ctypes
+    from slotscan_b200 import _lib
+    L, P = _lib.lib(), ctypes.byref
+    st = (9 * 6 * 64, 6 * 64, 64)
+    norm = lambda **kw: _with(_lib.NormParams(2, 9, 4, 2, 64, 32, 16, _lib.BF16, 1e-6, st, st), kw)               # noqa: E731
+    append = lambda base={}, **kw: _with(_lib.AppendParams(norm(**base), 16, st, st, st), kw)                     # noqa: E731
+    attn = lambda **kw: _with(_lib.AttnParams(2, 9, 9, 4, 2, 64, 16, _lib.BF16, 0.1, 0.0, st, st, st), kw)        # noqa: E731
+    step = lambda **kw: _with(_lib.AttnStepParams(2, 4, 2, 64, 16, 16, _lib.BF16, 0.1, 0.0, (64 * 6, 64), st, st), kw)    # noqa: E731
+
+    def _with(p, kw):
+        for n, x in kw.items():
+            setattr(p, n, x)
+        return p
+    odd = (ctypes.c_int64 * 3)(9 * 6 * 64, 6 * 64 + 4, 64)
+    for check, make, bad in (
+            (L.slotscan_norm_rope_check, norm, [("dtype", 7), ("H", 0), ("KV", 0), ("D", 12), ("D", 264), ("R", 24), ("R", 80), ("table_len", 0), ("B", -1), ("q_stride", odd)]),
+            (L.slotscan_attn_check, attn, [("dtype", 7), ("B", 65536), ("Tq", 10), ("Tk", 2 ** 29 + 1), ("H", 5), ("KV", 0), ("D", 136), ("D", 12), ("window", -1), ("cap", -1.0),
+                                           ("cap", float("nan")), ("cap", float("inf")), ("scale", 0.0), ("scale", float("nan")), ("k_stride", odd)]),
+            (L.slotscan_attn_step_check, step, [("dtype", 7), ("B", 65536), ("H", 5), ("L", 0), ("L", 2 ** 29 + 1), ("D", 136), ("window", -1), ("cap", float("nan")), ("v_stride", odd)])):
+        assert check(P(make())) == 0 and check(None) == -1
+        for n, x in bad:
+            assert check(P(make(**{n: x}))) < 0, (check.__name__, n, x)
+    # NULL pointers, scratch that is missing and rings that are too short are refused before any launch
+    assert L.slotscan_norm_rope_fwd(P(norm()), *[None] * 9) == -1
+    assert L.slotscan_norm_rope_bwd(P(norm()), *[None] * 13, 0, None) == -1
+    assert L.slotscan_norm_rope_append(P(append()), *[None] * 11) == -1
+    assert L.slotscan_norm_rope_append(P(append(L=8)), *[None] * 11) == L.slotscan_norm_rope_append(P(append(L=0)), *[None] * 11) == -2
+    assert L.slotscan_attn_fwd(P(attn()), *[None] * 10) == L.slotscan_attn_bwd(P(attn()), *[None] * 15) == -1
+    assert L.slotscan_attn_step(P(step()), *[None] * 8, 0, None) == -1
+    # nothing to do is no error
+    assert L.slotscan_norm_rope_fwd(P(norm(B=0)), *[None] * 9) == L.slotscan_attn_fwd(P(attn(B=0)), *[None] * 10) == L.slotscan_attn_step(P(step(B=0)), *[None] * 8, 0, None) == 0
+    assert L.slotscan_attn_step_scratch_bytes(P(step())) == 0 < L.slotscan_attn_step_scratch_bytes(P(step(L=4096, window=0)))
+    assert L.slotscan_norm_rope_bwd_scratch_bytes(P(norm())) >= 2 * 64 * 4

@@ -235,3 +235,71 @@ def test_compiled_generation_step():
         with torch.no_grad():
             assert torch.equal(f(q, k, v, kc, vc, pos), step(q, k, v, ke, ve, pos))
         assert torch.equal(kc, ke) and torch.equal(vc, ve)
+
+
+# ------------------------------------------------------------------------------------------------ layouts and far offsets
+
+def _layouts(t):
+    """The same values where they lie: heads before tokens, tokens before sequences, every second token, in a wider projection."""
+    B, T, H, D = t.shape
+    yield t.transpose(1, 2).contiguous().transpose(1, 2)
+    yield t.transpose(0, 1).contiguous().transpose(0, 1)
+    yield t.repeat_interleave(2, 1)[:, ::2]
+    yield torch.cat((t, t), 2)[:, :, H:]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 16])
+def test_layouts_are_read_in_place(dtype, window):
+    S = _S()
+    g, q, k, v, do = _attn_inputs(dtype, 3, 200, 200, 4, 2, 64, seed=53)
+    x = [t.detach().contiguous().requires_grad_() for t in (q, k, v)]
+    table = S.rope_table(200, 32, device="cuda")
+    o, n = S.token_attention(*x, window=window), S.norm_rope(*x[:2], table)
+    want = (o, *torch.autograd.grad(o, x, do), *n, *torch.autograd.grad(n, x[:2], (do, do[:, :, :2])))
+    caches = [_rand(g, 3, 40, 2, 64).to(DT[dtype]) for _ in range(2)]
+    pos = torch.tensor([0, 7, 90], device="cuda")
+    step = S.token_attention_step(x[0][:, :1].detach(), *caches, pos, window=window)
+    for lay in zip(*(list(_layouts(t)) for t in x)):
+        y = [t.detach().requires_grad_() for t in lay]
+        assert not y[0].is_contiguous() and y[0].data_ptr() % 16 == 0
+        o, n = S.token_attention(*y, window=window), S.norm_rope(*y[:2], table)
+        got = (o, *torch.autograd.grad(o, y, do), *n, *torch.autograd.grad(n, y[:2], (do, do[:, :, :2])))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for lay in zip(*(list(_layouts(t)) for t in (x[0][:, :1].detach(), *caches))):
+        assert torch.equal(S.token_attention_step(*lay, pos, window=window), step)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_offsets_beyond_32_bits(dtype):
+    """Caches and keys of more than 2^31 elements: the last rows are the ones that are written and read.  All other rows are left as
+    the allocator gave them: none of them is seen."""
+    S = _S()
+    g = _gen(55)
+    dt, H, KV, D, W = DT[dtype], 4, 4, 128, 200
+    L = 2 ** 31 // (KV * D) + 3000
+    kc, vc = (torch.empty(1, L, KV, D, device="cuda", dtype=dt) for _ in range(2))
+    n = 500                                              # rows that hold something
+    few = [_rand(g, 1, n, KV, D).to(dt) for _ in range(2)]
+    for big, small in zip((kc, vc), few):
+        big[:, L - n:] = small
+    q, k, v = (_rand(g, 1, 3, h, D).to(dt) for h in (H, KV, KV))
+    pos = torch.tensor([7 * L + L - 3], dtype=torch.int32, device="cuda")
+    near = torch.tensor([n - 3], dtype=torch.int32, device="cuda")
+    q1, q2 = S.norm_rope_append(q, k, v, kc, vc, pos, None), S.norm_rope_append(q, k, v, *few, near, None)
+    assert torch.equal(q1, q2) and all(torch.equal(big[:, L - n:], small) for big, small in zip((kc, vc), few))
+    kw = dict(window=W, slopes=torch.tensor([0.5, 0.1, 0.02, 0.0], device="cuda"))
+    a, b = (S.token_attention_step(q1[:, :1], *c, p + 2, **kw) for c, p in (((kc, vc), pos), (few, near)))
+    assert torch.equal(a, b)
+    o, grads = [], []
+    for c in ((kc, vc), few):
+        x = [t.detach().requires_grad_() for t in (q1, *c)]
+        o.append(S.token_attention(*x, **kw))
+        grads.append(torch.autograd.grad(o[-1], x, q))
+    # tiles begin elsewhere, so sums run in another order: twice the roundings of a weight, as for the kernels against the formula
+    off = 2.0 ** -7 if dtype == "bf16" else 2.0 ** -16
+    within(o[0], o[1].double(), off * few[1].abs().double().amax() + torch.zeros_like(o[1]).double(), "o")
+    for name, far, at in zip(("dq", "dk", "dv"), *grads):
+        far = far if name == "dq" else far[:, L - n:]
+        within(far, at.double(), 8 * off * at.abs().double().amax() + torch.zeros_like(at).double(), name)
+    assert not grads[0][1][:, :L - n:4099].any() and not grads[0][2][:, :L - n:4099].any()
