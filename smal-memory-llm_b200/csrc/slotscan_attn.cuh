@@ -95,7 +95,8 @@ __device__ __forceinline__ float score2(const Score& sc, float s, int dist, floa
 
 // ---- A row at a time, by a warp, over the visible pairs alone ----
 // The tiles' products take hidden keys with weight zero, and zero times infinity or NaN is NaN.  Where a row's result is not finite, it is
-// done anew here: what a row does not see then cannot reach it, and what it sees does.  Costs nothing where all is finite.
+// done anew here: what a row does not see then cannot reach it, and what it sees does.  Costs nothing where all is finite, and
+// much where it is not: one NaN in the padding of 8,192 tokens takes a forward of six heads from 0.18 to 135 ms.
 // A lane holds channels lane + 32 c.
 template <typename T>
 struct RowInputs { const T *q, *k, *v, *dout; };         // dout (B,Tq,H,D) contiguous

@@ -365,7 +365,8 @@ static StepArgs step_args(const slotscan_attn_step_params& p) {
     const int group = p.H / p.KV, G = heads_at_once(group, p.dtype);
     a.chunks = (group + G - 1) / G;
     // 128 rows at least; bf16: two CTAs for each SM at a time (their rings), six rounds of them (8 x 131,072 rows: two rounds 384 us, four
-    // 363, six 341, eight 351); float32: eight for each SM
+    // 363, six 341, eight 351); float32: eight for each SM.  Rounded up: 32 sequences over four key heads take 14 splits, 1,792 CTAs, the last
+    // 16 of them in a seventh round
     const long long ctas = (long long)p.B * p.KV * a.chunks, want = 148 * (p.dtype == SLOTSCAN_BF16 ? 12 : 8);
     long long s = (want + ctas - 1) / (ctas > 0 ? ctas : 1);
     if (s > (a.window + 127) / 128) s = (a.window + 127) / 128;
