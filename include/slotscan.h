@@ -363,6 +363,66 @@ size_t slotscan_attn_step_scratch_bytes(const slotscan_attn_step_params* p);
 int slotscan_attn_step(const slotscan_attn_step_params* p, const void* q, const void* k, const void* v, const int32_t* pos,
                        const int32_t* start, const float* slopes, void* o, void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Serving over pages: requests of uneven lengths share a pool of pages of `page` tokens (a power of two, 8 to 1024).  Token j of request b
+ * lies in page tables[b, j / page], row j mod page; its slot is that page's id times `page` plus the row.  The new tokens of all requests
+ * are packed: rows starts[b] to starts[b + 1] of a batch of `tokens` rows are request b's, and rows behind the last belong to none.
+ * [The reference has none of this: it scans a context in one call, memlm_sh.py:676.]
+ *
+ * Turn of a scheduler.  lengths (B) int32: tokens held;  tables (B, M) int32, rows table_stride apart;  free_pages (pages) int32: a stack,
+ * of which the first n_free (1) int32 entries are free.  All four are changed in place.
+ * slotscan_release_pages: each request with done[b] != 0 gives its pages back, in the order of requests and pages, behind the free
+ * ones; its length becomes 0 and its table minus ones.
+ * slotscan_extend_pages: fresh[b] new tokens for each request (negative: none).  A request is served whole or not at all: not where its
+ * table or the batch has no room for them, and not where it needs pages and the pages needed by it and the requests before it (the ones
+ * that had no room left out) are more than there are.  Pages are taken from the end of the stack, in the order of requests and pages.
+ *   slots, pos (tokens) int32: slot and position of each row's token, minus ones where there is none (rows of requests not served
+ *   among them);  starts (B + 1) int32, at most `tokens`;  taken (B) int32: fresh[b], or 0 where it is not served
+ * scratch of slotscan_pages_scratch_bytes for either.  Results are equal from run to run. */
+typedef struct {
+    int32_t B, M, page, pages, tokens;
+    int64_t table_stride;
+} slotscan_pages_params;
+int slotscan_pages_check(const slotscan_pages_params* p);
+size_t slotscan_pages_scratch_bytes(const slotscan_pages_params* p);
+int slotscan_extend_pages(const slotscan_pages_params* p, const int32_t* fresh, int32_t* lengths, int32_t* tables, int32_t* free_pages,
+                          int32_t* n_free, int32_t* slots, int32_t* pos, int32_t* starts, int32_t* taken, void* scratch, size_t scratch_bytes,
+                          void* stream);
+int slotscan_release_pages(const slotscan_pages_params* p, const uint8_t* done, int32_t* lengths, int32_t* tables, int32_t* free_pages,
+                           int32_t* n_free, void* scratch, size_t scratch_bytes, void* stream);
+/* slotscan_norm_rope_fwd for the rows of a packed batch (base.B 1, base.T rows, the sequence strides unused): row i stands at position
+ * pos[i], and its rotated key and its value v (rows, KV, D) go to slot slots[i] of the pages (pages, page, KV, D), whose strides are of a
+ * page, a row and a head.  A slot outside the pages stores nothing; a row with a negative position stores nothing and gives zeros. */
+typedef struct {
+    slotscan_norm_params base;
+    int32_t pages, page;
+    int64_t v_stride[3], kp_stride[3], vp_stride[3];
+} slotscan_page_append_params;
+int slotscan_norm_rope_pages(const slotscan_page_append_params* p, const void* q, const void* k, const void* v, const float* table,
+                             const int32_t* slots, const int32_t* pos, const float* qw, const float* kw, void* qo, void* kp, void* vp,
+                             void* stream);
+/* Attention over pages: query row i, of request b, stands at position pos[i] and sees the positions j of its request with
+ *     max(start[b], 0) <= j <= pos[i],   pos[i] - j < window (if window > 0),   j < M * page
+ * (start NULL: 0); scores, cap and slopes as in slotscan_attn_fwd with |i - j| = pos[i] - j.  A row that sees nothing, one with a negative
+ * position among them, gives zeros.  A page outside the pool reads as zeros.  Rows of pages that a query does not see do not
+ * reach it, whatever they hold.
+ *   q (rows, H, D), strides of a row and a head;  kp, vp (pages, page, KV, D), strides of a page, a row and a head;  tables (B, M) int32
+ *   slotscan_paged_step: a row for each request, N = B, starts NULL.   slotscan_paged_attn: rows starts[b] to starts[b + 1]; rows behind
+ *   the last and before the first give zeros; starts does not fall (what rows of a falling one hold is not said), and lies within 0 to N
+ *   o (N, H, D) contiguous.  scratch of slotscan_paged_{step,attn}_scratch_bytes, which depends on p alone */
+typedef struct {
+    int32_t N, B, H, KV, D, pages, page, M, window, dtype;
+    float scale, cap;
+    int64_t q_stride[2], k_stride[3], v_stride[3], table_stride;
+} slotscan_paged_params;
+int slotscan_paged_check(const slotscan_paged_params* p);
+size_t slotscan_paged_step_scratch_bytes(const slotscan_paged_params* p);
+int slotscan_paged_step(const slotscan_paged_params* p, const void* q, const void* kp, const void* vp, const int32_t* tables, const int32_t* pos,
+                        const int32_t* start, const float* slopes, void* o, void* scratch, size_t scratch_bytes, void* stream);
+size_t slotscan_paged_attn_scratch_bytes(const slotscan_paged_params* p);
+int slotscan_paged_attn(const slotscan_paged_params* p, const void* q, const void* kp, const void* vp, const int32_t* tables, const int32_t* starts,
+                        const int32_t* pos, const int32_t* start, const float* slopes, void* o, void* scratch, size_t scratch_bytes, void* stream);
+
 /* Registers / spilled bytes / static shared memory / max threads of each kernel, the analogue of kernel_attrs
  * (gqa25/slotkern_cuda.py:467-479).  Fills up to `cap` entries (HOST memory), returns how many kernels exist. */
 typedef struct {

@@ -17,6 +17,7 @@
 #include "slotscan_attn.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_tensor.cuh"
+#include "slotscan_warp_mma.cuh"
 
 namespace slotscan {
 
@@ -147,22 +148,6 @@ __global__ void __launch_bounds__(ST_THREADS) attn_step_kernel(StepArgs a, const
 
 // ---- bf16 ----
 constexpr int SM_WARPS = 4, SM_KEYS = 16, SM_STAGES = 3;
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
-}
-// 16 bytes into shared memory, zeros unless `in`
-__device__ __forceinline__ void cp_async16_or0(uint32_t dst, const void* src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
 
 // WIDE: 16 query heads to a CTA, else 8
 template <int DP, bool WIDE>

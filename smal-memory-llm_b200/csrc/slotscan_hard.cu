@@ -458,7 +458,7 @@ extern "C" int slotscan_device_status(void) {
     if (cudaDeviceSynchronize() != cudaSuccess) return -1;
     int all = 0;
     for (int (*status)() : {rows_bwd_status_f32, rows_bwd_status_bf16, read_mma_status, gather_status_f32, gather_status_bf16, replay_status,
-                            attn_mma_status, attn_bwd_mma_status, attn_narrow_status}) {
+                            attn_mma_status, attn_bwd_mma_status, attn_narrow_status, paged_attn_status}) {
         const int one = status();
         all = one < 0 || all < 0 ? -1 : all | one;
     }

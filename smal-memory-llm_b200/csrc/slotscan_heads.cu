@@ -1,4 +1,4 @@
-// Norms of queries and keys per head with the position rotation in the same pass, forward, backward and into ring caches.
+// Norms of queries and keys per head with the position rotation in the same pass, forward, backward, into ring caches and into pages.
 //
 // Per row x of D channels:  r = (mean x^2 + eps)^(-1/2),  y = x r w,  and the pairs (i, i + R/2) turned by the position's angle.
 // Backward, with g the upstream gradient turned back by the same angle:  dw += g x r,  h = g w,
@@ -41,8 +41,13 @@ struct NormArgs {
     const int32_t* pos;
     const float *qw, *kw;
 };
-struct AppendArgs {                                      // L 0: no caches
-    int L;
+// Where keys and values go: rows of their own, ring caches (row = position mod L), or slots in the pages of a pool
+enum Dest { OUT, RING, PAGES };
+struct AppendArgs {
+    int L;                                               // of a ring
+    int shift;                                           // of pages: log2 of their tokens
+    long long slots;                                     // of pages: how many there are
+    const int32_t* slot;                                 // of pages: of each token
     long long vs[3], kcs[3], vcs[3];
 };
 
@@ -132,10 +137,11 @@ __device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[4], const 
     }
 }
 
-// T: bf16 or float.  CACHE: the keys and the values go into the caches.
-template <typename T, int LPG, bool CACHE>
-__global__ void __launch_bounds__(NR_THREADS, CACHE ? 3 : NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
+// T: bf16 or float
+template <typename T, int LPG, Dest DEST>
+__global__ void __launch_bounds__(NR_THREADS, DEST != OUT ? 3 : NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
+    constexpr bool CACHE = DEST != OUT;
     constexpr int SLOTS = NR_FWD_SLOTS<T>;
     __shared__ uint4 ring[Ahead<T, LPG, 1, SLOTS>::BYTES / 16];
     Ahead<T, LPG, 1, SLOTS> rows(ring);
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(NR_THREADS, CACHE ? 3 : NR_FWD_CTAS) norm_rope
     const int h0 = (int)(unit % a.slices) * a.per_slice, all = a.H + a.KV + (CACHE ? a.KV : 0);
     const bool token = tok < a.tokens, live = token && c * 8 < a.D;                // a lane without channels still fetches for the others
     const unsigned b = token ? tok / a.T : 0, t = token ? tok % a.T : 0;
-    const long long at = CACHE ? (long long)a.pos[b] + t : a.pos != nullptr ? (long long)a.pos[token ? tok : 0] : t;
+    const long long at = DEST == RING ? (long long)a.pos[b] + t : a.pos != nullptr ? (long long)a.pos[token ? tok : 0] : t;
     const T* qt = q + b * a.qs[0] + t * a.qs[1];         // of the token
     const T* kt = k + b * a.ks[0] + t * a.ks[1];
     const T* vt = CACHE ? v + b * ap.vs[0] + t * ap.vs[1] : nullptr;
@@ -163,9 +169,17 @@ __global__ void __launch_bounds__(NR_THREADS, CACHE ? 3 : NR_FWD_CTAS) norm_rope
     const bool rot = c * 8 < a.R;
     float cs[4], sn[4], w[8];
     load_turn(a, at, c, cs, sn);
-    const long long row = CACHE && at >= 0 ? (unsigned)at % (unsigned)ap.L : 0;
-    T* kot = CACHE ? kc + b * ap.kcs[0] + row * ap.kcs[1] : ko + (size_t)tok * a.KV * a.D;
-    T* vot = CACHE ? vc + b * ap.vcs[0] + row * ap.vcs[1] : nullptr;
+    long long outer = b, row = 0;                        // sequence and row of a ring, page and row within it
+    bool stored = at >= 0;
+    if constexpr (DEST == RING) row = stored ? (unsigned)at % (unsigned)ap.L : 0;
+    if constexpr (DEST == PAGES) {
+        const long long slot = token ? ap.slot[tok] : -1;
+        stored = stored && slot >= 0 && slot < ap.slots;
+        outer = stored ? slot >> ap.shift : 0;
+        row = stored ? slot & ((1 << ap.shift) - 1) : 0;
+    }
+    T* kot = CACHE ? kc + outer * ap.kcs[0] + row * ap.kcs[1] : ko + (size_t)tok * a.KV * a.D;
+    T* vot = CACHE ? vc + outer * ap.vcs[0] + row * ap.vcs[1] : nullptr;
     const long long kos = CACHE ? ap.kcs[2] : a.D;
     const float inv_d = 1.f / a.D;
     for (int u = 0; u < a.per_slice; u++) {
@@ -189,8 +203,12 @@ __global__ void __launch_bounds__(NR_THREADS, CACHE ? 3 : NR_FWD_CTAS) norm_rope
         for (int i = 0; i < 8; i++) y[i] = x[i] * r * w[i];
         if (rot) turn<1>(y, cs, sn);
         if (!live || h >= all) continue;
+        if (DEST == PAGES && at < 0) {                   // a row of no token
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = 0.f;
+        }
         if (is_q) st_pieces(qot + h * a.D, y, pc);
-        else if (!CACHE || at >= 0) {
+        else if (!CACHE || stored) {
             if (!is_v) st_pieces(kot + (h - a.H) * kos, y, pc);
             else st_pieces(vot + (h - a.H - a.KV) * ap.vcs[2], x, pc);
         }
@@ -329,15 +347,15 @@ static int bwd_ctas(const NormArgs& a) {
     return (int)(want < NR_MAX_CTAS ? want : NR_MAX_CTAS);
 }
 
-template <typename T, bool CACHE>
+template <typename T, Dest DEST>
 static cudaError_t launch_norm(const NormArgs& a, const AppendArgs& ap, const void* q, const void* k, const void* v, void* qo, void* ko, void* kc,
                                void* vc, cudaStream_t st) {
     const int groups = NR_THREADS / lanes_of(a.D);
     const unsigned grid = (unsigned)((a.tokens * a.slices + groups - 1) / groups);
     auto go = [&](auto kern) { kern<<<grid, NR_THREADS, 0, st>>>(a, ap, (const T*)q, (const T*)k, (const T*)v, (T*)qo, (T*)ko, (T*)kc, (T*)vc); };
-    if (lanes_of(a.D) == 8) go(norm_rope_kernel<T, 8, CACHE>);
-    else if (lanes_of(a.D) == 16) go(norm_rope_kernel<T, 16, CACHE>);
-    else go(norm_rope_kernel<T, 32, CACHE>);
+    if (lanes_of(a.D) == 8) go(norm_rope_kernel<T, 8, DEST>);
+    else if (lanes_of(a.D) == 16) go(norm_rope_kernel<T, 16, DEST>);
+    else go(norm_rope_kernel<T, 32, DEST>);
     return cudaGetLastError();
 }
 template <typename T>
@@ -385,8 +403,8 @@ extern "C" int slotscan_norm_rope_fwd(const slotscan_norm_params* p, const void*
     if (!aligned16(q) || !aligned16(k) || !aligned16(qo) || !aligned16(ko) || !aligned16(table) || !aligned16(qw) || !aligned16(kw)) return SLOTSCAN_E_ALIGN;
     const NormArgs a = norm_args(*p, table, pos, qw, kw, p->H + p->KV);
     const AppendArgs none = {};
-    return (int)(p->dtype == SLOTSCAN_BF16 ? launch_norm<bf16, false>(a, none, q, k, nullptr, qo, ko, nullptr, nullptr, (cudaStream_t)stream)
-                                           : launch_norm<float, false>(a, none, q, k, nullptr, qo, ko, nullptr, nullptr, (cudaStream_t)stream));
+    return (int)(p->dtype == SLOTSCAN_BF16 ? launch_norm<bf16, OUT>(a, none, q, k, nullptr, qo, ko, nullptr, nullptr, (cudaStream_t)stream)
+                                           : launch_norm<float, OUT>(a, none, q, k, nullptr, qo, ko, nullptr, nullptr, (cudaStream_t)stream));
 }
 
 extern "C" size_t slotscan_norm_rope_bwd_scratch_bytes(const slotscan_norm_params* p) {
@@ -433,9 +451,32 @@ extern "C" int slotscan_norm_rope_append(const slotscan_append_params* p, const 
         !aligned16(kw))
         return SLOTSCAN_E_ALIGN;
     const NormArgs a = norm_args(n, table, pos, qw, kw, n.H + 2 * n.KV);
-    AppendArgs ap;
+    AppendArgs ap = {};
     ap.L = p->L;
     for (int i = 0; i < 3; i++) { ap.vs[i] = p->v_stride[i]; ap.kcs[i] = p->kc_stride[i]; ap.vcs[i] = p->vc_stride[i]; }
-    return (int)(n.dtype == SLOTSCAN_BF16 ? launch_norm<bf16, true>(a, ap, q, k, v, qo, nullptr, kc, vc, (cudaStream_t)stream)
-                                          : launch_norm<float, true>(a, ap, q, k, v, qo, nullptr, kc, vc, (cudaStream_t)stream));
+    return (int)(n.dtype == SLOTSCAN_BF16 ? launch_norm<bf16, RING>(a, ap, q, k, v, qo, nullptr, kc, vc, (cudaStream_t)stream)
+                                          : launch_norm<float, RING>(a, ap, q, k, v, qo, nullptr, kc, vc, (cudaStream_t)stream));
+}
+
+extern "C" int slotscan_norm_rope_pages(const slotscan_page_append_params* p, const void* q, const void* k, const void* v, const float* table,
+                                        const int32_t* slots, const int32_t* pos, const float* qw, const float* kw, void* qo, void* kp, void* vp,
+                                        void* stream) {
+    const int rc = slotscan_norm_rope_check(p == nullptr ? nullptr : &p->base);
+    if (rc != SLOTSCAN_OK) return rc;
+    const slotscan_norm_params& n = p->base;
+    if (n.B != 1 || p->pages < 1 || p->page < 8 || p->page > 1024 || (p->page & (p->page - 1))) return SLOTSCAN_E_SHAPE;
+    if (!strides16(p->v_stride, 3, n.dtype) || !strides16(p->kp_stride, 3, n.dtype) || !strides16(p->vp_stride, 3, n.dtype)) return SLOTSCAN_E_ALIGN;
+    if (n.T == 0) return SLOTSCAN_OK;
+    if (!q || !k || !v || !slots || !pos || !qo || !kp || !vp || (n.R && !table)) return SLOTSCAN_E_NULL;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(qo) || !aligned16(kp) || !aligned16(vp) || !aligned16(table) || !aligned16(qw) ||
+        !aligned16(kw))
+        return SLOTSCAN_E_ALIGN;
+    const NormArgs a = norm_args(n, table, pos, qw, kw, n.H + 2 * n.KV);
+    AppendArgs ap = {};
+    while ((1 << ap.shift) < p->page) ap.shift++;
+    ap.slots = (long long)p->pages << ap.shift;
+    ap.slot = slots;
+    for (int i = 0; i < 3; i++) { ap.vs[i] = p->v_stride[i]; ap.kcs[i] = p->kp_stride[i]; ap.vcs[i] = p->vp_stride[i]; }
+    return (int)(n.dtype == SLOTSCAN_BF16 ? launch_norm<bf16, PAGES>(a, ap, q, k, v, qo, nullptr, kp, vp, (cudaStream_t)stream)
+                                          : launch_norm<float, PAGES>(a, ap, q, k, v, qo, nullptr, kp, vp, (cudaStream_t)stream));
 }

@@ -85,6 +85,7 @@ int read_mma_status();
 int attn_mma_status();
 int attn_bwd_mma_status();
 int attn_narrow_status();
+int paged_attn_status();
 int gather_status_f32();
 int gather_status_bf16();
 int rows_bwd_status_f32();

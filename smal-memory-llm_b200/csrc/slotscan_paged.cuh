@@ -1,0 +1,94 @@
+// Attention over pages of a pool: what its kernels share.
+#pragma once
+#include <cfloat>
+
+#include "slotscan_attn.cuh"
+
+namespace slotscan {
+
+struct PagedArgs {
+    int N, B, H, KV, D;
+    int pages, shift, M;                                 // pages of the pool, log2 of a page's tokens, pages of a request at most
+    int window;                                          // 0: none
+    int chunks;                                          // of the query heads of a key head
+    float scale, cap;
+    long long qs[2], ks[3], vs[3], table_stride;
+    const int32_t *tables, *starts, *pos, *start;
+    const float* slopes;
+};
+
+// keys that a query at position `at` of request b sees, [lo, hi); empty where hi <= lo.  What its table does not reach is not seen.
+__device__ __forceinline__ Span paged_keys(const PagedArgs& a, int b, int at) {
+    const int first = a.start != nullptr ? max(a.start[b], 0) : 0;
+    const int hi = at < 0 ? 0 : min(at, (a.M << a.shift) - 1) + 1;
+    return {a.window > 0 && at >= a.window ? max(first, at - a.window + 1) : first, hi};
+}
+// id of the page of key j; minus one where it is not of the pool
+__device__ __forceinline__ int page_of(const PagedArgs& a, int b, int j) {
+    const int id = a.tables[b * a.table_stride + (j >> a.shift)];
+    return id < a.pages ? id : -1;
+}
+
+__device__ __forceinline__ Score paged_score(const PagedArgs& a, int h) {
+    AttnArgs s;
+    s.scale = a.scale; s.cap = a.cap; s.slopes = a.slopes;
+    return Score(s, min(h, a.H - 1));
+}
+// packed rows of request b
+__device__ __forceinline__ int rows_begin(const PagedArgs& a, int b) { return min(max(a.starts[b], 0), a.N); }
+__device__ __forceinline__ int rows_end(const PagedArgs& a, int b) { return max(min(a.starts[b + 1], a.N), rows_begin(a, b)); }
+// Rows of a tile: `heads` query heads (of the `chunks`-th part of a group) of `tokens` tokens, the heads of a token side by side
+struct RowShape { int heads, tokens; };                  // of a tile, or of a half of it
+
+// ---- a row at a time, by a warp, over the keys that it sees within [lo, hi): where hidden values have made a result not finite ----
+template <typename T>
+__device__ __forceinline__ void careful_row(const PagedArgs& a, const Score& sc, const T* q, const T* kp, const T* vp, int b, int hk, int at, int lo, int hi,
+                                            float (&o)[4], float& m, float& l) {
+    float x[4], y[4], unused;
+    lane_row(x, q, a.D);
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] = 0.f;
+    for (int j = lo; j < hi; j++) {
+        const int id = page_of(a, b, j), row = j & ((1 << a.shift) - 1);
+#pragma unroll
+        for (int c = 0; c < 4; c++) y[c] = 0.f;
+        if (id >= 0) lane_row(y, kp + id * a.ks[0] + row * a.ks[1] + hk * a.ks[2], a.D);
+        const float z = score2(sc, lane_dot(x, y), at - j, unused);
+        const float top = fmaxf(m, z), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), p = exp2f(z - base);
+        if (id >= 0) lane_row(y, vp + id * a.vs[0] + row * a.vs[1] + hk * a.vs[2], a.D);
+        l = fmaf(l, f, p);
+        bool gone = true;                                // NaN stays NaN
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            o[c] = p != 0.f ? fmaf(p, y[c], o[c] * f) : o[c] * f;
+            gone = gone && (isnan(o[c]) || (threadIdx.x & 31) + 32 * c >= a.D);
+        }
+        m = top;
+        if (__all_sync(FULL, gone)) break;
+    }
+}
+
+static inline PagedArgs paged_args(const slotscan_paged_params& p, const int32_t* tables, const int32_t* starts, const int32_t* pos, const int32_t* start,
+                                   const float* slopes) {
+    PagedArgs a;
+    a.N = p.N; a.B = p.B; a.H = p.H; a.KV = p.KV; a.D = p.D; a.pages = p.pages; a.M = p.M;
+    a.window = p.window; a.chunks = 1;
+    a.shift = 0;
+    while ((1 << a.shift) < p.page) a.shift++;
+    a.scale = p.scale; a.cap = p.cap;
+    for (int i = 0; i < 2; i++) a.qs[i] = p.q_stride[i];
+    for (int i = 0; i < 3; i++) { a.ks[i] = p.k_stride[i]; a.vs[i] = p.v_stride[i]; }
+    a.table_stride = p.table_stride;
+    a.tables = tables; a.starts = starts; a.pos = pos; a.start = start; a.slopes = slopes;
+    return a;
+}
+
+// attention of packed rows, by type
+size_t paged_attn_scratch_bf16(const PagedArgs& a);
+size_t paged_attn_scratch_f32(const PagedArgs& a);
+cudaError_t run_paged_attn_bf16(const PagedArgs& a, const void* q, const void* k, const void* v, void* o, void* scratch, cudaStream_t st);
+cudaError_t run_paged_attn_f32(const PagedArgs& a, const void* q, const void* k, const void* v, void* o, void* scratch, cudaStream_t st);
+
+}  // namespace slotscan

@@ -1,0 +1,236 @@
+// Pages of a pool handed to requests and taken back, and the slots of a packed batch of new tokens, on the GPU: a scheduler's turn without
+// a copy to the host.
+//
+// With n the new tokens of a request, len what it holds and P the tokens of a page
+//     ends = inclusive sum of n,   need = ceil((len + n) / P) - ceil(len / P),   upto = inclusive sum of need
+// a request is served if its table and the batch have room and need = 0 or upto <= free pages; page j of it, the (upto - need + j - have)-th
+// handed out, is taken from the end of the stack of free ones.  So everything is two sums over the requests, then independent per token.
+//
+// The sums are one CTA's, 1,024 requests at a time; what follows is its own too while it is little (one launch is the floor of a small turn),
+// and a second kernel's beyond.  Nothing is chosen by an order of arrival, so results repeat.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "slotscan.h"
+#include "slotscan_common.cuh"
+
+namespace slotscan {
+
+constexpr int PG_THREADS = 1024;
+constexpr int PG_OWN_ROWS = 8192;                        // rows, or entries of tables, that the CTA of the sums sees to itself
+
+struct PageArgs {
+    int B, M, shift, pages, tokens;
+    long long table_stride;
+    int32_t *lengths, *tables, *free_pages, *n_free;
+};
+// What the sums leave for the rows: per request the tokens held before (minus one: not served) and the rank of its first page; once the
+// free pages before
+struct PagePlan {
+    int32_t *held, *rank, *n_free;
+    __host__ __device__ explicit PagePlan(int32_t* scratch, int B) : held(scratch), rank(scratch + B), n_free(scratch + 2 * (size_t)B) {}
+};
+
+__device__ __forceinline__ long long pages_of(long long n, int shift) { return (n + (1 << shift) - 1) >> shift; }
+
+// inclusive sum over the CTA; `carry` (shared) is what came before, and gets the total added by the last thread
+__device__ __forceinline__ long long cta_sum(long long v, long long* s_warp, long long* carry) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+#pragma unroll
+    for (int off = 1; off < 32; off *= 2) {
+        const long long up = __shfl_up_sync(FULL, v, off);
+        if (lane >= off) v += up;
+    }
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        long long w = s_warp[lane];
+#pragma unroll
+        for (int off = 1; off < 32; off *= 2) {
+            const long long up = __shfl_up_sync(FULL, w, off);
+            if (lane >= off) w += up;
+        }
+        s_warp[lane] = w;
+    }
+    __syncthreads();
+    v += *carry + (warp > 0 ? s_warp[warp - 1] : 0);
+    __syncthreads();
+    if (threadIdx.x == PG_THREADS - 1) *carry = v;
+    __syncthreads();
+    return v;
+}
+__device__ __forceinline__ int free_before(const PageArgs& a) { return min(max(*a.n_free, 0), a.pages); }
+
+// slot and position of packed row i, and the table's entry of a page that begins with it
+__device__ __forceinline__ void place_row(const PageArgs& a, const PagePlan& plan, const int32_t* starts, int32_t* slots, int32_t* pos, int i) {
+    int slot = -1, at = -1;
+    if (i < starts[a.B]) {
+        int lo = 0, hi = a.B - 1;                        // the first request that ends behind i
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (starts[mid + 1] > i) hi = mid; else lo = mid + 1;
+        }
+        const int held = plan.held[lo];
+        if (held >= 0) {
+            at = held + i - starts[lo];
+            const int page = at >> a.shift, have = (int)pages_of(held, a.shift);
+            int32_t* entry = a.tables + lo * a.table_stride + page;
+            const int id = page < have ? *entry : a.free_pages[*plan.n_free - 1 - (plan.rank[lo] + page - have)];
+            const int in_page = at & ((1 << a.shift) - 1);
+            if (in_page == 0) *entry = id;
+            const long long s = ((long long)id << a.shift) + in_page;
+            slot = id >= 0 && s <= BIGI ? (int)s : -1;
+        }
+    }
+    slots[i] = slot;
+    pos[i] = at;
+}
+
+template <bool OWN>
+__global__ void __launch_bounds__(PG_THREADS) extend_kernel(PageArgs a, const int32_t* fresh, int32_t* scratch, int32_t* slots, int32_t* pos, int32_t* starts,
+                                                            int32_t* taken) {
+    __shared__ long long s_warp[32], s_tokens, s_pages;
+    __shared__ int s_handed;
+    const PagePlan plan(scratch, a.B);
+    const int tid = threadIdx.x;
+    if (tid == 0) { s_tokens = s_pages = 0; s_handed = 0; starts[0] = 0; }
+    const int nf = free_before(a);
+    __syncthreads();
+    for (int b0 = 0; b0 < a.B; b0 += PG_THREADS) {
+        const int b = b0 + tid;
+        const bool in = b < a.B;
+        const long long n = in ? max(fresh[b], 0) : 0, held = in ? max(a.lengths[b], 0) : 0;
+        const long long ends = cta_sum(n, s_warp, &s_tokens);
+        const bool fits = in && held + n <= ((long long)a.M << a.shift) && ends <= a.tokens;
+        const long long need = fits ? pages_of(held + n, a.shift) - pages_of(held, a.shift) : 0;
+        const long long upto = cta_sum(need, s_warp, &s_pages);
+        const bool served = fits && (need == 0 || upto <= nf);
+        if (in) {
+            starts[b + 1] = (int)min(ends, (long long)a.tokens);
+            taken[b] = served ? (int)n : 0;
+            plan.held[b] = served ? (int)held : -1;
+            plan.rank[b] = (int)min(upto - need, (long long)BIGI);
+            if (served && n > 0) a.lengths[b] = (int)(held + n);
+            if (served && need > 0) atomicMax(&s_handed, (int)upto);
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        *plan.n_free = nf;
+        *a.n_free = nf - s_handed;
+    }
+    if constexpr (OWN) {
+        __syncthreads();
+        for (int i = tid; i < a.tokens; i += PG_THREADS) place_row(a, plan, starts, slots, pos, i);
+    }
+}
+__global__ void __launch_bounds__(256) place_kernel(PageArgs a, int32_t* scratch, const int32_t* starts, int32_t* slots, int32_t* pos) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < a.tokens) place_row(a, PagePlan(scratch, a.B), starts, slots, pos, i);
+}
+
+// a request's pages onto the stack, in their order, and its table emptied; `held`: its pages, minus one where it stays
+__device__ __forceinline__ void give_back(const PageArgs& a, const PagePlan& plan, int b, int tid, int threads) {
+    const int n = plan.held[b];
+    if (n < 0) return;
+    int32_t* row = a.tables + b * a.table_stride;
+    const long long to = (long long)*plan.n_free + plan.rank[b];
+    for (int j = tid; j < a.M; j += threads) {
+        if (j < n && to + j < a.pages) a.free_pages[to + j] = row[j];
+        row[j] = -1;
+    }
+}
+
+template <bool OWN>
+__global__ void __launch_bounds__(PG_THREADS) release_kernel(PageArgs a, const uint8_t* done, int32_t* scratch) {
+    __shared__ long long s_warp[32], s_pages;
+    const PagePlan plan(scratch, a.B);
+    const int tid = threadIdx.x;
+    if (tid == 0) s_pages = 0;
+    const int nf = free_before(a);
+    __syncthreads();
+    for (int b0 = 0; b0 < a.B; b0 += PG_THREADS) {
+        const int b = b0 + tid;
+        const bool ends = b < a.B && done[b] != 0;
+        const long long n = ends ? min(pages_of(max(a.lengths[b], 0), a.shift), (long long)a.M) : 0;
+        const long long upto = cta_sum(n, s_warp, &s_pages);
+        if (b < a.B) {
+            plan.held[b] = ends ? (int)n : -1;
+            plan.rank[b] = (int)min(upto - n, (long long)BIGI);
+            if (ends) a.lengths[b] = 0;
+        }
+    }
+    if (tid == 0) {
+        *plan.n_free = nf;
+        *a.n_free = (int)min(nf + s_pages, (long long)a.pages);
+    }
+    if constexpr (OWN) {
+        __syncthreads();
+        for (int b = tid / 32; b < a.B; b += PG_THREADS / 32) give_back(a, plan, b, tid & 31, 32);
+    }
+}
+__global__ void __launch_bounds__(256) give_back_kernel(PageArgs a, int32_t* scratch) {
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) give_back(a, PagePlan(scratch, a.B), b, threadIdx.x, 256);
+}
+
+static PageArgs page_args(const slotscan_pages_params& p, int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* n_free) {
+    PageArgs a;
+    a.B = p.B; a.M = p.M; a.pages = p.pages; a.tokens = p.tokens;
+    a.shift = 0;
+    while ((1 << a.shift) < p.page) a.shift++;
+    a.table_stride = p.table_stride;
+    a.lengths = lengths; a.tables = tables; a.free_pages = free_pages; a.n_free = n_free;
+    return a;
+}
+
+}  // namespace slotscan
+
+using namespace slotscan;
+
+extern "C" int slotscan_pages_check(const slotscan_pages_params* p) {
+    if (p == nullptr) return SLOTSCAN_E_NULL;
+    if (p->B < 0 || p->B > (1 << 24) || p->M < 1 || p->M > (1 << 26) || p->pages < 1 || p->tokens < 0 || p->tokens > (1 << 30) || p->page < 8 ||
+        p->page > 1024 || (p->page & (p->page - 1)) || (int64_t)p->M * p->page > (1 << 29) || p->table_stride < p->M)
+        return SLOTSCAN_E_SHAPE;
+    return SLOTSCAN_OK;
+}
+
+extern "C" size_t slotscan_pages_scratch_bytes(const slotscan_pages_params* p) {
+    return slotscan_pages_check(p) == SLOTSCAN_OK ? sizeof(int32_t) * (2 * (size_t)p->B + 1) : 0;
+}
+
+extern "C" int slotscan_extend_pages(const slotscan_pages_params* p, const int32_t* fresh, int32_t* lengths, int32_t* tables, int32_t* free_pages,
+                                     int32_t* n_free, int32_t* slots, int32_t* pos, int32_t* starts, int32_t* taken, void* scratch,
+                                     size_t scratch_bytes, void* stream) {
+    const int rc = slotscan_pages_check(p);
+    if (rc != SLOTSCAN_OK) return rc;
+    if (!starts || !n_free || !free_pages || (p->B && (!fresh || !lengths || !tables || !taken)) || (p->tokens && (!slots || !pos))) return SLOTSCAN_E_NULL;
+    if (scratch == nullptr || scratch_bytes < slotscan_pages_scratch_bytes(p)) return SLOTSCAN_E_NULL;
+    const PageArgs a = page_args(*p, lengths, tables, free_pages, n_free);
+    cudaStream_t st = (cudaStream_t)stream;
+    int32_t* s = (int32_t*)scratch;
+    if (a.tokens <= PG_OWN_ROWS) extend_kernel<true><<<1, PG_THREADS, 0, st>>>(a, fresh, s, slots, pos, starts, taken);
+    else {
+        extend_kernel<false><<<1, PG_THREADS, 0, st>>>(a, fresh, s, slots, pos, starts, taken);
+        place_kernel<<<(a.tokens + 255) / 256, 256, 0, st>>>(a, s, starts, slots, pos);
+    }
+    return (int)cudaGetLastError();
+}
+
+extern "C" int slotscan_release_pages(const slotscan_pages_params* p, const uint8_t* done, int32_t* lengths, int32_t* tables, int32_t* free_pages,
+                                      int32_t* n_free, void* scratch, size_t scratch_bytes, void* stream) {
+    const int rc = slotscan_pages_check(p);
+    if (rc != SLOTSCAN_OK) return rc;
+    if (p->B == 0) return SLOTSCAN_OK;
+    if (!done || !lengths || !tables || !free_pages || !n_free) return SLOTSCAN_E_NULL;
+    if (scratch == nullptr || scratch_bytes < slotscan_pages_scratch_bytes(p)) return SLOTSCAN_E_NULL;
+    const PageArgs a = page_args(*p, lengths, tables, free_pages, n_free);
+    cudaStream_t st = (cudaStream_t)stream;
+    int32_t* s = (int32_t*)scratch;
+    if ((int64_t)a.B * a.M <= PG_OWN_ROWS) release_kernel<true><<<1, PG_THREADS, 0, st>>>(a, done, s);
+    else {
+        release_kernel<false><<<1, PG_THREADS, 0, st>>>(a, done, s);
+        give_back_kernel<<<(unsigned)(a.B < 148 * 8 ? a.B : 148 * 8), 256, 0, st>>>(a, s);
+    }
+    return (int)cudaGetLastError();
+}

@@ -107,6 +107,12 @@ __device__ __forceinline__ void tile_s2g(const CUtensorMap* map, int col, int ro
                  "r"(row), "r"(head), "r"(seq), "r"(smem_u32(src))
                  : "memory");
 }
+// of a (row, head, channel) tensor
+__device__ __forceinline__ void box_g2s(void* dst, const CUtensorMap* map, int col, int head, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(head), "r"(row), "r"(smem_u32(bar))
+                 : "memory");
+}
 // byte offset of the 16-byte piece `piece` (of 8) of row `row` in a sub-tile
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 
@@ -133,19 +139,34 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // strides in elements, of a sequence, a token and a head (any value where that dimension has one element).
 typedef CUresult (*TileMapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                     const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static inline bool tile_map(CUtensorMap* m, const void* base, int B, int T, int H, int D, const long long* stride, int rows) {
+static inline TileMapEncodeFn tile_map_encoder() {
     static TileMapEncodeFn enc = [] {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
         return (TileMapEncodeFn)f;
     }();
+    return enc;
+}
+static inline bool tile_map(CUtensorMap* m, const void* base, int B, int T, int H, int D, const long long* stride, int rows) {
+    const TileMapEncodeFn enc = tile_map_encoder();
     if (enc == nullptr) return false;
     auto bytes = [&](long long s, int n) { return (cuuint64_t)(n == 1 ? 2ll * D : 2ll * s); };
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
     const cuuint64_t strides[3] = {bytes(stride[1], T), bytes(stride[2], H), bytes(stride[0], B)};
     const cuuint32_t box[4] = {64u, (cuuint32_t)rows, 1u, 1u}, es[4] = {1u, 1u, 1u, 1u};
     return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// (row, head, channel) bf16 tensor, boxes of 64 channels x `heads` heads x `rows` rows, the heads of a row side by side; strides of a row and
+// a head
+static inline bool box_map(CUtensorMap* m, const void* base, int N, int H, int D, const long long* stride, int heads, int rows) {
+    const TileMapEncodeFn enc = tile_map_encoder();
+    if (enc == nullptr) return false;
+    auto bytes = [&](long long s, int n) { return (cuuint64_t)(n == 1 ? 2ll * D : 2ll * s); };
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)N}, strides[2] = {bytes(stride[1], H), bytes(stride[0], N)};
+    const cuuint32_t box[3] = {64u, (cuuint32_t)heads, (cuuint32_t)rows}, es[3] = {1u, 1u, 1u};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -316,6 +316,132 @@ py::object token_attention_step(const Tensor& q, const Tensor& kc, const Tensor&
     return py::cast(o);
 }
 
+// ---- pages ----
+// rows of integers side by side, in place
+bool table_laid(const Tensor& t, const Tensor& like, int64_t B) {
+    return t.dim() == 2 && t.scalar_type() == at::kInt && t.device() == like.device() && t.size(0) == B && t.size(1) > 0 && t.size(1) <= 0x7fffffff &&
+           (t.size(1) == 1 || t.stride(1) == 1) && (B <= 1 || t.stride(0) >= t.size(1));
+}
+int64_t table_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+bool ints(const Tensor& t, int64_t n, const Tensor& like) { return t.dim() == 1 && t.size(0) == n && fits(Maybe(t), at::kInt, {n}, like); }
+
+bool pages_params(slotscan_pages_params& p, const Tensor& lengths, const Tensor& tables, const Tensor& free_pages, const Tensor& n_free, int64_t page, int64_t tokens) {
+    if (!lengths.is_cuda() || lengths.dim() != 1 || free_pages.dim() != 1) return false;
+    const int64_t B = lengths.size(0);
+    if (!ints(lengths, B, lengths) || !ints(free_pages, free_pages.size(0), lengths) || !ints(n_free, 1, lengths) || !table_laid(tables, lengths, B)) return false;
+    if (std::max({B, free_pages.size(0), page, tokens}) > 0x7fffffff || page < 0 || tokens < 0) return false;
+    const Maybe ts[] = {lengths, tables, free_pages, n_free};
+    if (wants_grad({&ts[0], &ts[1], &ts[2], &ts[3]})) return false;
+    p.B = (int32_t)B; p.M = (int32_t)tables.size(1); p.page = (int32_t)page; p.pages = (int32_t)free_pages.size(0); p.tokens = (int32_t)tokens;
+    p.table_stride = table_stride(tables);
+    return slotscan_pages_check(&p) == SLOTSCAN_OK;
+}
+
+py::object extend_pages(const Tensor& any_new, const Tensor& lengths, const Tensor& tables, const Tensor& free_pages, const Tensor& n_free, int64_t page,
+                        int64_t tokens) {
+    slotscan_pages_params p;
+    const Tensor fresh = in_32_bits(any_new);
+    if (!pages_params(p, lengths, tables, free_pages, n_free, page, tokens) || !ints(fresh, p.B, lengths)) return py::none();
+    const c10::cuda::CUDAGuard here(lengths.device());
+    const size_t bytes = slotscan_pages_scratch_bytes(&p);
+    Tensor slots = at::empty({tokens}, lengths.options()), pos = at::empty({tokens}, lengths.options());
+    Tensor starts = at::empty({p.B + 1}, lengths.options()), taken = at::empty({p.B}, lengths.options());
+    Tensor scratch = at::empty({(int64_t)(bytes / sizeof(int32_t))}, lengths.options());
+    check(slotscan_extend_pages(&p, (const int32_t*)in(fresh), (int32_t*)out(lengths), (int32_t*)out(tables), (int32_t*)out(free_pages), (int32_t*)out(n_free),
+                                (int32_t*)out(slots), (int32_t*)out(pos), (int32_t*)out(starts), (int32_t*)out(taken), out(scratch), bytes, stream_of(lengths)),
+          "slotscan_extend_pages");
+    for (const Tensor& t : {lengths, tables, free_pages, n_free}) changed(t);
+    return py::cast(std::make_tuple(slots, pos, starts, taken));
+}
+
+bool release_pages(const Tensor& done, const Tensor& lengths, const Tensor& tables, const Tensor& free_pages, const Tensor& n_free, int64_t page) {
+    slotscan_pages_params p;
+    if (!pages_params(p, lengths, tables, free_pages, n_free, page, 0) || done.dim() != 1 || done.size(0) != p.B || done.device() != lengths.device() ||
+        (done.scalar_type() != at::kBool && done.scalar_type() != at::kByte) || !done.is_contiguous())
+        return false;
+    const c10::cuda::CUDAGuard here(lengths.device());
+    const size_t bytes = slotscan_pages_scratch_bytes(&p);
+    Tensor scratch = at::empty({(int64_t)(bytes / sizeof(int32_t))}, lengths.options());
+    check(slotscan_release_pages(&p, (const uint8_t*)in(done), (int32_t*)out(lengths), (int32_t*)out(tables), (int32_t*)out(free_pages), (int32_t*)out(n_free),
+                                 out(scratch), bytes, stream_of(lengths)),
+          "slotscan_release_pages");
+    for (const Tensor& t : {lengths, tables, free_pages, n_free}) changed(t);
+    return true;
+}
+
+py::object norm_rope_pages(const Tensor& q3, const Tensor& k3, const Tensor& v3, const Tensor& kp, const Tensor& vp, const Tensor& any_slots, const Tensor& any_pos,
+                           const Maybe& table, const Maybe& qw, const Maybe& kw, double eps) {
+    if (q3.dim() != 3 || k3.dim() != 3 || v3.dim() != 3) return py::none();
+    slotscan_page_append_params p;
+    const Tensor q = q3.unsqueeze(0), k = k3.unsqueeze(0), v = v3.unsqueeze(0), slots = in_32_bits(any_slots), pos = in_32_bits(any_pos);
+    if (!norm_params(p.base, q, k, table, qw, kw, eps)) return py::none();
+    const int64_t N = q.size(1), D = q.size(3), KV = k.size(2);
+    if (v.sizes() != k.sizes() || code(v) != code(q) || v.device() != q.device() || kp.dim() != 4 || vp.sizes() != kp.sizes() || code(kp) != code(q) ||
+        code(vp) != code(q) || kp.device() != q.device() || vp.device() != q.device() || kp.size(2) != KV || kp.size(3) != D ||
+        std::max(kp.size(0), kp.size(1)) > 0x7fffffff || !ints(slots, N, q) || !ints(pos, N, q))
+        return py::none();
+    const Maybe ts[] = {q3, k3, v3, kp, vp};
+    if (wants_grad({&ts[0], &ts[1], &ts[2], &ts[3], &ts[4], &table, &qw, &kw})) return py::none();
+    if (!laid(v, p.v_stride) || !laid(kp, p.kp_stride) || !laid(vp, p.vp_stride)) return py::none();
+    if ((some(table) && (uintptr_t)table->const_data_ptr() % 16) || (some(qw) && (uintptr_t)qw->const_data_ptr() % 16) ||
+        (some(kw) && (uintptr_t)kw->const_data_ptr() % 16))
+        return py::none();
+    p.pages = (int32_t)kp.size(0);
+    p.page = (int32_t)kp.size(1);
+    if (p.pages < 1 || p.page < 8 || p.page > 1024 || (p.page & (p.page - 1))) return py::none();
+    const c10::cuda::CUDAGuard here(q.device());
+    Tensor qo = at::empty(q3.sizes(), q3.options());
+    check(slotscan_norm_rope_pages(&p, in(q), in(k), in(v), ptr<float>(table), (const int32_t*)in(slots), (const int32_t*)in(pos), ptr<float>(qw), ptr<float>(kw),
+                                   out(qo), out(kp), out(vp), stream_of(q)),
+          "slotscan_norm_rope_pages");
+    changed(kp);
+    changed(vp);
+    return py::cast(qo);
+}
+
+// q: (N, 1, H, D), a row for each request (starts absent), or (N, H, D)
+py::object paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& any_tables, const Maybe& any_starts, const Tensor& any_pos,
+                           const Maybe& slopes, const Maybe& any_start, int64_t window, double cap, double scale) {
+    const bool step = !some(any_starts);
+    const Tensor tables = in_32_bits(any_tables), pos = in_32_bits(any_pos);
+    const Maybe starts = in_32_bits(any_starts), start = in_32_bits(any_start);
+    if (q.dim() != (step ? 4 : 3) || (step && q.size(1) != 1) || kp.dim() != 4 || vp.sizes() != kp.sizes() || code(q) < 0 || code(kp) != code(q) ||
+        code(vp) != code(q) || !q.is_cuda() || kp.device() != q.device() || vp.device() != q.device())
+        return py::none();
+    const int64_t N = q.size(0), H = q.size(-2), D = q.size(-1), KV = kp.size(2), B = step ? N : starts->numel() - 1;
+    if (kp.size(3) != D || KV == 0 || H % KV || std::max({N, H, D, kp.size(0), kp.size(1), window}) > 0x7fffffff || B < 0) return py::none();
+    if (!table_laid(tables, q, B) || !ints(pos, N, q) || !fits(starts, at::kInt, {B + 1}, q) || !fits(start, at::kInt, {B}, q) || !fits(slopes, at::kFloat, {H}, q))
+        return py::none();
+    const Maybe ts[] = {q, kp, vp, tables, pos};
+    if (wants_grad({&ts[0], &ts[1], &ts[2], &ts[3], &ts[4], &slopes, &start})) return py::none();
+    slotscan_paged_params p;
+    int64_t qs[3];
+    if (!laid(q, qs) || !laid(kp, p.k_stride) || !laid(vp, p.v_stride)) return py::none();
+    p.N = (int32_t)N; p.B = (int32_t)B; p.H = (int32_t)H; p.KV = (int32_t)KV; p.D = (int32_t)D;
+    p.pages = (int32_t)kp.size(0); p.page = (int32_t)kp.size(1); p.M = (int32_t)tables.size(1);
+    p.window = (int32_t)window;
+    p.dtype = code(q);
+    p.scale = (float)scale;
+    p.cap = (float)cap;
+    p.q_stride[0] = qs[0];
+    p.q_stride[1] = qs[step ? 2 : 1];
+    p.table_stride = table_stride(tables);
+    if (slotscan_paged_check(&p) != SLOTSCAN_OK) return py::none();
+    const c10::cuda::CUDAGuard here(q.device());
+    Tensor o = at::empty(q.sizes(), q.options()), scratch;
+    const size_t bytes = step ? slotscan_paged_step_scratch_bytes(&p) : slotscan_paged_attn_scratch_bytes(&p);
+    if (bytes) scratch = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    if (step)
+        check(slotscan_paged_step(&p, in(q), in(kp), in(vp), (const int32_t*)in(tables), (const int32_t*)in(pos), ptr<int32_t>(start), ptr<float>(slopes), out(o),
+                                  out(scratch), bytes, stream_of(q)),
+              "slotscan_paged_step");
+    else
+        check(slotscan_paged_attn(&p, in(q), in(kp), in(vp), (const int32_t*)in(tables), ptr<int32_t>(starts), (const int32_t*)in(pos), ptr<int32_t>(start),
+                                  ptr<float>(slopes), out(o), out(scratch), bytes, stream_of(q)),
+              "slotscan_paged_attn");
+    return py::cast(o);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tokens_host, m) {
@@ -323,4 +449,8 @@ PYBIND11_MODULE(_tokens_host, m) {
     m.def("norm_rope_append", &norm_rope_append);
     m.def("token_attention", &token_attention);
     m.def("token_attention_step", &token_attention_step);
+    m.def("extend_pages", &extend_pages);
+    m.def("release_pages", &release_pages);
+    m.def("norm_rope_pages", &norm_rope_pages);
+    m.def("paged_attention", &paged_attention);
 }

@@ -7,3 +7,4 @@ from .epilogue import E4M3, fq, quantize_mem, writer_epilogue  # noqa: F401
 from .read import read_snapshots  # noqa: F401
 from .keyless import slot_scan_v  # noqa: F401
 from .tokens import document_bounds, norm_rope, norm_rope_append, rope_table, token_attention, token_attention_step  # noqa: F401
+from .pages import extend_pages, norm_rope_pages, page_tables, paged_attention, paged_attention_step, release_pages  # noqa: F401

@@ -86,6 +86,24 @@ class AttnStepParams(ctypes.Structure):
                [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_stride", ctypes.c_int64 * 2), ("k_stride", _Strides), ("v_stride", _Strides)]
 
 
+class PagesParams(ctypes.Structure):
+    """slotscan_pages_params of include/slotscan.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "M", "page", "pages", "tokens")] + [("table_stride", ctypes.c_int64)]
+
+
+class PageAppendParams(ctypes.Structure):
+    """slotscan_page_append_params of include/slotscan.h."""
+    _fields_ = [("base", NormParams), ("pages", ctypes.c_int32), ("page", ctypes.c_int32), ("v_stride", _Strides), ("kp_stride", _Strides),
+                ("vp_stride", _Strides)]
+
+
+class PagedParams(ctypes.Structure):
+    """slotscan_paged_params of include/slotscan.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("N", "B", "H", "KV", "D", "pages", "page", "M", "window", "dtype")] + \
+               [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("q_stride", ctypes.c_int64 * 2), ("k_stride", _Strides), ("v_stride", _Strides),
+                ("table_stride", ctypes.c_int64)]
+
+
 class KernelAttr(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 48), ("regs", ctypes.c_int32), ("local_bytes", ctypes.c_int32),
                 ("static_smem", ctypes.c_int32), ("max_threads", ctypes.c_int32)]
@@ -156,11 +174,16 @@ def lib():
         L.slotscan_read_bwd.argtypes = [ctypes.POINTER(ReadParams)] + [vp] * 13
         L.slotscan_read_bwd.restype = ci
         NP, TP, SP_ = ctypes.POINTER(NormParams), ctypes.POINTER(AttnParams), ctypes.POINTER(AttnStepParams)
+        GP, QP = ctypes.POINTER(PagesParams), ctypes.POINTER(PagedParams)
         for name, args, res in (
                 ("norm_rope_check", [NP], ci), ("norm_rope_fwd", [NP] + [vp] * 9, ci), ("norm_rope_bwd_scratch_bytes", [NP], sz),
                 ("norm_rope_bwd", [NP] + [vp] * 13 + [sz, vp], ci), ("norm_rope_append", [ctypes.POINTER(AppendParams)] + [vp] * 11, ci),
                 ("attn_check", [TP], ci), ("attn_keeps", [TP, ci], ci), ("attn_fwd", [TP] + [vp] * 10, ci), ("attn_bwd", [TP] + [vp] * 15, ci),
-                ("attn_step_check", [SP_], ci), ("attn_step_scratch_bytes", [SP_], sz), ("attn_step", [SP_] + [vp] * 8 + [sz, vp], ci)):
+                ("attn_step_check", [SP_], ci), ("attn_step_scratch_bytes", [SP_], sz), ("attn_step", [SP_] + [vp] * 8 + [sz, vp], ci),
+                ("pages_check", [GP], ci), ("pages_scratch_bytes", [GP], sz), ("extend_pages", [GP] + [vp] * 10 + [sz, vp], ci),
+                ("release_pages", [GP] + [vp] * 6 + [sz, vp], ci), ("norm_rope_pages", [ctypes.POINTER(PageAppendParams)] + [vp] * 12, ci),
+                ("paged_check", [QP], ci), ("paged_step_scratch_bytes", [QP], sz), ("paged_step", [QP] + [vp] * 9 + [sz, vp], ci),
+                ("paged_attn_scratch_bytes", [QP], sz), ("paged_attn", [QP] + [vp] * 10 + [sz, vp], ci)):
             f = getattr(L, "slotscan_" + name)
             f.argtypes, f.restype = args, res
         L.slotscan_device_status.restype = ci
