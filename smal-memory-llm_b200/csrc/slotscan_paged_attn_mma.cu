@@ -21,28 +21,32 @@ static __device__ int g_paged_status = 0;                // a bounded wait gave 
 constexpr float PA_GROWN = 8.f;                          // in powers of two
 constexpr int PA_HALVES = 2, PA_KEYS = 128, PA_ROWS = PA_HALVES * 128;
 constexpr int PA_THREADS = PA_ROWS + 128;
+constexpr int PA_OUT_ROW = 64 + 16, PA_OUT = 32 * PA_OUT_ROW;             // bytes of a warp's outputs on their way: 64 of a row, and what keeps banks apart
+constexpr int PA_TILE_COST = 2;                          // of a tile of rows itself, in tiles of keys: its queries and its results
 constexpr int PA_STAGES = 4;                             // tiles of the ring, keys and values in turn
 template <int DP>
 struct PagedShape {
     static constexpr int SUBS = DP / 64;                 // 64-column sub-tiles of a tile
     static constexpr int QTILE = 128 * DP * 2, KTILE = PA_KEYS * DP * 2;           // bytes
-    static constexpr int SMEM = PA_HALVES * QTILE + PA_STAGES * KTILE + 1024;
+    static constexpr int SMEM = PA_HALVES * QTILE + PA_STAGES * KTILE + PA_HALVES * 4 * PA_OUT + 1024;
 };
 struct PagedMaps { CUtensorMap q, k, v; };
 
-// What the first CTA leaves for the join: of each tile of rows its place in the line and its request, and the length of a CTA's share
+// What the CTAs leave for the join: each the tile of rows that its end is the first to cut (tokens 0: none), and its parts, at most two: of the
+// tile that its share begins in, and of the one that it ends in
+struct Cut {
+    int b, row0, tokens, at0, first, h0, heads;
+    int begun;                                           // the share that begins the tile begins with it
+    int shares;                                          // CTAs that have a part of it
+};
 struct LinePlan {
-    long long* before;                                   // most + 1
-    long long* per;
-    long long* tiles;
-    int2* tile;                                          // request, tile of its rows
+    Cut* cuts;
     float* parts;
-    long long most;                                      // tiles that the scratch has room for: all, unless starts falls
-    static size_t head_bytes(long long most) { return (sizeof(long long) * (most + 3) + sizeof(int2) * most + 15) / 16 * 16; }
-    LinePlan(void* scratch, long long most_) : before((long long*)scratch), per(before + most_ + 1), tiles(per + 1), tile((int2*)(tiles + 1)),
-                                               parts((float*)((char*)scratch + head_bytes(most_))), most(most_) {}
+    long long most;                                      // tiles of rows, unless starts falls
+    static size_t head_bytes() { return (sizeof(Cut) * 148 + 15) / 16 * 16; }
+    LinePlan(void* scratch, long long most_) : cuts((Cut*)scratch), parts((float*)((char*)scratch + head_bytes())), most(most_) {}
     // outputs, unscaled, then maximum and sum of each row
-    __device__ __forceinline__ float* part(int cta, bool begun, int D) const { return parts + (2 * (size_t)cta + begun) * PA_ROWS * (D + 2); }
+    __device__ __forceinline__ float* part(int cta, bool begun, int D) const { return parts + (2 * (size_t)cta + !begun) * PA_ROWS * (D + 2); }
 };
 
 // A tile of rows of one request
@@ -65,25 +69,15 @@ __device__ __forceinline__ RowTile row_tile(const PagedArgs& a, const RowShape& 
     }
     return t;
 }
-// key tiles [first, last) that a half of the tile sees within [n0, n1); first = last where it sees none
-struct HalfRange { int first, last; };
-__device__ __forceinline__ HalfRange half_range(const PagedArgs& a, const RowShape& rs, int b, const RowTile& t, int half, int n0, int n1) {
-    const int from = half * rs.tokens, n = min(rs.tokens, t.tokens - from);
-    if (n <= 0 || t.at0 < 0) return {n0, n0};
-    const int lo = paged_keys(a, b, t.at0 + from).lo, hi = paged_keys(a, b, t.at0 + from + n - 1).hi;
-    if (hi <= lo) return {n0, n0};
-    const int first = max(lo / PA_KEYS, n0), last = min((hi + PA_KEYS - 1) / PA_KEYS, n1);
-    return last > first ? HalfRange{first, last} : HalfRange{n0, n0};
-}
-
-// A place in the line, and what of it lies ahead
+// A place in the line, and what of it lies ahead.  A tile of rows takes PA_TILE_COST steps of the line before its key tiles do.
 struct LineCursor {
-    int b, tile, pair, n;                                // pair: key head and chunk of its query heads; n: key tiles of the tile passed
+    int b, tile, pair, n;                                // pair: key head and chunk of its query heads; n: steps of the tile passed
     long long left;
     RowTile t;
-    __device__ __forceinline__ int steps() const { return t.n1 - t.n0; }
-    // the piece of the current tile that is this CTA's
+    __device__ __forceinline__ int steps() const { return PA_TILE_COST + t.n1 - t.n0; }
+    // the steps of the current tile that are this CTA's, and the key tile that step n begins with
     __device__ __forceinline__ int piece() const { return (int)min((long long)(steps() - n), left); }
+    __device__ __forceinline__ int key(int n) const { return t.n0 + max(n - PA_TILE_COST, 0); }
     __device__ __forceinline__ void next_tile(const PagedArgs& a, const RowShape& rs) {
         n = 0;
         if (++pair < a.KV * a.chunks) return;
@@ -130,7 +124,7 @@ __device__ __forceinline__ int first_above(const long long* s_sum, int threads, 
 }
 // The CTA's share of the line, by all its threads
 template <int THREADS>
-__device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& rs, const LinePlan& plan, LineCursor* out) {
+__device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& rs, long long most_tiles, LineCursor* out, long long* out_per) {
     __shared__ long long s_tiles[THREADS], s_steps[THREADS];
     const int tid = threadIdx.x, most = PA_HALVES * rs.tokens, pairs = a.KV * a.chunks;
     auto tiles_of = [&](int b) { return (rows_end(a, b) - rows_begin(a, b) + most - 1) / most; };
@@ -138,7 +132,7 @@ __device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& r
     long long v = 0;
     for (int b = b0; b < b1; b++) v += tiles_of(b);
     line_sum(v, s_tiles);
-    const long long tiles = min(s_tiles[THREADS - 1], plan.most), per_u = (tiles + THREADS - 1) / THREADS;
+    const long long tiles = min(s_tiles[THREADS - 1], most_tiles), per_u = (tiles + THREADS - 1) / THREADS;
     // request and tile of the u-th tile of rows
     auto find = [&](long long u, int& b, int& tile) {
         const int t = first_above(s_tiles, THREADS, u);
@@ -159,18 +153,9 @@ __device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& r
     };
     const long long u0 = min(tid * per_u, tiles), u1 = min(u0 + per_u, tiles);
     v = 0;
-    walk(u0, u1, [&](long long, int, int, const RowTile& t) { v += t.n1 - t.n0; return true; });
-    const long long upto = line_sum(v, s_steps), total = s_steps[THREADS - 1] * pairs, per = (total + gridDim.x - 1) / gridDim.x;
-    if (blockIdx.x == 0) {
-        long long at = upto - v;
-        walk(u0, u1, [&](long long u, int b, int tile, const RowTile& t) {
-            plan.before[u] = at * pairs;
-            plan.tile[u] = make_int2(b, tile);
-            at += t.n1 - t.n0;
-            return true;
-        });
-        if (tid == 0) { plan.before[tiles] = total; *plan.per = per; *plan.tiles = tiles; }
-    }
+    walk(u0, u1, [&](long long, int, int, const RowTile& t) { v += PA_TILE_COST + t.n1 - t.n0; return true; });
+    line_sum(v, s_steps);
+    const long long total = s_steps[THREADS - 1] * pairs, per = (total + gridDim.x - 1) / gridDim.x;
     const long long x0 = blockIdx.x * per, x1 = min(x0 + per, total);
     if (tid == 0) {
         LineCursor c = {};
@@ -179,7 +164,7 @@ __device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& r
             const int t = first_above(s_steps, THREADS, x0 / pairs);
             long long at = t > 0 ? s_steps[t - 1] : 0;
             walk(t * per_u, tiles, [&](long long, int b, int tile, const RowTile& rt) {
-                const int steps = rt.n1 - rt.n0;
+                const int steps = PA_TILE_COST + rt.n1 - rt.n0;
                 if ((at + steps) * pairs <= x0) { at += steps; return true; }
                 c.b = b; c.tile = tile; c.t = rt;
                 c.pair = (int)((x0 - at * pairs) / steps);
@@ -188,8 +173,51 @@ __device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& r
             });
         }
         *out = c;
+        *out_per = per;
     }
     __syncthreads();
+}
+
+// A piece of a CTA's share: a tile of rows over some of its key tiles.  One warp writes them ahead of the others, whose addresses
+// in global memory it thereby keeps out of their way.
+struct Piece {
+    int b, hk, h0, heads;                                // h0: its first query head
+    int row0, tokens, at0, first;                        // first: where the request begins to see
+    int n0, n1;                                          // key tiles
+    int lo, hi;                                          // keys that some row of the tile sees
+    int from[PA_HALVES], to[PA_HALVES];                  // key tiles of each half
+    int cut, begun;                                      // it has not all key tiles of its tile; it begins the share
+    int twin;                                            // rows for one half alone: both take them, each every other key tile
+    int last;
+};
+constexpr int PA_PIECES = 4;
+
+__device__ __forceinline__ Piece make_piece(const PagedArgs& a, const RowShape& rs, const LineCursor& c, bool begun) {
+    Piece p;
+    p.b = c.b;
+    p.hk = c.pair / a.chunks;
+    const int g0 = c.pair % a.chunks * rs.heads, group = a.H / a.KV;
+    p.h0 = p.hk * group + g0;
+    p.heads = min(rs.heads, group - g0);
+    p.row0 = c.t.row0; p.tokens = c.t.tokens; p.at0 = c.t.at0;
+    p.first = a.start != nullptr ? max(a.start[c.b], 0) : 0;
+    p.n0 = c.key(c.n);
+    p.n1 = c.key(c.n + c.piece());
+    p.lo = paged_keys(a, c.b, c.t.at0).lo;
+    p.hi = paged_keys(a, c.b, c.t.at0 < 0 ? -1 : c.t.at0 + c.t.tokens - 1).hi;
+    for (int t = 0; t < PA_HALVES; t++) {
+        const int at = t * rs.tokens, n = min(rs.tokens, p.tokens - at);
+        p.from[t] = p.to[t] = p.n0;
+        if (n <= 0 || p.at0 < 0) continue;
+        const int lo = paged_keys(a, c.b, p.at0 + at).lo, hi = paged_keys(a, c.b, p.at0 + at + n - 1).hi;
+        const int from = max(lo / PA_KEYS, p.n0), to = min((hi + PA_KEYS - 1) / PA_KEYS, p.n1);
+        if (hi > lo && to > from) { p.from[t] = from; p.to[t] = to; }
+    }
+    p.cut = p.n0 > c.t.n0 || p.n1 < c.t.n1;
+    p.begun = begun;
+    p.twin = p.tokens <= rs.tokens && p.to[0] - p.from[0] >= 2;
+    p.last = 0;
+    return p;
 }
 
 template <int DP, bool CAP, bool BIAS>
@@ -201,19 +229,29 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
     char* Qs = smem;
     char* Ks = smem + PA_HALVES * Sh::QTILE;
     __shared__ uint64_t q_full, q_empty, s_full[PA_HALVES], p_full[PA_HALVES], o_full[PA_HALVES], full[PA_STAGES], empty[PA_STAGES];
+    __shared__ uint64_t piece_full[PA_PIECES], piece_empty[PA_PIECES], merge_full, merge_empty;
+    __shared__ Piece s_piece[PA_PIECES];
+    __shared__ float2 s_merge[128];
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
     __shared__ LineCursor s_at;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, group = a.H / a.KV;
+    __shared__ long long s_per;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(&q_full, 1); mbar_init(&q_empty, 1);
+        mbar_init(&q_full, 1); mbar_init(&q_empty, 1); mbar_init(&merge_full, 4); mbar_init(&merge_empty, 4);
         for (int t = 0; t < PA_HALVES; t++) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); }
         for (int s = 0; s < PA_STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < PA_PIECES; s++) { mbar_init(&piece_full[s], 1); mbar_init(&piece_empty[s], PA_HALVES * 4 + 2); }
         mbar_fence_init();
         s_fail = 0;
     }
     if (warp == PA_HALVES * 4) tmem_alloc(&s_tmem, 512);
-    line_share<PA_THREADS>(a, rs, plan, &s_at);
+    if (tid == 32) {
+        prefetch_map(&maps.q);
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
+    }
+    line_share<PA_THREADS>(a, rs, plan.most, &s_at, &s_per);
     {                                                    // rows of no request
         const int r0 = a.B > 0 ? rows_begin(a, 0) : a.N, r1 = a.B > 0 ? max(rows_end(a, a.B - 1), r0) : a.N;
         const long long pieces = (long long)a.H * a.D / 8, n = (long long)(r0 + a.N - r1) * pieces;
@@ -226,32 +264,43 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
     __syncthreads();
     tmem_fence_after();
     constexpr uint32_t tmem = 0;                         // all 512 columns are this CTA's, so they begin at the first
-    LineCursor c = s_at;
-    bool ok = true;
+    bool ok = s_at.n + s_at.left > PA_TILE_COST, failed = false;                   // ok: there is a next piece (of a tile's own cost alone there is nothing to do)
+    unsigned turn = 0;                                   // pieces so far
+    auto next = [&]() -> const Piece& {                  // waits for the piece; `failed` where none came
+        failed = failed || !wait_soon_warp(&piece_full[turn % PA_PIECES], (turn / PA_PIECES) & 1);
+        return s_piece[turn % PA_PIECES];
+    };
+    auto passed = [&](const Piece& p) {                  // by a whole warp that reads no more of it
+        ok = !failed && !p.last;
+        __syncwarp();
+        if (lane == 0) arrive(&piece_empty[turn % PA_PIECES]);
+        turn++;
+    };
     // 3 x 128 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72; a row of 128 scores stays in registers
     if (warp < PA_HALVES * 4) {                          // ---- softmax of a half ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int half = tid / 128, r = tid % 128, token = r / rs.heads, g = r % rs.heads;
         const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
         const uint32_t S = tmem + half * PA_KEYS + lane_at, O = tmem + PA_HALVES * PA_KEYS + half * DP + lane_at;
-        unsigned done = 0, x0 = 0;                       // key tiles of this half so far; tiles of the ring before this piece
-        const long long share = c.left;
-        for (; c.left > 0 && ok; c.next_piece(a, rs)) {
-            const int n0 = c.t.n0 + c.n, n1 = n0 + c.piece(), b = c.b, hk = c.pair / a.chunks, h = hk * group + c.pair % a.chunks * rs.heads + g;
-            const bool cut = n0 > c.t.n0 || n1 < c.t.n1;
-            const HalfRange hr = half_range(a, rs, b, c.t, half, n0, n1);
-            const int tk = half * rs.tokens + token;     // of the tile
-            const bool row = token < rs.tokens && tk < c.t.tokens && c.pair % a.chunks * rs.heads + g < group;
-            const Span sp = row && c.t.at0 >= 0 ? paged_keys(a, b, c.t.at0 + tk) : Span{0, 0};
-            const int all_lo = paged_keys(a, b, c.t.at0).lo, all_hi = paged_keys(a, b, c.t.at0 + c.t.tokens - 1).hi;
+        unsigned done = 0, others = 0, x0 = 0, merges = 0;   // key tiles of this half and of the other so far; tiles of the ring before this piece
+        while (ok) {
+            const Piece& p = next();
+            if (failed) break;
+            const int tk = (p.twin ? 0 : half) * rs.tokens + token;                // of the tile
+            const bool row = token < rs.tokens && tk < p.tokens && g < p.heads;
+            const int where = p.at0 + tk;
+            const Span sp = row && p.at0 >= 0 ? Span{a.window > 0 && where >= a.window ? max(p.first, where - a.window + 1) : p.first, min(where, (a.M << a.shift) - 1) + 1}
+                                              : Span{0, 0};
             const WarpSpan ws(sp);
-            const Score sc = paged_score(a, h);
+            const Score sc = paged_score(a, p.h0 + g);
+            const int by = p.twin ? 2 : 1, n_first = p.twin ? p.from[0] + half : p.from[half], n_last = p.twin ? p.to[0] : p.to[half];
+            const int all_lo = p.lo, all_hi = p.hi, n_base = p.n0;
             float m = -INFINITY, l = 0.f;                // m in base-2 exponents
-            const float at = (float)(c.t.at0 + tk);
-            for (int n = hr.first; n < hr.last; n++, done++) {
+            const float at = (float)where;
+            for (int n = n_first; n < n_last; n += by, done++) {
                 const int j0 = n * PA_KEYS;
                 const bool masked = !ws.clear(j0, PA_KEYS);
-                if (!(ok = wait_soon_warp(&s_full[half], done & 1))) break;
+                if (!wait_soon_warp(&s_full[half], done & 1)) { failed = true; break; }
                 tmem_fence_after();
                 uint32_t raw[PA_KEYS / 32][32];
 #pragma unroll
@@ -272,8 +321,8 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 if (m == -INFINITY) m = top;
                 if (__any_sync(FULL, grown)) {
                     const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_fast(m - to);
-                    if (n > hr.first) {
-                        if (!(ok = wait_soon_warp(&o_full[half], (done - 1) & 1))) break;
+                    if (n > n_first) {
+                        if (!wait_soon_warp(&o_full[half], (done - 1) & 1)) { failed = true; break; }
                         tmem_fence_after();
 #pragma unroll
                         for (int i = 0; i < DP / 32; i++) {
@@ -308,8 +357,8 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 l += total.x + total.y;
                 if (j0 < all_lo || j0 + PA_KEYS > all_hi) {
                     // values that no row of the tile sees (the rest of a page, another request's) must not reach the product: zeros
-                    const unsigned xv = x0 + 2 * (n - n0) + 1, s = xv % PA_STAGES;
-                    if (!(ok = wait_soon_warp(&full[s], (xv / PA_STAGES) & 1))) break;
+                    const unsigned xv = x0 + 2 * (n - n_base) + 1, s = xv % PA_STAGES;
+                    if (!wait_soon_warp(&full[s], (xv / PA_STAGES) & 1)) { failed = true; break; }
                     if (j0 + r < all_lo || j0 + r >= all_hi) {
 #pragma unroll
                         for (int i = 0; i < DP / 8; i++)
@@ -322,101 +371,177 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 __syncwarp();
                 if (lane == 0) arrive(&p_full[half]);
             }
-            if (ok && hr.last > hr.first) ok = wait_soon_warp(&o_full[half], (done - 1) & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            const bool none = sp.hi <= sp.lo;
-            const float inv = none ? 0.f : 1.f / l;
-            // at the share's first step a part continues what the CTA before has begun
-            float* part = plan.part(blockIdx.x, c.left != share, a.D);
-            const int pr = half * 128 + r;
-            bf16* to = o + ((size_t)(c.t.row0 + tk) * a.H + h) * a.D;
-            float seen = 0.f;
+            if (failed) break;
+            others += p.twin ? (p.to[0] - p.from[0] + half) / 2 : p.to[1 - half] - p.from[1 - half];
+            if (n_last > n_first && !wait_soon_warp(&o_full[half], (done - 1) & 1)) { failed = true; break; }
+            float f0 = 1.f, f1 = 0.f;                    // of a twin: what the halves' outputs count
+            if (p.twin && half == 1) {                   // its rows are the other half's to finish
+                s_merge[r] = make_float2(m, l);
+                __syncwarp();
+                if (lane == 0) arrive(&merge_full);
+                if (!wait_soon_warp(&merge_empty, merges & 1)) { failed = true; break; }
+            } else {
+                if (p.twin) {
+                    if (!wait_soon_warp(&merge_full, merges & 1) || !wait_soon_warp(&o_full[1], (others - 1) & 1)) { failed = true; break; }
+                    const float2 other = s_merge[r];
+                    const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
+                    f0 = exp2f(m - base);
+                    f1 = exp2f(other.x - base);
+                    l = l * f0 + other.y * f1;
+                    m = top;
+                }
+                tmem_fence_after();
+                const bool none = sp.hi <= sp.lo;
+                const float inv = none ? 0.f : 1.f / l;
+                float* part = plan.part(blockIdx.x, p.begun, a.D);
+                const int pr = (p.twin ? 0 : half) * 128 + r;
+                const unsigned rows = __ballot_sync(FULL, row);
+                // rows of 64 bytes through shared memory, so that a store covers 8 of them and not 32
+                const uint32_t out = smem_u32(smem + PA_HALVES * Sh::QTILE + PA_STAGES * Sh::KTILE) + warp * PA_OUT;
+                auto put = [&](const uint32_t (&w)[16], auto store) {
 #pragma unroll
-            for (int i = 0; i < DP / 32; i++) {
-                uint32_t y[32];
+                    for (int e = 0; e < 4; e++) st_shared16(out + lane * PA_OUT_ROW + e * 16, w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                    __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 32; e++) y[e] = 0u;
-                if (hr.last > hr.first) { tmem_ld(O + i * 32, y); tmem_ld_wait(y); }
+                    for (int e = 0; e < 4; e++) {
+                        const int x = e * 8 + lane / 4;  // row of the warp
+                        const uint4 v = ld_shared16(out + x * PA_OUT_ROW + (lane % 4) * 16);
+                        if (rows >> x & 1) store(r - lane + x, lane % 4, v);
+                    }
+                    __syncwarp();
+                };
+                float seen = 0.f;
 #pragma unroll
-                for (int e = 0; e < 32; e++) watch(seen, __uint_as_float(y[e]));
-                if (!row) continue;
-                if (cut) {
+                for (int i = 0; i < DP / 32; i++) {
+                    uint32_t y[32];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        if (i * 32 + e < a.D)
-                            *reinterpret_cast<uint4*>(part + (size_t)pr * a.D + i * 32 + e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-                } else {
+                    for (int e = 0; e < 32; e++) y[e] = 0u;
+                    if (n_last > n_first) { tmem_ld(O + i * 32, y); tmem_ld_wait(y); }
+                    if (p.twin) {
+                        uint32_t z[32];
+                        tmem_ld(O + DP + i * 32, z);
+                        tmem_ld_wait(z);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t w[4];
+                        for (int e = 0; e < 32; e++) y[e] = __float_as_uint(fmaf(__uint_as_float(z[e]), f1, __uint_as_float(y[e]) * f0));
+                    }
 #pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            w[u] = none ? 0u : pack_bf16(__uint_as_float(y[e + 2 * u]) * inv, __uint_as_float(y[e + 2 * u + 1]) * inv);
-                        if (i * 32 + e < a.D) *reinterpret_cast<uint4*>(to + i * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int e = 0; e < 32; e++) watch(seen, __uint_as_float(y[e]));
+                    if (p.cut) {
+#pragma unroll
+                        for (int s = 0; s < 2; s++)
+                            put(reinterpret_cast<const uint32_t(&)[16]>(y[16 * s]), [&](int x, int piece, uint4 v) {
+                                const int d = i * 32 + s * 16 + piece * 4;
+                                if (d < a.D) *reinterpret_cast<uint4*>(part + (size_t)(pr - r + x) * a.D + d) = v;
+                            });
+                    } else {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            w[e] = none ? 0u : pack_bf16(__uint_as_float(y[2 * e]) * inv, __uint_as_float(y[2 * e + 1]) * inv);
+                        put(w, [&](int x, int piece, uint4 v) {
+                            const int d = i * 32 + piece * 8, xt = x / rs.heads;
+                            if (d < a.D) *reinterpret_cast<uint4*>(o + ((size_t)(p.row0 + tk - token + xt) * a.H + p.h0 + x - xt * rs.heads) * a.D + d) = v;
+                        });
                     }
                 }
-            }
-            if (cut && row) *reinterpret_cast<float2*>(part + (size_t)PA_ROWS * a.D + 2 * pr) = make_float2(fmaxf(m, -FLT_MAX), l);
-            for (unsigned bad = __ballot_sync(FULL, row && !none && (seen != seen)); bad != 0; bad &= bad - 1) {
-                const int from = __ffs(bad) - 1;
-                const int xr = __shfl_sync(FULL, r, from), xtk = __shfl_sync(FULL, tk, from), xh = __shfl_sync(FULL, h, from);
-                const int lo = max(__shfl_sync(FULL, sp.lo, from), n0 * PA_KEYS), hi = min(__shfl_sync(FULL, sp.hi, from), n1 * PA_KEYS);
-                float y[4], xm, xl;
-                careful_row(a, paged_score(a, xh), q + (long long)(c.t.row0 + xtk) * a.qs[0] + xh * a.qs[1], kp, vp, b, hk, c.t.at0 + xtk, lo, hi, y, xm, xl);
-                __syncwarp();
+                if (p.cut && row) *reinterpret_cast<float2*>(part + (size_t)PA_ROWS * a.D + 2 * pr) = make_float2(fmaxf(m, -FLT_MAX), l);
+                for (unsigned bad = __ballot_sync(FULL, row && !none && (seen != seen)); bad != 0; bad &= bad - 1) {
+                    const int from = __ffs(bad) - 1;
+                    const int xpr = __shfl_sync(FULL, pr, from), xtk = __shfl_sync(FULL, tk, from), xh = p.h0 + __shfl_sync(FULL, g, from);
+                    const int lo = max(__shfl_sync(FULL, sp.lo, from), p.n0 * PA_KEYS), hi = min(__shfl_sync(FULL, sp.hi, from), p.n1 * PA_KEYS);
+                    float y[4], xm, xl;
+                    careful_row(a, paged_score(a, xh), q + (long long)(p.row0 + xtk) * a.qs[0] + xh * a.qs[1], kp, vp, p.b, p.hk, p.at0 + xtk, lo, hi, y, xm, xl);
+                    __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int d = lane + 32 * e;
-                    if (d >= a.D) continue;
-                    if (cut) part[(size_t)(half * 128 + xr) * a.D + d] = y[e];
-                    else o[((size_t)(c.t.row0 + xtk) * a.H + xh) * a.D + d] = __float2bfloat16_rn(y[e] / xl);
+                    for (int e = 0; e < 4; e++) {
+                        const int d = lane + 32 * e;
+                        if (d >= a.D) continue;
+                        if (p.cut) part[(size_t)xpr * a.D + d] = y[e];
+                        else o[((size_t)(p.row0 + xtk) * a.H + xh) * a.D + d] = __float2bfloat16_rn(y[e] / xl);
+                    }
+                    if (p.cut && lane == 0) *reinterpret_cast<float2*>(part + (size_t)PA_ROWS * a.D + 2 * xpr) = make_float2(fmaxf(xm, -FLT_MAX), xl);
                 }
-                if (cut && lane == 0) *reinterpret_cast<float2*>(part + (size_t)PA_ROWS * a.D + 2 * (half * 128 + xr)) = make_float2(fmaxf(xm, -FLT_MAX), xl);
+                tmem_fence_before();
+                __syncwarp();
+                if (p.twin && lane == 0) arrive(&merge_empty);
             }
-            x0 += 2 * (n1 - n0);
-            tmem_fence_before();
-            __syncwarp();
+            merges += p.twin;
+            x0 += 2 * (p.n1 - p.n0);
+            passed(p);
         }
-        if (!ok) s_fail = 1;
+        if (failed) s_fail = 1;
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == PA_HALVES * 4 + 1) {                 // ---- copies ----
-            unsigned x = 0, piece = 0;
-            const int rows = min(1 << a.shift, PA_KEYS), boxes = PA_KEYS / rows;
-            for (; c.left > 0 && ok; c.next_piece(a, rs), piece++) {
-                const int n0 = c.t.n0 + c.n, n1 = n0 + c.piece(), hk = c.pair / a.chunks, h0 = hk * group + c.pair % a.chunks * rs.heads;
-                if (piece > 0 && !(ok = wait_soon_warp(&q_empty, (piece - 1) & 1))) break;
+        if (warp == PA_HALVES * 4 + 2) {                 // ---- pieces ----
+            LineCursor c = s_at;
+            Cut cut = {};
+            for (bool begun = true; ok; begun = false, turn++) {
+                const unsigned slot = turn % PA_PIECES;
+                const int steps = c.piece();
+                const bool whole_left = c.n + steps == c.steps();
+                Piece p = make_piece(a, rs, c, begun);
+                ok = c.left - steps > (whole_left ? PA_TILE_COST : 0);
+                p.last = !ok;
+                if (!whole_left && p.n0 == c.t.n0)
+                    cut = {p.b, p.row0, p.tokens, p.at0, p.first, p.h0, p.heads, begun, 1 + (int)((c.steps() - c.n - steps + s_per - 1) / s_per)};
+                if (turn >= PA_PIECES && !wait_soon_warp(&piece_empty[slot], (turn / PA_PIECES - 1) & 1)) { failed = true; break; }
                 if (lane == 0) {
-                    const int halves = c.t.tokens > rs.tokens ? 2 : 1;
-                    mbar_arrive_expect_tx(&q_full, halves * Sh::SUBS * rs.heads * rs.tokens * 128);
-                    for (int t = 0; t < halves; t++)
-                        for (int s = 0; s < Sh::SUBS; s++)
-                            box_g2s(Qs + t * Sh::QTILE + s * 128 * 128, &maps.q, s * 64, h0, c.t.row0 + t * rs.tokens, &q_full);
+                    s_piece[slot] = p;
+                    arrive(&piece_full[slot]);
                 }
-                for (int n = n0; n < n1 && ok; n++) {
+                __syncwarp();
+                c.next_piece(a, rs);
+            }
+            if (lane == 0) plan.cuts[blockIdx.x] = cut;
+            if (failed && lane == 0) s_fail = 1;
+        } else if (warp == PA_HALVES * 4 + 1) {          // ---- copies ----
+            unsigned x = 0;
+            const int rows = min(1 << a.shift, PA_KEYS), boxes = PA_KEYS / rows;
+            // this lane's box of a tile: sub-tile of channels, rows; its page's id is fetched a tile ahead
+            const int sub = lane / boxes, box = lane % boxes;
+            const bool mine = sub < Sh::SUBS;
+            while (ok) {
+                const Piece& p = next();
+                if (failed) break;
+                auto id_of = [&](int n) {                // a page outside the pool, or beyond the table: zeros
+                    const int j = n * PA_KEYS + box * rows;
+                    return mine && n < p.n1 && (j >> a.shift) < a.M ? max(page_of(a, p.b, j), -1) : -1;
+                };
+                int id = id_of(p.n0);
+                for (int n = p.n0; n < p.n1 && !failed; n++) {
+                    const int then = id_of(n + 1);
                     for (int w = 0; w < 2; w++, x++) {   // keys, values
-                        const unsigned s = x % PA_STAGES, turn = x / PA_STAGES;
-                        if (turn > 0 && !(ok = wait_soon_warp(&empty[s], (turn - 1) & 1))) break;
+                        const unsigned s = x % PA_STAGES, round = x / PA_STAGES;
+                        if (round > 0 && !wait_soon_warp(&empty[s], (round - 1) & 1)) { failed = true; break; }
                         if (lane == 0) mbar_arrive_expect_tx(&full[s], Sh::KTILE);
                         __syncwarp();
-                        for (int i = lane; i < boxes * Sh::SUBS; i += 32) {        // a page outside the pool, or beyond the table: zeros
-                            const int sub = i / boxes, box = i % boxes, j = n * PA_KEYS + box * rows;
-                            const int id = (j >> a.shift) < a.M ? page_of(a, c.b, j) : -1;
-                            tile_g2s(Ks + s * Sh::KTILE + sub * PA_KEYS * 128 + box * rows * 128, w ? &maps.v : &maps.k, sub * 64, j & ((1 << a.shift) - 1), hk,
-                                     max(id, -1), &full[s]);
-                        }
+                        if (mine)
+                            tile_g2s(Ks + s * Sh::KTILE + sub * PA_KEYS * 128 + box * rows * 128, w ? &maps.v : &maps.k, sub * 64,
+                                     (n * PA_KEYS + box * rows) & ((1 << a.shift) - 1), p.hk, id, &full[s]);
+                    }
+                    id = then;
+                    if (n > p.n0) continue;
+                    // the queries, whose place is the last piece's until its scores are done, behind the first keys and values
+                    if (turn > 0 && !wait_soon_warp(&q_empty, (turn - 1) & 1)) { failed = true; break; }
+                    if (lane == 0) {
+                        const int halves = p.tokens > rs.tokens ? 2 : 1;
+                        mbar_arrive_expect_tx(&q_full, halves * Sh::SUBS * rs.heads * rs.tokens * 128);
+                        for (int t = 0; t < halves; t++)
+                            for (int s = 0; s < Sh::SUBS; s++)
+                                box_g2s(Qs + t * Sh::QTILE + s * 128 * 128, &maps.q, s * 64, p.h0, p.row0 + t * rs.tokens, &q_full);
                     }
                 }
+                if (failed) break;
+                passed(p);
             }
-            if (!ok && lane == 0) s_fail = 1;
+            if (failed && lane == 0) s_fail = 1;
         } else if (warp == PA_HALVES * 4) {              // ---- products ----
             const bool lead = elected();
-            unsigned x = 0, piece = 0, done[PA_HALVES] = {0, 0};
+            unsigned x = 0, done[PA_HALVES] = {0, 0};
             auto stage = [](unsigned i) { return i % PA_STAGES; };
-            auto arrived = [&](unsigned i) { return wait_soon_warp(&full[stage(i)], (i / PA_STAGES) & 1); };
-            auto scores = [&](int t, unsigned i) {       // s = q k^T
-                const uint32_t qd = tile_desc(smem_u32(Qs + t * Sh::QTILE), 16), kd = tile_desc(smem_u32(Ks + stage(i) * Sh::KTILE), 16);
+            auto arrived = [&](unsigned i) { failed = failed || !wait_soon_warp(&full[stage(i)], (i / PA_STAGES) & 1); return !failed; };
+            auto scores = [&](int t, int tile, unsigned i) {                       // s = q k^T of a half, with the queries of tile 0 or 1
+                const uint32_t qd = tile_desc(smem_u32(Qs + tile * Sh::QTILE), 16), kd = tile_desc(smem_u32(Ks + stage(i) * Sh::KTILE), 16);
                 if (lead) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; k++)
@@ -426,47 +551,62 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 }
                 __syncwarp();
             };
-            for (; c.left > 0 && ok; c.next_piece(a, rs), piece++) {
-                const int n0 = c.t.n0 + c.n, n1 = n0 + c.piece();
-                HalfRange hr[PA_HALVES];
+            auto outputs = [&](int t, unsigned i, bool add) {                      // o += p v of a half
+                failed = failed || !wait_soon_warp(&p_full[t], done[t] & 1);
+                if (failed) return;
+                done[t]++;
+                tmem_fence_after();
+                const uint32_t vd = tile_desc(smem_u32(Ks + stage(i) * Sh::KTILE), PA_KEYS * 128);
+                if (lead) {
 #pragma unroll
-                for (int t = 0; t < PA_HALVES; t++) hr[t] = half_range(a, rs, c.b, c.t, t, n0, n1);
-                ok = wait_soon_warp(&q_full, piece & 1) && arrived(x);
-#pragma unroll
-                for (int t = 0; t < PA_HALVES; t++)
-                    if (ok && hr[t].first == n0 && hr[t].last > hr[t].first) scores(t, x);
-                if (lead) mma_commit(&empty[stage(x)]);
-                __syncwarp();
-                for (int n = n0; n < n1 && ok; n++, x += 2) {
-                    ok = arrived(x + 1) && (n + 1 == n1 || arrived(x + 2));
-                    const uint32_t vd = tile_desc(smem_u32(Ks + stage(x + 1) * Sh::KTILE), PA_KEYS * 128);
-#pragma unroll
-                    for (int t = 0; t < PA_HALVES; t++) {
-                        if (!ok) break;
-                        if (n >= hr[t].first && n < hr[t].last) {
-                            ok = wait_soon_warp(&p_full[t], done[t] & 1);
-                            done[t]++;
-                            tmem_fence_after();
-                            if (lead) {
-#pragma unroll
-                                for (int k = 0; k < PA_KEYS / 16; k++)
-                                    mma_ts(tmem + PA_HALVES * PA_KEYS + t * DP, tmem + t * PA_KEYS + k * 8, vd + k * 2048 / 16, mma_shape(DP, true), n > hr[t].first || k > 0);
-                                mma_commit(&o_full[t]);
-                            }
-                            __syncwarp();
-                        }
-                        if (n + 1 >= hr[t].first && n + 1 < hr[t].last) scores(t, x + 2);
-                    }
-                    if (lead) {
-                        mma_commit(&empty[stage(x + 1)]);
-                        if (n + 1 < n1) mma_commit(&empty[stage(x + 2)]);
-                    }
-                    __syncwarp();
+                    for (int k = 0; k < PA_KEYS / 16; k++)
+                        mma_ts(tmem + PA_HALVES * PA_KEYS + t * DP, tmem + t * PA_KEYS + k * 8, vd + k * 2048 / 16, mma_shape(DP, true), add || k > 0);
+                    mma_commit(&o_full[t]);
                 }
-                if (lead) mma_commit(&q_empty);
                 __syncwarp();
+            };
+            auto used = [&](unsigned i) {
+                if (lead) mma_commit(&empty[stage(i)]);
+                __syncwarp();
+            };
+            while (ok) {
+                const Piece& p = next();
+                failed = failed || !wait_soon_warp(&q_full, turn & 1);
+                if (failed) break;
+                const int n0 = p.n0, n1 = p.n1, from[PA_HALVES] = {p.from[0], p.from[1]}, to[PA_HALVES] = {p.to[0], p.to[1]};
+                if (p.twin) {                            // p.from[0] is n0 and p.to[0] n1: all its key tiles are seen by some row
+                    if (arrived(x)) { scores(0, 0, x); used(x); }
+                    if (arrived(x + 2)) { scores(1, 0, x + 2); used(x + 2); }
+                    if (n0 + 2 == n1 && lead) mma_commit(&q_empty);
+                    for (int n = n0; n < n1 && arrived(x + 1); n++, x += 2) {
+                        const int t = (n - n0) & 1;
+                        outputs(t, x + 1, n >= n0 + 2);
+                        used(x + 1);
+                        if (n + 2 < n1 && arrived(x + 4)) { scores(t, 0, x + 4); used(x + 4); }
+                        if (n + 3 == n1 && lead) mma_commit(&q_empty);
+                    }
+                } else {
+                    arrived(x);
+#pragma unroll
+                    for (int t = 0; t < PA_HALVES; t++)
+                        if (!failed && from[t] == n0 && to[t] > n0) scores(t, t, x);
+                    used(x);
+                    if (n0 + 1 == n1 && lead) mma_commit(&q_empty);
+                    for (int n = n0; n < n1 && arrived(x + 1) && (n + 1 == n1 || arrived(x + 2)); n++, x += 2) {
+#pragma unroll
+                        for (int t = 0; t < PA_HALVES; t++) {
+                            if (n >= from[t] && n < to[t]) outputs(t, x + 1, n > from[t]);
+                            if (!failed && n + 1 >= from[t] && n + 1 < to[t]) scores(t, t, x + 2);
+                        }
+                        used(x + 1);
+                        if (n + 1 < n1) used(x + 2);
+                        if (n + 2 == n1 && lead) mma_commit(&q_empty);
+                    }
+                }
+                if (failed) break;
+                passed(p);
             }
-            if (!ok) s_fail = 1;
+            if (failed) s_fail = 1;
         }
     }
     tmem_fence_before();
@@ -478,43 +618,42 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
     if (warp == PA_HALVES * 4) { tmem_fence_after(); tmem_free(s_tmem, 512); }
 }
 
-// The tile of rows that the end of a CTA's share cuts, joined in the order of its parts: blockIdx.x the share, the first that cuts it
-// does; a warp to a row
-constexpr int LJ_ROWS = 32;
+// The tile of rows that the end of a share is the first to cut, joined in the order of its parts; a warp to a row
+constexpr int LJ_ROWS = 16;
 __global__ void __launch_bounds__(256) line_join_kernel(PagedArgs a, RowShape rs, LinePlan plan, bf16* o) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, group = a.H / a.KV, pairs = a.KV * a.chunks;
-    const long long tiles = *plan.tiles, per = *plan.per;
-    const long long x = (blockIdx.x + 1ll) * per;        // the cut
-    if (per == 0 || x >= plan.before[tiles]) return;
-    long long lo = 0, hi = tiles - 1;                    // the tile that holds it
-    while (lo < hi) {
-        const long long mid = (lo + hi + 1) / 2;
-        if (plan.before[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    const long long steps = (plan.before[lo + 1] - plan.before[lo]) / pairs, pair = (x - plan.before[lo]) / steps, x0 = plan.before[lo] + pair * steps;
-    if (x == x0 || x - per > x0) return;                 // cuts nothing, or is not the first to cut it
-    const int w0 = (int)(x0 / per), w1 = (int)((x0 + steps - 1) / per);
-    const int2 at = plan.tile[lo];
-    const RowTile t = row_tile(a, rs, at.x, at.y);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const Cut c = plan.cuts[blockIdx.x];
     for (int pr = blockIdx.y * LJ_ROWS + warp; pr < (blockIdx.y + 1) * LJ_ROWS; pr += 8) {
-        const int half = pr / 128, r = pr % 128, token = r / rs.heads, g = (int)(pair % a.chunks) * rs.heads + r % rs.heads, tk = half * rs.tokens + token;
-        if (token >= rs.tokens || tk >= t.tokens || g >= group) continue;
-        const Span sp = t.at0 >= 0 ? paged_keys(a, at.x, t.at0 + tk) : Span{0, 0};
+        const int half = pr / 128, r = pr % 128, token = r / rs.heads, g = r % rs.heads, tk = half * rs.tokens + token;
+        if (token >= rs.tokens || tk >= c.tokens || g >= c.heads) continue;
+        const Span sp = c.at0 >= 0 ? paged_keys(a, c.b, c.at0 + tk) : Span{0, 0};
         float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int w = w0; w <= w1; w++) {
-            const float* part = plan.part(w, w * per < x0, a.D);
-            const float2 ml = *reinterpret_cast<const float2*>(part + (size_t)PA_ROWS * a.D + 2 * pr);
-            const float top = fmaxf(m, ml.x), f = exp2f(m - top), pf = exp2f(ml.x - top);
-            l = l * f + ml.y * pf;
+        for (int s0 = 0; s0 < c.shares; s0 += 32) {
+            const int n = min(c.shares - s0, 32);
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (lane < n) ml = *reinterpret_cast<const float2*>(plan.part(blockIdx.x + s0 + lane, s0 + lane > 0 || c.begun, a.D) + (size_t)PA_ROWS * a.D + 2 * pr);
+            float top = ml.x;
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 32 * c < a.D) acc[c] = acc[c] * f + part[(size_t)pr * a.D + lane + 32 * c] * pf;
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, off));
+            top = fmaxf(m, top);
+            const float f = exp2f(m - top), weight = exp2f(ml.x - top);
+            l = l * f + warp_sum(ml.y * weight);
             m = top;
-        }
-        bf16* to = o + ((size_t)(t.row0 + tk) * a.H + (pair / a.chunks) * group + g) * a.D;
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-            if (lane + 32 * c < a.D) to[lane + 32 * c] = __float2bfloat16_rn(sp.hi > sp.lo ? acc[c] / l : 0.f);
+            for (int e = 0; e < 4; e++) acc[e] *= f;
+#pragma unroll 4
+            for (int s = 0; s < n; s++) {
+                const float* part = plan.part(blockIdx.x + s0 + s, s0 + s > 0 || c.begun, a.D) + (size_t)pr * a.D;
+                const float w = __shfl_sync(FULL, weight, s);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (lane + 32 * e < a.D) acc[e] = fmaf(part[lane + 32 * e], w, acc[e]);
+            }
+        }
+        bf16* to = o + ((size_t)(c.row0 + tk) * a.H + c.h0 + g) * a.D;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (lane + 32 * e < a.D) to[lane + 32 * e] = __float2bfloat16_rn(sp.hi > sp.lo ? acc[e] / l : 0.f);
     }
 }
 
@@ -525,7 +664,7 @@ static RowShape row_shape(const PagedArgs& a) {
 static long long most_tiles(const PagedArgs& a) { return a.N / (PA_HALVES * row_shape(a).tokens) + (long long)a.B; }
 
 size_t paged_attn_scratch_bf16(const PagedArgs& a) {
-    return LinePlan::head_bytes(most_tiles(a)) + sizeof(float) * 148 * 2 * PA_ROWS * (size_t)(a.D + 2);
+    return LinePlan::head_bytes() + sizeof(float) * 148 * 2 * PA_ROWS * (size_t)(a.D + 2);
 }
 
 template <int DP, bool CAP, bool BIAS>

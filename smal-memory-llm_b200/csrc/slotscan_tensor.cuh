@@ -107,6 +107,7 @@ __device__ __forceinline__ void tile_s2g(const CUtensorMap* map, int col, int ro
                  "r"(row), "r"(head), "r"(seq), "r"(smem_u32(src))
                  : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
 // of a (row, head, channel) tensor
 __device__ __forceinline__ void box_g2s(void* dst, const CUtensorMap* map, int col, int head, int row, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
