@@ -17,12 +17,14 @@ struct PagedArgs {
     const float* slopes;
 };
 
-// keys that a query at position `at` of request b sees, [lo, hi); empty where hi <= lo.  What its table does not reach is not seen.
-__device__ __forceinline__ Span paged_keys(const PagedArgs& a, int b, int at) {
-    const int first = a.start != nullptr ? max(a.start[b], 0) : 0;
+// keys that a query at position `at` sees, [lo, hi), of a request that sees from `first` on; empty where hi <= lo.  What a table does not reach
+// is not seen.
+__device__ __forceinline__ Span paged_keys_from(const PagedArgs& a, int first, int at) {
     const int hi = at < 0 ? 0 : min(at, (a.M << a.shift) - 1) + 1;
     return {a.window > 0 && at >= a.window ? max(first, at - a.window + 1) : first, hi};
 }
+__device__ __forceinline__ int first_key(const PagedArgs& a, int b) { return a.start != nullptr ? max(a.start[b], 0) : 0; }
+__device__ __forceinline__ Span paged_keys(const PagedArgs& a, int b, int at) { return paged_keys_from(a, first_key(a, b), at); }
 // id of the page of key j; minus one where it is not of the pool
 __device__ __forceinline__ int page_of(const PagedArgs& a, int b, int j) {
     const int id = a.tables[b * a.table_stride + (j >> a.shift)];
@@ -34,9 +36,15 @@ __device__ __forceinline__ Score paged_score(const PagedArgs& a, int h) {
     s.scale = a.scale; s.cap = a.cap; s.slopes = a.slopes;
     return Score(s, min(h, a.H - 1));
 }
-// packed rows of request b
+// Packed rows of a request [begin, end), the position of the first (minus one: they see nothing) and the first key that they see
+struct Request { int begin, end, at, first; };
 __device__ __forceinline__ int rows_begin(const PagedArgs& a, int b) { return min(max(a.starts[b], 0), a.N); }
 __device__ __forceinline__ int rows_end(const PagedArgs& a, int b) { return max(min(a.starts[b + 1], a.N), rows_begin(a, b)); }
+__device__ __forceinline__ Request request(const PagedArgs& a, int b) {
+    Request r = {rows_begin(a, b), rows_end(a, b), -1, first_key(a, b)};
+    if (r.end > r.begin) r.at = min(max(a.pos[r.begin], -1), 1 << 30);
+    return r;
+}
 // Rows of a tile: `heads` query heads (of the `chunks`-th part of a group) of `tokens` tokens, the heads of a token side by side
 struct RowShape { int heads, tokens; };                  // of a tile, or of a half of it
 

@@ -35,7 +35,7 @@ struct PagedMaps { CUtensorMap q, k, v; };
 // What the CTAs leave for the join: each the tile of rows that its end is the first to cut (tokens 0: none), and its parts, at most two: of the
 // tile that its share begins in, and of the one that it ends in
 struct Cut {
-    int b, row0, tokens, at0, first, h0, heads;
+    int row0, tokens, at0, first, h0, heads;
     int begun;                                           // the share that begins the tile begins with it
     int shares;                                          // CTAs that have a part of it
 };
@@ -54,21 +54,25 @@ struct RowTile {
     int row0, tokens, at0;                               // first packed row, its tokens, position of the first (minus one: they see nothing)
     int n0, n1;                                          // key tiles; one that nobody sees where there are none
 };
-__device__ __forceinline__ RowTile row_tile(const PagedArgs& a, const RowShape& rs, int b, int tile) {
-    const int begin = rows_begin(a, b), most = PA_HALVES * rs.tokens;
+__device__ __forceinline__ RowTile row_tile(const PagedArgs& a, const RowShape& rs, const Request& r, int tile) {
+    const int most = PA_HALVES * rs.tokens;
     RowTile t;
-    t.row0 = begin + tile * most;
-    t.tokens = min(most, rows_end(a, b) - t.row0);
-    const int at = a.pos[begin];
-    t.at0 = at < 0 ? -1 : min(at, 1 << 30) + tile * most;
+    t.row0 = r.begin + tile * most;
+    t.tokens = min(most, r.end - t.row0);
+    t.at0 = r.at < 0 ? -1 : r.at + tile * most;
     t.n0 = 0;
     t.n1 = 1;
-    if (at >= 0) {
-        const int lo = paged_keys(a, b, t.at0).lo, hi = paged_keys(a, b, t.at0 + t.tokens - 1).hi;
+    if (r.at >= 0) {
+        const int lo = paged_keys_from(a, r.first, t.at0).lo, hi = paged_keys_from(a, r.first, t.at0 + t.tokens - 1).hi;
         if (hi > lo) { t.n0 = lo / PA_KEYS; t.n1 = (hi + PA_KEYS - 1) / PA_KEYS; }
     }
     return t;
 }
+// The first requests, kept in shared memory: a CTA looks them up again and again while it finds its share
+struct Requests {
+    Request* kept;                                       // PA_THREADS
+    __device__ __forceinline__ Request at(const PagedArgs& a, int b) const { return b < PA_THREADS ? kept[b] : request(a, b); }
+};
 // A place in the line, and what of it lies ahead.  A tile of rows takes PA_TILE_COST steps of the line before its key tiles do.
 struct LineCursor {
     int b, tile, pair, n;                                // pair: key head and chunk of its query heads; n: steps of the tile passed
@@ -78,44 +82,45 @@ struct LineCursor {
     // the steps of the current tile that are this CTA's, and the key tile that step n begins with
     __device__ __forceinline__ int piece() const { return (int)min((long long)(steps() - n), left); }
     __device__ __forceinline__ int key(int n) const { return t.n0 + max(n - PA_TILE_COST, 0); }
-    __device__ __forceinline__ void next_tile(const PagedArgs& a, const RowShape& rs) {
+    __device__ __forceinline__ void next_tile(const PagedArgs& a, const RowShape& rs, const Requests& all) {
         n = 0;
         if (++pair < a.KV * a.chunks) return;
         pair = 0;
         tile++;
-        while (rows_begin(a, b) + (long long)tile * PA_HALVES * rs.tokens >= rows_end(a, b)) {
+        Request r = all.at(a, b);
+        while (tile * PA_HALVES * rs.tokens >= r.end - r.begin) {
             tile = 0;
             if (++b >= a.B) return;
+            r = all.at(a, b);
         }
-        t = row_tile(a, rs, b, tile);
+        t = row_tile(a, rs, r, tile);
     }
-    __device__ __forceinline__ void next_piece(const PagedArgs& a, const RowShape& rs) {
+    __device__ __forceinline__ void next_piece(const PagedArgs& a, const RowShape& rs, const Requests& all) {
         const int p = piece();
         n += p;
         left -= p;
-        if (left > 0 && n == steps()) next_tile(a, rs);
+        if (left > 0 && n == steps()) next_tile(a, rs, all);
     }
 };
 
-__device__ __forceinline__ long long line_sum(long long v, long long* s_sum) {     // inclusive over the CTA's threads, kept in s_sum
+// inclusive over the CTA's threads, kept in s_sum; s_warp: a place for each warp, of this call alone
+template <typename T>
+__device__ __forceinline__ void line_sum(T v, T* s_sum, T* s_warp) {
     const int tid = threadIdx.x, lane = tid & 31;
 #pragma unroll
     for (int off = 1; off < 32; off *= 2) {
-        const long long up = __shfl_up_sync(FULL, v, off);
+        const T up = __shfl_up_sync(FULL, v, off);
         if (lane >= off) v += up;
     }
+    if (lane == 31) s_warp[tid / 32] = v;
     __syncthreads();
+    for (int i = 0; i < tid / 32; i++) v += s_warp[i];
     s_sum[tid] = v;
     __syncthreads();
-    long long base = 0;
-    for (int i = 0; i < tid / 32; i++) base += s_sum[32 * i + 31];
-    __syncthreads();
-    s_sum[tid] = v + base;
-    __syncthreads();
-    return v + base;
 }
-__device__ __forceinline__ int first_above(const long long* s_sum, int threads, long long x) {      // first thread whose sum is greater
-    int lo = 0, hi = threads - 1;
+template <typename T>
+__device__ __forceinline__ int first_above(const T* s_sum, T x) {                  // first thread whose sum is greater
+    int lo = 0, hi = PA_THREADS - 1;
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
         if (s_sum[mid] > x) hi = mid; else lo = mid + 1;
@@ -123,52 +128,48 @@ __device__ __forceinline__ int first_above(const long long* s_sum, int threads, 
     return lo;
 }
 // The CTA's share of the line, by all its threads
-template <int THREADS>
-__device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& rs, long long most_tiles, LineCursor* out, long long* out_per) {
-    __shared__ long long s_tiles[THREADS], s_steps[THREADS];
+__device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& rs, int most_tiles, const Requests& all, LineCursor* out, long long* out_per) {
+    __shared__ int s_tiles[PA_THREADS], s_warp0[PA_THREADS / 32];
+    __shared__ long long s_steps[PA_THREADS], s_warp1[PA_THREADS / 32];
     const int tid = threadIdx.x, most = PA_HALVES * rs.tokens, pairs = a.KV * a.chunks;
-    auto tiles_of = [&](int b) { return (rows_end(a, b) - rows_begin(a, b) + most - 1) / most; };
-    const int per_b = (a.B + THREADS - 1) / THREADS, b0 = min(tid * per_b, a.B), b1 = min(b0 + per_b, a.B);
-    long long v = 0;
-    for (int b = b0; b < b1; b++) v += tiles_of(b);
-    line_sum(v, s_tiles);
-    const long long tiles = min(s_tiles[THREADS - 1], most_tiles), per_u = (tiles + THREADS - 1) / THREADS;
-    // request and tile of the u-th tile of rows
-    auto find = [&](long long u, int& b, int& tile) {
-        const int t = first_above(s_tiles, THREADS, u);
-        b = t * per_b;
-        long long in = u - (t > 0 ? s_tiles[t - 1] : 0);
-        for (int n = tiles_of(b); in >= n; n = tiles_of(b)) { in -= n; b++; }
-        tile = (int)in;
-    };
-    auto walk = [&](long long u0, long long u1, auto each) {
+    if (tid < a.B) all.kept[tid] = request(a, tid);
+    __syncthreads();
+    auto tiles_of = [&](const Request& r) { return (r.end - r.begin + most - 1) / most; };
+    const int per_b = (a.B + PA_THREADS - 1) / PA_THREADS, b0 = min(tid * per_b, a.B), b1 = min(b0 + per_b, a.B);
+    int n = 0;
+    for (int b = b0; b < b1; b++) n = min(n + tiles_of(all.at(a, b)), most_tiles);                   // more there are not, unless starts falls
+    line_sum(n, s_tiles, s_warp0);
+    const int tiles = min(s_tiles[PA_THREADS - 1], most_tiles), per_u = (tiles + PA_THREADS - 1) / PA_THREADS;
+    auto walk = [&](int u0, int u1, auto each) {         // tiles of rows [u0, u1)
         if (u0 >= u1) return;
-        int b, tile;
-        find(u0, b, tile);
-        for (long long u = u0; u < u1; u++) {
-            const RowTile t = row_tile(a, rs, b, tile);
-            if (!each(u, b, tile, t)) return;
-            if (++tile >= tiles_of(b) && u + 1 < u1) { tile = 0; do b++; while (tiles_of(b) == 0); }
+        const int t = first_above(s_tiles, u0);
+        int b = t * per_b, tile = u0 - (t > 0 ? s_tiles[t - 1] : 0);
+        Request r = all.at(a, b);
+        for (int k = tiles_of(r); tile >= k; k = tiles_of(r)) { tile -= k; r = all.at(a, ++b); }
+        for (int u = u0; u < u1; u++) {
+            if (!each(b, tile, row_tile(a, rs, r, tile))) return;
+            if (++tile >= tiles_of(r) && u + 1 < u1) {
+                tile = 0;
+                do r = all.at(a, ++b); while (r.end == r.begin);
+            }
         }
     };
-    const long long u0 = min(tid * per_u, tiles), u1 = min(u0 + per_u, tiles);
-    v = 0;
-    walk(u0, u1, [&](long long, int, int, const RowTile& t) { v += PA_TILE_COST + t.n1 - t.n0; return true; });
-    line_sum(v, s_steps);
-    const long long total = s_steps[THREADS - 1] * pairs, per = (total + gridDim.x - 1) / gridDim.x;
-    const long long x0 = blockIdx.x * per, x1 = min(x0 + per, total);
+    long long v = 0;
+    walk(min(tid * per_u, tiles), min((tid + 1) * per_u, tiles), [&](int, int, const RowTile& t) { v += PA_TILE_COST + t.n1 - t.n0; return true; });
+    line_sum(v, s_steps, s_warp1);
     if (tid == 0) {
+        const long long total = s_steps[PA_THREADS - 1] * pairs, per = (total + gridDim.x - 1) / gridDim.x, x0 = blockIdx.x * per;
         LineCursor c = {};
-        c.left = max(x1 - x0, 0ll);
+        c.left = max(min(per, total - x0), 0ll);
         if (c.left > 0) {
-            const int t = first_above(s_steps, THREADS, x0 / pairs);
-            long long at = t > 0 ? s_steps[t - 1] : 0;
-            walk(t * per_u, tiles, [&](long long, int b, int tile, const RowTile& rt) {
+            const int t = first_above(s_steps, x0 / pairs);
+            long long at = (t > 0 ? s_steps[t - 1] : 0) * pairs;
+            walk(t * per_u, tiles, [&](int b, int tile, const RowTile& rt) {
                 const int steps = PA_TILE_COST + rt.n1 - rt.n0;
-                if ((at + steps) * pairs <= x0) { at += steps; return true; }
+                if (at + (long long)steps * pairs <= x0) { at += (long long)steps * pairs; return true; }
                 c.b = b; c.tile = tile; c.t = rt;
-                c.pair = (int)((x0 - at * pairs) / steps);
-                c.n = (int)((x0 - at * pairs) % steps);
+                c.pair = (int)((x0 - at) / steps);
+                c.n = (int)((x0 - at) % steps);
                 return false;
             });
         }
@@ -191,8 +192,18 @@ struct Piece {
     int last;
 };
 constexpr int PA_PIECES = 4;
+// Tiles of a piece in the ring: keys and values in turn.  Of a twin the keys come one tile earlier, as they are used: k0 k1 v0 k2 v1 k3 ...
+__device__ __forceinline__ unsigned twin_key(unsigned i) { return i < 2 ? i : 2 * i - 1; }
+__device__ __forceinline__ unsigned twin_value(unsigned i, unsigned n) { return i + 1 == n ? 2 * n - 1 : 2 * i + 2; }
+struct RingTile { int i; bool value; };                  // the inverse: what stands at a place
+__device__ __forceinline__ RingTile ring_tile(bool twin, int place, int n) {
+    if (!twin) return {place / 2, (place & 1) != 0};
+    if (place < 2) return {place, false};
+    if (place == 2 * n - 1) return {n - 1, true};
+    return place & 1 ? RingTile{(place + 1) / 2, false} : RingTile{(place - 2) / 2, true};
+}
 
-__device__ __forceinline__ Piece make_piece(const PagedArgs& a, const RowShape& rs, const LineCursor& c, bool begun) {
+__device__ __forceinline__ Piece make_piece(const PagedArgs& a, const RowShape& rs, const LineCursor& c, int first, bool begun) {
     Piece p;
     p.b = c.b;
     p.hk = c.pair / a.chunks;
@@ -200,16 +211,16 @@ __device__ __forceinline__ Piece make_piece(const PagedArgs& a, const RowShape& 
     p.h0 = p.hk * group + g0;
     p.heads = min(rs.heads, group - g0);
     p.row0 = c.t.row0; p.tokens = c.t.tokens; p.at0 = c.t.at0;
-    p.first = a.start != nullptr ? max(a.start[c.b], 0) : 0;
+    p.first = first;
     p.n0 = c.key(c.n);
     p.n1 = c.key(c.n + c.piece());
-    p.lo = paged_keys(a, c.b, c.t.at0).lo;
-    p.hi = paged_keys(a, c.b, c.t.at0 < 0 ? -1 : c.t.at0 + c.t.tokens - 1).hi;
+    p.lo = paged_keys_from(a, first, c.t.at0).lo;
+    p.hi = paged_keys_from(a, first, c.t.at0 < 0 ? -1 : c.t.at0 + c.t.tokens - 1).hi;
     for (int t = 0; t < PA_HALVES; t++) {
         const int at = t * rs.tokens, n = min(rs.tokens, p.tokens - at);
         p.from[t] = p.to[t] = p.n0;
         if (n <= 0 || p.at0 < 0) continue;
-        const int lo = paged_keys(a, c.b, p.at0 + at).lo, hi = paged_keys(a, c.b, p.at0 + at + n - 1).hi;
+        const int lo = paged_keys_from(a, first, p.at0 + at).lo, hi = paged_keys_from(a, first, p.at0 + at + n - 1).hi;
         const int from = max(lo / PA_KEYS, p.n0), to = min((hi + PA_KEYS - 1) / PA_KEYS, p.n1);
         if (hi > lo && to > from) { p.from[t] = from; p.to[t] = to; }
     }
@@ -236,6 +247,8 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
     __shared__ int s_fail;
     __shared__ LineCursor s_at;
     __shared__ long long s_per;
+    __shared__ Request s_request[PA_THREADS];
+    const Requests all = {s_request};
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     if (tid == 0) {
         mbar_init(&q_full, 1); mbar_init(&q_empty, 1); mbar_init(&merge_full, 4); mbar_init(&merge_empty, 4);
@@ -251,7 +264,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
         prefetch_map(&maps.k);
         prefetch_map(&maps.v);
     }
-    line_share<PA_THREADS>(a, rs, plan.most, &s_at, &s_per);
+    line_share(a, rs, (int)plan.most, all, &s_at, &s_per);
     {                                                    // rows of no request
         const int r0 = a.B > 0 ? rows_begin(a, 0) : a.N, r1 = a.B > 0 ? max(rows_end(a, a.B - 1), r0) : a.N;
         const long long pieces = (long long)a.H * a.D / 8, n = (long long)(r0 + a.N - r1) * pieces;
@@ -276,9 +289,9 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
         if (lane == 0) arrive(&piece_empty[turn % PA_PIECES]);
         turn++;
     };
-    // 3 x 128 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72; a row of 128 scores stays in registers
+    // 3 x 128 threads x 168 registers at launch = 2 x 128 x 200 + 128 x 104 (with 72 the product warp spilled)
     if (warp < PA_HALVES * 4) {                          // ---- softmax of a half ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int half = tid / 128, r = tid % 128, token = r / rs.heads, g = r % rs.heads;
         const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
         const uint32_t S = tmem + half * PA_KEYS + lane_at, O = tmem + PA_HALVES * PA_KEYS + half * DP + lane_at;
@@ -289,39 +302,63 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
             const int tk = (p.twin ? 0 : half) * rs.tokens + token;                // of the tile
             const bool row = token < rs.tokens && tk < p.tokens && g < p.heads;
             const int where = p.at0 + tk;
-            const Span sp = row && p.at0 >= 0 ? Span{a.window > 0 && where >= a.window ? max(p.first, where - a.window + 1) : p.first, min(where, (a.M << a.shift) - 1) + 1}
-                                              : Span{0, 0};
-            const WarpSpan ws(sp);
+            const Span sp = row && p.at0 >= 0 ? paged_keys_from(a, p.first, where) : Span{0, 0};
+            const WarpSpan ws(row ? sp : Span{0, BIGI});  // rows that are none ask for no mask
             const Score sc = paged_score(a, p.h0 + g);
             const int by = p.twin ? 2 : 1, n_first = p.twin ? p.from[0] + half : p.from[half], n_last = p.twin ? p.to[0] : p.to[half];
             const int all_lo = p.lo, all_hi = p.hi, n_base = p.n0;
             float m = -INFINITY, l = 0.f;                // m in base-2 exponents
             const float at = (float)where;
+            const bool rows_here = __any_sync(FULL, row);                          // of this warp
             for (int n = n_first; n < n_last; n += by, done++) {
                 const int j0 = n * PA_KEYS;
                 const bool masked = !ws.clear(j0, PA_KEYS);
+                const bool edge = j0 < all_lo || j0 + PA_KEYS > all_hi;
                 if (!wait_soon_warp(&s_full[half], done & 1)) { failed = true; break; }
-                tmem_fence_after();
-                uint32_t raw[PA_KEYS / 32][32];
-#pragma unroll
-                for (int i = 0; i < PA_KEYS / 32; i++) tmem_ld(S + i * 32, raw[i]);
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < PA_KEYS / 32; i++) {
-                    tmem_ld_wait(raw[i]);
-                    float(&s)[32] = reinterpret_cast<float(&)[32]>(raw[i]);
-                    scores32<CAP, BIAS>(s, sc, at - (float)(j0 + i * 32), masked, sp.lo - j0 - i * 32, sp.hi - j0 - i * 32);
-                    float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
-#pragma unroll
-                    for (int e = 4; e < 32; e += 4) { t0 = fmaxf(t0, s[e]); t1 = fmaxf(t1, s[e + 1]); t2 = fmaxf(t2, s[e + 2]); t3 = fmaxf(t3, s[e + 3]); }
-                    top = fmaxf(top, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
+                if (!rows_here && !edge) {               // products of rows that are none: whatever stands there
+                    if (lane == 0) arrive(&p_full[half]);
+                    continue;
                 }
-                if constexpr (!CAP && !BIAS) top *= sc.lin;
-                const bool grown = top > m + PA_GROWN && m != -INFINITY;           // a row that has seen nothing so far has only zeros to rescale
-                if (m == -INFINITY) m = top;
-                if (__any_sync(FULL, grown)) {
-                    const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2_fast(m - to);
-                    if (n > n_first) {
+                tmem_fence_after();
+                // The weights are taken relative to the maximum so far, and the new one is found beside them; only where it has grown too
+                // much (or the row begins) are they taken once more, out of the scores that still stand in tensor memory.
+                uint32_t w[PA_KEYS / 2];
+                float total;
+                while (true) {
+                    float top = -INFINITY;
+                    const float base = m == -INFINITY ? 0.f : m;
+                    f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+                    const f32x2 lin = pack2(sc.lin, sc.lin), back = pack2(-base, -base);
+                    uint32_t raw[2][32];
+                    tmem_ld(S, raw[0]);
+#pragma unroll
+                    for (int i = 0; i < PA_KEYS / 32; i++) {
+                        uint32_t(&x)[32] = raw[i % 2];
+                        tmem_ld_wait(x);
+                        if (i + 1 < PA_KEYS / 32) tmem_ld(S + (i + 1) * 32, raw[(i + 1) % 2]);
+                        float(&s)[32] = reinterpret_cast<float(&)[32]>(x);
+                        scores32<CAP, BIAS>(s, sc, at - (float)(j0 + i * 32), masked, sp.lo - j0 - i * 32, sp.hi - j0 - i * 32);
+                        float t0 = s[0], t1 = s[1];
+#pragma unroll
+                        for (int e = 2; e < 32; e += 4) { t0 = fmaxf(fmaxf(t0, s[e]), s[e + 1]); if (e + 2 < 32) t1 = fmaxf(fmaxf(t1, s[e + 2]), s[e + 3]); }
+                        top = fmaxf(top, fmaxf(t0, t1));
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const f32x2 y = pack2(s[e], s[e + 1]);
+                            const float2 z = unpack2(CAP || BIAS ? add2(y, back) : fma2(y, lin, back));
+                            const float p0 = exp2_fast(z.x), p1 = exp2_fast(z.y);
+                            sum[(e / 2) % 2] = add2(sum[(e / 2) % 2], pack2(p0, p1));
+                            w[i * 16 + e / 2] = pack_bf16(p0, p1);
+                        }
+                    }
+                    if constexpr (!CAP && !BIAS) top *= sc.lin;
+                    const float2 both = unpack2(add2(sum[0], sum[1]));
+                    total = both.x + both.y;
+                    const bool grown = row && top > m + PA_GROWN;                         // minus infinity: a row begins
+                    if (!__any_sync(FULL, grown)) break;
+                    const float to = fmaxf(m, top);
+                    if (__any_sync(FULL, m != -INFINITY) && n > n_first) {         // a row that has seen nothing so far has only zeros to rescale
+                        const float f = m == -INFINITY ? 1.f : exp2_fast(m - to);
                         if (!wait_soon_warp(&o_full[half], (done - 1) & 1)) { failed = true; break; }
                         tmem_fence_after();
 #pragma unroll
@@ -333,31 +370,17 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                             for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
                             tmem_st(O + i * 32, y);
                         }
+                        l *= f;
                     }
                     m = to;
-                    l *= f;
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-                const f32x2 lin = pack2(sc.lin, sc.lin), back = pack2(-base, -base);
+                if (failed) break;
+                l += total;
 #pragma unroll
-                for (int i = 0; i < PA_KEYS / 32; i++) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const f32x2 y = pack2(__uint_as_float(raw[i][e]), __uint_as_float(raw[i][e + 1]));
-                        const float2 z = unpack2(CAP || BIAS ? add2(y, back) : fma2(y, lin, back));
-                        const float p0 = exp2_fast(z.x), p1 = exp2_fast(z.y);
-                        sum[(e / 2) % 2] = add2(sum[(e / 2) % 2], pack2(p0, p1));
-                        w[e / 2] = pack_bf16(p0, p1);
-                    }
-                    tmem_st(S + i * 16, w);
-                }
-                const float2 total = unpack2(add2(sum[0], sum[1]));
-                l += total.x + total.y;
-                if (j0 < all_lo || j0 + PA_KEYS > all_hi) {
+                for (int i = 0; i < PA_KEYS / 32; i++) tmem_st(S + i * 16, reinterpret_cast<const uint32_t(&)[16]>(w[16 * i]));
+                if (edge) {
                     // values that no row of the tile sees (the rest of a page, another request's) must not reach the product: zeros
-                    const unsigned xv = x0 + 2 * (n - n_base) + 1, s = xv % PA_STAGES;
+                    const unsigned xv = x0 + (p.twin ? twin_value(n - n_base, p.n1 - n_base) : 2 * (n - n_base) + 1), s = xv % PA_STAGES;
                     if (!wait_soon_warp(&full[s], (xv / PA_STAGES) & 1)) { failed = true; break; }
                     if (j0 + r < all_lo || j0 + r >= all_hi) {
 #pragma unroll
@@ -398,7 +421,14 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 const unsigned rows = __ballot_sync(FULL, row);
                 // rows of 64 bytes through shared memory, so that a store covers 8 of them and not 32
                 const uint32_t out = smem_u32(smem + PA_HALVES * Sh::QTILE + PA_STAGES * Sh::KTILE) + warp * PA_OUT;
-                auto put = [&](const uint32_t (&w)[16], auto store) {
+                size_t to[4];                            // where this lane's four rows of the warp go
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int x = r - lane + e * 8 + lane / 4, xt = x / rs.heads;
+                    to[e] = p.cut ? (size_t)(pr - r + x) * a.D : ((size_t)(p.row0 + tk - token + xt) * a.H + p.h0 + x - xt * rs.heads) * a.D;
+                }
+                auto put = [&](const uint32_t (&w)[16], auto* base, int d) {       // channels from d on
+                    typedef typename std::remove_reference<decltype(*base)>::type E;
 #pragma unroll
                     for (int e = 0; e < 4; e++) st_shared16(out + lane * PA_OUT_ROW + e * 16, w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
                     __syncwarp();
@@ -406,7 +436,8 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     for (int e = 0; e < 4; e++) {
                         const int x = e * 8 + lane / 4;  // row of the warp
                         const uint4 v = ld_shared16(out + x * PA_OUT_ROW + (lane % 4) * 16);
-                        if (rows >> x & 1) store(r - lane + x, lane % 4, v);
+                        if ((rows >> x & 1) && d + (lane % 4) * (16 / (int)sizeof(E)) < a.D)
+                            *reinterpret_cast<uint4*>(base + to[e] + d + (lane % 4) * (16 / (int)sizeof(E))) = v;
                     }
                     __syncwarp();
                 };
@@ -429,19 +460,13 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     if (p.cut) {
 #pragma unroll
                         for (int s = 0; s < 2; s++)
-                            put(reinterpret_cast<const uint32_t(&)[16]>(y[16 * s]), [&](int x, int piece, uint4 v) {
-                                const int d = i * 32 + s * 16 + piece * 4;
-                                if (d < a.D) *reinterpret_cast<uint4*>(part + (size_t)(pr - r + x) * a.D + d) = v;
-                            });
+                            put(reinterpret_cast<const uint32_t(&)[16]>(y[16 * s]), part, i * 32 + s * 16);
                     } else {
                         uint32_t w[16];
 #pragma unroll
                         for (int e = 0; e < 16; e++)
                             w[e] = none ? 0u : pack_bf16(__uint_as_float(y[2 * e]) * inv, __uint_as_float(y[2 * e + 1]) * inv);
-                        put(w, [&](int x, int piece, uint4 v) {
-                            const int d = i * 32 + piece * 8, xt = x / rs.heads;
-                            if (d < a.D) *reinterpret_cast<uint4*>(o + ((size_t)(p.row0 + tk - token + xt) * a.H + p.h0 + x - xt * rs.heads) * a.D + d) = v;
-                        });
+                        put(w, o, i * 32);
                     }
                 }
                 if (p.cut && row) *reinterpret_cast<float2*>(part + (size_t)PA_ROWS * a.D + 2 * pr) = make_float2(fmaxf(m, -FLT_MAX), l);
@@ -471,7 +496,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
         }
         if (failed) s_fail = 1;
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == PA_HALVES * 4 + 2) {                 // ---- pieces ----
             LineCursor c = s_at;
             Cut cut = {};
@@ -479,18 +504,18 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 const unsigned slot = turn % PA_PIECES;
                 const int steps = c.piece();
                 const bool whole_left = c.n + steps == c.steps();
-                Piece p = make_piece(a, rs, c, begun);
+                Piece p = make_piece(a, rs, c, all.at(a, c.b).first, begun);
                 ok = c.left - steps > (whole_left ? PA_TILE_COST : 0);
                 p.last = !ok;
                 if (!whole_left && p.n0 == c.t.n0)
-                    cut = {p.b, p.row0, p.tokens, p.at0, p.first, p.h0, p.heads, begun, 1 + (int)((c.steps() - c.n - steps + s_per - 1) / s_per)};
+                    cut = {p.row0, p.tokens, p.at0, p.first, p.h0, p.heads, begun, 1 + (int)((c.steps() - c.n - steps + s_per - 1) / s_per)};
                 if (turn >= PA_PIECES && !wait_soon_warp(&piece_empty[slot], (turn / PA_PIECES - 1) & 1)) { failed = true; break; }
                 if (lane == 0) {
                     s_piece[slot] = p;
                     arrive(&piece_full[slot]);
                 }
                 __syncwarp();
-                c.next_piece(a, rs);
+                c.next_piece(a, rs, all);
             }
             if (lane == 0) plan.cuts[blockIdx.x] = cut;
             if (failed && lane == 0) s_fail = 1;
@@ -503,33 +528,37 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
             while (ok) {
                 const Piece& p = next();
                 if (failed) break;
-                auto id_of = [&](int n) {                // a page outside the pool, or beyond the table: zeros
-                    const int j = n * PA_KEYS + box * rows;
-                    return mine && n < p.n1 && (j >> a.shift) < a.M ? max(page_of(a, p.b, j), -1) : -1;
+                const int n = p.n1 - p.n0;
+                const bool twin = p.twin != 0;
+                auto id_of = [&](int place) {            // a page outside the pool, or beyond the table: zeros
+                    const int j = (p.n0 + ring_tile(twin, place, n).i) * PA_KEYS + box * rows;
+                    return mine && place < 2 * n && (j >> a.shift) < a.M ? max(page_of(a, p.b, j), -1) : -1;
                 };
-                int id = id_of(p.n0);
-                for (int n = p.n0; n < p.n1 && !failed; n++) {
-                    const int then = id_of(n + 1);
-                    for (int w = 0; w < 2; w++, x++) {   // keys, values
-                        const unsigned s = x % PA_STAGES, round = x / PA_STAGES;
-                        if (round > 0 && !wait_soon_warp(&empty[s], (round - 1) & 1)) { failed = true; break; }
-                        if (lane == 0) mbar_arrive_expect_tx(&full[s], Sh::KTILE);
-                        __syncwarp();
-                        if (mine)
-                            tile_g2s(Ks + s * Sh::KTILE + sub * PA_KEYS * 128 + box * rows * 128, w ? &maps.v : &maps.k, sub * 64,
-                                     (n * PA_KEYS + box * rows) & ((1 << a.shift) - 1), p.hk, id, &full[s]);
-                    }
+                int id = id_of(0);
+                auto queries = [&] {
+                    if (lane != 0) return;
+                    const int halves = p.tokens > rs.tokens ? 2 : 1;
+                    mbar_arrive_expect_tx(&q_full, halves * Sh::SUBS * rs.heads * rs.tokens * 128);
+                    for (int t = 0; t < halves; t++)
+                        for (int s = 0; s < Sh::SUBS; s++)
+                            box_g2s(Qs + t * Sh::QTILE + s * 128 * 128, &maps.q, s * 64, p.h0, p.row0 + t * rs.tokens, &q_full);
+                };
+                if (turn == 0) queries();
+                for (int place = 0; place < 2 * n; place++, x++) {
+                    const int then = id_of(place + 1);
+                    const RingTile t = ring_tile(twin, place, n);
+                    const unsigned s = x % PA_STAGES, round = x / PA_STAGES;
+                    if (round > 0 && !wait_soon_warp(&empty[s], (round - 1) & 1)) { failed = true; break; }
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], Sh::KTILE);
+                    __syncwarp();
+                    if (mine)
+                        tile_g2s(Ks + s * Sh::KTILE + sub * PA_KEYS * 128 + box * rows * 128, t.value ? &maps.v : &maps.k, sub * 64,
+                                 ((p.n0 + t.i) * PA_KEYS + box * rows) & ((1 << a.shift) - 1), p.hk, id, &full[s]);
                     id = then;
-                    if (n > p.n0) continue;
-                    // the queries, whose place is the last piece's until its scores are done, behind the first keys and values
-                    if (turn > 0 && !wait_soon_warp(&q_empty, (turn - 1) & 1)) { failed = true; break; }
-                    if (lane == 0) {
-                        const int halves = p.tokens > rs.tokens ? 2 : 1;
-                        mbar_arrive_expect_tx(&q_full, halves * Sh::SUBS * rs.heads * rs.tokens * 128);
-                        for (int t = 0; t < halves; t++)
-                            for (int s = 0; s < Sh::SUBS; s++)
-                                box_g2s(Qs + t * Sh::QTILE + s * 128 * 128, &maps.q, s * 64, p.h0, p.row0 + t * rs.tokens, &q_full);
-                    }
+                    if (place != 1 || turn == 0) continue;
+                    // the queries, whose place is the last piece's until its scores are done, behind the first two tiles
+                    if (!wait_soon_warp(&q_empty, (turn - 1) & 1)) { failed = true; break; }
+                    queries();
                 }
                 if (failed) break;
                 passed(p);
@@ -537,7 +566,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
             if (failed && lane == 0) s_fail = 1;
         } else if (warp == PA_HALVES * 4) {              // ---- products ----
             const bool lead = elected();
-            unsigned x = 0, done[PA_HALVES] = {0, 0};
+            unsigned x = 0, phase = 0;                       // phase: a bit to a half, the parity of its weights' next hand-over
             auto stage = [](unsigned i) { return i % PA_STAGES; };
             auto arrived = [&](unsigned i) { failed = failed || !wait_soon_warp(&full[stage(i)], (i / PA_STAGES) & 1); return !failed; };
             auto scores = [&](int t, int tile, unsigned i) {                       // s = q k^T of a half, with the queries of tile 0 or 1
@@ -552,9 +581,9 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 __syncwarp();
             };
             auto outputs = [&](int t, unsigned i, bool add) {                      // o += p v of a half
-                failed = failed || !wait_soon_warp(&p_full[t], done[t] & 1);
+                failed = failed || !wait_soon_warp(&p_full[t], phase >> t & 1);
                 if (failed) return;
-                done[t]++;
+                phase ^= 1u << t;
                 tmem_fence_after();
                 const uint32_t vd = tile_desc(smem_u32(Ks + stage(i) * Sh::KTILE), PA_KEYS * 128);
                 if (lead) {
@@ -575,16 +604,19 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 if (failed) break;
                 const int n0 = p.n0, n1 = p.n1, from[PA_HALVES] = {p.from[0], p.from[1]}, to[PA_HALVES] = {p.to[0], p.to[1]};
                 if (p.twin) {                            // p.from[0] is n0 and p.to[0] n1: all its key tiles are seen by some row
-                    if (arrived(x)) { scores(0, 0, x); used(x); }
-                    if (arrived(x + 2)) { scores(1, 0, x + 2); used(x + 2); }
-                    if (n0 + 2 == n1 && lead) mma_commit(&q_empty);
-                    for (int n = n0; n < n1 && arrived(x + 1); n++, x += 2) {
-                        const int t = (n - n0) & 1;
-                        outputs(t, x + 1, n >= n0 + 2);
-                        used(x + 1);
-                        if (n + 2 < n1 && arrived(x + 4)) { scores(t, 0, x + 4); used(x + 4); }
-                        if (n + 3 == n1 && lead) mma_commit(&q_empty);
+                    const unsigned n = n1 - n0;
+                    for (unsigned i = 0; i < 2; i++)
+                        if (arrived(x + i)) { scores(i, 0, x + i); used(x + i); }
+                    if (n == 2 && lead) mma_commit(&q_empty);
+                    for (unsigned i = 0; i < n; i++) {
+                        const unsigned v = x + twin_value(i, n), k = x + twin_key(i + 2);
+                        if (!arrived(v)) break;
+                        outputs(i & 1, v, i >= 2);
+                        used(v);
+                        if (i + 2 < n && arrived(k)) { scores(i & 1, 0, k); used(k); }
+                        if (i + 3 == n && lead) mma_commit(&q_empty);
                     }
+                    x += 2 * n;
                 } else {
                     arrived(x);
 #pragma unroll
@@ -626,7 +658,7 @@ __global__ void __launch_bounds__(256) line_join_kernel(PagedArgs a, RowShape rs
     for (int pr = blockIdx.y * LJ_ROWS + warp; pr < (blockIdx.y + 1) * LJ_ROWS; pr += 8) {
         const int half = pr / 128, r = pr % 128, token = r / rs.heads, g = r % rs.heads, tk = half * rs.tokens + token;
         if (token >= rs.tokens || tk >= c.tokens || g >= c.heads) continue;
-        const Span sp = c.at0 >= 0 ? paged_keys(a, c.b, c.at0 + tk) : Span{0, 0};
+        const Span sp = c.at0 >= 0 ? paged_keys_from(a, c.first, c.at0 + tk) : Span{0, 0};
         float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
         for (int s0 = 0; s0 < c.shares; s0 += 32) {
             const int n = min(c.shares - s0, 32);
