@@ -22,7 +22,9 @@ constexpr float PA_GROWN = 8.f;                          // in powers of two
 constexpr int PA_HALVES = 2, PA_KEYS = 128, PA_ROWS = PA_HALVES * 128;
 constexpr int PA_THREADS = PA_ROWS + 128;
 constexpr int PA_OUT_ROW = 64 + 16, PA_OUT = 32 * PA_OUT_ROW;             // bytes of a warp's outputs on their way: 64 of a row, and what keeps banks apart
-constexpr int PA_TILE_COST = 2;                          // of a tile of rows itself, in tiles of keys: its queries and its results
+// Steps of the line, as their times are: of a tile of keys with rows in both halves, in one, and of a tile of rows itself (its queries and
+// results)
+constexpr int PA_TWO = 3, PA_ONE = 2, PA_TILE_COST = 6;
 constexpr int PA_STAGES = 4;                             // tiles of the ring, keys and values in turn
 template <int DP>
 struct PagedShape {
@@ -68,20 +70,23 @@ __device__ __forceinline__ RowTile row_tile(const PagedArgs& a, const RowShape& 
     }
     return t;
 }
+__device__ __forceinline__ int step_cost(const RowShape& rs, const RowTile& t) { return t.tokens > rs.tokens ? PA_TWO : PA_ONE; }
 // The first requests, kept in shared memory: a CTA looks them up again and again while it finds its share
 struct Requests {
     Request* kept;                                       // PA_THREADS
     __device__ __forceinline__ Request at(const PagedArgs& a, int b) const { return b < PA_THREADS ? kept[b] : request(a, b); }
 };
-// A place in the line, and what of it lies ahead.  A tile of rows takes PA_TILE_COST steps of the line before its key tiles do.
+// A place in the line, and what of it lies ahead.  A tile of rows takes PA_TILE_COST steps of the line, then its key tiles theirs; a key
+// tile is the share's in which its last step lies.
 struct LineCursor {
     int b, tile, pair, n;                                // pair: key head and chunk of its query heads; n: steps of the tile passed
     long long left;
     RowTile t;
-    __device__ __forceinline__ int steps() const { return PA_TILE_COST + t.n1 - t.n0; }
-    // the steps of the current tile that are this CTA's, and the key tile that step n begins with
+    int each;                                            // steps of a key tile
+    __device__ __forceinline__ int steps() const { return PA_TILE_COST + (t.n1 - t.n0) * each; }
+    // the steps of the current tile that are this CTA's, and the key tiles whose last step is before the n-th
     __device__ __forceinline__ int piece() const { return (int)min((long long)(steps() - n), left); }
-    __device__ __forceinline__ int key(int n) const { return t.n0 + max(n - PA_TILE_COST, 0); }
+    __device__ __forceinline__ int key(int n) const { return t.n0 + max(n - PA_TILE_COST, 0) / each; }
     __device__ __forceinline__ void next_tile(const PagedArgs& a, const RowShape& rs, const Requests& all) {
         n = 0;
         if (++pair < a.KV * a.chunks) return;
@@ -94,6 +99,7 @@ struct LineCursor {
             r = all.at(a, b);
         }
         t = row_tile(a, rs, r, tile);
+        each = step_cost(rs, t);
     }
     __device__ __forceinline__ void next_piece(const PagedArgs& a, const RowShape& rs, const Requests& all) {
         const int p = piece();
@@ -155,19 +161,19 @@ __device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& r
         }
     };
     long long v = 0;
-    walk(min(tid * per_u, tiles), min((tid + 1) * per_u, tiles), [&](int, int, const RowTile& t) { v += PA_TILE_COST + t.n1 - t.n0; return true; });
+    walk(min(tid * per_u, tiles), min((tid + 1) * per_u, tiles), [&](int, int, const RowTile& t) { v += PA_TILE_COST + (t.n1 - t.n0) * step_cost(rs, t); return true; });
     line_sum(v, s_steps, s_warp1);
     if (tid == 0) {
-        const long long total = s_steps[PA_THREADS - 1] * pairs, per = (total + gridDim.x - 1) / gridDim.x, x0 = blockIdx.x * per;
+        const long long total = s_steps[PA_THREADS - 1] * pairs, per = max((total + gridDim.x - 1) / gridDim.x, (long long)PA_TWO), x0 = blockIdx.x * per;     // a key tile to each
         LineCursor c = {};
         c.left = max(min(per, total - x0), 0ll);
         if (c.left > 0) {
             const int t = first_above(s_steps, x0 / pairs);
             long long at = (t > 0 ? s_steps[t - 1] : 0) * pairs;
             walk(t * per_u, tiles, [&](int b, int tile, const RowTile& rt) {
-                const int steps = PA_TILE_COST + rt.n1 - rt.n0;
+                const int each = step_cost(rs, rt), steps = PA_TILE_COST + (rt.n1 - rt.n0) * each;
                 if (at + (long long)steps * pairs <= x0) { at += (long long)steps * pairs; return true; }
-                c.b = b; c.tile = tile; c.t = rt;
+                c.b = b; c.tile = tile; c.t = rt; c.each = each;
                 c.pair = (int)((x0 - at) / steps);
                 c.n = (int)((x0 - at) % steps);
                 return false;
@@ -189,7 +195,7 @@ struct Piece {
     int from[PA_HALVES], to[PA_HALVES];                  // key tiles of each half
     int cut, begun;                                      // it has not all key tiles of its tile; it begins the share
     int twin;                                            // rows for one half alone: both take them, each every other key tile
-    int last;
+    int stop;                                            // nothing more
 };
 constexpr int PA_PIECES = 4;
 // Tiles of a piece in the ring: keys and values in turn.  Of a twin the keys come one tile earlier, as they are used: k0 k1 v0 k2 v1 k3 ...
@@ -227,7 +233,7 @@ __device__ __forceinline__ Piece make_piece(const PagedArgs& a, const RowShape& 
     p.cut = p.n0 > c.t.n0 || p.n1 < c.t.n1;
     p.begun = begun;
     p.twin = p.tokens <= rs.tokens && p.to[0] - p.from[0] >= 2;
-    p.last = 0;
+    p.stop = 0;
     return p;
 }
 
@@ -254,7 +260,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
         mbar_init(&q_full, 1); mbar_init(&q_empty, 1); mbar_init(&merge_full, 4); mbar_init(&merge_empty, 4);
         for (int t = 0; t < PA_HALVES; t++) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); }
         for (int s = 0; s < PA_STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < PA_PIECES; s++) { mbar_init(&piece_full[s], 1); mbar_init(&piece_empty[s], PA_HALVES * 4 + 2); }
+        for (int s = 0; s < PA_PIECES; s++) { mbar_init(&piece_full[s], 1); mbar_init(&piece_empty[s], PA_HALVES * 4 + 3); }
         mbar_fence_init();
         s_fail = 0;
     }
@@ -277,14 +283,13 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
     __syncthreads();
     tmem_fence_after();
     constexpr uint32_t tmem = 0;                         // all 512 columns are this CTA's, so they begin at the first
-    bool ok = s_at.n + s_at.left > PA_TILE_COST, failed = false;                   // ok: there is a next piece (of a tile's own cost alone there is nothing to do)
+    bool failed = false;
     unsigned turn = 0;                                   // pieces so far
     auto next = [&]() -> const Piece& {                  // waits for the piece; `failed` where none came
         failed = failed || !wait_soon_warp(&piece_full[turn % PA_PIECES], (turn / PA_PIECES) & 1);
         return s_piece[turn % PA_PIECES];
     };
-    auto passed = [&](const Piece& p) {                  // by a whole warp that reads no more of it
-        ok = !failed && !p.last;
+    auto passed = [&] {                                  // by a whole warp that reads no more of it
         __syncwarp();
         if (lane == 0) arrive(&piece_empty[turn % PA_PIECES]);
         turn++;
@@ -296,9 +301,9 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
         const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
         const uint32_t S = tmem + half * PA_KEYS + lane_at, O = tmem + PA_HALVES * PA_KEYS + half * DP + lane_at;
         unsigned done = 0, others = 0, x0 = 0, merges = 0;   // key tiles of this half and of the other so far; tiles of the ring before this piece
-        while (ok) {
+        while (true) {
             const Piece& p = next();
-            if (failed) break;
+            if (failed || p.stop) break;
             const int tk = (p.twin ? 0 : half) * rs.tokens + token;                // of the tile
             const bool row = token < rs.tokens && tk < p.tokens && g < p.heads;
             const int where = p.at0 + tk;
@@ -442,31 +447,38 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     __syncwarp();
                 };
                 float seen = 0.f;
+                // 16 or 32 columns at a time, in loops that are not unrolled: code that a CTA runs this seldom is fetched as it runs
+                auto columns = [&](auto n, int first, auto& y) {
+                    constexpr int N = decltype(n)::value;
 #pragma unroll
-                for (int i = 0; i < DP / 32; i++) {
-                    uint32_t y[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) y[e] = 0u;
-                    if (n_last > n_first) { tmem_ld(O + i * 32, y); tmem_ld_wait(y); }
+                    for (int e = 0; e < N; e++) y[e] = 0u;
+                    if (n_last > n_first) { tmem_ld(O + first, y); tmem_ld_wait(y); }
                     if (p.twin) {
-                        uint32_t z[32];
-                        tmem_ld(O + DP + i * 32, z);
+                        uint32_t z[N];
+                        tmem_ld(O + DP + first, z);
                         tmem_ld_wait(z);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) y[e] = __float_as_uint(fmaf(__uint_as_float(z[e]), f1, __uint_as_float(y[e]) * f0));
+                        for (int e = 0; e < N; e++) y[e] = __float_as_uint(fmaf(__uint_as_float(z[e]), f1, __uint_as_float(y[e]) * f0));
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) watch(seen, __uint_as_float(y[e]));
-                    if (p.cut) {
-#pragma unroll
-                        for (int s = 0; s < 2; s++)
-                            put(reinterpret_cast<const uint32_t(&)[16]>(y[16 * s]), part, i * 32 + s * 16);
-                    } else {
-                        uint32_t w[16];
+                    for (int e = 0; e < N; e++) watch(seen, __uint_as_float(y[e]));
+                };
+                if (p.cut) {
+#pragma unroll 1
+                    for (int d = 0; d < DP; d += 16) {
+                        uint32_t y[16];
+                        columns(std::integral_constant<int, 16>(), d, y);
+                        put(y, part, d);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int d = 0; d < DP; d += 32) {
+                        uint32_t y[32], w[16];
+                        columns(std::integral_constant<int, 32>(), d, y);
 #pragma unroll
                         for (int e = 0; e < 16; e++)
                             w[e] = none ? 0u : pack_bf16(__uint_as_float(y[2 * e]) * inv, __uint_as_float(y[2 * e + 1]) * inv);
-                        put(w, o, i * 32);
+                        put(w, o, d);
                     }
                 }
                 if (p.cut && row) *reinterpret_cast<float2*>(part + (size_t)PA_ROWS * a.D + 2 * pr) = make_float2(fmaxf(m, -FLT_MAX), l);
@@ -492,7 +504,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
             }
             merges += p.twin;
             x0 += 2 * (p.n1 - p.n0);
-            passed(p);
+            passed();
         }
         if (failed) s_fail = 1;
     } else {
@@ -500,43 +512,49 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
         if (warp == PA_HALVES * 4 + 2) {                 // ---- pieces ----
             LineCursor c = s_at;
             Cut cut = {};
-            for (bool begun = true; ok; begun = false, turn++) {
+            for (bool begun = true; !failed; begun = false) {
+                Piece p;
+                p.stop = c.left <= 0;
+                if (!p.stop) {
+                    p = make_piece(a, rs, c, all.at(a, c.b).first, begun);
+                    const int left = c.steps() - c.n - c.piece();                  // of the tile, to the next shares
+                    if (left > 0 && p.n0 == c.t.n0 && p.n1 > p.n0)
+                        cut = {p.row0, p.tokens, p.at0, p.first, p.h0, p.heads, begun, 1 + (int)((left + s_per - 1) / s_per)};
+                    c.next_piece(a, rs, all);
+                    if (p.n1 == p.n0) continue;
+                }
                 const unsigned slot = turn % PA_PIECES;
-                const int steps = c.piece();
-                const bool whole_left = c.n + steps == c.steps();
-                Piece p = make_piece(a, rs, c, all.at(a, c.b).first, begun);
-                ok = c.left - steps > (whole_left ? PA_TILE_COST : 0);
-                p.last = !ok;
-                if (!whole_left && p.n0 == c.t.n0)
-                    cut = {p.row0, p.tokens, p.at0, p.first, p.h0, p.heads, begun, 1 + (int)((c.steps() - c.n - steps + s_per - 1) / s_per)};
                 if (turn >= PA_PIECES && !wait_soon_warp(&piece_empty[slot], (turn / PA_PIECES - 1) & 1)) { failed = true; break; }
                 if (lane == 0) {
                     s_piece[slot] = p;
                     arrive(&piece_full[slot]);
                 }
                 __syncwarp();
-                c.next_piece(a, rs, all);
+                turn++;
+                if (p.stop) break;
             }
             if (lane == 0) plan.cuts[blockIdx.x] = cut;
             if (failed && lane == 0) s_fail = 1;
-        } else if (warp == PA_HALVES * 4 + 1) {          // ---- copies ----
+        } else if (warp != PA_HALVES * 4) {              // ---- copies, by two warps ----
+            // Pages of 8 to 32 rows make 32 to 8 boxes a tile, whose issue takes longer than their bytes: a warp issued one in 130 cycles with a
+            // lane to each.  So two warps share them, and a box's coordinates are the same in all lanes, of which the elected one issues.
             unsigned x = 0;
+            const bool lead = elected(), second = warp == PA_HALVES * 4 + 3;
             const int rows = min(1 << a.shift, PA_KEYS), boxes = PA_KEYS / rows;
-            // this lane's box of a tile: sub-tile of channels, rows; its page's id is fetched a tile ahead
-            const int sub = lane / boxes, box = lane % boxes;
-            const bool mine = sub < Sh::SUBS;
-            while (ok) {
+            const int sub = Sh::SUBS == 2 && second, by = Sh::SUBS == 2 ? 1 : 2, mine = Sh::SUBS == 2 ? boxes : (boxes + !second) / 2;
+            const int box = lane * by + (Sh::SUBS == 1 && second);                 // this lane fetches the id of its page, a tile ahead
+            while (true) {
                 const Piece& p = next();
-                if (failed) break;
-                const int n = p.n1 - p.n0;
+                if (failed || p.stop) break;
+                const int n = p.n1 - p.n0, hk = p.hk;
                 const bool twin = p.twin != 0;
                 auto id_of = [&](int place) {            // a page outside the pool, or beyond the table: zeros
                     const int j = (p.n0 + ring_tile(twin, place, n).i) * PA_KEYS + box * rows;
-                    return mine && place < 2 * n && (j >> a.shift) < a.M ? max(page_of(a, p.b, j), -1) : -1;
+                    return lane < mine && place < 2 * n && (j >> a.shift) < a.M ? max(page_of(a, p.b, j), -1) : -1;
                 };
                 int id = id_of(0);
                 auto queries = [&] {
-                    if (lane != 0) return;
+                    if (second || !lead) return;
                     const int halves = p.tokens > rs.tokens ? 2 : 1;
                     mbar_arrive_expect_tx(&q_full, halves * Sh::SUBS * rs.heads * rs.tokens * 128);
                     for (int t = 0; t < halves; t++)
@@ -549,11 +567,15 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     const RingTile t = ring_tile(twin, place, n);
                     const unsigned s = x % PA_STAGES, round = x / PA_STAGES;
                     if (round > 0 && !wait_soon_warp(&empty[s], (round - 1) & 1)) { failed = true; break; }
-                    if (lane == 0) mbar_arrive_expect_tx(&full[s], Sh::KTILE);
+                    if (!second && lead) mbar_arrive_expect_tx(&full[s], Sh::KTILE);
+                    const int row = (p.n0 + t.i) * PA_KEYS & ((1 << a.shift) - 1);     // of pages of more than a tile
+                    char* to = Ks + s * Sh::KTILE + sub * PA_KEYS * 128;
+#pragma unroll 4
+                    for (int i = 0; i < mine; i++) {
+                        const int at = i * by + (Sh::SUBS == 1 && second), page = __shfl_sync(FULL, id, i);
+                        if (lead) tile_g2s(to + at * rows * 128, t.value ? &maps.v : &maps.k, sub * 64, row, hk, page, &full[s]);
+                    }
                     __syncwarp();
-                    if (mine)
-                        tile_g2s(Ks + s * Sh::KTILE + sub * PA_KEYS * 128 + box * rows * 128, t.value ? &maps.v : &maps.k, sub * 64,
-                                 ((p.n0 + t.i) * PA_KEYS + box * rows) & ((1 << a.shift) - 1), p.hk, id, &full[s]);
                     id = then;
                     if (place != 1 || turn == 0) continue;
                     // the queries, whose place is the last piece's until its scores are done, behind the first two tiles
@@ -561,7 +583,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     queries();
                 }
                 if (failed) break;
-                passed(p);
+                passed();
             }
             if (failed && lane == 0) s_fail = 1;
         } else if (warp == PA_HALVES * 4) {              // ---- products ----
@@ -598,9 +620,10 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                 if (lead) mma_commit(&empty[stage(i)]);
                 __syncwarp();
             };
-            while (ok) {
+            while (true) {
                 const Piece& p = next();
-                failed = failed || !wait_soon_warp(&q_full, turn & 1);
+                if (failed || p.stop) break;
+                failed = !wait_soon_warp(&q_full, turn & 1);
                 if (failed) break;
                 const int n0 = p.n0, n1 = p.n1, from[PA_HALVES] = {p.from[0], p.from[1]}, to[PA_HALVES] = {p.to[0], p.to[1]};
                 if (p.twin) {                            // p.from[0] is n0 and p.to[0] n1: all its key tiles are seen by some row
@@ -636,7 +659,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     }
                 }
                 if (failed) break;
-                passed(p);
+                passed();
             }
             if (failed) s_fail = 1;
         }
