@@ -18,6 +18,21 @@ static inline cudaError_t opt_in_smem(F f, size_t bytes) {
     return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
+// A kernel that may start while the one before it in the stream ends, and begins with cudaGridDependencySynchronize()
+template <typename... P, typename... A>
+static inline cudaError_t launch_behind(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t st, A&&... args) {
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.stream = st;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kern, P(args)...);
+}
+
 // in_dtype / snap_dtype of p select the instantiation
 // initial state of the address scan (all NULL: the empty memory) and where its carried squared key norms go
 struct AddrFwdState { const float* K0; const float* o0; const double* nsq0; double* nsqfin; };

@@ -677,6 +677,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
 constexpr int LJ_ROWS = 16;
 __global__ void __launch_bounds__(256) line_join_kernel(PagedArgs a, RowShape rs, LinePlan plan, bf16* o) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    cudaGridDependencySynchronize();
     const Cut c = plan.cuts[blockIdx.x];
     for (int pr = blockIdx.y * LJ_ROWS + warp; pr < (blockIdx.y + 1) * LJ_ROWS; pr += 8) {
         const int half = pr / 128, r = pr % 128, token = r / rs.heads, g = r % rs.heads, tk = half * rs.tokens + token;
@@ -735,8 +736,7 @@ static cudaError_t paged_tensor(const PagedArgs& a, const void* q, const void* k
         return cudaErrorInvalidValue;
     const LinePlan plan(scratch, most_tiles(a));
     kern<<<148, PA_THREADS, Sh::SMEM, st>>>(a, rs, plan, maps, (const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o);
-    line_join_kernel<<<dim3(147, PA_ROWS / LJ_ROWS), 256, 0, st>>>(a, rs, plan, (bf16*)o);
-    return cudaGetLastError();
+    return launch_behind(line_join_kernel, dim3(147, PA_ROWS / LJ_ROWS), dim3(256), st, a, rs, plan, (bf16*)o);
 }
 template <int DP>
 static cudaError_t paged_tensor_score(const PagedArgs& a, const void* q, const void* k, const void* v, void* o, void* scratch, cudaStream_t st) {

@@ -125,29 +125,42 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
     Cursor ahead = c;
     Ids ids;
     ids.fetch(a, ahead);
-    const int piece = lane % PIECES, sub = lane / PIECES;
+    // A lane fetches piece `piece` of rows sub, sub + PER_PASS, ...  The instructions of a step are what bounds this kernel once its bytes come
+    // fast enough (690 of them: 5.5 TB/s), so addresses are sums of what a lane knows beforehand, and a step that is seen whole asks for
+    // no mask.
+    const int piece = lane % PIECES, sub = lane / PIECES, in_page = (1 << a.shift) - 1;
+    const bool live = piece * 8 < a.D;
+    const uint32_t put_at = sub * ROW + (((piece & ~7) | ((piece ^ sub) & 7)) << 4);
+    const bf16* kl = k + sub * a.ks[1] + (live ? piece * 8 : 0);
+    const bf16* vl = v + sub * a.vs[1] + (live ? piece * 8 : 0);
+    const long long k_pass = PER_PASS * a.ks[1], v_pass = PER_PASS * a.vs[1];
     long long fetched = x0;
     int put = 0, get = 0;
     auto fetch = [&] {                                   // the next step's 16 keys and values into the ring
         if (fetched < x1) {
             if (ahead.s < ids.base || ahead.s - ids.base >= 32) ids.fetch(a, ahead);
-            const int id[2] = {__shfl_sync(FULL, ids.lo, ahead.s - ids.base), __shfl_sync(FULL, ids.hi, ahead.s - ids.base)};
-            const int j0 = ahead.w.from + ahead.s * PS_KEYS, in_page = (1 << a.shift) - 1, hk = ahead.pair / a.chunks;
+            const int id0 = __shfl_sync(FULL, ids.lo, ahead.s - ids.base), id1 = __shfl_sync(FULL, ids.hi, ahead.s - ids.base);
+            const int j0 = ahead.w.from + ahead.s * PS_KEYS, hk = ahead.pair / a.chunks;
             const uint32_t to = ring + put * 2 * TILE;
-            const bf16 *kr[2], *vr[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const long long id0 = max(id[i], 0);
-                kr[i] = k + id0 * a.ks[0] + ((j0 + 8 * i) & in_page) * a.ks[1] + hk * a.ks[2] + piece * 8;
-                vr[i] = v + id0 * a.vs[0] + ((j0 + 8 * i) & in_page) * a.vs[1] + hk * a.vs[2] + piece * 8;
-            }
+            const bf16* kr = kl + max(id0, 0) * a.ks[0] + (j0 & in_page) * a.ks[1] + hk * a.ks[2];
+            const bf16* vr = vl + max(id0, 0) * a.vs[0] + (j0 & in_page) * a.vs[1] + hk * a.vs[2];
+            const bool whole = j0 >= ahead.w.lo && j0 + PS_KEYS <= ahead.w.hi && id0 >= 0 && id1 >= 0;
 #pragma unroll
             for (int i = 0; i < PS_KEYS / PER_PASS; i++) {
-                const int key = i * PER_PASS + sub, half = (i * PER_PASS) / 8 == ((i + 1) * PER_PASS - 1) / 8 ? (i * PER_PASS) / 8 : key / 8;
-                const bool in = j0 + key >= ahead.w.lo && j0 + key < ahead.w.hi && id[half] >= 0 && piece * 8 < a.D;
-                const uint32_t at = to + key * ROW + (((piece & ~7) | ((piece ^ key) & 7)) << 4);
-                cp_async16_or0(at, in ? kr[half] + (key & 7) * a.ks[1] : k, in);
-                cp_async16_or0(at + TILE, in ? vr[half] + (key & 7) * a.vs[1] : v, in);
+                if (i * PER_PASS == 8 && a.shift < 4) {  // the second half lies in another page
+                    kr = kl + max(id1, 0) * a.ks[0] + hk * a.ks[2];
+                    vr = vl + max(id1, 0) * a.vs[0] + hk * a.vs[2];
+                }
+                bool in = live;
+                if (!whole) {
+                    const int j = j0 + i * PER_PASS + sub;
+                    in = live && j >= ahead.w.lo && j < ahead.w.hi && (i * PER_PASS < 8 ? id0 : id1) >= 0;
+                }
+                const uint32_t at = to + (put_at ^ ((i * PER_PASS & 7) << 4)) + i * PER_PASS * ROW;
+                cp_async16_or0(at, in ? kr : k, in);
+                cp_async16_or0(at + TILE, in ? vr : v, in);
+                kr += k_pass;
+                vr += v_pass;
             }
             put = put + 1 == PS_STAGES ? 0 : put + 1;
             fetched++;
@@ -162,6 +175,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
     const bool capped = a.cap > 0.f;
     const float lin = capped ? a.scale / a.cap * (2.f * LOG2E) : a.scale * LOG2E, cap2 = a.cap * LOG2E;
     const long long me = (long long)warp * gridDim.x + blockIdx.x;
+    // of fewer than 9 heads rows 8 to 15 of the products take the lower parts of the weights, whose sums are added at the end
     uint32_t qf[DP / 16][4];
     float slope[R], m[R], l[R], acc[DP / 8][4];
     bool begins = true;                                  // a pair, at this step
@@ -212,19 +226,28 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
             mma16(s[1], qf[kk], f[2], f[3]);
         }
         uint32_t ph[4], pl[4];
-        if (!WIDE) ph[1] = ph[3] = pl[1] = pl[3] = 0u;
+        const bool seen = j0 >= c.w.lo && j0 + PS_KEYS <= c.w.hi;                  // whole
 #pragma unroll
         for (int r = 0; r < R; r++) {
             float z[4], top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int j = j0 + (i / 2) * 8 + (lane % 4) * 2 + i % 2;
-                float y = s[i / 2][2 * r + i % 2] * lin;
-                if (capped) y = fmaf(-2.f * cap2, __fdividef(1.f, exp2f(y) + 1.f), cap2);      // tanh x = 1 - 2 / (e^2x + 1)
-                y = fmaf(-slope[r], (float)(pos - j), y);
-                z[i] = j >= c.w.lo && j < c.w.hi ? y : -INFINITY;
-                top = fmaxf(top, z[i]);
+                z[i] = s[i / 2][2 * r + i % 2] * lin;
+                if (capped) z[i] = fmaf(-2.f * cap2, __fdividef(1.f, exp2f(z[i]) + 1.f), cap2);        // tanh x = 1 - 2 / (e^2x + 1)
             }
+            if (a.slopes != nullptr) {
+                const float dist = (float)(pos - j0 - (lane % 4) * 2);
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[i] = fmaf(-slope[r], dist - (float)((i / 2) * 8 + i % 2), z[i]);
+            }
+            if (!seen) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = j0 + (i / 2) * 8 + (lane % 4) * 2 + i % 2;
+                    z[i] = j >= c.w.lo && j < c.w.hi ? z[i] : -INFINITY;
+                }
+            }
+            top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
             top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
             top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
             top = fmaxf(top, m[r]);
@@ -233,7 +256,9 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
                 const float shrink = exp2f(m[r] - base);
                 l[r] *= shrink;
 #pragma unroll
-                for (int i = 0; i < DP / 8; i++) { acc[i][2 * r] *= shrink; acc[i][2 * r + 1] *= shrink; }
+                for (int i = 0; i < DP / 8; i++)
+#pragma unroll
+                    for (int e = 0; e < (WIDE ? 2 : 4); e++) acc[i][2 * r + e] *= shrink;
                 m[r] = top;
             }
             float p[4];
@@ -243,7 +268,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
             for (int t = 0; t < 2; t++) {
                 const uint32_t w = pack_bf16(p[2 * t], p[2 * t + 1]);
                 ph[2 * t + r] = w;
-                pl[2 * t + r] = pack_bf16(p[2 * t] - __uint_as_float(w << 16), p[2 * t + 1] - __uint_as_float(w & 0xffff0000u));
+                (WIDE ? pl : ph)[2 * t + (WIDE ? r : 1)] = pack_bf16(p[2 * t] - __uint_as_float(w << 16), p[2 * t + 1] - __uint_as_float(w & 0xffff0000u));
             }
         }
 #pragma unroll
@@ -252,9 +277,11 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
             const int key = ((lane / 8) % 2) * 8 + lane % 8, pc = i + lane / 16;
             ldsm4_t(f, vs + key * ROW + (((pc & ~7) | ((pc ^ key) & 7)) << 4));
             mma16(acc[i], ph, f[0], f[1]);
-            mma16(acc[i], pl, f[0], f[1]);
             mma16(acc[i + 1], ph, f[2], f[3]);
-            mma16(acc[i + 1], pl, f[2], f[3]);
+            if (WIDE) {
+                mma16(acc[i], pl, f[0], f[1]);
+                mma16(acc[i + 1], pl, f[2], f[3]);
+            }
         }
         __syncwarp();
         get = get + 1 == PS_STAGES ? 0 : get + 1;
@@ -262,6 +289,10 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
         const bool ends = c.s + 1 == c.w.steps;
         if (ends || x + 1 == x1) {
             const bool whole = ends && x - begun + 1 == c.w.steps;
+            if (!WIDE) {
+#pragma unroll
+                for (int i = 0; i < DP / 8; i++) { acc[i][0] += acc[i][2]; acc[i][1] += acc[i][3]; }
+            }
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 float sum = l[r];
@@ -414,45 +445,61 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_kernel(PagedArgs a, Ste
     }
 }
 
-// o of a (request, head) whose pair several warps took, joined in their order; zeros where it sees nothing
+// o of a (request, head) whose pair several warps took, joined in their order; zeros where it sees nothing.  W warps to a (request, head):
+// one where there are many of them, most of which have nothing to join
 constexpr int PJ_WARPS = 8;
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(PJ_WARPS * 32) paged_join_kernel(PagedArgs a, StepPlan plan, T* o) {
-    __shared__ float s_acc[PJ_WARPS][128], s_m[PJ_WARPS], s_l[PJ_WARPS];
-    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, lane = threadIdx.x & 31, warp = threadIdx.x / 32, group = a.H / a.KV;
-    const int hk = h / group, g = h % group, pair = hk * a.chunks + g / plan.heads, pairs = a.KV * a.chunks;
-    const long long steps = (plan.before[b + 1] - plan.before[b]) / pairs, per = *plan.per;
-    T* to = o + (size_t)blockIdx.x * a.D;
+    __shared__ float s_acc[W > 1 ? W : 1][128], s_m[PJ_WARPS], s_l[PJ_WARPS];
+    cudaGridDependencySynchronize();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, x = blockIdx.x * (PJ_WARPS / W) + warp / W, mine = warp % W;
+    if (x >= a.B * a.H) return;                          // W > 1: never, a CTA has one
+    const int b = x / a.H, h = x % a.H, group = a.H / a.KV, hk = h / group, g = h % group, pair = hk * a.chunks + g / plan.heads, pairs = a.KV * a.chunks;
+    const long long before = plan.before[b], steps = (plan.before[b + 1] - before) / pairs, per = *plan.per;
+    T* to = o + (size_t)x * a.D;
     if (steps == 0) {
-        for (int d = threadIdx.x; d < a.D; d += PJ_WARPS * 32) st1(to + d, 0.f);
+        for (int d = mine * 32 + lane; d < a.D; d += W * 32) st1(to + d, 0.f);
         return;
     }
-    const long long x0 = plan.before[b] + pair * steps, w0 = x0 / per, w1 = (x0 + steps - 1) / per;
+    const long long x0 = before + pair * steps, w0 = x0 / per, w1 = (x0 + steps - 1) / per;
     if (w0 == w1) return;                                // one warp had it all
     float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (long long w = w0 + warp; w <= w1; w += PJ_WARPS) {
+#pragma unroll 4
+    for (long long w = w0 + mine; w <= w1; w += W) {
         const float* from = plan.part(w, w * per < x0, g % plan.heads, a.D);
-        const float pm = from[a.D], pl = from[a.D + 1], top = fmaxf(m, pm), f = exp2f(m - top), pf = exp2f(pm - top);
-        l = l * f + pl * pf;
+        const float2 ml = *reinterpret_cast<const float2*>(from + a.D);
+        const float top = fmaxf(m, ml.x), f = exp2f(m - top), pf = exp2f(ml.x - top);
+        l = l * f + ml.y * pf;
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-            if (lane + 32 * c < a.D) acc[c] = acc[c] * f + from[lane + 32 * c] * pf;
+        for (int c = 0; c < 4; c++) acc[c] = acc[c] * f + (lane + 32 * c < a.D ? from[lane + 32 * c] : 0.f) * pf;
         m = top;
     }
+    if constexpr (W == 1) {
 #pragma unroll
-    for (int c = 0; c < 4; c++) s_acc[warp][lane + 32 * c] = acc[c];
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-    __syncthreads();
-    for (int d = threadIdx.x; d < a.D; d += PJ_WARPS * 32) {
-        float top = -INFINITY, sum = 0.f, x = 0.f;
-        for (int i = 0; i < PJ_WARPS; i++) top = fmaxf(top, s_m[i]);
-        for (int i = 0; i < PJ_WARPS; i++) {
-            const float f = exp2f(s_m[i] - top);
-            sum = fmaf(s_l[i], f, sum);
-            x = fmaf(s_acc[i][d], f, x);
+        for (int c = 0; c < 4; c++)
+            if (lane + 32 * c < a.D) st1(to + lane + 32 * c, acc[c] / l);
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++) s_acc[warp][lane + 32 * c] = acc[c];
+        if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+        __syncthreads();
+        for (int d = threadIdx.x; d < a.D; d += PJ_WARPS * 32) {
+            float top = -INFINITY, sum = 0.f, y = 0.f;
+            for (int i = 0; i < W; i++) top = fmaxf(top, s_m[i]);
+            for (int i = 0; i < W; i++) {
+                const float f = exp2f(s_m[i] - top);
+                sum = fmaf(s_l[i], f, sum);
+                y = fmaf(s_acc[i][d], f, y);
+            }
+            st1(to + d, y / sum);
         }
-        st1(to + d, x / sum);
     }
+}
+template <typename T>
+static cudaError_t launch_join(const PagedArgs& a, const StepPlan& plan, void* o, cudaStream_t st) {
+    const int n = a.B * a.H;
+    return n < 148 * 4 ? launch_behind(paged_join_kernel<T, PJ_WARPS>, dim3(n), dim3(PJ_WARPS * 32), st, a, plan, (T*)o)
+                       : launch_behind(paged_join_kernel<T, 1>, dim3((n + PJ_WARPS - 1) / PJ_WARPS), dim3(PJ_WARPS * 32), st, a, plan, (T*)o);
 }
 
 static int paged_heads(int group, int dtype) { return dtype == SLOTSCAN_BF16 ? (group > 8 ? 16 : 8) : group > 4 ? 8 : group; }
@@ -536,11 +583,10 @@ extern "C" int slotscan_paged_step(const slotscan_paged_params* p, const void* q
     if (p->dtype == SLOTSCAN_BF16) {
         const cudaError_t e = p->D <= 64 ? launch_step_bf16<64>(a, plan, ctas, q, kp, vp, o, st) : launch_step_bf16<128>(a, plan, ctas, q, kp, vp, o, st);
         if (e != cudaSuccess) return (int)e;
-        paged_join_kernel<bf16><<<a.B * a.H, PJ_WARPS * 32, 0, st>>>(a, plan, (bf16*)o);
+        return (int)launch_join<bf16>(a, plan, o, st);
     } else {
         if (p->D <= 64) launch_step_f32<8>(a, plan, ctas, q, kp, vp, o, st);
         else launch_step_f32<16>(a, plan, ctas, q, kp, vp, o, st);
-        paged_join_kernel<float><<<a.B * a.H, PJ_WARPS * 32, 0, st>>>(a, plan, (float*)o);
+        return (int)launch_join<float>(a, plan, o, st);
     }
-    return (int)cudaGetLastError();
 }
