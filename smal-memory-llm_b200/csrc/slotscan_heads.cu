@@ -139,7 +139,7 @@ __device__ __forceinline__ void turn(float (&y)[8], const float (&cs)[4], const 
 
 // T: bf16 or float
 template <typename T, int LPG, Dest DEST>
-__global__ void __launch_bounds__(NR_THREADS, DEST != OUT ? 3 : NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
+__global__ void __launch_bounds__(NR_THREADS, DEST == RING ? 3 : NR_FWD_CTAS) norm_rope_kernel(NormArgs a, AppendArgs ap, const T* q, const T* k, const T* v, T* qo, T* ko,
                                                                T* kc, T* vc) {
     constexpr bool CACHE = DEST != OUT;
     constexpr int SLOTS = NR_FWD_SLOTS<T>;

@@ -13,6 +13,7 @@
 
 #include "slotscan.h"
 #include "slotscan_common.cuh"
+#include "slotscan_launch.h"
 
 namespace slotscan {
 
@@ -33,8 +34,8 @@ struct PagePlan {
 
 __device__ __forceinline__ long long pages_of(long long n, int shift) { return (n + (1 << shift) - 1) >> shift; }
 
-// inclusive sum over the CTA; `carry` (shared) is what came before, and gets the total added by the last thread
-__device__ __forceinline__ long long cta_sum(long long v, long long* s_warp, long long* carry) {
+// inclusive sum over the CTA on top of `carry`, which becomes the total; s_warp: 32 places that the call before this one did not have
+__device__ __forceinline__ long long cta_sum(long long v, long long* s_warp, long long& carry) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
 #pragma unroll
     for (int off = 1; off < 32; off *= 2) {
@@ -43,67 +44,84 @@ __device__ __forceinline__ long long cta_sum(long long v, long long* s_warp, lon
     }
     if (lane == 31) s_warp[warp] = v;
     __syncthreads();
-    if (warp == 0) {
-        long long w = s_warp[lane];
+    long long w = s_warp[lane];                          // every warp sums the warps' totals for itself
 #pragma unroll
-        for (int off = 1; off < 32; off *= 2) {
-            const long long up = __shfl_up_sync(FULL, w, off);
-            if (lane >= off) w += up;
-        }
-        s_warp[lane] = w;
+    for (int off = 1; off < 32; off *= 2) {
+        const long long up = __shfl_up_sync(FULL, w, off);
+        if (lane >= off) w += up;
     }
-    __syncthreads();
-    v += *carry + (warp > 0 ? s_warp[warp - 1] : 0);
-    __syncthreads();
-    if (threadIdx.x == PG_THREADS - 1) *carry = v;
-    __syncthreads();
+    const long long before = __shfl_sync(FULL, w, (warp + 31) % 32), all = __shfl_sync(FULL, w, 31);
+    v += carry + (warp > 0 ? before : 0);
+    carry += all;
     return v;
 }
 __device__ __forceinline__ int free_before(const PageArgs& a) { return min(max(*a.n_free, 0), a.pages); }
 
-// slot and position of packed row i, and the table's entry of a page that begins with it
-__device__ __forceinline__ void place_row(const PageArgs& a, const PagePlan& plan, const int32_t* starts, int32_t* slots, int32_t* pos, int i) {
+// Slots and positions of packed rows, 32 to a warp, and the table's entries of pages that begin with them.  `i`: the lane's row.  The first
+// row's request is found in steps of 32, so that few loads wait for one another, and the others' among the 32 that follow it.
+__device__ __forceinline__ void place_rows(const PageArgs& a, const PagePlan& plan, const int32_t* starts, int32_t* slots, int32_t* pos, int i) {
+    const int lane = threadIdx.x & 31, i0 = i - lane;
     int slot = -1, at = -1;
-    if (i < starts[a.B]) {
-        int lo = 0, hi = a.B - 1;                        // the first request that ends behind i
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (starts[mid + 1] > i) hi = mid; else lo = mid + 1;
+    if (i0 < starts[a.B]) {                              // the same in all lanes
+        int lo = 0, n = a.B;                             // the first request that ends behind i0 is one of n from lo on
+        while (n > 1) {
+            const int step = (n + 31) / 32, mine = lo + min((lane + 1) * step, n);
+            const int below = __popc(__ballot_sync(FULL, (lane + 1) * step < n && starts[mine] <= i0));
+            lo += below * step;
+            n = min(step, n - below * step);
         }
-        const int held = plan.held[lo];
-        if (held >= 0) {
-            at = held + i - starts[lo];
-            const int page = at >> a.shift, have = (int)pages_of(held, a.shift);
-            int32_t* entry = a.tables + lo * a.table_stride + page;
-            const int id = page < have ? *entry : a.free_pages[*plan.n_free - 1 - (plan.rank[lo] + page - have)];
-            const int in_page = at & ((1 << a.shift) - 1);
-            if (in_page == 0) *entry = id;
-            const long long s = ((long long)id << a.shift) + in_page;
-            slot = id >= 0 && s <= BIGI ? (int)s : -1;
+        int b = lo;
+        for (int b0 = lo;; b0 += 32) {                   // those without rows among them
+            const int end = b0 + lane < a.B ? starts[b0 + lane + 1] : BIGI;
+            int behind = 0;                              // of the 32, how many end at or before i
+#pragma unroll
+            for (int step = 16; step > 0; step /= 2)
+                if (__shfl_sync(FULL, end, behind + step - 1) <= i) behind += step;
+            const int last = __shfl_sync(FULL, end, 31);
+            if (behind == 31 && last <= i) behind = 32;
+            if (b == b0) b += behind;
+            if (!__any_sync(FULL, b == b0 + 32 && b < a.B)) break;
+        }
+        if (i < starts[a.B]) {
+            const int held = plan.held[b];
+            if (held >= 0) {
+                at = held + i - starts[b];
+                const int page = at >> a.shift, have = (int)pages_of(held, a.shift);
+                int32_t* entry = a.tables + b * a.table_stride + page;
+                const int id = page < have ? *entry : a.free_pages[*plan.n_free - 1 - (plan.rank[b] + page - have)];
+                const int in_page = at & ((1 << a.shift) - 1);
+                if (in_page == 0) *entry = id;
+                const long long s = ((long long)id << a.shift) + in_page;
+                slot = id >= 0 && s <= BIGI ? (int)s : -1;
+            }
         }
     }
-    slots[i] = slot;
-    pos[i] = at;
+    if (i < a.tokens) {
+        slots[i] = slot;
+        pos[i] = at;
+    }
 }
 
 template <bool OWN>
 __global__ void __launch_bounds__(PG_THREADS) extend_kernel(PageArgs a, const int32_t* fresh, int32_t* scratch, int32_t* slots, int32_t* pos, int32_t* starts,
                                                             int32_t* taken) {
-    __shared__ long long s_warp[32], s_tokens, s_pages;
+    __shared__ long long s_warp[2][32];
     __shared__ int s_handed;
     const PagePlan plan(scratch, a.B);
     const int tid = threadIdx.x;
-    if (tid == 0) { s_tokens = s_pages = 0; s_handed = 0; starts[0] = 0; }
+    if (tid == 0) { s_handed = 0; starts[0] = 0; }
+    if (tid < 64) s_warp[tid / 32][tid % 32] = 0;        // of warps that the CTA does not have
     const int nf = free_before(a);
+    long long tokens = 0, pages = 0;
     __syncthreads();
-    for (int b0 = 0; b0 < a.B; b0 += PG_THREADS) {
+    for (int b0 = 0; b0 < a.B; b0 += blockDim.x) {
         const int b = b0 + tid;
         const bool in = b < a.B;
         const long long n = in ? max(fresh[b], 0) : 0, held = in ? max(a.lengths[b], 0) : 0;
-        const long long ends = cta_sum(n, s_warp, &s_tokens);
+        const long long ends = cta_sum(n, s_warp[0], tokens);
         const bool fits = in && held + n <= ((long long)a.M << a.shift) && ends <= a.tokens;
         const long long need = fits ? pages_of(held + n, a.shift) - pages_of(held, a.shift) : 0;
-        const long long upto = cta_sum(need, s_warp, &s_pages);
+        const long long upto = cta_sum(need, s_warp[1], pages);
         const bool served = fits && (need == 0 || upto <= nf);
         if (in) {
             starts[b + 1] = (int)min(ends, (long long)a.tokens);
@@ -121,12 +139,13 @@ __global__ void __launch_bounds__(PG_THREADS) extend_kernel(PageArgs a, const in
     }
     if constexpr (OWN) {
         __syncthreads();
-        for (int i = tid; i < a.tokens; i += PG_THREADS) place_row(a, plan, starts, slots, pos, i);
+        for (int i = tid; i - (tid & 31) < a.tokens; i += blockDim.x) place_rows(a, plan, starts, slots, pos, i);
     }
 }
 __global__ void __launch_bounds__(256) place_kernel(PageArgs a, int32_t* scratch, const int32_t* starts, int32_t* slots, int32_t* pos) {
+    cudaGridDependencySynchronize();
     const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < a.tokens) place_row(a, PagePlan(scratch, a.B), starts, slots, pos, i);
+    if (i - (int)(threadIdx.x & 31) < a.tokens) place_rows(a, PagePlan(scratch, a.B), starts, slots, pos, i);
 }
 
 // a request's pages onto the stack, in their order, and its table emptied; `held`: its pages, minus one where it stays
@@ -143,17 +162,19 @@ __device__ __forceinline__ void give_back(const PageArgs& a, const PagePlan& pla
 
 template <bool OWN>
 __global__ void __launch_bounds__(PG_THREADS) release_kernel(PageArgs a, const uint8_t* done, int32_t* scratch) {
-    __shared__ long long s_warp[32], s_pages;
+    __shared__ long long s_warp[2][32];
     const PagePlan plan(scratch, a.B);
     const int tid = threadIdx.x;
-    if (tid == 0) s_pages = 0;
+    if (tid < 64) s_warp[tid / 32][tid % 32] = 0;
     const int nf = free_before(a);
+    long long pages = 0;
+    int turn = 0;
     __syncthreads();
-    for (int b0 = 0; b0 < a.B; b0 += PG_THREADS) {
+    for (int b0 = 0; b0 < a.B; b0 += blockDim.x, turn ^= 1) {
         const int b = b0 + tid;
         const bool ends = b < a.B && done[b] != 0;
         const long long n = ends ? min(pages_of(max(a.lengths[b], 0), a.shift), (long long)a.M) : 0;
-        const long long upto = cta_sum(n, s_warp, &s_pages);
+        const long long upto = cta_sum(n, s_warp[turn], pages);
         if (b < a.B) {
             plan.held[b] = ends ? (int)n : -1;
             plan.rank[b] = (int)min(upto - n, (long long)BIGI);
@@ -162,16 +183,20 @@ __global__ void __launch_bounds__(PG_THREADS) release_kernel(PageArgs a, const u
     }
     if (tid == 0) {
         *plan.n_free = nf;
-        *a.n_free = (int)min(nf + s_pages, (long long)a.pages);
+        *a.n_free = (int)min(nf + pages, (long long)a.pages);
     }
     if constexpr (OWN) {
         __syncthreads();
-        for (int b = tid / 32; b < a.B; b += PG_THREADS / 32) give_back(a, plan, b, tid & 31, 32);
+        for (int b = tid / 32; b < a.B; b += blockDim.x / 32) give_back(a, plan, b, tid & 31, 32);
     }
 }
 __global__ void __launch_bounds__(256) give_back_kernel(PageArgs a, int32_t* scratch) {
+    cudaGridDependencySynchronize();
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) give_back(a, PagePlan(scratch, a.B), b, threadIdx.x, 256);
 }
+
+// threads of the sums' CTA: fewer where there are few requests and rows
+static int sum_threads(long long most) { return most <= 256 ? 256 : PG_THREADS; }
 
 static PageArgs page_args(const slotscan_pages_params& p, int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* n_free) {
     PageArgs a;
@@ -209,12 +234,12 @@ extern "C" int slotscan_extend_pages(const slotscan_pages_params* p, const int32
     const PageArgs a = page_args(*p, lengths, tables, free_pages, n_free);
     cudaStream_t st = (cudaStream_t)stream;
     int32_t* s = (int32_t*)scratch;
-    if (a.tokens <= PG_OWN_ROWS) extend_kernel<true><<<1, PG_THREADS, 0, st>>>(a, fresh, s, slots, pos, starts, taken);
-    else {
-        extend_kernel<false><<<1, PG_THREADS, 0, st>>>(a, fresh, s, slots, pos, starts, taken);
-        place_kernel<<<(a.tokens + 255) / 256, 256, 0, st>>>(a, s, starts, slots, pos);
+    if (a.tokens <= PG_OWN_ROWS) {
+        extend_kernel<true><<<1, sum_threads(a.tokens > a.B ? a.tokens : a.B), 0, st>>>(a, fresh, s, slots, pos, starts, taken);
+        return (int)cudaGetLastError();
     }
-    return (int)cudaGetLastError();
+    extend_kernel<false><<<1, sum_threads(a.B), 0, st>>>(a, fresh, s, slots, pos, starts, taken);
+    return (int)launch_behind(place_kernel, dim3((a.tokens + 255) / 256), dim3(256), st, a, s, (const int32_t*)starts, slots, pos);
 }
 
 extern "C" int slotscan_release_pages(const slotscan_pages_params* p, const uint8_t* done, int32_t* lengths, int32_t* tables, int32_t* free_pages,
@@ -227,10 +252,10 @@ extern "C" int slotscan_release_pages(const slotscan_pages_params* p, const uint
     const PageArgs a = page_args(*p, lengths, tables, free_pages, n_free);
     cudaStream_t st = (cudaStream_t)stream;
     int32_t* s = (int32_t*)scratch;
-    if ((int64_t)a.B * a.M <= PG_OWN_ROWS) release_kernel<true><<<1, PG_THREADS, 0, st>>>(a, done, s);
-    else {
-        release_kernel<false><<<1, PG_THREADS, 0, st>>>(a, done, s);
-        give_back_kernel<<<(unsigned)(a.B < 148 * 8 ? a.B : 148 * 8), 256, 0, st>>>(a, s);
+    if ((int64_t)a.B * a.M <= PG_OWN_ROWS) {
+        release_kernel<true><<<1, sum_threads((int64_t)a.B * a.M), 0, st>>>(a, done, s);
+        return (int)cudaGetLastError();
     }
-    return (int)cudaGetLastError();
+    release_kernel<false><<<1, sum_threads(a.B), 0, st>>>(a, done, s);
+    return (int)launch_behind(give_back_kernel, dim3((unsigned)(a.B < 148 * 8 ? a.B : 148 * 8)), dim3(256), st, a, s);
 }
