@@ -719,8 +719,16 @@ static RowShape row_shape(const PagedArgs& a) {
 }
 static long long most_tiles(const PagedArgs& a) { return a.N / (PA_HALVES * row_shape(a).tokens) + (long long)a.B; }
 
+// one to an SM; fewer where the longest requests that the tables hold would not give each a tile of keys
+static int line_ctas(const PagedArgs& a) {
+    const int heads = row_shape(a).heads;
+    const long long keys = (((long long)a.M << a.shift) + PA_KEYS - 1) / PA_KEYS, pairs = (long long)a.KV * ((a.H / a.KV + heads - 1) / heads);
+    const long long tiles = most_tiles(a) < 148 ? most_tiles(a) : 148, most = (tiles * pairs * (PA_TILE_COST + PA_TWO * keys) + PA_TWO - 1) / PA_TWO;
+    return (int)(most < 1 ? 1 : most < 148 ? most : 148);
+}
+
 size_t paged_attn_scratch_bf16(const PagedArgs& a) {
-    return LinePlan::head_bytes() + sizeof(float) * 148 * 2 * PA_ROWS * (size_t)(a.D + 2);
+    return LinePlan::head_bytes() + sizeof(float) * line_ctas(a) * 2 * PA_ROWS * (size_t)(a.D + 2);
 }
 
 template <int DP, bool CAP, bool BIAS>
@@ -735,8 +743,9 @@ static cudaError_t paged_tensor(const PagedArgs& a, const void* q, const void* k
     if (!box_map(&maps.q, q, a.N, a.H, a.D, a.qs, rs.heads, rs.tokens) || !tile_map(&maps.k, k, a.pages, page, a.KV, a.D, a.ks, rows) || !tile_map(&maps.v, v, a.pages, page, a.KV, a.D, a.vs, rows))
         return cudaErrorInvalidValue;
     const LinePlan plan(scratch, most_tiles(a));
-    kern<<<148, PA_THREADS, Sh::SMEM, st>>>(a, rs, plan, maps, (const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o);
-    return launch_behind(line_join_kernel, dim3(147, PA_ROWS / LJ_ROWS), dim3(256), st, a, rs, plan, (bf16*)o);
+    const int ctas = line_ctas(a);
+    kern<<<ctas, PA_THREADS, Sh::SMEM, st>>>(a, rs, plan, maps, (const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o);
+    return ctas == 1 ? cudaGetLastError() : launch_behind(line_join_kernel, dim3(ctas - 1, PA_ROWS / LJ_ROWS), dim3(256), st, a, rs, plan, (bf16*)o);
 }
 template <int DP>
 static cudaError_t paged_tensor_score(const PagedArgs& a, const void* q, const void* k, const void* v, void* o, void* scratch, cudaStream_t st) {

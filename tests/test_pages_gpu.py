@@ -222,12 +222,13 @@ class Batch:
             at += new
         return o, size, worst, max(h for h, _ in self.requests)
 
-    def hold(self, got, dtype, window, cap, slopes, start, step, scale=None):
+    def hold(self, got, dtype, window, cap, slopes, start, step, scale=None, large=False):
+        """`large`: scores so large that their float32 sums are off by more than the roundings to bf16."""
         o, size, worst, keys = self.want(window, cap, slopes, start, scale)
+        E = (self.D + 16) * 2.0 ** -24 * worst
         if dtype == "bf16" and not step:
-            allowed = 2.0 ** -8 * (size + o.abs())
+            allowed = 2.0 ** -8 * (size + o.abs()) + (4 * E * size if large else 0.0)
         else:
-            E = (self.D + 16) * 2.0 ** -24 * worst
             allowed = (4 * E + (keys + 64) * 2.0 ** -24) * size + (2.0 ** -8 if dtype == "bf16" else 2.0 ** -23) * o.abs()
         within(got, o, allowed, "o")
 
@@ -243,7 +244,10 @@ CHUNKS = [([(1, 1), (17, 17), (300, 5), (128, 128), (1000, 1), (129, 3)], 16, 12
           ([(5000, 700)], 16, 2, 1, 128, 0, 30.0, False, False, 0),
           ([(9000, 4)], 16, 1, 1, 64, 0, 0.0, False, False, 1),
           ([(1, 1)] * 200, 8, 1, 1, 128, 0, 0.0, False, False, 0),
-          ([(260, 129), (385, 256)], 512, 5, 5, 72, 33, 0.0, True, False, 0)]
+          ([(260, 129), (385, 256)], 512, 5, 5, 72, 33, 0.0, True, False, 0),
+          # more requests than a CTA looks up at a time, several pieces to a CTA, some without rows
+          ([(1 + 37 * i % 301, min(1 + 37 * i % 301, (0, 1, 1, 7, 150)[i % 5])) for i in range(900)], 16, 6, 2, 64, 0, 0.0, False, True, 11),
+          ([(2000 + 40 * i, (1, 90, 2)[i % 3]) for i in range(12)], 32, 8, 8, 128, 0, 0.0, True, False, 0)]
 
 
 def _start(requests, use):
@@ -341,6 +345,97 @@ def test_rows_of_nobody_and_pages_of_no_pool(dtype):
     a = S.paged_attention_step(x.q[:3].unsqueeze(1), x.kp, x.vp, short, torch.tensor([299, 69, 199], device="cuda"))
     b = S.paged_attention_step(x.q[:3].unsqueeze(1), x.kp, x.vp, x.tables, torch.tensor([63, 63, 63], device="cuda"))
     within(a, b.double(), 2.0 ** (-7 if dtype == "bf16" else -20) * (b.double().abs() + 1e-3), "what the table reaches")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 512, 1024])
+def test_pages_of_every_size(page, dtype):
+    """The size of a page changes no bit: one tensor of keys cut into pages of each size."""
+    S = _S()
+    g = _gen(30)
+    dt = DT[dtype]
+    L, KV, D = 4096, 2, 64
+    k, v = _rand(g, L, KV, D).to(dt), _rand(g, L, KV, D).to(dt)
+    q, starts = (2 * _rand(g, 140, 6, D)).to(dt), torch.tensor([0, 100, 140], device="cuda")
+    pos = torch.cat((torch.arange(900, 1000), torch.arange(1960, 2000))).cuda()
+
+    def run(page):
+        tables = torch.stack((torch.arange(2048 // page), 2048 // page + torch.arange(2048 // page))).cuda()
+        kp, vp = k.view(-1, page, KV, D), v.view(-1, page, KV, D)
+        return (S.paged_attention(q, kp, vp, tables, starts, pos, window=700), S.paged_attention_step(q[[99, 139]].unsqueeze(1), kp, vp, tables, pos[[99, 139]]))
+    for a, b in zip(run(page), run(1024 if page != 1024 else 8)):
+        assert torch.equal(a, b)
+
+
+def test_infinite_values_that_are_seen():
+    """A query that sees an infinite value gets infinity or NaN in its channel, and numbers in the others."""
+    S = _S()
+    for dtype in ("f32", "bf16"):
+        x = Batch([(300, 40), (90, 1)], 16, 4, 2, 64, dtype, seed=31)
+        x.vp[x.tables[0, 2].long(), 5, 0, 7] = math.inf
+        o = S.paged_attention(x.q, x.kp, x.vp, x.tables, x.starts, x.pos)
+        assert not o[:40, :2, 7].isfinite().any() and o[:40, 2:].isfinite().all() and o[40:].isfinite().all()
+        assert o[:40, :2, :7].isfinite().all() and o[:40, :2, 8:].isfinite().all()
+        x.kp[x.tables[1, 0].long(), 3, 1] = math.nan
+        q1, p1 = x.q[[39, 40]].unsqueeze(1), x.pos[[39, 40]]
+        s = S.paged_attention_step(q1, x.kp, x.vp, x.tables, p1)
+        assert not s[0, 0, :2, 7].isfinite().any() and s[0, 0, 2:].isfinite().all() and s[1, 0, 2:].isnan().all() and s[1, 0, :2].isfinite().all()
+
+
+def test_scores_far_apart():
+    """Maxima that grow by hundreds along the keys, and fall: weights and sums are taken relative to the running one."""
+    S = _S()
+    for dtype in ("f32", "bf16"):
+        x = Batch([(1500, 300), (1500, 1)], 16, 4, 2, 64, dtype, seed=32)
+        for b, rising in ((0, True), (1, False)):
+            ramp = torch.linspace(0.1, 12, 1500, device="cuda")[:, None, None]
+            x.k[b] = (x.k[b].float() * (ramp if rising else ramp.flip(0))).to(x.k[b].dtype)
+            j = torch.arange(1500, device="cuda")
+            x.kp[x.tables[b, j // 16].long(), j % 16] = x.k[b]
+        x.hold(S.paged_attention(x.q, x.kp, x.vp, x.tables, x.starts, x.pos), dtype, 0, 0.0, None, None, step=False, large=True)
+        y = Batch([(1500, 1), (1500, 1)], 16, 4, 2, 64, dtype, seed=32)
+        y.k, y.v, y.kp, y.vp, y.tables = x.k, x.v, x.kp, x.vp, x.tables
+        y.hold(S.paged_attention_step(y.q.unsqueeze(1), x.kp, x.vp, x.tables, y.pos).squeeze(1), dtype, 0, 0.0, None, None, step=True)
+
+
+def test_two_calls_at_once():
+    """On two streams, and in two graphs that are replayed in turn: each call has a workspace of its own."""
+    S = _S()
+    a, b = (Batch([(3000, 40), (2000 + i, 1), (700, 130)], 16, 6, 2, 128, "bf16", seed=33 + i) for i in range(2))
+    last = {id(x): (x.q[[39, 40, 170]].unsqueeze(1), x.pos[[39, 40, 170]]) for x in (a, b)}
+
+    def call(x):
+        q, pos = last[id(x)]
+        return S.paged_attention(x.q, x.kp, x.vp, x.tables, x.starts, x.pos), S.paged_attention_step(q, x.kp, x.vp, x.tables, pos)
+    want = call(a), call(b)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(x))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(p, q) for r in got[i] for p, q in zip(r, want[i]))
+    graphs, held = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i, x in enumerate((a, b)):
+        with torch.cuda.graph(graphs[i]):
+            held.append(call(x))
+    for _ in range(5):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(held[i], want[i]))
+
+
+def test_no_wait_was_given_up():
+    from slotscan_b200 import _lib
+    S = _S()
+    x = Batch([(4000, 700), (3000, 1), (100, 100)], 16, 6, 2, 128, "bf16", seed=40)
+    _lib.device_status()
+    S.paged_attention(x.q, x.kp, x.vp, x.tables, x.starts, x.pos)
+    assert _lib.device_status() == 0
 
 
 def test_starts_that_are_no_starts():
