@@ -2,7 +2,8 @@
 //
 // A CTA holds 32 rows, (token, query head) pairs of one request and one key head, and passes over their keys 64 at a time with the running
 // maximum and sum of each row's softmax.  Where the tiles of rows would leave SMs idle, their keys are split evenly among several CTAs, and
-// a second kernel joins the parts in their order.  Bound by shared memory, as the attention over tokens in float32 is.
+// a second kernel joins the parts in their order.  Bound by shared memory, as the attention over tokens in float32 is; small calls by
+// their launches (two chunks of 40 tokens: 12 us with the host's side).
 #include "slotscan_attn_cores.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_paged.cuh"

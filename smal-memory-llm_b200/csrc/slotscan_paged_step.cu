@@ -9,6 +9,8 @@
 // bf16: the heads of a group are the rows of m16n8k16 products (up to 16 of them, the others zero), the keys the columns.  p is split into
 // two bf16 (p = hi + lo, off by 2^-17): the second product costs nothing here and keeps the float32 weights' precision.
 // float32: the CUDA cores.  A row is read by LPG lanes, 8 channels each.
+// 8 requests of up to 131,072 tokens over six key heads: 324 us, 6.67 TB/s; 32 of up to 8,192 over four: 50, and 5 for the join.  One
+// round of warps: with two to six shorter ones the ends of shares and the search for them took 370 to 393 us (of then 370).
 #include "slotscan_async.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_paged.cuh"

@@ -7,7 +7,8 @@
 // handed out, is taken from the end of the stack of free ones.  So everything is two sums over the requests, then independent per token.
 //
 // The sums are one CTA's, 1,024 requests at a time; what follows is its own too while it is little (one launch is the floor of a small turn),
-// and a second kernel's beyond.  Nothing is chosen by an order of arrival, so results repeat.
+// and a second kernel's beyond.  Nothing is chosen by an order of arrival, so results repeat.  Bound by latency: 5 us a call for four
+// requests, 10 for 1,024 with 99,000 tokens (cold, under the profiler), of which the host's side takes as long.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
