@@ -325,6 +325,14 @@ bool table_laid(const Tensor& t, const Tensor& like, int64_t B) {
 int64_t table_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 bool ints(const Tensor& t, int64_t n, const Tensor& like) { return t.dim() == 1 && t.size(0) == n && fits(Maybe(t), at::kInt, {n}, like); }
 
+// `n` elements of `t` from the `from`-th on, as a tensor of its own that shares the memory
+Tensor part_of(const Tensor& t, int64_t from, int64_t n) {
+    Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+    r.unsafeGetTensorImpl()->set_storage_offset(from);
+    r.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return r;
+}
+
 bool pages_params(slotscan_pages_params& p, const Tensor& lengths, const Tensor& tables, const Tensor& free_pages, const Tensor& n_free, int64_t page, int64_t tokens) {
     if (!lengths.is_cuda() || lengths.dim() != 1 || free_pages.dim() != 1) return false;
     const int64_t B = lengths.size(0);
@@ -343,10 +351,14 @@ py::object extend_pages(const Tensor& any_new, const Tensor& lengths, const Tens
     const Tensor fresh = in_32_bits(any_new);
     if (!pages_params(p, lengths, tables, free_pages, n_free, page, tokens) || !ints(fresh, p.B, lengths)) return py::none();
     const c10::cuda::CUDAGuard here(lengths.device());
+    // the results and the scratch lie in one allocation: five of them were a third of a small call's host time
     const size_t bytes = slotscan_pages_scratch_bytes(&p);
-    Tensor slots = at::empty({tokens}, lengths.options()), pos = at::empty({tokens}, lengths.options());
-    Tensor starts = at::empty({p.B + 1}, lengths.options()), taken = at::empty({p.B}, lengths.options());
-    Tensor scratch = at::empty({(int64_t)(bytes / sizeof(int32_t))}, lengths.options());
+    const int64_t sizes[] = {tokens, tokens, p.B + 1, p.B, (int64_t)(bytes / sizeof(int32_t))};
+    int64_t at[6] = {0};
+    for (int i = 0; i < 5; i++) at[i + 1] = at[i] + (sizes[i] + 3) / 4 * 4;        // each on 16 bytes
+    const Tensor all = at::empty({at[5]}, lengths.options());
+    const Tensor slots = part_of(all, at[0], sizes[0]), pos = part_of(all, at[1], sizes[1]), starts = part_of(all, at[2], sizes[2]),
+                 taken = part_of(all, at[3], sizes[3]), scratch = part_of(all, at[4], sizes[4]);
     check(slotscan_extend_pages(&p, (const int32_t*)in(fresh), (int32_t*)out(lengths), (int32_t*)out(tables), (int32_t*)out(free_pages), (int32_t*)out(n_free),
                                 (int32_t*)out(slots), (int32_t*)out(pos), (int32_t*)out(starts), (int32_t*)out(taken), out(scratch), bytes, stream_of(lengths)),
           "slotscan_extend_pages");
