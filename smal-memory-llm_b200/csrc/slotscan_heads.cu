@@ -12,7 +12,7 @@
 // registers: 4 in flight to a group and four CTAs to an SM, backward 5 rows with their gradients and two CTAs.  64 x 1,024 tokens of
 // 6 + 6 heads of 128, bf16: 76 us (5.3 TB/s), backward 120 us (5.0 TB/s).  Before: 101 and 150 us with rows in registers and a pair's
 // sides 8 lanes apart; 80 and 129 with the ring alone.  Three, five or six CTAs: 78, 85, 84 us; backward three CTAs 129, four 204.
-// Into pages: 6,200 packed tokens of 12 + 4 + 4 heads of 128 in 22 us, 49,000 in 100 (5.0 TB/s), four CTAs to an SM (three took as long).
+// Into pages: 6,456 packed tokens of 12 + 4 + 4 heads of 128 in 19 us, 49,000 in 100 (5.0 TB/s), four CTAs to an SM (three took as long).
 // Now bound by the issue of instructions (84 % of the slots, backward 76 %); paired multiply-adds took 81 and 126: their operands
 // have to be moved into pairs.  float32 is as fast either way (8 x 4,096 tokens of 12 + 4 heads of 64: 44 + 71 us, 6.1 TB/s).
 #include <cuda_bf16.h>
@@ -344,8 +344,8 @@ static NormArgs norm_args(const slotscan_norm_params& p, const float* table, con
     return a;
 }
 // Slices of a token's heads for packed tokens, whose number is any: the ones of least time, which is rounds of four CTAs to an SM, each of its
-// rows and of some six more until the first are there.  4,300 tokens of 12 + 4 + 4 heads: two slices, one round; with three, 1.36
-// rounds, 22.7 us
+// rows and of some six more until the first are there.  6,456 tokens of 12 + 4 + 4 heads: whole tokens, two thirds of a round, 19 us; two
+// slices are 1.36 rounds, 23 us
 static void slice_for_rounds(NormArgs& a, int heads, int lanes) {
     const long long round = 148ll * NR_FWD_CTAS * (NR_THREADS / lanes);
     long long best = 0;
