@@ -8,15 +8,21 @@
 namespace slotscan {
 
 // 32 scores of a row as base-2 exponents (CAP or BIAS: whole; else still without the factor `lin`), minus infinity where the row does
-// not see them
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void scores32(float (&s)[32], const Score& sc, float ahead, bool masked, int lo, int hi) {
+// not see them.  A warp's block is capped by one of two forms, which are rounded differently, and by its greatest score: rows that do not count
+// (whatever stands there) have no say in that, nor, with SEEN, have columns that a row does not see.
+template <bool CAP, bool BIAS, bool SEEN = false>
+__device__ __forceinline__ void scores32(float (&s)[32], const Score& sc, float ahead, bool masked, int lo, int hi, bool counts = true) {
     bool small = true;                                   // the capped scores' polynomial serves this warp's block
     if constexpr (CAP) {
         float m0 = 0.f, m1 = 0.f;
+        if (SEEN && masked) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) { m0 = fmaxf(m0, fabsf(s[i])); m1 = fmaxf(m1, fabsf(s[i + 1])); }
-        small = __all_sync(FULL, fmaxf(m0, m1) * sc.cap_in <= CAP_POLY_MOST);
+            for (int i = 0; i < 32; i++) m0 = i >= lo && i < hi ? fmaxf(m0, fabsf(s[i])) : m0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) { m0 = fmaxf(m0, fabsf(s[i])); m1 = fmaxf(m1, fabsf(s[i + 1])); }
+        }
+        small = __all_sync(FULL, !counts || fmaxf(m0, m1) * sc.cap_in <= CAP_POLY_MOST);
     }
     if constexpr (CAP || BIAS) {
         auto whole = [&](auto poly) {

@@ -349,7 +349,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                         tmem_ld_wait(x);
                         if (i + 1 < PA_KEYS / 32) tmem_ld(S + (i + 1) * 32, raw[(i + 1) % 2]);
                         float(&s)[32] = reinterpret_cast<float(&)[32]>(x);
-                        scores32<CAP, BIAS>(s, sc, at - (float)(j0 + i * 32), masked, sp.lo - j0 - i * 32, sp.hi - j0 - i * 32);
+                        scores32<CAP, BIAS, true>(s, sc, at - (float)(j0 + i * 32), masked, sp.lo - j0 - i * 32, sp.hi - j0 - i * 32, row);
                         float t0 = s[0], t1 = s[1];
 #pragma unroll
                         for (int e = 2; e < 32; e += 4) { t0 = fmaxf(fmaxf(t0, s[e]), s[e + 1]); if (e + 2 < 32) t1 = fmaxf(fmaxf(t1, s[e + 2]), s[e + 3]); }
