@@ -104,12 +104,14 @@ __device__ __forceinline__ void step_range(const PagedArgs& a, const StepPlan& p
 
 // cap tanh(x) in base-2 exponents, of y = 2 log2(e) x.  1 - 2 / (e^2x + 1) is off by 1.2e-7 of the cap wherever x is, which of a small x, under
 // a cap far above the scores, is all of it (1 % of a weight for cap 1e5); so below 1/4 the series of tanh, to x^9, which is off by 1e-8 of the
-// score.  Both are formed, as lanes differ: 32 requests of up to 8,192 tokens, capped at 30, take the 58 us that they took before.
-__device__ __forceinline__ float capped_score(float y, float cap2) {
+// score.  A warp whose scores are all small forms that one alone: 32 requests of up to 8,192 tokens, capped at 30,
+// 57.3 us (59.2 with the exponential form alone, 60.5 with both for every score).
+constexpr float CAP_SMALL = 0.25f * 2.f * LOG2E;
+__device__ __forceinline__ float cap_small(float y, float cap2) {
     const float x = y * (0.5f / LOG2E), w = x * x;
-    const float near = x * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
-    return fabsf(x) < 0.25f ? cap2 * near : fmaf(-2.f * cap2, __fdividef(1.f, exp2f(y) + 1.f), cap2);
+    return cap2 * (x * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f));
 }
+__device__ __forceinline__ float cap_large(float y, float cap2) { return fmaf(-2.f * cap2, __fdividef(1.f, exp2f(y) + 1.f), cap2); }
 
 // Page ids of 32 steps from `base` on, a lane to a step; of both halves of 8 keys
 struct Ids {
@@ -242,9 +244,16 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
         for (int r = 0; r < R; r++) {
             float z[4], top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                z[i] = s[i / 2][2 * r + i % 2] * lin;
-                if (capped) z[i] = capped_score(z[i], cap2);
+            for (int i = 0; i < 4; i++) z[i] = s[i / 2][2 * r + i % 2] * lin;
+            if (capped) {
+                const bool small = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3]))) < CAP_SMALL;
+                if (__all_sync(FULL, small)) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) z[i] = cap_small(z[i], cap2);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) z[i] = fabsf(z[i]) < CAP_SMALL ? cap_small(z[i], cap2) : cap_large(z[i], cap2);
+                }
             }
             if (a.slopes != nullptr) {
                 const float dist = (float)(pos - j0 - (lane % 4) * 2);
