@@ -320,7 +320,6 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
             const int by = p.twin ? 2 : 1, n_first = p.twin ? p.from[0] + half : p.from[half], n_last = p.twin ? p.to[0] : p.to[half];
             const int all_lo = p.lo, all_hi = p.hi, n_base = p.n0;
             float m = -INFINITY, l = 0.f;                // m in base-2 exponents
-            const float at = (float)where;
             const bool rows_here = __any_sync(FULL, row);                          // of this warp
             for (int n = n_first; n < n_last; n += by, done++) {
                 const int j0 = n * PA_KEYS;
@@ -349,7 +348,8 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                         tmem_ld_wait(x);
                         if (i + 1 < PA_KEYS / 32) tmem_ld(S + (i + 1) * 32, raw[(i + 1) % 2]);
                         float(&s)[32] = reinterpret_cast<float(&)[32]>(x);
-                        scores32<CAP, BIAS, true>(s, sc, at - (float)(j0 + i * 32), masked, sp.lo - j0 - i * 32, sp.hi - j0 - i * 32, row);
+                        // the distance is taken between whole numbers: float32 does not hold the positions beyond 2^24
+                        scores32<CAP, BIAS, true>(s, sc, (float)(where - j0 - i * 32), masked, sp.lo - j0 - i * 32, sp.hi - j0 - i * 32, row);
                         float t0 = s[0], t1 = s[1];
 #pragma unroll
                         for (int e = 2; e < 32; e += 4) { t0 = fmaxf(fmaxf(t0, s[e]), s[e + 1]); if (e + 2 < 32) t1 = fmaxf(fmaxf(t1, s[e + 2]), s[e + 3]); }

@@ -7,11 +7,55 @@ import pytest
 import torch
 
 from tests.test_pages_gpu import Batch, _S
+from tests.test_tokens_gpu import DT, _gen, _rand, within
 
 pytestmark = pytest.mark.gpu
 
 
 # ------------------------------------------------------------------------------------------------ scores
+
+def _formula(q, keys, values, dist, slopes, cap, scale):
+    """(o, sum p |v|, greatest magnitude of a score's terms) of rows q (n, H, D) over keys (n, L, KV, D) at distances (n, L), float64."""
+    n = q.shape[1] // keys.shape[2]
+    k, v = (t.double().repeat_interleave(n, 2) for t in (keys, values))
+    s = torch.einsum("nhd,nlhd->nhl", q.double(), k) * scale
+    mag = torch.einsum("nhd,nlhd->nhl", q.double().abs(), k.abs()) * scale
+    s = cap * torch.tanh(s / cap) if cap else s
+    bias = slopes.double()[:, None] * dist.double()[:, None, :] if slopes is not None else 0.0 * s
+    p = torch.softmax(s - bias, -1)
+    return torch.einsum("nhl,nlhd->nhd", p, v), torch.einsum("nhl,nlhd->nhd", p, v.abs()), float((mag + bias).max())
+
+
+def _allowed(o, size, worst, D, keys, dtype, step):
+    E = (D + 16) * 2.0 ** -24 * worst
+    if dtype == "bf16" and not step:
+        return 2.0 ** -8 * (size + o.abs())
+    return (4 * E + (keys + 64) * 2.0 ** -24) * size + (2.0 ** -8 if dtype == "bf16" else 2.0 ** -23) * o.abs()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("at", [2 ** 24 - 2, 2 ** 24 + 1, 2 ** 25 + 3, 2 ** 28 + 7, 2 ** 29 - 9])
+def test_distance_bias_at_far_positions(at, dtype):
+    """Positions that float32 does not hold: the distances are taken between whole numbers."""
+    S = _S()
+    g = _gen(50)
+    dt = DT[dtype]
+    H, KV, D, page, rows, window = 4, 2, 64, 1024, 7, 300
+    tables = torch.zeros(1, (at + rows - 1) // page + 1, dtype=torch.int32, device="cuda")     # one page named often, others at the end
+    tables[0, -2:] = torch.tensor([1, 2])
+    kp, vp = _rand(g, 3, page, KV, D).to(dt), _rand(g, 3, page, KV, D).to(dt)
+    q = _rand(g, rows, H, D).to(dt)
+    slopes = torch.tensor([0.5, 0.3, 0.125, 0.02], device="cuda")
+    i = at + torch.arange(rows, device="cuda")
+    j = i[:, None] - torch.arange(window, device="cuda")
+    ids = tables[0, j // page].long()
+    o, size, worst = _formula(q, kp[ids, j % page], vp[ids, j % page], i[:, None] - j, slopes, 0.0, D ** -0.5)
+    starts = torch.tensor([0, rows], device="cuda")
+    got = S.paged_attention(q, kp, vp, tables, starts, i, window=window, slopes=slopes)
+    within(got, o, _allowed(o, size, worst, D, window, dtype, False), "packed")
+    got = S.paged_attention_step(q[:1].unsqueeze(1), kp, vp, tables, i[:1], window=window, slopes=slopes)[0]
+    within(got, o[:1], _allowed(o, size, worst, D, window, dtype, True)[:1], "step")
+
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cap", [0.5, 30.0, 1e3, 1e5, 1e7])
