@@ -40,9 +40,12 @@ __device__ __forceinline__ Score paged_score(const PagedArgs& a, int h) {
 struct Request { int begin, end, at, first; };
 __device__ __forceinline__ int rows_begin(const PagedArgs& a, int b) { return min(max(a.starts[b], 0), a.N); }
 __device__ __forceinline__ int rows_end(const PagedArgs& a, int b) { return max(min(a.starts[b + 1], a.N), rows_begin(a, b)); }
+// Position of a request's first row, minus one where its rows see nothing; so that those behind it, and the rows that a tile does not have, stay
+// within an int
+__device__ __forceinline__ int first_position(const PagedArgs& a, int begin, int end) { return min(max(a.pos[begin], -1), BIGI - 512 - (end - begin)); }
 __device__ __forceinline__ Request request(const PagedArgs& a, int b) {
     Request r = {rows_begin(a, b), rows_end(a, b), -1, first_key(a, b)};
-    if (r.end > r.begin) r.at = min(max(a.pos[r.begin], -1), 1 << 30);
+    if (r.end > r.begin) r.at = first_position(a, r.begin, r.end);
     return r;
 }
 // Rows of a tile: `heads` query heads (of the `chunks`-th part of a group) of `tokens` tokens, the heads of a token side by side

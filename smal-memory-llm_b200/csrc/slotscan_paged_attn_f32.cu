@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(PC_THREADS, 3) paged_attn_cores_kernel(PagedAr
     int b, tile;
     if (!find_tile(a, rs, blockIdx.x, b, tile)) return;
     const int begin = rows_begin(a, b), t0 = tile * rs.tokens, tokens = min(rs.tokens, rows_end(a, b) - begin - t0), row0 = begin + t0;
-    const int at = a.pos[begin], at0 = at < 0 ? -1 : min(at, 1 << 30) + t0;
+    const int at = first_position(a, begin, rows_end(a, b)), at0 = at < 0 ? -1 : at + t0;
     auto exists = [&](int r) { return r / rs.heads < tokens && r % rs.heads < heads; };
     auto span = [&](int r) { return exists(r) && at0 >= 0 ? paged_keys(a, b, at0 + r / rs.heads) : Span{0, 0}; };
     auto query = [&](int r) { return q + (long long)(row0 + r / rs.heads) * a.qs[0] + (long long)(hk * group + g0 + r % rs.heads) * a.qs[1]; };
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_cores_join_kernel(PagedArgs 
     int b, tile;
     if (!find_tile(a, rs, blockIdx.x, b, tile)) return;
     const int begin = rows_begin(a, b), t0 = tile * rs.tokens, tokens = min(rs.tokens, rows_end(a, b) - begin - t0);
-    const int at = a.pos[begin], at0 = at < 0 ? -1 : min(at, 1 << 30) + t0;
+    const int at = first_position(a, begin, rows_end(a, b)), at0 = at < 0 ? -1 : at + t0;
     const float* from = parts + ((size_t)blockIdx.x * pairs + pair) * splits * PC_ROWS * (a.D + 2);
     for (int r = warp; r < PC_ROWS; r += PC_THREADS / 32) {
         if (r / rs.heads >= tokens || r % rs.heads >= heads) continue;

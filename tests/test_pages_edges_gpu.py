@@ -58,6 +58,29 @@ def test_distance_bias_at_far_positions(at, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_windows_that_reach_back_from_beyond_the_tables(dtype):
+    """Positions near 2^31, whose windows end in what the table holds."""
+    S = _S()
+    g = _gen(51)
+    dt = DT[dtype]
+    H, KV, D, page, M, rows = 6, 2, 64, 16, 64, 40
+    at, end = 2 ** 31 - 2000, page * M
+    window = at - 700 + 1                                              # the first row sees [700, end)
+    tables = torch.randperm(M, device="cuda", generator=g).int().unsqueeze(0)
+    kp, vp = _rand(g, M, page, KV, D).to(dt), _rand(g, M, page, KV, D).to(dt)
+    k, v = kp[tables[0].long()].view(1, end, KV, D), vp[tables[0].long()].view(1, end, KV, D)
+    q = (2 * _rand(g, rows, H, D)).to(dt)
+    i = at + torch.arange(rows, device="cuda")
+    starts = torch.tensor([0, rows], device="cuda")
+    got = S.paged_attention(q, kp, vp, tables, starts, i, window=window)
+    for r in (0, 1, 17, rows - 1):
+        o, size, worst = _formula(q[r:r + 1], k[:, 700 + r:], v[:, 700 + r:], torch.zeros(1, end - 700 - r, device="cuda"), None, 0.0, D ** -0.5)
+        within(got[r:r + 1], o, _allowed(o, size, worst, D, end, dtype, False), "packed, row %d" % r)
+        s = S.paged_attention_step(q[r:r + 1].unsqueeze(1), kp, vp, tables, i[r:r + 1], window=window)[0]
+        within(s, o, _allowed(o, size, worst, D, end, dtype, True), "step, row %d" % r)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cap", [0.5, 30.0, 1e3, 1e5, 1e7])
 def test_caps_of_a_step(cap, dtype):
     """A cap far above the scores leaves them as they are; one below them bends them all."""
