@@ -87,7 +87,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
         const int cg = warp / 4;                         // columns 32 cg ..
         const uint32_t lane_at = (uint32_t)((warp % 4) * 32) << 16;
         const uint32_t S = tmem + cg * 32 + lane_at;
-        const float at = (float)(KEYS ? row - off : row + off);                    // this row's place among the stream's
+        const int at = KEYS ? row - off : row + off;     // this row's place among the stream's
         bool ok = true;
         float my_lse = 0.f, my_delta = 0.f;              // negated
         if constexpr (!KEYS) {
@@ -132,6 +132,7 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
         if (KEYS && steps > 0) fetch();
         for (int s = 0; s < steps; s++) {
             const int y0 = (y_first + y_at) * AB_N + cg * 32;
+            const float ahead = (float)(at - y0);        // float32 does not hold the places beyond 2^24
             const Score sc(a, head);
             const bool masked = y0 < ts.lo_max || y0 + 32 > ts.hi_min;
             float* stat = s_stat + (s & 1) * 2 * AB_N + cg * 32;
@@ -142,7 +143,6 @@ attn_bwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ B
                 sync_group(2 + cg, 128);
             }
             const int lo = sp.lo - y0, hi = sp.hi - y0;
-            const float ahead = at - (float)y0;
             uint32_t xs[32];                             // s, then p (1 - tanh^2)
             // a warp that has given up stays with its group's barrier, at which the others would wait for it without a limit
             if (!(ok = ok && wait_soon_warp(&s_full, s & 1))) continue;

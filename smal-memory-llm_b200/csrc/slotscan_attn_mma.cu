@@ -91,7 +91,7 @@ attn_fwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ F
         const uint32_t S = tmem + t * KT + lane_at, O = tmem + NT * KT + t * DP + lane_at;
         const Score sc(a, h);
         float m = -INFINITY, l = 0.f;                    // m in base-2 exponents
-        const float at = (float)(row + a.Tk - a.Tq);
+        const int at = row + a.Tk - a.Tq;
         bool ok = true;
         for (int n = f0; n < l0; n++) {
             const int j0 = n * KT;
@@ -106,7 +106,7 @@ attn_fwd_tensor_kernel(AttnArgs a, RowInputs<bf16> in, const __grid_constant__ F
             for (int c = 0; c < KT / 32; c++) {
                 tmem_ld_wait(raw[c]);
                 float(&s)[32] = reinterpret_cast<float(&)[32]>(raw[c]);
-                scores32<CAP, BIAS>(s, sc, at - (float)(j0 + c * 32), masked, sp.lo - j0 - c * 32, sp.hi - j0 - c * 32);
+                scores32<CAP, BIAS>(s, sc, (float)(at - j0 - c * 32), masked, sp.lo - j0 - c * 32, sp.hi - j0 - c * 32);
                 float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
 #pragma unroll
                 for (int i = 4; i < 32; i += 4) { t0 = fmaxf(t0, s[i]); t1 = fmaxf(t1, s[i + 1]); t2 = fmaxf(t2, s[i + 2]); t3 = fmaxf(t3, s[i + 3]); }
