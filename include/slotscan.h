@@ -372,7 +372,8 @@ int slotscan_attn_step(const slotscan_attn_step_params* p, const void* q, const 
  * Turn of a scheduler.  lengths (B) int32: tokens held;  tables (B, M) int32, rows table_stride apart;  free_pages (pages) int32: a stack,
  * of which the first n_free (1) int32 entries are free.  All four are changed in place.
  * slotscan_release_pages: each request with done[b] != 0 gives its pages back, in the order of requests and pages, behind the free
- * ones; its length becomes 0 and its table minus ones.
+ * ones; its length becomes 0 and its table minus ones.  Entries outside 0 to pages - 1 are not given back: where requests share pages, those
+ * of a request that ends and does not own them are set to minus one first.
  * slotscan_extend_pages: fresh[b] new tokens for each request (negative: none).  A request is served whole or not at all: not where its
  * table or the batch has no room for them, and not where it needs pages and the pages needed by it and the requests before it (the ones
  * that had no room left out) are more than there are.  Pages are taken from the end of the stack, in the order of requests and pages.

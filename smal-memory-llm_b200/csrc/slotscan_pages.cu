@@ -9,6 +9,9 @@
 // The sums are one CTA's, 1,024 requests at a time; what follows is its own too while it is little (one launch is the floor of a small turn),
 // and a second kernel's beyond.  Nothing is chosen by an order of arrival, so results repeat.  Bound by latency: 5 us a call for four
 // requests, 10 for 1,024 with 99,000 tokens (cold, under the profiler), of which the host's side takes as long.
+//
+// Back go the entries of a request's table that are pages of the pool: the others (minus ones where another request owns the page) are counted
+// out before the sum over the requests, since an id that no page has would be handed out again and its tokens stored nowhere.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -27,10 +30,14 @@ struct PageArgs {
     int32_t *lengths, *tables, *free_pages, *n_free;
 };
 // What the sums leave for the rows: per request the tokens held before (minus one: not served) and the rank of its first page; once the
-// free pages before
+// free pages before.  Of requests that end: the entries of their table, the rank within their CTA's requests and how many go back, and per CTA
+// how many in all.
+constexpr int PG_CTAS = 148 * 8;
 struct PagePlan {
-    int32_t *held, *rank, *n_free;
-    __host__ __device__ explicit PagePlan(int32_t* scratch, int B) : held(scratch), rank(scratch + B), n_free(scratch + 2 * (size_t)B) {}
+    int32_t *held, *rank, *n_free, *back, *total;
+    static size_t ints(int B) { return 3 * (size_t)B + 1 + PG_CTAS; }
+    __host__ __device__ explicit PagePlan(int32_t* scratch, int B)
+        : held(scratch), rank(scratch + B), n_free(scratch + 2 * (size_t)B), back(n_free + 1), total(back + B) {}
 };
 
 __device__ __forceinline__ long long pages_of(long long n, int shift) { return (n + (1 << shift) - 1) >> shift; }
@@ -149,51 +156,118 @@ __global__ void __launch_bounds__(256) place_kernel(PageArgs a, int32_t* scratch
     if (i - (int)(threadIdx.x & 31) < a.tokens) place_rows(a, PagePlan(scratch, a.B), starts, slots, pos, i);
 }
 
-// a request's pages onto the stack, in their order, and its table emptied; `held`: its pages, minus one where it stays
-__device__ __forceinline__ void give_back(const PageArgs& a, const PagePlan& plan, int b, int tid, int threads) {
+// how many of a table's first n entries are pages of the pool, as far as this thread sees them
+__device__ __forceinline__ int pool_pages(const PageArgs& a, const int32_t* row, int n, int tid, int threads) {
+    int mine = 0;
+    for (int j = tid; j < n; j += threads) mine += row[j] >= 0 && row[j] < a.pages;
+    return mine;
+}
+__device__ __forceinline__ int held_pages(const PageArgs& a, int b) { return (int)min(pages_of(max(a.lengths[b], 0), a.shift), (long long)a.M); }
+
+// a request's pages onto the stack from place `to` on, in their order, and its table emptied
+__device__ __forceinline__ void give_back(const PageArgs& a, const PagePlan& plan, int b, long long to, int tid, int threads) {
     const int n = plan.held[b];
     if (n < 0) return;
     int32_t* row = a.tables + b * a.table_stride;
-    const long long to = (long long)*plan.n_free + plan.rank[b];
-    for (int j = tid; j < a.M; j += threads) {
+    const bool all = plan.back[b] == n;
+    if (!all && tid < 32) {                              // some are none: those before them are counted, 32 at a time
+        for (int j0 = 0; j0 < n; j0 += 32) {
+            const int id = j0 + tid < n ? row[j0 + tid] : -1;
+            const bool page = id >= 0 && id < a.pages;
+            const unsigned pages = __ballot_sync(FULL, page);
+            const long long at = to + __popc(pages & ((1u << tid) - 1));
+            if (page && at < a.pages) a.free_pages[at] = id;
+            if (j0 + tid < n) row[j0 + tid] = -1;
+            to += __popc(pages);
+        }
+    }
+    for (int j = (all ? 0 : n) + tid; j < a.M; j += threads) {
         if (j < n && to + j < a.pages) a.free_pages[to + j] = row[j];
         row[j] = -1;
     }
 }
 
-template <bool OWN>
+// by one CTA: a warp to a request
 __global__ void __launch_bounds__(PG_THREADS) release_kernel(PageArgs a, const uint8_t* done, int32_t* scratch) {
     __shared__ long long s_warp[2][32];
     const PagePlan plan(scratch, a.B);
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31;
     if (tid < 64) s_warp[tid / 32][tid % 32] = 0;
     const int nf = free_before(a);
+    for (int b = tid / 32; b < a.B; b += blockDim.x / 32) {
+        const int n = done[b] != 0 ? held_pages(a, b) : -1;
+        const int pages = __reduce_add_sync(FULL, pool_pages(a, a.tables + b * a.table_stride, n, lane, 32));
+        if (lane == 0) { plan.held[b] = n; plan.back[b] = pages; }
+    }
     long long pages = 0;
     int turn = 0;
     __syncthreads();
     for (int b0 = 0; b0 < a.B; b0 += blockDim.x, turn ^= 1) {
-        const int b = b0 + tid;
-        const bool ends = b < a.B && done[b] != 0;
-        const long long n = ends ? min(pages_of(max(a.lengths[b], 0), a.shift), (long long)a.M) : 0;
+        const int b = b0 + tid, n = b < a.B ? plan.back[b] : 0;
         const long long upto = cta_sum(n, s_warp[turn], pages);
         if (b < a.B) {
-            plan.held[b] = ends ? (int)n : -1;
             plan.rank[b] = (int)min(upto - n, (long long)BIGI);
-            if (ends) a.lengths[b] = 0;
+            if (plan.held[b] >= 0) a.lengths[b] = 0;
         }
     }
-    if (tid == 0) {
-        *plan.n_free = nf;
-        *a.n_free = (int)min(nf + pages, (long long)a.pages);
-    }
-    if constexpr (OWN) {
-        __syncthreads();
-        for (int b = tid / 32; b < a.B; b += blockDim.x / 32) give_back(a, plan, b, tid & 31, 32);
-    }
+    if (tid == 0) *a.n_free = (int)min(nf + pages, (long long)a.pages);
+    __syncthreads();
+    for (int b = tid / 32; b < a.B; b += blockDim.x / 32) give_back(a, plan, b, (long long)nf + plan.rank[b], lane, 32);
 }
-__global__ void __launch_bounds__(256) give_back_kernel(PageArgs a, int32_t* scratch) {
+
+// By many: a CTA counts a run of requests, one after the other, and another one like it, which knows the counts of those before it, gives
+// their pages back.
+struct Run { int b0, b1; };
+__device__ __forceinline__ Run run_of(const PageArgs& a) {
+    const int per = (a.B + gridDim.x - 1) / gridDim.x, b0 = min((int)blockIdx.x * per, a.B);
+    return {b0, min(b0 + per, a.B)};
+}
+constexpr int PG_RUN_THREADS = 256;
+__device__ __forceinline__ long long run_sum(long long v, long long* s_warp) {     // over the CTA; s_warp: a place to a warp
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(FULL, v, off);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < PG_RUN_THREADS / 32; i++) v += s_warp[i];
+    return v;
+}
+__global__ void __launch_bounds__(PG_RUN_THREADS) count_back_kernel(PageArgs a, const uint8_t* done, int32_t* scratch) {
+    __shared__ long long s_warp[PG_RUN_THREADS / 32];
+    const PagePlan plan(scratch, a.B);
+    const int tid = threadIdx.x;
+    const Run r = run_of(a);
+    if (blockIdx.x == 0 && tid == 0) *plan.n_free = free_before(a);
+    long long sum = 0;
+    for (int b = r.b0; b < r.b1; b++) {
+        const bool ends = done[b] != 0;                  // the same in all threads
+        const int n = ends ? held_pages(a, b) : -1;
+        const int pages = ends ? (int)run_sum(pool_pages(a, a.tables + b * a.table_stride, n, tid, PG_RUN_THREADS), s_warp) : 0;
+        if (tid == 0) {
+            plan.held[b] = n;
+            plan.back[b] = pages;
+            plan.rank[b] = (int)min(sum, (long long)BIGI);
+        }
+        sum += pages;
+    }
+    if (tid == 0) plan.total[blockIdx.x] = (int)min(sum, (long long)BIGI);
+}
+__global__ void __launch_bounds__(PG_RUN_THREADS) give_back_kernel(PageArgs a, int32_t* scratch) {
+    __shared__ long long s_warp[PG_RUN_THREADS / 32];
+    const PagePlan plan(scratch, a.B);
+    const int tid = threadIdx.x;
     cudaGridDependencySynchronize();
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) give_back(a, PagePlan(scratch, a.B), b, threadIdx.x, 256);
+    const Run r = run_of(a);
+    long long before = 0;
+    for (int i = tid; i < blockIdx.x; i += PG_RUN_THREADS) before += plan.total[i];
+    const long long to = *plan.n_free + run_sum(before, s_warp);
+    for (int b = r.b0; b < r.b1; b++) {
+        give_back(a, plan, b, to + plan.rank[b], tid, PG_RUN_THREADS);
+        if (tid == 0 && plan.held[b] >= 0) a.lengths[b] = 0;
+    }
+    if (blockIdx.x == gridDim.x - 1 && tid == 0) *a.n_free = (int)min(to + plan.total[blockIdx.x], (long long)a.pages);
 }
 
 // threads of the sums' CTA: fewer where there are few requests and rows
@@ -222,7 +296,7 @@ extern "C" int slotscan_pages_check(const slotscan_pages_params* p) {
 }
 
 extern "C" size_t slotscan_pages_scratch_bytes(const slotscan_pages_params* p) {
-    return slotscan_pages_check(p) == SLOTSCAN_OK ? sizeof(int32_t) * (2 * (size_t)p->B + 1) : 0;
+    return slotscan_pages_check(p) == SLOTSCAN_OK ? sizeof(int32_t) * PagePlan::ints(p->B) : 0;
 }
 
 extern "C" int slotscan_extend_pages(const slotscan_pages_params* p, const int32_t* fresh, int32_t* lengths, int32_t* tables, int32_t* free_pages,
@@ -254,9 +328,10 @@ extern "C" int slotscan_release_pages(const slotscan_pages_params* p, const uint
     cudaStream_t st = (cudaStream_t)stream;
     int32_t* s = (int32_t*)scratch;
     if ((int64_t)a.B * a.M <= PG_OWN_ROWS) {
-        release_kernel<true><<<1, sum_threads((int64_t)a.B * a.M), 0, st>>>(a, done, s);
+        release_kernel<<<1, sum_threads((int64_t)a.B * a.M), 0, st>>>(a, done, s);
         return (int)cudaGetLastError();
     }
-    release_kernel<false><<<1, sum_threads(a.B), 0, st>>>(a, done, s);
-    return (int)launch_behind(give_back_kernel, dim3((unsigned)(a.B < 148 * 8 ? a.B : 148 * 8)), dim3(256), st, a, s);
+    const int ctas = a.B < PG_CTAS ? a.B : PG_CTAS;
+    count_back_kernel<<<ctas, PG_RUN_THREADS, 0, st>>>(a, done, s);
+    return (int)launch_behind(give_back_kernel, dim3(ctas), dim3(PG_RUN_THREADS), st, a, s);
 }

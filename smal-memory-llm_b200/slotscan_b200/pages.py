@@ -132,8 +132,11 @@ def _(done, lengths, tables, free, n_free, page):
 
 def release_pages(done, lengths, tables, free, n_free, page):
     """Requests whose `done` (B) is true give their pages back, in the order of requests and pages; their lengths become 0 and their tables
-    minus ones.  In place, as `extend_pages`.  A page that several tables name goes back once for each: share pages only with a request
-    that outlives the others and is the one to give them back."""
+    minus ones.  In place, as `extend_pages`.
+
+    Entries that are no page of the pool are not given back, which is how requests share pages (a common system prompt): one request owns
+    them and outlives the others, and a request that ends without owning them has those entries set to minus one first,
+    `tables[:, :n].masked_fill_((done & shares).unsqueeze(1), -1)`.  A page that is named twice goes back twice."""
     ts = (done, lengths, tables, free, n_free)
     _no_tangents("release_pages", *ts)
     page = _count("release_pages", "page", page)

@@ -2,14 +2,103 @@
 starts mean nothing.  Tolerances as in test_pages_gpu.py, whose batches are used: one rounding to bf16 is off by 2^-8 of the value at most
 (two in the packed attention, of its weights and of the result); a float32 score by E = (D + 16) 2^-24 of the greatest magnitude of
 its terms, a weight by 4 E of itself, a sum over the keys by (keys + 64) 2^-24."""
+import random
 
 import pytest
 import torch
 
-from tests.test_pages_gpu import Batch, _S
+from tests.test_pages_gpu import Batch, Pool, _S
 from tests.test_tokens_gpu import DT, _gen, _rand, within
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ pages that requests share
+
+class SharingPool(Pool):
+    """The turn's definition where entries of a table may be none of the pool: they are not given back."""
+
+    def __init__(self, requests, pages, page, max_pages):
+        super().__init__(requests, pages, page, max_pages)
+        self.pages = pages
+
+    def release(self, done):
+        for b, d in enumerate(done):
+            if d:
+                for p in self.tables[b][:-(-self.lengths[b] // self.page)]:
+                    if 0 <= p < self.pages:
+                        self.free[self.n_free] = p
+                        self.n_free += 1
+                self.lengths[b], self.tables[b] = 0, [-1] * len(self.tables[b])
+
+
+@pytest.mark.parametrize("requests,max_pages,page,registered", [(5, 12, 8, False), (40, 150, 16, False), (300, 70, 8, False), (1500, 40, 8, True), (3, 9000, 8, False)])
+def test_shared_pages_are_given_back_by_their_owner_alone(requests, max_pages, page, registered):
+    """Request 0 owns a prompt that others name in front of their own pages.  They end and come again, with the shared entries taken out
+    of their tables first: every page stays named once, on the stack or by its owner."""
+    S = _S()
+    from slotscan_b200 import pages as P
+    release = P._release if registered else S.release_pages
+    r = random.Random(requests)
+    pages = requests * max_pages
+    pool, state = SharingPool(requests, pages, page, max_pages), S.page_tables(requests, pages, page, max_pages * page)
+    lengths, tables, free, n_free = state
+    common = max_pages // 3
+
+    def extend(new):
+        got = S.extend_pages(torch.tensor(new, device="cuda"), *state, page, 2 ** 17)
+        for a, b in zip(got, pool.extend(new, 2 ** 17)):
+            assert a.tolist() == b
+        return got
+    extend([common * page] + [0] * (requests - 1))
+    for turn in range(3):
+        shares = [False] + [r.random() < 0.6 for _ in range(requests - 1)]
+        for b in range(1, requests):
+            if shares[b]:
+                pool.lengths[b], pool.tables[b][:common] = common * page, pool.tables[0][:common]
+        sh = torch.tensor(shares, device="cuda")
+        lengths[sh], tables[:, :common] = common * page, torch.where(sh[:, None], tables[0, :common], tables[:, :common])
+        extend([0] + [r.randrange(1, 1 + min(60, (max_pages - common) * page)) for _ in range(requests - 1)])
+        done = [False] + [r.random() < 0.7 for _ in range(requests - 1)]
+        gone = torch.tensor(done, device="cuda")
+        # what the requests that end do not own, minus ones in front
+        tables[:, :common].masked_fill_((gone & sh)[:, None], -1)
+        for b in range(1, requests):
+            if done[b] and shares[b]:
+                pool.tables[b][:common] = [-1] * common
+        release(gone, *state, page)
+        pool.release(done)
+        assert tables.tolist() == pool.tables and lengths.tolist() == pool.lengths and n_free.tolist() == [pool.n_free]
+        assert free[:pool.n_free].tolist() == pool.free[:pool.n_free]
+        own = [p for b, row in enumerate(pool.tables) for p in row[common if shares[b] else 0:] if p >= 0]
+        assert sorted(own + pool.free[:pool.n_free]) == list(range(pages)), "a page is lost or held twice"
+        # the sharers that go on end too, so that the next turn begins alike
+        left = [b > 0 for b in range(requests)]
+        tables[1:, :common].masked_fill_((sh & ~gone)[1:, None], -1)
+        for b in range(1, requests):
+            if shares[b] and not done[b]:
+                pool.tables[b][:common] = [-1] * common
+        S.release_pages(torch.tensor(left, device="cuda"), *state, page)
+        pool.release(left)
+        assert n_free.tolist() == [pages - common] == [pool.n_free] and free[:pool.n_free].tolist() == pool.free[:pool.n_free]
+
+
+@pytest.mark.parametrize("M", [40, 5000])
+def test_entries_that_are_none_of_the_pool_are_not_given_back(M):
+    """Anywhere in a table, and more of them than the stack has room for."""
+    S = _S()
+    pages, page = 200, 8
+    pool, state = SharingPool(3, pages, page, M), S.page_tables(3, pages, page, M * page)
+    S.extend_pages(torch.tensor([31 * page, 40 * page - 7, 9], device="cuda"), *state, page, 600)
+    pool.extend([31 * page, 40 * page - 7, 9], 600)
+    for b, j, bad in ((0, 30, -1), (0, 3, pages), (0, 4, 2 ** 31 - 1), (1, 0, -2 ** 31), (1, 39, -7), (1, 33, pages + 1)):
+        state[1][b, j] = pool.tables[b][j] = bad
+    S.release_pages(torch.tensor([True, True, False], device="cuda"), *state, page)
+    pool.release([True, True, False])
+    assert state[3].tolist() == [pool.n_free] and state[2][:pool.n_free].tolist() == pool.free[:pool.n_free] and state[1].tolist() == pool.tables
+    state[0][2], state[1][2, :40] = 40 * page, -1
+    S.release_pages(torch.tensor([False, False, True], device="cuda"), *state, page)
+    assert state[3].tolist() == [pool.n_free]
 
 
 # ------------------------------------------------------------------------------------------------ scores
