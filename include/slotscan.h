@@ -369,6 +369,8 @@ int slotscan_attn_step(const slotscan_attn_step_params* p, const void* q, const 
  * are packed: rows starts[b] to starts[b + 1] of a batch of `tokens` rows are request b's, and rows behind the last belong to none.
  * [The reference has none of this: it scans a context in one call, memlm_sh.py:676.]
  *
+ * A slot is an int32, and what lies beyond those saturates at 2^31 - 1: so pages x page stays below 2^31 wherever slots are made or used.
+ *
  * Turn of a scheduler.  lengths (B) int32: tokens held;  tables (B, M) int32, rows table_stride apart;  free_pages (pages) int32: a stack,
  * of which the first n_free (1) int32 entries are free.  All four are changed in place.
  * slotscan_release_pages: each request with done[b] != 0 gives its pages back, in the order of requests and pages, behind the free

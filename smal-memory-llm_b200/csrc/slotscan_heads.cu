@@ -477,7 +477,7 @@ extern "C" int slotscan_norm_rope_pages(const slotscan_page_append_params* p, co
     const int rc = slotscan_norm_rope_check(p == nullptr ? nullptr : &p->base);
     if (rc != SLOTSCAN_OK) return rc;
     const slotscan_norm_params& n = p->base;
-    if (n.B != 1 || p->pages < 1 || p->page < 8 || p->page > 1024 || (p->page & (p->page - 1))) return SLOTSCAN_E_SHAPE;
+    if (n.B != 1 || p->pages < 1 || p->page < 8 || p->page > 1024 || (p->page & (p->page - 1)) || (int64_t)p->pages * p->page > BIGI) return SLOTSCAN_E_SHAPE;
     if (!strides16(p->v_stride, 3, n.dtype) || !strides16(p->kp_stride, 3, n.dtype) || !strides16(p->vp_stride, 3, n.dtype)) return SLOTSCAN_E_ALIGN;
     if (n.T == 0) return SLOTSCAN_OK;
     if (!q || !k || !v || !slots || !pos || !qo || !kp || !vp || (n.R && !table)) return SLOTSCAN_E_NULL;

@@ -100,7 +100,7 @@ __device__ __forceinline__ void place_rows(const PageArgs& a, const PagePlan& pl
                 const int in_page = at & ((1 << a.shift) - 1);
                 if (in_page == 0) *entry = id;
                 const long long s = ((long long)id << a.shift) + in_page;
-                slot = id >= 0 && s <= BIGI ? (int)s : -1;
+                slot = id >= 0 && s < BIGI ? (int)s : -1;                          // of a page of the pool it is one (slotscan_pages_check)
             }
         }
     }
@@ -290,7 +290,7 @@ using namespace slotscan;
 extern "C" int slotscan_pages_check(const slotscan_pages_params* p) {
     if (p == nullptr) return SLOTSCAN_E_NULL;
     if (p->B < 0 || p->B > (1 << 24) || p->M < 1 || p->M > (1 << 26) || p->pages < 1 || p->tokens < 0 || p->tokens > (1 << 30) || p->page < 8 ||
-        p->page > 1024 || (p->page & (p->page - 1)) || (int64_t)p->M * p->page > (1 << 29) || p->table_stride < p->M)
+        p->page > 1024 || (p->page & (p->page - 1)) || (int64_t)p->M * p->page > (1 << 29) || (int64_t)p->pages * p->page > BIGI || p->table_stride < p->M)
         return SLOTSCAN_E_SHAPE;
     return SLOTSCAN_OK;
 }

@@ -400,7 +400,7 @@ py::object norm_rope_pages(const Tensor& q3, const Tensor& k3, const Tensor& v3,
         return py::none();
     p.pages = (int32_t)kp.size(0);
     p.page = (int32_t)kp.size(1);
-    if (p.pages < 1 || p.page < 8 || p.page > 1024 || (p.page & (p.page - 1))) return py::none();
+    if (p.pages < 1 || p.page < 8 || p.page > 1024 || (p.page & (p.page - 1)) || (int64_t)p.pages * p.page > INT32_MAX) return py::none();
     const c10::cuda::CUDAGuard here(q.device());
     Tensor qo = at::empty(q3.sizes(), q3.options());
     check(slotscan_norm_rope_pages(&p, in(q), in(k), in(v), ptr<float>(table), (const int32_t*)in(slots), (const int32_t*)in(pos), ptr<float>(qw), ptr<float>(kw),

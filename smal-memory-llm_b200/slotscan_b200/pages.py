@@ -21,8 +21,8 @@ from .tokens import (_CODE, _cache_bases, _f32, _host, _i32, _integers, _laid, _
 
 def page_tables(requests, pages, page, max_tokens, device="cuda"):
     """(lengths, tables, free, n_free) of an empty pool: what `extend_pages` and `release_pages` change in place.  `pages` pages of `page`
-    tokens, `requests` places for requests of up to `max_tokens` tokens.  The keys and values themselves are the caller's, for each layer
-    (pages, page, KV, D)."""
+    tokens, fewer than 2^31 - 1 tokens in all, `requests` places for requests of up to `max_tokens` tokens.  The keys and values themselves
+    are the caller's, for each layer (pages, page, KV, D); pages are named 0 to pages - 1."""
     i32 = dict(dtype=torch.int32, device=device)
     return (torch.zeros(requests, **i32), torch.full((requests, max(1, -(-max_tokens // page))), -1, **i32),
             torch.arange(pages - 1, -1, -1, **i32), torch.full((1,), pages, **i32))
@@ -51,6 +51,13 @@ def _pages_params(*sizes):
     return p
 
 
+def _fake_limits(free, page):
+    """The library's limits, of sizes that may be symbols."""
+    _pages_params(1, 1, int(page), 1, 0, 1)
+    if free.shape[0] * page >= 2 ** 31:
+        raise ValueError("slots are int32, so a pool has fewer than 2^31 - 1 of them; got %s pages of %s" % (free.shape[0], page))
+
+
 def _extend_shapes(new, lengths, tables, free, n_free, page, tokens):
     _integers("extend_pages", _sig(new))
     return _state("extend_pages", _sig(new), _sig(lengths), _sig(tables), _sig(free), _sig(n_free), page, tokens)
@@ -75,7 +82,7 @@ _extend_op = torch.library.custom_op("slotscan::extend_pages", mutates_args=("le
 @_extend_op.register_fake
 def _(new, lengths, tables, free, n_free, page, tokens):
     _extend_shapes(new, lengths, tables, free, n_free, page, tokens)
-    _pages_params(1, 1, int(page), 1, 0, 1)                            # the library's limits, of sizes whose others may be symbols
+    _fake_limits(free, page)
     return tuple(lengths.new_empty((n,)) for n in (tokens, tokens, lengths.shape[0] + 1, lengths.shape[0]))
 
 
@@ -127,7 +134,7 @@ _release_op = torch.library.custom_op("slotscan::release_pages", mutates_args=("
 @_release_op.register_fake
 def _(done, lengths, tables, free, n_free, page):
     _release_shapes(done, lengths, tables, free, n_free, page)
-    _pages_params(1, 1, int(page), 1, 0, 1)
+    _fake_limits(free, page)
 
 
 def release_pages(done, lengths, tables, free, n_free, page):
@@ -178,6 +185,8 @@ def _into_shapes(q, k, v, k_pages, v_pages, slots, pos, table, q_weight, k_weigh
     sizes = _norm_checked(what, _one(q), _one(k), table, q_weight, k_weight)
     _type_check(what, q, k, v)
     ks, vs = _pool(what, k_pages, v_pages, q[2], sizes[3], sizes[4])
+    if k_pages[0][0] * k_pages[0][1] >= 2 ** 31:
+        raise ValueError("%s: slots are int32, so a pool has fewer than 2^31 - 1 of them; got %s pages of %s" % (what, k_pages[0][0], k_pages[0][1]))
     if slots[0] != q[0][:1] or pos[0] != q[0][:1]:
         raise ValueError("%s: a slot and a position for each of the %d rows, got %s and %s" % (what, q[0][0], tuple(slots[0]), tuple(pos[0])))
     _integers(what, slots, pos)

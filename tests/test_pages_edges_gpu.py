@@ -101,6 +101,25 @@ def test_entries_that_are_none_of_the_pool_are_not_given_back(M):
     assert state[3].tolist() == [pool.n_free]
 
 
+def test_pools_whose_slots_pass_32_bits_are_refused():
+    """A slot is an int32: tokens of the upper pages would be taken and stored nowhere."""
+    S = _S()
+    many = 2 ** 31 // 1024
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def turn(pages):
+        state = torch.zeros(1, **i32), torch.full((1, 4), -1, **i32), torch.arange(pages, **i32), torch.full((1,), pages, **i32)
+        return state, S.extend_pages(torch.tensor([3], device="cuda"), *state, 1024, 3)
+    for pages in (many, many + 5):
+        with pytest.raises(ValueError):
+            turn(pages)
+        state = torch.zeros(1, **i32), torch.full((1, 4), -1, **i32), torch.arange(pages, **i32), torch.full((1,), pages, **i32)
+        with pytest.raises(ValueError):
+            S.release_pages(torch.tensor([True], device="cuda"), *state, 1024)
+    state, (slots, _, _, taken) = turn(many - 1)
+    assert taken.tolist() == [3] and slots.tolist() == [(many - 2) * 1024 + i for i in range(3)]
+
+
 # ------------------------------------------------------------------------------------------------ scores
 
 def _formula(q, keys, values, dist, slopes, cap, scale):
