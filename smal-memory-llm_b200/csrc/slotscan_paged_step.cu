@@ -560,7 +560,8 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 extern "C" int slotscan_paged_check(const slotscan_paged_params* p) {
     if (p == nullptr) return SLOTSCAN_E_NULL;
     if (p->dtype != SLOTSCAN_F32 && p->dtype != SLOTSCAN_BF16) return SLOTSCAN_E_DTYPE;
-    if (p->N < 0 || p->N > (1 << 28) || p->B < 0 || p->B > (1 << 24) || p->H < 1 || p->H > 65535 || p->KV < 1 || p->H % p->KV || (int64_t)p->N * p->H > 0x7fffffff ||
+    // rows times heads, rounded up to whole CTAs of the join, stay an int
+    if (p->N < 0 || p->N > (1 << 28) || p->B < 0 || p->B > (1 << 24) || p->H < 1 || p->H > 65535 || p->KV < 1 || p->H % p->KV || (int64_t)p->N * p->H > 0x7ffffff8 ||
         p->D < 8 || p->D > 128 || p->D % 8 || p->pages < 1 || p->M < 1 || p->page < 8 || p->page > 1024 || (p->page & (p->page - 1)) ||
         (int64_t)p->M * p->page > (1 << 29) || p->table_stride < p->M)
         return SLOTSCAN_E_SHAPE;

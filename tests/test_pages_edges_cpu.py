@@ -35,3 +35,12 @@ def test_pools_whose_slots_pass_32_bits_are_refused():
                     with pytest.raises(ValueError):
                         call()
             assert S.paged_attention(x, pool, pool, i(2, 5), i(3), pos).shape == x.shape
+
+
+def test_rows_whose_number_passes_32_bits_are_refused():
+    """Requests times heads, rounded up to whole CTAs of the join, fit an int."""
+    from slotscan_b200 import _lib
+    L = _lib.lib()
+    for N, H, ok in ((42966, 49980, True), (49981, 42966, False), (2 ** 24, 2 ** 7, False), (2 ** 24, 2 ** 7 - 1, True)):
+        p = _lib.PagedParams(N, N, H, 1, 8, 4, 16, 5, 0, _lib.BF16, 0.1, 0.0, (8 * H, 8), (128, 8, 8), (128, 8, 8), 5)
+        assert (L.slotscan_paged_check(ctypes.byref(p)) == 0) == ok, (N, H)
