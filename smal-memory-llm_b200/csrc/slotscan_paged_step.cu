@@ -338,6 +338,30 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
                     if (lane % 4 == 0) *reinterpret_cast<float2*>(to + a.D) = make_float2(fmaxf(m[r], -FLT_MAX), sum);
                 }
             }
+            // infinity times the lower part of a weight, which is zero or negative, is not what it is times the weight: such a row anew
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float seen_all = 0.f;
+#pragma unroll
+                for (int i = 0; i < DP / 8; i++) { watch(seen_all, acc[i][2 * r]); watch(seen_all, acc[i][2 * r + 1]); }
+                for (unsigned bad = __ballot_sync(FULL, seen_all != seen_all && g0 + lane / 4 + 8 * r < group); bad != 0;) {
+                    const int from = __ffs(bad) - 1, g = from / 4 + 8 * r, h = hk * group + g0 + g;
+                    bad &= ~(15u << (from & ~3));        // a row's four lanes
+                    const int first = max(c.w.lo, c.w.from + (c.s - (int)(x - begun)) * PS_KEYS), end = min(c.w.hi, c.w.from + (c.s + 1) * PS_KEYS);
+                    float y[4], xm, xl;
+                    careful_row(a, paged_score(a, h), q + c.b * a.qs[0] + h * a.qs[1], k, v, c.b, hk, pos, first, end, y, xm, xl);
+                    __syncwarp();
+                    float* part = plan.part(me, begun != x0, g, a.D);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int d = lane + 32 * e;
+                        if (d >= a.D) continue;
+                        if (whole) o[((size_t)c.b * a.H + h) * a.D + d] = __float2bfloat16_rn(y[e] / xl);
+                        else part[d] = y[e];
+                    }
+                    if (!whole && lane == 0) *reinterpret_cast<float2*>(part + a.D) = make_float2(fmaxf(xm, -FLT_MAX), xl);
+                }
+            }
             begins = true;
         }
         c.next(a);

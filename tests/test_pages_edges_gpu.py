@@ -2,6 +2,7 @@
 starts mean nothing.  Tolerances as in test_pages_gpu.py, whose batches are used: one rounding to bf16 is off by 2^-8 of the value at most
 (two in the packed attention, of its weights and of the result); a float32 score by E = (D + 16) 2^-24 of the greatest magnitude of
 its terms, a weight by 4 E of itself, a sum over the keys by (keys + 64) 2^-24."""
+import math
 import random
 
 import pytest
@@ -212,3 +213,40 @@ def test_caps_of_packed_tokens(cap, dtype):
     for y in (1e30, -2e38, 0.0):
         x.kp[rest] = y
         assert torch.equal(o, call())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("H,KV,D", [(6, 2, 64), (12, 1, 128), (4, 4, 40)])
+def test_a_step_that_sees_infinite_values(H, KV, D, dtype):
+    """Infinity times a weight is infinity, of its sign; infinities of both signs, and NaN, are NaN; the other channels and heads have their
+    numbers.  Requests that one warp has whole, and some that many share."""
+    S = _S()
+    held = [(300, 1), (5, 1), (9000, 1), (40, 1), (16, 1), (1, 1)]
+    x = Batch(held, 16, H, KV, D, dtype, seed=54, peak=0.3)            # weights far from zero
+    call = lambda: S.paged_attention_step(x.q.unsqueeze(1), x.kp, x.vp, x.tables, x.pos).squeeze(1)                        # noqa: E731
+    clean, n = call(), H // KV
+    plus, minus, both, nan = 7, 9, 12, 30
+    want = {}
+    for b, (h, _) in enumerate(held):
+        put = lambda j, c, y: x.vp[x.tables[b, j // 16].long(), j % 16].__setitem__((0, c), y)                                  # noqa: B023, E731
+        put(h // 2, plus, math.inf)
+        put(h - 1, minus, -math.inf)
+        put(0, nan, math.nan)
+        if h > 1:
+            put(h - 1, both, math.inf)
+            put(0, both, -math.inf)
+        want[b] = {plus: math.inf, minus: -math.inf}
+    got = call()
+    for b, (h, _) in enumerate(held):
+        mine = got[b, :n].float()
+        for c, y in want[b].items():
+            assert (mine[:, c] == y).all(), (b, c)
+        assert mine[:, nan].isnan().all() and (h == 1 or mine[:, both].isnan().all())
+    other = torch.ones(D, dtype=torch.bool, device="cuda")
+    other[[plus, minus, both, nan]] = False
+    assert torch.equal(got[:, n:], clean[:, n:])
+    c = clean[:, :n][..., other].double()
+    assert got[:, :n][..., other].isfinite().all()
+    # the row is done anew in another order: both results are within the tolerance of the formula; |v| < 5, scale |q| |k| < 0.3 * 25 * D^(1/2)
+    E = (D + 16) * 2.0 ** -24 * 0.3 * 25 * D ** 0.5
+    within(got[:, :n][..., other], c, 2 * (4 * E + (9000 + 64) * 2.0 ** -24) * 5 + (2.0 ** -7 if dtype == "bf16" else 2.0 ** -22) * (c.abs() + 1e-3), "other channels")
