@@ -22,6 +22,14 @@ namespace slotscan {
 constexpr int PS_WARPS = 4, PS_THREADS = PS_WARPS * 32, PS_KEYS = 16, PS_STAGES = 3;
 constexpr int PS_LEAST = 4;                              // steps of a warp, at least: a part's own cost
 
+// CTAs that an SM holds at a time, which the kernels are compiled for: as many are launched, one round.  bf16: by their rings beyond 64 channels,
+// by registers below; float32: by the registers that its heads take.  Where more were launched than fit, 1.4 GB of keys and values took
+// 291 us in place of 210 (bf16, 12 heads over four, 64 channels), 356 in place of 286 (16 heads over one), 314 in place of 230 (float32,
+// three heads to a key head).
+__host__ __device__ constexpr int step_ctas_per_sm(int dtype, int D, int heads) {
+    return dtype == SLOTSCAN_BF16 ? (D > 64 ? 2 : 4) : heads == 1 ? 4 : heads <= 3 ? 3 : 2;
+}
+
 // What a request's query sees, in steps of 16 keys from a multiple of 16 on (so that no step but those of pages of 8 meets two pages)
 struct Walk {
     int lo, hi, from, steps;
@@ -126,7 +134,7 @@ struct Ids {
 
 // WIDE: 16 query heads to a pair, else 8
 template <int DP, bool WIDE>
-__global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a, StepPlan plan, const bf16* q, const bf16* k, const bf16* v, bf16* o) {
+__global__ void __launch_bounds__(PS_THREADS, step_ctas_per_sm(SLOTSCAN_BF16, DP, 0)) paged_step_mma_kernel(PagedArgs a, StepPlan plan, const bf16* q, const bf16* k, const bf16* v, bf16* o) {
     constexpr int PIECES = DP / 8, PER_PASS = 32 / PIECES, ROW = DP * 2, TILE = PS_KEYS * ROW, R = WIDE ? 2 : 1, HEADS = 8 * R;
     extern __shared__ float4 smem4[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, group = a.H / a.KV;
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_step_mma_kernel(PagedArgs a,
 
 // LPG lanes to a row, G heads to a pair
 template <int LPG, int G>
-__global__ void __launch_bounds__(PS_THREADS) paged_step_kernel(PagedArgs a, StepPlan plan, const float* q, const float* k, const float* v, float* o) {
+__global__ void __launch_bounds__(PS_THREADS, step_ctas_per_sm(SLOTSCAN_F32, LPG * 8, G)) paged_step_kernel(PagedArgs a, StepPlan plan, const float* q, const float* k, const float* v, float* o) {
     constexpr int GROUPS = 32 / LPG, U = 4;              // rows of a turn of a group of lanes
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, group = a.H / a.KV, ch = lane % LPG, grp = lane / LPG;
     const bool live = ch * 8 < a.D;
@@ -548,8 +556,7 @@ static cudaError_t launch_join(const PagedArgs& a, const StepPlan& plan, void* o
 
 static int paged_heads(int group, int dtype) { return dtype == SLOTSCAN_BF16 ? (group > 8 ? 16 : 8) : group > 4 ? 8 : group; }
 static int step_ctas(const PagedArgs& a, int dtype) {
-    // one round: two CTAs of bf16 to an SM, four of narrow rows or float32
-    const int round = 148 * (dtype == SLOTSCAN_BF16 && a.D > 64 ? 2 : 4);
+    const int round = 148 * step_ctas_per_sm(dtype, a.D, paged_heads(a.H / a.KV, dtype));
     const long long steps = (long long)a.B * a.KV * a.chunks * (((long long)a.M << a.shift) / PS_KEYS + 1), want = (steps + PS_LEAST * PS_WARPS - 1) / (PS_LEAST * PS_WARPS);
     return (int)(want < round ? want : round);
 }
