@@ -244,6 +244,21 @@ __device__ __forceinline__ Piece make_piece(const PagedArgs& a, const RowShape& 
     return p;
 }
 
+// A wait for a piece or for the place of one, which may last as long as others' whole pieces (up to 4 million key tiles, 8 s) or the search for
+// the next request that has rows.  It is given up where a warp has given up one of the other waits, each of which is for a tile's time
+// and bounded, and is bounded itself.
+__device__ __forceinline__ bool wait_piece(uint64_t* bar, unsigned parity, const int* fail) {
+    bool ok = false;
+    for (int it = 0; it < (1 << 28); it++) {
+        if ((ok = mbar_try_wait(bar, parity))) break;
+        if (it > (1 << 12)) {
+            __nanosleep(100);
+            if (*reinterpret_cast<const volatile int*>(fail) != 0) break;
+        }
+    }
+    return __all_sync(FULL, ok);
+}
+
 template <int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(PA_THREADS, 1)
 paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant__ PagedMaps maps, const bf16* q, const bf16* kp, const bf16* vp, bf16* o) {
@@ -293,7 +308,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
     bool failed = false;
     unsigned turn = 0;                                   // pieces so far
     auto next = [&]() -> const Piece& {                  // waits for the piece; `failed` where none came
-        failed = failed || !wait_soon_warp(&piece_full[turn % PA_PIECES], (turn / PA_PIECES) & 1);
+        failed = failed || !wait_piece(&piece_full[turn % PA_PIECES], (turn / PA_PIECES) & 1, &s_fail);
         return s_piece[turn % PA_PIECES];
     };
     auto passed = [&] {                                  // by a whole warp that reads no more of it
@@ -531,7 +546,7 @@ paged_attn_kernel(PagedArgs a, RowShape rs, LinePlan plan, const __grid_constant
                     if (p.n1 == p.n0) continue;
                 }
                 const unsigned slot = turn % PA_PIECES;
-                if (turn >= PA_PIECES && !wait_soon_warp(&piece_empty[slot], (turn / PA_PIECES - 1) & 1)) { failed = true; break; }
+                if (turn >= PA_PIECES && !wait_piece(&piece_empty[slot], (turn / PA_PIECES - 1) & 1, &s_fail)) { failed = true; break; }
                 if (lane == 0) {
                     s_piece[slot] = p;
                     arrive(&piece_full[slot]);

@@ -250,3 +250,49 @@ def test_a_step_that_sees_infinite_values(H, KV, D, dtype):
     # the row is done anew in another order: both results are within the tolerance of the formula; |v| < 5, scale |q| |k| < 0.3 * 25 * D^(1/2)
     E = (D + 16) * 2.0 ** -24 * 0.3 * 25 * D ** 0.5
     within(got[:, :n][..., other], c, 2 * (4 * E + (9000 + 64) * 2.0 ** -24) * 5 + (2.0 ** -7 if dtype == "bf16" else 2.0 ** -22) * (c.abs() + 1e-3), "other channels")
+
+
+# ------------------------------------------------------------------------------------------------ layouts and arguments
+
+def test_pieces_that_take_long():
+    """One request of 2^29 positions (one page named often) over 16 heads: a CTA's piece is of 450,000 key tiles, for which the warp that writes the
+    pieces waits."""
+    from slotscan_b200 import _lib
+    S = _S()
+    g = _gen(56)
+    H, D, page, M = 16, 64, 1024, 2 ** 19
+    kp, vp = _rand(g, 1, page, H, D).bfloat16(), _rand(g, 1, page, H, D).bfloat16()
+    q = _rand(g, 1, H, D).bfloat16()
+    tables = torch.zeros(1, M, dtype=torch.int32, device="cuda")
+    _lib.device_status()
+    o = S.paged_attention(q, kp, vp, tables, torch.tensor([0, 1], device="cuda"), torch.tensor([M * page - 1], device="cuda"))
+    assert _lib.device_status() == 0
+    want, size, _ = _formula(q, kp, vp, torch.zeros(1, page, device="cuda"), None, 0.0, D ** -0.5)
+    # a half adds up 8 products a key tile, and its share of the sum of the weights: each addition off by 2^-23 of what is there at most
+    tiles = M * page // 128 * H / 148 / 2
+    within(o, want, 9 * tiles * 2.0 ** -23 * size + 2.0 ** -8 * (size + want.abs()), "o")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_requests_without_rows(dtype):
+    """Half a million places, of which the first and the last have rows: the search from one to the other takes longer than a key tile by far."""
+    from slotscan_b200 import _lib
+    S = _S()
+    g = _gen(57)
+    dt = DT[dtype]
+    B, H, KV, D, page = 2 ** 19, 4, 2, 64, 64
+    kp, vp = _rand(g, 2, page, KV, D).to(dt), _rand(g, 2, page, KV, D).to(dt)
+    q = (2 * _rand(g, 40, H, D)).to(dt)
+    starts = torch.full((B + 1,), 25, dtype=torch.int32, device="cuda")
+    starts[0], starts[-1] = 0, 40
+    tables = torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    tables[-1] = 1
+    pos = torch.cat((torch.arange(30, 55), torch.arange(40, 55))).cuda()
+    _lib.device_status()
+    o = S.paged_attention(q, kp, vp, tables, starts, pos)
+    assert _lib.device_status() == 0
+    for r in (0, 24, 25, 39):
+        n = int(pos[r]) + 1
+        k, v = (t[int(r >= 25), :n].unsqueeze(0) for t in (kp, vp))
+        want, size, worst = _formula(q[r:r + 1], k, v, torch.zeros(1, n, device="cuda"), None, 0.0, D ** -0.5)
+        within(o[r:r + 1], want, _allowed(want, size, worst, D, n, dtype, False), "row %d" % r)
