@@ -129,8 +129,6 @@ __device__ __forceinline__ void line_sum(T v, T* s_sum, T* s_warp) {
     s_sum[tid] = v;
     __syncthreads();
 }
-// x / d of x >= 0, d > 0; by 32 bits where they do: the shares are found before anything else can begin
-__device__ __forceinline__ long long line_div(long long x, int d) { return x >> 32 == 0 ? (unsigned)x / (unsigned)d : x / d; }
 template <typename T>
 __device__ __forceinline__ int first_above(const T* s_sum, T x) {                  // first thread whose sum is greater
     int lo = 0, hi = PA_THREADS - 1;
@@ -171,17 +169,17 @@ __device__ __forceinline__ void line_share(const PagedArgs& a, const RowShape& r
     walk(min(tid * per_u, tiles), min((tid + 1) * per_u, tiles), [&](int, int, const RowTile& t) { v += PA_TILE_COST + (t.n1 - t.n0) * step_cost(rs, t); return true; });
     line_sum(v, s_steps, s_warp1);
     if (tid == 0) {
-        const long long total = s_steps[PA_THREADS - 1] * pairs, per = max(line_div(total + gridDim.x - 1, gridDim.x), (long long)PA_TWO), x0 = blockIdx.x * per;     // a key tile to each
+        const long long total = s_steps[PA_THREADS - 1] * pairs, per = max((total + gridDim.x - 1) / gridDim.x, (long long)PA_TWO), x0 = blockIdx.x * per;     // a key tile to each
         LineCursor c = {};
         c.left = max(min(per, total - x0), 0ll);
         if (c.left > 0) {
-            const int t = first_above(s_steps, line_div(x0, pairs));
+            const int t = first_above(s_steps, x0 / pairs);
             long long at = (t > 0 ? s_steps[t - 1] : 0) * pairs;
             walk(t * per_u, tiles, [&](int b, int tile, const RowTile& rt) {
                 const int each = step_cost(rs, rt), steps = PA_TILE_COST + (rt.n1 - rt.n0) * each;
                 if (at + (long long)steps * pairs <= x0) { at += (long long)steps * pairs; return true; }
                 c.b = b; c.tile = tile; c.t = rt; c.each = each;
-                c.pair = (int)line_div(x0 - at, steps);
+                c.pair = (int)((x0 - at) / steps);
                 c.n = (int)(x0 - at - (long long)c.pair * steps);
                 return false;
             });
