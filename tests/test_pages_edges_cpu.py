@@ -37,6 +37,21 @@ def test_pools_whose_slots_pass_32_bits_are_refused():
             assert S.paged_attention(x, pool, pool, i(2, 5), i(3), pos).shape == x.shape
 
 
+def test_scratch_of_the_step_is_bounded():
+    """20 MB of parts and 8 bytes a request, whatever the heads, the channels and the types."""
+    from slotscan_b200 import _lib
+    L, most = _lib.lib(), 0
+    for dtype in (_lib.F32, _lib.BF16):
+        for D in (8, 40, 64, 72, 128):
+            for H, KV in ((1, 1), (3, 1), (4, 2), (8, 1), (12, 4), (16, 1), (40, 1), (64, 8), (200, 2)):
+                for B, M in ((1, 1), (64, 4096), (5000, 65536)):
+                    p = _lib.PagedParams(B, B, H, KV, D, 1000, 16, M, 0, dtype, 0.1, 0.0, (H * D, D), (16 * KV * D, KV * D, D), (16 * KV * D, KV * D, D), M)
+                    size = L.slotscan_paged_step_scratch_bytes(ctypes.byref(p))
+                    assert 0 < size <= 20.1e6 + 8 * B + 32, (dtype, D, H, KV, B, M, size)
+                    most = max(most, size)
+    assert most > 19e6
+
+
 def test_rows_whose_number_passes_32_bits_are_refused():
     """Requests times heads, rounded up to whole CTAs of the join, fit an int."""
     from slotscan_b200 import _lib

@@ -2,6 +2,7 @@
 starts mean nothing.  Tolerances as in test_pages_gpu.py, whose batches are used: one rounding to bf16 is off by 2^-8 of the value at most
 (two in the packed attention, of its weights and of the result); a float32 score by E = (D + 16) 2^-24 of the greatest magnitude of
 its terms, a weight by 4 E of itself, a sum over the keys by (keys + 64) 2^-24."""
+import ctypes
 import math
 import random
 
@@ -254,6 +255,26 @@ def test_a_step_that_sees_infinite_values(H, KV, D, dtype):
 
 # ------------------------------------------------------------------------------------------------ layouts and arguments
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 8), (40, 256)])
+def test_pages_whose_heads_lie_outside_their_rows(D, page, dtype):
+    """A pool laid out (pages, KV, page, D), read and written in place through its transposed view."""
+    S = _S()
+    x = Batch([(300, 40), (1000, 1), (90, 90)], page, 6, 3, D, dtype, seed=55)
+    kt, vt = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (x.kp, x.vp))
+    assert not kt.is_contiguous() and kt.stride(2) == page * D
+    kw = dict(window=500, slopes=x.slopes)
+    assert torch.equal(S.paged_attention(x.q, x.kp, x.vp, x.tables, x.starts, x.pos, **kw), S.paged_attention(x.q, kt, vt, x.tables, x.starts, x.pos, **kw))
+    q1, p1 = x.q[[39, 40, 130]].unsqueeze(1), x.pos[[39, 40, 130]]
+    assert torch.equal(S.paged_attention_step(q1, x.kp, x.vp, x.tables, p1, **kw), S.paged_attention_step(q1, kt, vt, x.tables, p1, **kw))
+    n = 37
+    slots = torch.randperm(x.kp.shape[0] * page, device="cuda", generator=x.g)[:n]
+    k, v = x.q[:n, :3], x.q[:n, 3:]
+    args = (slots, torch.arange(n, device="cuda"), S.rope_table(n, 32 if D >= 32 else 16, device="cuda"))
+    assert torch.equal(S.norm_rope_pages(x.q[:n], k, v, x.kp, x.vp, *args), S.norm_rope_pages(x.q[:n], k, v, kt, vt, *args))
+    assert torch.equal(x.kp.nan_to_num(), kt.nan_to_num()) and torch.equal(x.vp.nan_to_num(7.0), vt.nan_to_num(7.0))
+
+
 def test_pieces_that_take_long():
     """One request of 2^29 positions (one page named often) over 16 heads: a CTA's piece is of 450,000 key tiles, for which the warp that writes the
     pieces waits."""
@@ -296,3 +317,37 @@ def test_many_requests_without_rows(dtype):
         k, v = (t[int(r >= 25), :n].unsqueeze(0) for t in (kp, vp))
         want, size, worst = _formula(q[r:r + 1], k, v, torch.zeros(1, n, device="cuda"), None, 0.0, D ** -0.5)
         within(o[r:r + 1], want, _allowed(want, size, worst, D, n, dtype, False), "row %d" % r)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_starts_that_are_no_starts_touch_nothing_else(dtype):
+    """The C call with an output and a scratch that lie between patterns: the patterns stay, whatever `starts` holds; starts that do not fall are
+    taken into the batch."""
+    from slotscan_b200 import _lib
+    from slotscan_b200 import pages as P
+    S = _S()
+    x = Batch([(300, 20), (70, 6), (200, 10)], 16, 6, 3, 64, dtype, seed=9)
+    N = len(x.pos)
+    p = P._paged_params("paged_attention", x.q, x.kp, x.vp, x.tables, x.starts, x.pos, None, None, 0, 0.0, 0.125)
+    L, ptr = _lib.lib(), lambda t: ctypes.c_void_p(t.data_ptr())                               # noqa: E731
+    size = L.slotscan_paged_attn_scratch_bytes(ctypes.byref(p))
+
+    def call(starts):
+        out = torch.full((3, N, 6, 64), 77.0, dtype=x.q.dtype, device="cuda")
+        room = (size + 255) // 256 * 256
+        scratch = torch.full((room + 2 * 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+        inner = scratch[4096:4096 + room]
+        st = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        rc = L.slotscan_paged_attn(ctypes.byref(p), ptr(x.q), ptr(x.kp), ptr(x.vp), ptr(x.tables), ptr(st), ptr(x.pos), None, None, ptr(out[1]), ptr(inner), size,
+                                   ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert (out[0] == 77).all() and (out[2] == 77).all() and (scratch[:4096] == 0x5a).all() and (scratch[4096 + size:] == 0x5a).all()
+        return out[1]
+    for starts in ([0, 36, 0, 36], [30, 20, 10, 0], [36, 0, 36, 0], [2 ** 31 - 1, -2 ** 31, 5, -1]):
+        call(starts)
+    for starts, same in (([-5, 20, 26, 2 ** 31 - 1], [0, 20, 26, 36]), ([-2 ** 31, -1, 0, 40], [0, 0, 0, 36]), ([36, 36, 36, 36], None), ([50, 60, 70, 80], None)):
+        got = call(starts)
+        want = torch.zeros_like(got) if same is None else S.paged_attention(x.q, x.kp, x.vp, x.tables, torch.tensor(same, device="cuda"), x.pos)
+        assert ((got == want) | (got.isnan() & want.isnan())).all(), starts                  # rows of pages that no token fills are NaN here, and seen
+    assert _lib.device_status() == 0
