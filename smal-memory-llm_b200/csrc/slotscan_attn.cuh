@@ -152,6 +152,36 @@ __device__ __forceinline__ void careful_query(const AttnArgs& a, const RowInputs
     lse = sp.hi - sp.lo == 1 ? INFINITY : m + log2f(l);
     delta = d * inv;
 }
+// The unscaled o of a query at `at` over keys [lo, hi), with the maximum (base-2 exponent) and the sum of their weights.  where(j, key, value) says
+// where they lie; a null key has zeros.
+template <typename T, typename W>
+__device__ __forceinline__ void careful_keys(const Score& sc, const T* q, int D, int at, int lo, int hi, W where, float (&o)[4], float& m, float& l) {
+    float x[4], y[4], unused;
+    lane_row(x, q, D);
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] = 0.f;
+    for (int j = lo; j < hi; j++) {
+        const T *key, *value;
+        where(j, key, value);
+#pragma unroll
+        for (int c = 0; c < 4; c++) y[c] = 0.f;
+        if (key != nullptr) lane_row(y, key, D);
+        const float z = score2(sc, lane_dot(x, y), at - j, unused);
+        const float top = fmaxf(m, z), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), p = exp2f(z - base);
+        if (key != nullptr) lane_row(y, value, D);
+        l = fmaf(l, f, p);
+        bool gone = true;                                // NaN stays NaN
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            o[c] = p != 0.f ? fmaf(p, y[c], o[c] * f) : o[c] * f;
+            gone = gone && (isnan(o[c]) || (threadIdx.x & 31) + 32 * c >= D);
+        }
+        m = top;
+        if (__all_sync(FULL, gone)) break;
+    }
+}
 // weight and scaled gradient of the score of a visible pair
 __device__ __forceinline__ void careful_pair(const AttnArgs& a, const Score& sc, float s, float dp, int dist, float lse, float delta, float& p, float& ds) {
     float f;

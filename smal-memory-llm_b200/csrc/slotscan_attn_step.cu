@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
     constexpr int PIECES = DP / 8, PER_PASS = 32 / PIECES, ROW = DP * 2, TILE = SM_KEYS * ROW, R = WIDE ? 2 : 1, HEADS = 8 * R;
     extern __shared__ float4 smem4[];
     __shared__ Softmax s_sm[SM_WARPS][HEADS];
+    __shared__ int s_bad[HEADS];                         // its output here is not finite
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const int split = blockIdx.x, hk = blockIdx.y / a.chunks, b = blockIdx.z, group = a.H / a.KV, g0 = (blockIdx.y % a.chunks) * HEADS;
     const long long pos = a.pos[b];
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                     // the ring becomes the warps' outputs
     float* s_acc = reinterpret_cast<float*>(smem4);      // [warp][head][DP]
+    if (threadIdx.x < HEADS) s_bad[threadIdx.x] = 0;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         l[r] += __shfl_xor_sync(FULL, l[r], 1);
@@ -289,7 +291,8 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
             *reinterpret_cast<float2*>(&s_acc[(warp * HEADS + lane / 4 + 8 * r) * DP + c * 8 + (lane % 4) * 2]) = make_float2(acc[c][2 * r], acc[c][2 * r + 1]);
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < min(HEADS, group - g0) * a.D; x += SM_WARPS * 32) {
+    const int heads = min(HEADS, group - g0);
+    for (int x = threadIdx.x; x < heads * a.D; x += SM_WARPS * 32) {
         const int g = x / a.D, d = x % a.D, h = hk * group + g0 + g;
         float top = -INFINITY, ll = 0.f, sum = 0.f;
 #pragma unroll
@@ -301,12 +304,38 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
             ll = fmaf(s_sm[i][g].l, f, ll);
             sum = fmaf(s_acc[(i * HEADS + g) * DP + d], f, sum);
         }
+        if (!isfinite(sum)) s_bad[g] = 1;
         if (a.splits == 1) o[((size_t)b * a.H + h) * a.D + d] = __float2bfloat16_rn(n == 0 ? 0.f : sum / ll);
         else {
             float* pp = part + (((size_t)b * a.H + h) * a.splits + split) * (a.D + 2);
             pp[d] = sum;
             if (d == 0) { pp[a.D] = split_max(n, top); pp[a.D + 1] = ll; }
         }
+    }
+    // infinity times the lower part of a weight, which is zero or negative, is not what it is times the weight: such a head anew
+    __syncthreads();
+    for (int g = warp; g < heads; g += SM_WARPS) {
+        if (s_bad[g] == 0) continue;
+        const int h = hk * group + g0 + g;
+        AttnArgs s;
+        s.scale = a.scale; s.cap = a.cap; s.slopes = a.slopes;
+        float y[4], m1, l1;
+        careful_keys(Score(s, h), q + b * a.qs[0] + h * a.qs[1], a.D, n - 1, lo, hi,
+                     [&](int j, const bf16*& key, const bf16*& value) {
+                         const int r = row0 + j, row = r >= a.L ? r - a.L : r;
+                         key = kb + row * a.ks[1];
+                         value = vb + row * a.vs[1];
+                     },
+                     y, m1, l1);
+        float* pp = part + (((size_t)b * a.H + h) * a.splits + split) * (a.D + 2);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = lane + 32 * e;
+            if (d >= a.D) continue;
+            if (a.splits == 1) o[((size_t)b * a.H + h) * a.D + d] = __float2bfloat16_rn(y[e] / l1);
+            else pp[d] = y[e];
+        }
+        if (a.splits > 1 && lane == 0) { pp[a.D] = split_max(n, m1); pp[a.D + 1] = l1; }
     }
 }
 

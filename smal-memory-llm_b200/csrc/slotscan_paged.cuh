@@ -55,30 +55,14 @@ struct RowShape { int heads, tokens; };                  // of a tile, or of a h
 template <typename T>
 __device__ __forceinline__ void careful_row(const PagedArgs& a, const Score& sc, const T* q, const T* kp, const T* vp, int b, int hk, int at, int lo, int hi,
                                             float (&o)[4], float& m, float& l) {
-    float x[4], y[4], unused;
-    lane_row(x, q, a.D);
-    m = -INFINITY;
-    l = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; c++) o[c] = 0.f;
-    for (int j = lo; j < hi; j++) {
-        const int id = page_of(a, b, j), row = j & ((1 << a.shift) - 1);
-#pragma unroll
-        for (int c = 0; c < 4; c++) y[c] = 0.f;
-        if (id >= 0) lane_row(y, kp + id * a.ks[0] + row * a.ks[1] + hk * a.ks[2], a.D);
-        const float z = score2(sc, lane_dot(x, y), at - j, unused);
-        const float top = fmaxf(m, z), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), p = exp2f(z - base);
-        if (id >= 0) lane_row(y, vp + id * a.vs[0] + row * a.vs[1] + hk * a.vs[2], a.D);
-        l = fmaf(l, f, p);
-        bool gone = true;                                // NaN stays NaN
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            o[c] = p != 0.f ? fmaf(p, y[c], o[c] * f) : o[c] * f;
-            gone = gone && (isnan(o[c]) || (threadIdx.x & 31) + 32 * c >= a.D);
-        }
-        m = top;
-        if (__all_sync(FULL, gone)) break;
-    }
+    const int in_page = (1 << a.shift) - 1;
+    careful_keys(sc, q, a.D, at, lo, hi,
+                 [&](int j, const T*& key, const T*& value) {
+                     const int id = page_of(a, b, j), row = j & in_page;
+                     key = id >= 0 ? kp + id * a.ks[0] + row * a.ks[1] + hk * a.ks[2] : nullptr;
+                     value = id >= 0 ? vp + id * a.vs[0] + row * a.vs[1] + hk * a.vs[2] : nullptr;
+                 },
+                 o, m, l);
 }
 
 static inline PagedArgs paged_args(const slotscan_paged_params& p, const int32_t* tables, const int32_t* starts, const int32_t* pos, const int32_t* start,

@@ -1,8 +1,10 @@
-"""Attention over tokens at places that float32 does not hold."""
+"""Attention over tokens at places that float32 does not hold, and single tokens that see infinite values."""
+import math
+
 import pytest
 import torch
 
-from tests.test_tokens_gpu import DT, _gen, _rand
+from tests.test_tokens_gpu import DT, _gen, _rand, within
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +29,32 @@ def test_distance_bias_at_far_places(window, cap, dtype):
         return o, qq.grad, kk.grad[:, before:], vv.grad[:, before:]
     for name, a, b in zip(("o", "dq", "dk", "dv"), run(0), run(2 ** 24)):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,H,KV,D", [(5, 100, 6, 2, 64), (2, 20000, 12, 1, 128), (3, 700, 4, 4, 40)])
+def test_a_step_that_sees_infinite_values(B, L, H, KV, D, dtype):
+    """Infinity times a weight is infinity, of its sign; infinities of both signs, and NaN, are NaN; other channels, heads and sequences have
+    their numbers."""
+    import slotscan_b200 as S
+    g = _gen(61)
+    dt = DT[dtype]
+    kc, vc = _rand(g, B, L, KV, D).to(dt), _rand(g, B, L, KV, D).to(dt)
+    q = (0.3 * _rand(g, B, 1, H, D)).to(dt)                            # weights far from zero
+    pos = torch.tensor([L + 30, L // 2, 3 * L - 1, 7, L][:B], device="cuda")
+    clean, n = S.token_attention_step(q, kc, vc, pos), H // KV
+    plus, minus, both, nan = 7, 9, 12, 30
+    for b in range(B - 1):                                             # the last sequence stays as it is
+        last = int(pos[b])
+        first = max(last - L + 1, 0)
+        for j, c, y in ((first, plus, math.inf), (last, minus, -math.inf), (first, both, math.inf), (last, both, -math.inf), ((first + last) // 2, nan, math.nan)):
+            vc[b, j % L, 0, c] = y
+    got = S.token_attention_step(q, kc, vc, pos)
+    assert torch.equal(got[B - 1], clean[B - 1]) and torch.equal(got[:, :, n:], clean[:, :, n:])
+    mine = got[:B - 1, 0, :n].float()
+    assert (mine[..., plus] == math.inf).all() and (mine[..., minus] == -math.inf).all() and mine[..., both].isnan().all() and mine[..., nan].isnan().all()
+    rest = [c for c in range(D) if c not in (plus, minus, both, nan)]
+    a, b = got[:B - 1, 0, :n][..., rest].double(), clean[:B - 1, 0, :n][..., rest].double()
+    # done anew in another order: both are within the tolerance of the formula; |v| < 5.5, scale |q| |k| < 0.3 * 30 * D^(1/2)
+    E = (D + 16) * 2.0 ** -24 * 0.3 * 30 * D ** 0.5
+    within(a, b, 2 * (4 * E + (L + 64) * 2.0 ** -24) * 5.5 + (2.0 ** -7 if dtype == "bf16" else 2.0 ** -22) * (b.abs() + 1e-3), "other channels")
