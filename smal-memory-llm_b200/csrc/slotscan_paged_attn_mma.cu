@@ -8,12 +8,14 @@
 // Requests are of uneven lengths, and few new tokens see many keys: so the work is cut by tiles of keys, not by tiles of rows.  All (tile of
 // rows, key head, tile of keys) stand in one line, which is shared out evenly among one CTA to an SM.  A CTA writes results where it has a tile
 // of rows whole, else its part (at most two to a CTA), and a second kernel joins the parts of the tiles that were cut, in their order.
-// p is rounded to bf16 for its product, as its operand type asks; the sum of the softmax takes it unrounded.
+// p is rounded to bf16 for its product, as its operand type asks; the sum of the softmax takes it unrounded.  Results are off by 0.0023 of
+// their norm so, 0.0017 of which is their own rounding.
 //
-// A chunk of 2,048 tokens of 12 heads over 65,536 keys of four: 750 us, 1,083 TFLOP/s.  A key tile takes 3,770 cycles: a half's softmax
-// 2,420 of them, its two products and their hand-overs 1,320, during which the other half's softmax runs.  A third of the special function
-// unit's and half of the tensor cores' time is left.  Handing the weights over 64 keys at a time took 793 us.  Few rows over many keys are bound by
-// memory: 16 x 5 tokens over 32,768 keys 134 us, 5.2 TB/s.
+// A chunk of 2,048 tokens of 12 heads over 65,536 keys of four: 826 us in a run of twenty (983 TFLOP/s), 930 in runs of seconds (873), in which
+// the power cap holds the clock at 1,680 MHz of 1,965.  A key tile takes 3,770 cycles: a half's softmax 2,420 of them, its two products and
+// their hand-overs 1,320, during which the other half's softmax runs.  A third of the special function unit's and half of the tensor cores'
+// time is left.  Handing the weights over 64 keys at a time took 6 % more.  Few rows over many keys are bound by memory: 16 x 5 tokens over
+// up to 32,768 keys 129 to 142 us, 5.4 to 4.9 TB/s.
 #include "slotscan_attn_scores.cuh"
 #include "slotscan_launch.h"
 #include "slotscan_paged.cuh"

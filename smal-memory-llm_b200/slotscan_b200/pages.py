@@ -99,7 +99,8 @@ def extend_pages(new, lengths, tables, free, n_free, page, tokens):
     The new tokens are packed into a batch of `tokens` rows: rows starts[b] to starts[b + 1] are request b's, `slots` and `pos` of a row say
     where its token goes and at which position it stands, minus ones where there is none.  A request is served whole (taken[b] = new[b]) or
     not at all (0; its length stays, its rows hold minus ones): not where its table or the batch has no room for it, and not where it needs
-    pages and, with the requests before it, more than are free.  Negative counts are none."""
+    pages and, with the requests before it, more than are free.  Negative counts are none.  The four results of an ordinary call lie side
+    by side in one allocation, which lives as long as any of them."""
     ts = (new, lengths, tables, free, n_free)
     _no_tangents("extend_pages", *ts)
     page, tokens = _count("extend_pages", "page", page), _count("extend_pages", "tokens", tokens)
@@ -337,7 +338,8 @@ def paged_attention(q, k_pages, v_pages, tables, starts, pos, window=0, cap=0.0,
     ones in one batch.  Rows starts[b] to starts[b + 1] of q (N,H,D) are request b's; the first stands at its pos (N), the others behind it
     (`extend_pages` gives both), and the keys of all of them are in the pages (`norm_rope_pages`).  A row sees the positions up to its own, of
     the last `window` (0: all), from start[b] on (None: 0); a row of no token, or that sees nothing, gives zeros.  `cap`, `slopes` and `scale` as
-    in `token_attention`.  A page outside the pool reads as zeros; rows of pages that a token does not see do not reach it."""
+    in `token_attention`.  A page outside the pool reads as zeros; rows of pages that a token does not see do not reach it.  An infinite value that
+    it sees gives infinity of its sign (NaN with one of the other sign)."""
     if starts is None:
         raise ValueError("paged_attention: packed queries need their starts; of one query for each request use paged_attention_step")
     return _attend("paged_attention", q, k_pages, v_pages, tables, starts, pos, window, cap, slopes, start, scale)
