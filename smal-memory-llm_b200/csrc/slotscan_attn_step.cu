@@ -149,13 +149,39 @@ __global__ void __launch_bounds__(ST_THREADS) attn_step_kernel(StepArgs a, const
 // ---- bf16 ----
 constexpr int SM_WARPS = 4, SM_KEYS = 16, SM_STAGES = 3;
 
-// WIDE: 16 query heads to a CTA, else 8
-template <int DP, bool WIDE>
+// What a query sees: positions first + 0 to first + n - 1, the first of them in row row0 of its ring
+struct Seen { int n, row0; };
+__device__ __forceinline__ Seen seen_of(const StepArgs& a, int b) {
+    const long long pos = a.pos[b];
+    const long long first = max(max(pos - a.window + 1, a.start != nullptr ? (long long)a.start[b] : 0ll), 0ll);
+    const int n = (int)max(pos - first + 1, 0ll);
+    return {n, n > 0 ? (int)(first % a.L) : 0};
+}
+// The output of a head over [lo, hi) of what it sees, unscaled, by a warp, where the products' is not finite: infinity times the lower part of
+// a weight, which is zero or negative, is not what it is times the weight.
+__device__ __forceinline__ void redo_head(const StepArgs& a, const bf16* q, const bf16* k, const bf16* v, int b, int h, Seen sn, int lo, int hi, float (&y)[4], float& m, float& l) {
+    const int hk = h / (a.H / a.KV);
+    const bf16* kb = k + b * a.ks[0] + hk * a.ks[2];
+    const bf16* vb = v + b * a.vs[0] + hk * a.vs[2];
+    AttnArgs s;
+    s.scale = a.scale; s.cap = a.cap; s.slopes = a.slopes;
+    careful_keys(Score(s, h), q + b * a.qs[0] + h * a.qs[1], a.D, sn.n - 1, lo, hi,
+                 [&](int j, const bf16*& key, const bf16*& value) {
+                     const int r = sn.row0 + j, row = r >= a.L ? r - a.L : r;
+                     key = kb + row * a.ks[1];
+                     value = vb + row * a.vs[1];
+                 },
+                 y, m, l);
+}
+
+// WIDE: 16 query heads to a CTA, else 8.
+// WHOLE: one split, whose heads that are not finite are redone here; those of several the join redoes (in here it cost 8 of 131,072 2 %).
+template <int DP, bool WIDE, bool WHOLE>
 __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a, const bf16* q, const bf16* k, const bf16* v, bf16* o, float* part) {
     constexpr int PIECES = DP / 8, PER_PASS = 32 / PIECES, ROW = DP * 2, TILE = SM_KEYS * ROW, R = WIDE ? 2 : 1, HEADS = 8 * R;
     extern __shared__ float4 smem4[];
     __shared__ Softmax s_sm[SM_WARPS][HEADS];
-    __shared__ int s_bad[HEADS];                         // its output here is not finite
+    __shared__ int s_bad[HEADS];                         // a warp's output of it is not finite
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const int split = blockIdx.x, hk = blockIdx.y / a.chunks, b = blockIdx.z, group = a.H / a.KV, g0 = (blockIdx.y % a.chunks) * HEADS;
     const long long pos = a.pos[b];
@@ -166,6 +192,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
     const uint32_t ring = smem_u32(smem4) + warp * SM_STAGES * 2 * TILE;
     const bf16* kb = k + b * a.ks[0] + hk * a.ks[2];
     const bf16* vb = v + b * a.vs[0] + hk * a.vs[2];
+    if (WHOLE && threadIdx.x < HEADS) s_bad[threadIdx.x] = 0;
     const int piece = lane % PIECES, sub = lane / PIECES;
     auto load = [&](int step) {                          // 16 keys and values of this warp's step into its ring
         const int j0 = lo + (step * SM_WARPS + warp) * SM_KEYS;
@@ -280,12 +307,17 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                     // the ring becomes the warps' outputs
     float* s_acc = reinterpret_cast<float*>(smem4);      // [warp][head][DP]
-    if (threadIdx.x < HEADS) s_bad[threadIdx.x] = 0;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         l[r] += __shfl_xor_sync(FULL, l[r], 1);
         l[r] += __shfl_xor_sync(FULL, l[r], 2);
         if (lane % 4 == 0) s_sm[warp][lane / 4 + 8 * r] = {m[r], l[r]};
+        if constexpr (WHOLE) {
+            float w = 0.f;
+#pragma unroll
+            for (int c = 0; c < DP / 8; c++) { watch(w, acc[c][2 * r]); watch(w, acc[c][2 * r + 1]); }
+            if (w != w) s_bad[lane / 4 + 8 * r] = 1;
+        }
 #pragma unroll
         for (int c = 0; c < DP / 8; c++)
             *reinterpret_cast<float2*>(&s_acc[(warp * HEADS + lane / 4 + 8 * r) * DP + c * 8 + (lane % 4) * 2]) = make_float2(acc[c][2 * r], acc[c][2 * r + 1]);
@@ -294,6 +326,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
     const int heads = min(HEADS, group - g0);
     for (int x = threadIdx.x; x < heads * a.D; x += SM_WARPS * 32) {
         const int g = x / a.D, d = x % a.D, h = hk * group + g0 + g;
+        if (WHOLE && s_bad[g] != 0) continue;
         float top = -INFINITY, ll = 0.f, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < SM_WARPS; i++) top = fmaxf(top, s_sm[i][g].m);
@@ -304,66 +337,79 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
             ll = fmaf(s_sm[i][g].l, f, ll);
             sum = fmaf(s_acc[(i * HEADS + g) * DP + d], f, sum);
         }
-        if (!isfinite(sum)) s_bad[g] = 1;
-        if (a.splits == 1) o[((size_t)b * a.H + h) * a.D + d] = __float2bfloat16_rn(n == 0 ? 0.f : sum / ll);
+        if (WHOLE) o[((size_t)b * a.H + h) * a.D + d] = __float2bfloat16_rn(n == 0 ? 0.f : sum / ll);
         else {
             float* pp = part + (((size_t)b * a.H + h) * a.splits + split) * (a.D + 2);
             pp[d] = sum;
             if (d == 0) { pp[a.D] = split_max(n, top); pp[a.D + 1] = ll; }
         }
     }
-    // infinity times the lower part of a weight, which is zero or negative, is not what it is times the weight: such a head anew
-    __syncthreads();
-    for (int g = warp; g < heads; g += SM_WARPS) {
-        if (s_bad[g] == 0) continue;
-        const int h = hk * group + g0 + g;
-        AttnArgs s;
-        s.scale = a.scale; s.cap = a.cap; s.slopes = a.slopes;
-        float y[4], m1, l1;
-        careful_keys(Score(s, h), q + b * a.qs[0] + h * a.qs[1], a.D, n - 1, lo, hi,
-                     [&](int j, const bf16*& key, const bf16*& value) {
-                         const int r = row0 + j, row = r >= a.L ? r - a.L : r;
-                         key = kb + row * a.ks[1];
-                         value = vb + row * a.vs[1];
-                     },
-                     y, m1, l1);
-        float* pp = part + (((size_t)b * a.H + h) * a.splits + split) * (a.D + 2);
+    if constexpr (WHOLE) {
+        for (int g = warp; g < heads; g += SM_WARPS) {
+            if (s_bad[g] == 0) continue;
+            const int h = hk * group + g0 + g;
+            float y[4], m1, l1;
+            redo_head(a, q, k, v, b, h, {n, row0}, lo, hi, y, m1, l1);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int d = lane + 32 * e;
-            if (d >= a.D) continue;
-            if (a.splits == 1) o[((size_t)b * a.H + h) * a.D + d] = __float2bfloat16_rn(y[e] / l1);
-            else pp[d] = y[e];
+            for (int e = 0; e < 4; e++)
+                if (lane + 32 * e < a.D) o[((size_t)b * a.H + h) * a.D + lane + 32 * e] = __float2bfloat16_rn(y[e] / l1);
         }
-        if (a.splits > 1 && lane == 0) { pp[a.D] = split_max(n, m1); pp[a.D + 1] = l1; }
     }
 }
 
 // o = the splits' sums joined, a CTA to a (sequence, head)
 template <typename T>
-__global__ void __launch_bounds__(128) attn_step_join_kernel(const float* part, int splits, int D, T* o) {
+__global__ void __launch_bounds__(128) attn_step_join_kernel(StepArgs a, const T* q, const T* k, const T* v, float* part, T* o) {
     __shared__ float s_f[ST_MAX_SPLITS], s_red[2];
-    const float* pp = part + (size_t)blockIdx.x * splits * (D + 2);
+    const int splits = a.splits, D = a.D;
+    float* pp = part + (size_t)blockIdx.x * splits * (D + 2);
     const int tid = threadIdx.x;
-    if (tid < 32) {
-        float top = -INFINITY, l = 0.f;
-        for (int i = tid; i < splits; i += 32) top = fmaxf(top, pp[(size_t)i * (D + 2) + D]);
+    auto join = [&] {                                    // whether the result is finite in this thread's channels
+        if (tid < 32) {
+            float top = -INFINITY, l = 0.f;
+            for (int i = tid; i < splits; i += 32) top = fmaxf(top, pp[(size_t)i * (D + 2) + D]);
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, off));
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int i = tid; i < splits; i += 32) {
-            const float f = exp2f(pp[(size_t)i * (D + 2) + D] - base);
-            s_f[i] = f;
-            l = fmaf(pp[(size_t)i * (D + 2) + D + 1], f, l);
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, off));
+            const float base = top == -INFINITY ? 0.f : top;
+            for (int i = tid; i < splits; i += 32) {
+                const float f = exp2f(pp[(size_t)i * (D + 2) + D] - base);
+                s_f[i] = f;
+                l = fmaf(pp[(size_t)i * (D + 2) + D + 1], f, l);
+            }
+            l = warp_sum(l);
+            if (tid == 0) { s_red[0] = l; s_red[1] = top; }
         }
-        l = warp_sum(l);
-        if (tid == 0) { s_red[0] = l; s_red[1] = top; }
-    }
-    __syncthreads();
-    for (int d = tid; d < D; d += 128) {
-        float s = 0.f;
-        for (int i = 0; i < splits; i++) s = fmaf(pp[(size_t)i * (D + 2) + d], s_f[i], s);
-        st1(o + (size_t)blockIdx.x * D + d, s_red[1] == -INFINITY ? 0.f : s / s_red[0]);
+        __syncthreads();
+        bool finite = true;
+        for (int d = tid; d < D; d += 128) {
+            float s = 0.f;
+            for (int i = 0; i < splits; i++) s = fmaf(pp[(size_t)i * (D + 2) + d], s_f[i], s);
+            finite = finite && isfinite(s);
+            st1(o + (size_t)blockIdx.x * D + d, s_red[1] == -INFINITY ? 0.f : s / s_red[0]);
+        }
+        return finite;
+    };
+    const bool finite = join();
+    if constexpr (sizeof(T) == 2) {                      // the parts that are not finite anew, a warp to a part, and the join once more
+        if (__syncthreads_and(finite)) return;
+        const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, lane = tid & 31;
+        const Seen sn = seen_of(a, b);
+        const int per = (sn.n + splits - 1) / splits;
+        for (int i = tid / 32; i < splits; i += 4) {
+            float* one = pp + (size_t)i * (D + 2);
+            float w = 0.f;
+            for (int d = lane; d < D; d += 32) watch(w, one[d]);
+            if (!__any_sync(FULL, w != w)) continue;
+            const int lo = min(i * per, sn.n), hi = min(lo + per, sn.n);
+            float y[4], m, l;
+            redo_head(a, q, k, v, b, h, sn, lo, hi, y, m, l);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (lane + 32 * e < D) one[lane + 32 * e] = y[e];
+            if (lane == 0) { one[D] = split_max(sn.n, m); one[D + 1] = l; }
+        }
+        __syncthreads();
+        join();
     }
 }
 
@@ -399,17 +445,23 @@ static cudaError_t launch_step_f32(const StepArgs& a, const void* q, const void*
         case 4: go(attn_step_kernel<float, LPG, 4>); break;
         default: go(attn_step_kernel<float, LPG, 8>); break;
     }
-    if (a.splits > 1) attn_step_join_kernel<float><<<a.B * a.H, 128, 0, st>>>(part, a.splits, a.D, (float*)o);
+    if (a.splits > 1) attn_step_join_kernel<float><<<a.B * a.H, 128, 0, st>>>(a, (const float*)q, (const float*)k, (const float*)v, part, (float*)o);
     return cudaGetLastError();
 }
-template <int DP>
-static cudaError_t launch_step_bf16(const StepArgs& a, const void* q, const void* k, const void* v, void* o, float* part, cudaStream_t st) {
+template <int DP, bool WHOLE>
+static cudaError_t launch_step_mma(const StepArgs& a, const void* q, const void* k, const void* v, void* o, float* part, cudaStream_t st) {
     const size_t sm = (size_t)SM_WARPS * SM_STAGES * 2 * SM_KEYS * DP * 2;
-    auto kern = heads_at_once(a.H / a.KV, SLOTSCAN_BF16) == 16 ? attn_step_mma_kernel<DP, true> : attn_step_mma_kernel<DP, false>;
+    auto kern = heads_at_once(a.H / a.KV, SLOTSCAN_BF16) == 16 ? attn_step_mma_kernel<DP, true, WHOLE> : attn_step_mma_kernel<DP, false, WHOLE>;
     const cudaError_t e = opt_in_smem(kern, sm);
     if (e != cudaSuccess) return e;
     kern<<<dim3(a.splits, a.KV * a.chunks, a.B), SM_WARPS * 32, sm, st>>>(a, (const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o, part);
-    if (a.splits > 1) attn_step_join_kernel<bf16><<<a.B * a.H, 128, 0, st>>>(part, a.splits, a.D, (bf16*)o);
+    return cudaSuccess;
+}
+template <int DP>
+static cudaError_t launch_step_bf16(const StepArgs& a, const void* q, const void* k, const void* v, void* o, float* part, cudaStream_t st) {
+    const cudaError_t e = a.splits == 1 ? launch_step_mma<DP, true>(a, q, k, v, o, part, st) : launch_step_mma<DP, false>(a, q, k, v, o, part, st);
+    if (e != cudaSuccess) return e;
+    if (a.splits > 1) attn_step_join_kernel<bf16><<<a.B * a.H, 128, 0, st>>>(a, (const bf16*)q, (const bf16*)k, (const bf16*)v, part, (bf16*)o);
     return cudaGetLastError();
 }
 
