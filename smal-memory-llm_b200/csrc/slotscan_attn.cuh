@@ -275,6 +275,16 @@ struct CapPoly {
     }
 };
 
+// cap tanh(x) in base-2 exponents, of y = 2 log2(e) x, for the steps.  1 - 2 / (e^2x + 1) is off by 1.2e-7 of the cap wherever x is, which of a
+// small x, under a cap far above the scores, is all of it (1 % of a weight for cap 1e5); so below 1/4 the series of tanh, to x^9, which is off by
+// 1e-8 of the score.
+constexpr float CAP_SMALL = 0.25f * 2.f * LOG2E;
+__device__ __forceinline__ float cap_small(float y, float cap2) {
+    const float x = y * (0.5f / LOG2E), w = x * x;
+    return cap2 * (x * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f));
+}
+__device__ __forceinline__ float cap_large(float y, float cap2) { return fmaf(-2.f * cap2, __fdividef(1.f, exp2f(y) + 1.f), cap2); }
+
 // the launches of the two families, float32 and bf16
 cudaError_t run_attn_fwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st);
 cudaError_t run_attn_bwd_f32(const AttnArgs& a, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,

@@ -174,9 +174,10 @@ __device__ __forceinline__ void redo_head(const StepArgs& a, const bf16* q, cons
                  y, m, l);
 }
 
-// WIDE: 16 query heads to a CTA, else 8.
+// WIDE: 16 query heads to a CTA, else 8.  HIGH_CAP: small scores are capped by a form of their own.  Up to a cap of 256 the large ones' form is off
+// by 2^-15 of a weight at most, far below the result's rounding; the choice within the kernel cost 32 capped sequences of 8,192 90 us for 84.
 // WHOLE: one split, whose heads that are not finite are redone here; those of several the join redoes (in here it cost 8 of 131,072 2 %).
-template <int DP, bool WIDE, bool WHOLE>
+template <int DP, bool WIDE, bool HIGH_CAP, bool WHOLE>
 __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a, const bf16* q, const bf16* k, const bf16* v, bf16* o, float* part) {
     constexpr int PIECES = DP / 8, PER_PASS = 32 / PIECES, ROW = DP * 2, TILE = SM_KEYS * ROW, R = WIDE ? 2 : 1, HEADS = 8 * R;
     extern __shared__ float4 smem4[];
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) attn_step_mma_kernel(StepArgs a
             for (int i = 0; i < 4; i++) {
                 const int j = j0 + (i / 2) * 8 + (lane % 4) * 2 + i % 2;
                 float x = s[i / 2][2 * r + i % 2] * lin;
-                if (capped) x = fmaf(-2.f * cap2, __fdividef(1.f, exp2f(x) + 1.f), cap2);      // tanh x = 1 - 2 / (e^2x + 1)
+                if (capped) x = HIGH_CAP && fabsf(x) < CAP_SMALL ? cap_small(x, cap2) : cap_large(x, cap2);
                 x = fmaf(-slope[r], (float)(n - 1 - j), x);
                 z[i] = j < hi ? x : -INFINITY;
                 top = fmaxf(top, z[i]);
@@ -448,10 +449,10 @@ static cudaError_t launch_step_f32(const StepArgs& a, const void* q, const void*
     if (a.splits > 1) attn_step_join_kernel<float><<<a.B * a.H, 128, 0, st>>>(a, (const float*)q, (const float*)k, (const float*)v, part, (float*)o);
     return cudaGetLastError();
 }
-template <int DP, bool WHOLE>
+template <int DP, bool HIGH_CAP, bool WHOLE>
 static cudaError_t launch_step_mma(const StepArgs& a, const void* q, const void* k, const void* v, void* o, float* part, cudaStream_t st) {
     const size_t sm = (size_t)SM_WARPS * SM_STAGES * 2 * SM_KEYS * DP * 2;
-    auto kern = heads_at_once(a.H / a.KV, SLOTSCAN_BF16) == 16 ? attn_step_mma_kernel<DP, true, WHOLE> : attn_step_mma_kernel<DP, false, WHOLE>;
+    auto kern = heads_at_once(a.H / a.KV, SLOTSCAN_BF16) == 16 ? attn_step_mma_kernel<DP, true, HIGH_CAP, WHOLE> : attn_step_mma_kernel<DP, false, HIGH_CAP, WHOLE>;
     const cudaError_t e = opt_in_smem(kern, sm);
     if (e != cudaSuccess) return e;
     kern<<<dim3(a.splits, a.KV * a.chunks, a.B), SM_WARPS * 32, sm, st>>>(a, (const bf16*)q, (const bf16*)k, (const bf16*)v, (bf16*)o, part);
@@ -459,7 +460,9 @@ static cudaError_t launch_step_mma(const StepArgs& a, const void* q, const void*
 }
 template <int DP>
 static cudaError_t launch_step_bf16(const StepArgs& a, const void* q, const void* k, const void* v, void* o, float* part, cudaStream_t st) {
-    const cudaError_t e = a.splits == 1 ? launch_step_mma<DP, true>(a, q, k, v, o, part, st) : launch_step_mma<DP, false>(a, q, k, v, o, part, st);
+    const bool high = a.cap > 256.f, whole = a.splits == 1;
+    const cudaError_t e = high ? (whole ? launch_step_mma<DP, true, true>(a, q, k, v, o, part, st) : launch_step_mma<DP, true, false>(a, q, k, v, o, part, st))
+                               : (whole ? launch_step_mma<DP, false, true>(a, q, k, v, o, part, st) : launch_step_mma<DP, false, false>(a, q, k, v, o, part, st));
     if (e != cudaSuccess) return e;
     if (a.splits > 1) attn_step_join_kernel<bf16><<<a.B * a.H, 128, 0, st>>>(a, (const bf16*)q, (const bf16*)k, (const bf16*)v, part, (bf16*)o);
     return cudaGetLastError();

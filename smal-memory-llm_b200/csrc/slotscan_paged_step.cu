@@ -111,17 +111,6 @@ __device__ __forceinline__ void step_range(const PagedArgs& a, const StepPlan& p
     c.s = (int)(in % c.w.steps);
 }
 
-// cap tanh(x) in base-2 exponents, of y = 2 log2(e) x.  1 - 2 / (e^2x + 1) is off by 1.2e-7 of the cap wherever x is, which of a small x, under
-// a cap far above the scores, is all of it (1 % of a weight for cap 1e5); so below 1/4 the series of tanh, to x^9, which is off by 1e-8 of the
-// score.  A warp whose scores are all small forms that one alone: 32 requests of up to 8,192 tokens, capped at 30,
-// 57.3 us (59.2 with the exponential form alone, 60.5 with both for every score).
-constexpr float CAP_SMALL = 0.25f * 2.f * LOG2E;
-__device__ __forceinline__ float cap_small(float y, float cap2) {
-    const float x = y * (0.5f / LOG2E), w = x * x;
-    return cap2 * (x * fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f));
-}
-__device__ __forceinline__ float cap_large(float y, float cap2) { return fmaf(-2.f * cap2, __fdividef(1.f, exp2f(y) + 1.f), cap2); }
-
 // Page ids of 32 steps from `base` on, a lane to a step; of both halves of 8 keys
 struct Ids {
     int base, lo, hi;
@@ -254,7 +243,7 @@ __global__ void __launch_bounds__(PS_THREADS, step_ctas_per_sm(SLOTSCAN_BF16, DP
             float z[4], top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; i++) z[i] = s[i / 2][2 * r + i % 2] * lin;
-            if (capped) {
+            if (capped) {                                // one form for a warp whose scores are all small: 57.3 us of 32 capped requests, both 60.5
                 const bool small = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3]))) < CAP_SMALL;
                 if (__all_sync(FULL, small)) {
 #pragma unroll

@@ -58,3 +58,27 @@ def test_a_step_that_sees_infinite_values(B, L, H, KV, D, dtype):
     # done anew in another order: both are within the tolerance of the formula; |v| < 5.5, scale |q| |k| < 0.3 * 30 * D^(1/2)
     E = (D + 16) * 2.0 ** -24 * 0.3 * 30 * D ** 0.5
     within(a, b, 2 * (4 * E + (L + 64) * 2.0 ** -24) * 5.5 + (2.0 ** -7 if dtype == "bf16" else 2.0 ** -22) * (b.abs() + 1e-3), "other channels")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap", [0.5, 30.0, 256.0, 1e3, 1e5, 1e7])
+def test_caps_of_a_step(cap, dtype):
+    """A cap far above the scores leaves them as they are; one below them bends them all.  Against the formula in float64: a score is off by
+    E = (D + 16) 2^-24 of the greatest magnitude of its terms, a weight by 4 E of itself, a sum over the keys by (keys + 64) 2^-24, the
+    result in bf16 by 2^-8; caps up to 256 by 2^-15 of a weight on top."""
+    import slotscan_b200 as S
+    g = _gen(62)
+    dt = DT[dtype]
+    B, L, D = 2, 1500, 64
+    for H, KV in ((12, 4), (12, 1)):
+        kc, vc, q = _rand(g, B, L, KV, D).to(dt), _rand(g, B, L, KV, D).to(dt), (2 * _rand(g, B, 1, H, D)).to(dt)
+        got = S.token_attention_step(q, kc, vc, torch.tensor([L - 1, 600], device="cuda"), cap=cap)
+        for b, n in enumerate((L, 601)):
+            k, v = (t[b, :n].double().transpose(0, 1).repeat_interleave(H // KV, 0) for t in (kc, vc))
+            x = q[b].double().transpose(0, 1)
+            s = x @ k.transpose(1, 2) * D ** -0.5
+            worst = float((x.abs() @ k.abs().transpose(1, 2) * D ** -0.5).max())
+            p = torch.softmax(cap * torch.tanh(s / cap), -1)
+            o, size = (p @ v).squeeze(1), (p @ v.abs()).squeeze(1)
+            E = (D + 16) * 2.0 ** -24 * worst
+            within(got[b, 0], o, (4 * E + (n + 64) * 2.0 ** -24 + (2 * 2.0 ** -15 if cap <= 256 else 0)) * size + (2.0 ** -8 if dtype == "bf16" else 2.0 ** -23) * o.abs(), "H %d" % H)
